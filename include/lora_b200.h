@@ -61,6 +61,13 @@ enum lora_status {
 
 enum lora_dtype { LORA_F16 = 0, LORA_BF16 = 1, LORA_F32 = 2 };
 
+/* Microscaled formats (codes with a scale per block of a row). */
+enum lora_mx_format {
+  LORA_MXFP4 = 0, /* E2M1 codes, a power of two (E8M0) per 32 values          */
+  LORA_NVFP4 = 1, /* E2M1 codes, E4M3 per 16 values, one fp32 per tensor      */
+  LORA_MXFP8 = 2  /* E4M3 codes, a power of two (E8M0) per 32 values          */
+};
+
 /* Layout of a LoRA up-projection B as seen by the expand kernels. */
 enum lora_b_layout {
   LORA_B_PEFT = 0,      /* B[n * ldb + j]  : lora_B.weight [N, R]            */
@@ -340,6 +347,56 @@ LORA_API int lora_sgmv_linear(const void* x, int64_t ldx, const void* w, int64_t
                      const int32_t* tiles, void* out, int64_t ldo, int64_t T, int64_t S, int64_t K, int64_t N,
                      int64_t r_max, float scale, int dtype, void* workspace, size_t workspace_bytes,
                      void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Microscaled tensors.  An [M, K] tensor (Kp = K rounded up to 32) is
+ *   codes   row-major, lora_mx_codes_size(M, K, fmt) bytes: Kp/2 a row for
+ *           4-bit codes (the even column in the low half of a byte), Kp for
+ *           8-bit ones; columns K..Kp-1 hold zeros
+ *   scales  lora_mx_scales_size(M, K, fmt) bytes: 512-byte chunks of 128 rows x
+ *           4 blocks, chunk (row / 128) * ceil(blocks / 4) + block / 4; row r,
+ *           block g of a chunk at byte 16 (r % 32) + 4 (r / 32) + g; zeros
+ *           beyond the tensor
+ * both 16-byte aligned, and a value is code x block scale x global_scale
+ * (global_scale 1 except for LORA_NVFP4, there in [2^-64, 2^64]).
+ *
+ * lora_mx_quantize: x [M, K] (any ldx >= K) to the format.  MXFP4 / MXFP8: the
+ * scale is 2^max(floor(log2 amax) - top, -127), top = 2 / 8.  NVFP4: the block
+ * scale is E4M3(amax / (6 global_scale)), quotients in fp32.  Codes are the
+ * scaled values rounded to nearest even, saturating.  A block with an infinity
+ * or a NaN becomes NaN as a whole.
+ * lora_mx_dequantize: the values in dtype, [M, K] or (transpose) [K, M].
+ * Limits: M <= 8388480, K <= 2^30.  No counterpart in the reference, whose
+ * base weights and activations are 16-bit.
+ * ------------------------------------------------------------------------- */
+LORA_API size_t lora_mx_codes_size(int64_t M, int64_t K, int fmt);
+LORA_API size_t lora_mx_scales_size(int64_t M, int64_t K, int fmt);
+LORA_API int lora_mx_quantize(const void* x, int64_t ldx, void* codes, void* scales, int64_t M, int64_t K, int fmt,
+                     float global_scale, int dtype, void* stream);
+LORA_API int lora_mx_dequantize(const void* codes, const void* scales, void* out, int64_t ldo, int64_t M, int64_t K,
+                       int fmt, float global_scale, int transpose, int dtype, void* stream);
+
+/* LoRA linear with 4-bit base operands (MXFP4 or NVFP4):
+ *   out[M,N] = q(x) . W^T + scale * (x . a^T) . b^T + bias
+ * W [N, K] as microscaled codes and scales (w_global its tensor scale); x is
+ * quantised to the same format inside the call (tensor scale x_global), the
+ * adapter's products take x in 16 bits.  a [R, K], b [N, R], R <= 256 (0: no
+ * adapter).  Launches: the quantisation, the shrink to a hi/lo pair
+ * z = (scale / zs) x . a^T, the block-scaled tensor-core GEMM with z . b^T as its
+ * last K steps.  z_out (NULL, or [M, 2 r16], r16 = R rounded up to 16, 16-byte
+ * aligned) receives z = [hi | lo] for the backward pass; zs =
+ * lora_mx_linear_z_scale(x_global, w_global, fmt), 1 for MXFP4.
+ * Workspace: lora_mx_linear_workspace_size bytes, 256-byte aligned, with a
+ * zeroed ticket region first as lora_shrink's; calls that share one must not
+ * overlap on the GPU.  Rows of b: 16-byte aligned (any layout when R is not a
+ * multiple of 8: it is copied); R > 128 also needs K, ldx, lda multiples of 8
+ * and x, a 16-byte aligned.  No counterpart in the reference. */
+LORA_API size_t lora_mx_linear_workspace_size(int64_t M, int64_t N, int64_t K, int64_t R, int fmt);
+LORA_API float lora_mx_linear_z_scale(float x_global, float w_global, int fmt);
+LORA_API int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, const void* w_scales, float w_global,
+                   const void* bias, const void* a, int64_t lda, const void* b, int64_t ldb, void* out,
+                   int64_t ldo, void* z_out, int64_t M, int64_t N, int64_t K, int64_t R, float scale,
+                   float x_global, int fmt, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

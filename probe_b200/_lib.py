@@ -35,6 +35,10 @@ LORA_F16 = 0
 LORA_BF16 = 1
 LORA_F32 = 2
 
+LORA_MXFP4 = 0
+LORA_NVFP4 = 1
+LORA_MXFP8 = 2
+
 LORA_B_PEFT = 0
 LORA_B_RANK_MAJOR = 1
 
@@ -83,6 +87,14 @@ SIGNATURES = {
     "lora_sgmv_linear_workspace_size": (_SZ, [_I64, _I64, _I64, _I64]),
     "lora_sgmv_linear": (_I, [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _I64,
                               _I64, _I64, _I64, _I64, _F, _I, _P, _SZ, _P]),
+    "lora_mx_codes_size": (_SZ, [_I64, _I64, _I]),
+    "lora_mx_scales_size": (_SZ, [_I64, _I64, _I]),
+    "lora_mx_quantize": (_I, [_P, _I64, _P, _P, _I64, _I64, _I, _F, _I, _P]),
+    "lora_mx_linear_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _I]),
+    "lora_mx_linear_z_scale": (_F, [_F, _F, _I]),
+    "lora_mx_linear": (_I, [_P, _I64, _P, _P, _F, _P, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _F, _F,
+                            _I, _I, _P, _SZ, _P]),
+    "lora_mx_dequantize": (_I, [_P, _P, _P, _I64, _I64, _I64, _I, _F, _I, _I, _P]),
 }
 
 

@@ -1,0 +1,103 @@
+// Microscaled formats (4- and 8-bit floating point with a scale per block).
+//
+//   mxfp4   E2M1 codes, a power of two (E8M0 byte) per 32 values of a row
+//   nvfp4   E2M1 codes, an E4M3 scale per 16 values, one fp32 scale per tensor
+//   mxfp8   E4M3 codes, a power of two (E8M0 byte) per 32 values
+//
+// Storage of an [M, K] tensor, Kp = K rounded up to 32:
+//   codes   row-major, Kp/2 bytes a row (two E2M1 codes a byte, the even column
+//           in the low half) or Kp bytes (E4M3); columns K..Kp-1 hold zeros
+//   scales  512-byte chunks of 128 rows x 4 blocks, chunk (row / 128) * GB +
+//           block / 4 with GB = ceil(blocks / 4); row r and block g of a chunk
+//           at byte 16 (r % 32) + 4 (r / 32) + g; rows and blocks beyond the
+//           tensor hold zeros.  One chunk is what tcgen05.cp.32x128b copies
+//           into 4 columns of TMEM for a block-scaled MMA, so neither the
+//           product nor its loads rearrange a byte.
+#pragma once
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "runtime.h"
+
+namespace lora {
+
+template <int FMT> struct MxFormat;
+template <> struct MxFormat<LORA_MXFP4> {
+  static constexpr int kBlock = 32, kBits = 4, kTop = 2;  // kTop: exponent of the largest code
+};
+template <> struct MxFormat<LORA_NVFP4> {
+  static constexpr int kBlock = 16, kBits = 4, kTop = 2;
+};
+template <> struct MxFormat<LORA_MXFP8> {
+  static constexpr int kBlock = 32, kBits = 8, kTop = 8;
+};
+
+inline int mx_block(int fmt) { return fmt == LORA_NVFP4 ? 16 : 32; }
+inline int mx_bits(int fmt) { return fmt == LORA_MXFP8 ? 8 : 4; }
+inline int64_t mx_padded_k(int64_t k) { return (k + 31) / 32 * 32; }
+inline int64_t mx_code_pitch(int64_t k, int fmt) { return mx_padded_k(k) * mx_bits(fmt) / 8; }
+inline int64_t mx_scale_chunks(int64_t k, int fmt) { return (mx_padded_k(k) / mx_block(fmt) + 3) / 4; }
+inline bool mx_format_ok(int fmt) { return fmt == LORA_MXFP4 || fmt == LORA_NVFP4 || fmt == LORA_MXFP8; }
+// The tensor-wide scale of nvfp4 (1 for the others): in this range scale x block
+// scale and its reciprocal are normal fp32 numbers.
+inline bool mx_global_ok(float g, int fmt) {
+  return fmt == LORA_NVFP4 ? (g >= 5.4210109e-20f && g <= 1.8446744e19f) : g == 1.0f;  // [2^-64, 2^64]
+}
+
+// 2^(byte - 127) of an E8M0 scale byte; 255 is NaN.
+LORA_DEVINL float mx_e8m0(uint32_t byte) {
+  const uint32_t bits = byte == 0 ? 0x00400000u : (byte == 255 ? 0x7fffffffu : byte << 23);
+  return __uint_as_float(bits);
+}
+// One E4M3 byte.
+LORA_DEVINL float mx_e4m3(uint32_t byte) {
+  uint32_t h2;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(byte)));
+  return __low2float(*reinterpret_cast<__half2*>(&h2));
+}
+// Two floats -> two E4M3 codes (lo in the low byte), nearest even, saturating.
+LORA_DEVINL uint32_t mx_to_e4m3x2(float lo, float hi) {
+  uint16_t d;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+// Eight floats -> eight E2M1 codes, the first in the low bits.
+LORA_DEVINL uint32_t mx_to_e2m1x8(const float* v) {
+  uint32_t d;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(d)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return d;
+}
+// Eight E2M1 codes -> four f16 pairs (exact).
+LORA_DEVINL void mx_from_e2m1x8(uint32_t w, uint32_t* h2) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h2[0]), "=r"(h2[1]), "=r"(h2[2]), "=r"(h2[3])
+      : "r"(w));
+}
+// Two E4M3 codes -> one f16 pair (exact).
+LORA_DEVINL uint32_t mx_from_e4m3x2(uint32_t w) {
+  uint32_t h2;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(w)));
+  return h2;
+}
+
+// Device entry points of the parts (host launchers), used by the C ABI and by
+// the composite operators.
+int mx_quantize_launch(const void* x, int64_t ldx, void* codes, void* scales, int64_t M, int64_t K, int fmt,
+                       float global_scale, int dtype, cudaStream_t stream);
+int mx_dequantize_launch(const void* codes, const void* scales, void* out, int64_t ldo, int64_t M, int64_t K, int fmt,
+                         float global_scale, int transpose, int dtype, cudaStream_t stream);
+
+}  // namespace lora

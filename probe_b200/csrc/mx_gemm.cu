@@ -1,0 +1,473 @@
+// 4-bit block-scaled GEMM with the LoRA expand folded in.
+//
+//   out[M,N] = alpha ( 2^-d sum_k xq[m,k] sx[m,k/b] wq[n,k] sw[n,k/b]
+//                      + sum_j (zh[m,j] + zl[m,j]) B[n,j] ) + bias[n]
+//
+// xq, wq: E2M1 codes, sx, sw: their block scales (mx.cuh), multiplied inside
+// tcgen05.mma.kind::mxf4nvf4 as the products are formed.  z = [zh | zl] is the
+// 16-bit hi/lo pair of the adapter's shrink; its products with B are kind::f16
+// MMAs into the same fp32 accumulator, after the base ones.  nvfp4 has
+// alpha 2^-d = the product of the two tensor scales with alpha in [1, 2): the
+// power of two is taken off the accumulator by the first tail MMA (scale-input-d,
+// exact, at most 2^-15; beyond that a stage of zeros takes off the first 2^-15),
+// so z stays within the range of fp16.
+//
+// Bound: the tensor pipe (K = 64 steps of M 256 x N 256 a pair) and, with it,
+// the operand intake of each SM: a 256-deep stage brings 32 KB of codes and 3
+// to 6 KB of scales for 4 MMAs, the byte ratio of a 16-bit GEMM with 256 x 256
+// tiles.  Layout: a cluster of two CTAs per 256 x 256 tile, persistent; warp 0
+// TMA (codes in 128-byte swizzled rows, scale chunks as they are stored), warp
+// 1 of the leader copies the stage's scales to TMEM (tcgen05.cp, each CTA from
+// its own shared memory) and issues the MMAs, warps 2..5 the epilogue.
+// TMEM: two 256-column accumulators and two buffers of scales do not fit 512
+// columns, so the accumulators share 48 (mxfp4) or 96 (nvfp4) columns: the
+// epilogue drains those first and only they hold up the next tile's MMAs.
+#include <cudaTypedefs.h>
+
+#include <cmath>
+#include <mutex>
+
+#include "mx_linear.h"
+
+namespace lora {
+namespace {
+
+constexpr int kMxEpiWarps = 4;
+constexpr int kMxGemmThreads = 64 + 32 * kMxEpiWarps;
+
+struct MxGemmArgs {
+  void* out;
+  const void* bias;
+  int* err;
+  int64_t ldo;
+  int M, N;
+  int num_kb;         // 256-deep base stages
+  int last_k64;       // MMA steps of the last one
+  int rank_kb;        // 64-deep tail stages of each z part (0: no adapter)
+  int last_k16;       // MMA steps of the last of them
+  int zero_kb;        // 1: a tail stage of zeros comes first
+  int chunks;         // scale chunks of a block of 128 rows
+  int num_m_tiles, num_n_tiles, num_tiles, group_m;
+  int dshift;         // 0..30
+  float alpha;
+};
+
+template <int FMT>
+struct MxSmem {
+  static constexpr int kChunks = 256 / MxFormat<FMT>::kBlock / 4;  // scale chunks of 128 rows a stage
+  static constexpr int kStages = FMT == LORA_MXFP4 ? 6 : 5;
+  static constexpr int kOpBytes = 128 * 128;                       // codes (or z, B) of 128 rows
+  static constexpr int kSfBytes = 3 * kChunks * 512;               // x rows, then the W rows of both CTAs
+  static constexpr int kMainBytes = 2 * kOpBytes + kSfBytes;
+  static constexpr int kSfOffset = kStages * 2 * kOpBytes;
+  static constexpr int kBarOffset = kSfOffset + kStages * kSfBytes;
+  static constexpr int kBytes = kBarOffset + 256 + 1024;
+  // TMEM columns
+  static constexpr int kSfCols = 3 * kChunks * 4;
+  static constexpr int kSfBase = 512 - 2 * kSfCols;
+  static constexpr int kAcc1 = kSfBase - 256;  // accumulator 1; accumulator 0 starts at 0
+  static constexpr int kOverlap = 256 - kAcc1;
+  static_assert(kOverlap % 16 == 0 && kBytes <= 227 * 1024, "layout");
+};
+
+// Descriptor of a scale chunk in shared memory: 32 rows of 16 bytes, no swizzle,
+// 8-row groups 128 bytes apart.
+LORA_DEVINL uint64_t mx_desc_scales(uint32_t addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((addr >> 4) & 0x3FFF);
+  d |= static_cast<uint64_t>(128 >> 4) << 16;
+  d |= static_cast<uint64_t>(128 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  return d;
+}
+
+LORA_DEVINL void mx_cp_scales_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+template <int FMT>
+LORA_DEVINL void mx_mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                             uint32_t accumulate) {
+  if constexpr (FMT == LORA_MXFP4) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  }
+}
+
+// D = A B^T + D 2^-S
+template <int S>
+LORA_DEVINL void mx_mma_f16_pair_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.eq.b32 p, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p, %4;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "n"(S)
+      : "memory");
+}
+LORA_DEVINL void mx_mma_f16_pair_shift(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int shift) {
+  switch (shift) {
+#define LORA_MX_CASE(S) \
+  case S: mx_mma_f16_pair_scaled<S>(d, a, b, idesc); break;
+    LORA_MX_CASE(1) LORA_MX_CASE(2) LORA_MX_CASE(3) LORA_MX_CASE(4) LORA_MX_CASE(5) LORA_MX_CASE(6) LORA_MX_CASE(7)
+    LORA_MX_CASE(8) LORA_MX_CASE(9) LORA_MX_CASE(10) LORA_MX_CASE(11) LORA_MX_CASE(12) LORA_MX_CASE(13)
+    LORA_MX_CASE(14) LORA_MX_CASE(15)
+#undef LORA_MX_CASE
+    default: tc_mma_f16_pair(d, a, b, idesc, 1u);
+  }
+}
+
+// Block-scaled instruction descriptor: E2M1 operands, K-major, fp32 accumulator;
+// the scale ids (the pair of bytes of a 32-bit scale word) are added per MMA.
+template <int FMT>
+__host__ __device__ constexpr uint32_t mx_idesc(int m, int n) {
+  return (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | ((FMT == LORA_MXFP4 ? 1u : 0u) << 23) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+LORA_DEVINL void mx_tile_coords(int tile, const MxGemmArgs& a, int& mt, int& nt) {
+  const int group_size = a.group_m * a.num_n_tiles;
+  const int group = tile / group_size;
+  const int first_m = group * a.group_m;
+  const int gm = min(a.num_m_tiles - first_m, a.group_m);
+  const int in_group = tile - group * group_size;
+  mt = first_m + in_group % gm;
+  nt = in_group / gm;
+}
+
+struct MxMaps {
+  CUtensorMap x, w, sx, sw, zh, zl, b;
+};
+
+template <typename T>
+LORA_DEVINL void mx_store16(const MxGemmArgs& args, T* out_row, int row, int col0, bool vec, const uint32_t* r) {
+  if (row >= args.M || col0 >= args.N) return;
+  const T* bias = static_cast<const T*>(args.bias);
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]) * args.alpha;
+  if (bias != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (col0 + i < args.N) v[i] += to_f32(bias[col0 + i]);
+  }
+  if (vec && col0 + 16 <= args.N) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    uint4* dst = reinterpret_cast<uint4*>(out_row + col0);
+    dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (col0 + i < args.N) out_row[col0 + i] = from_f32<T>(v[i]);
+  }
+}
+
+template <typename T, int FMT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
+    mx_gemm_pair_kernel(const __grid_constant__ MxMaps maps, const MxGemmArgs args) {
+  using L = MxSmem<FMT>;
+  constexpr uint32_t kIdesc = mx_idesc<FMT>(256, 256);
+  constexpr uint32_t kIdescTail = umma_idesc_f16(256, 256, std::is_same<T, __nv_bfloat16>::value ? 1 : 0);
+  constexpr uint16_t kBoth = 0x3;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* sm_a = smem;
+  uint8_t* sm_b = smem + L::kStages * L::kOpBytes;
+  uint8_t* sm_sf = smem + L::kSfOffset;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOffset);
+  uint64_t* empty = full + L::kStages;
+  uint64_t* acc_full = empty + L::kStages;  // a tile's MMAs are complete
+  uint64_t* acc_free = acc_full + 1;        // its shared columns are drained
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_free + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int pair = blockIdx.x >> 1;
+  const int npairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < L::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_free, 2 * kMxEpiWarps);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&maps.x);
+    tma_prefetch_desc(&maps.w);
+    tma_prefetch_desc(&maps.sx);
+    tma_prefetch_desc(&maps.sw);
+  }
+  if (warp == 2) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int tail_kb = 2 * args.rank_kb + args.zero_kb;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < args.num_tiles; tile += npairs) {
+        int mt, nt;
+        mx_tile_coords(tile, args, mt, nt);
+        const int row_a = mt * 256 + static_cast<int>(rank) * 128;
+        const int row_b = nt * 256 + static_cast<int>(rank) * 128;
+        for (int kb = 0; kb < args.num_kb + tail_kb; ++kb) {
+          if (!mbar_wait_bounded(&empty[stage], phase ^ 1, abort_flag, args.err, kDevErrTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);
+          uint8_t* a = sm_a + stage * L::kOpBytes;
+          uint8_t* b = sm_b + stage * L::kOpBytes;
+          if (kb < args.num_kb) {
+            if (leader) mbar_arrive_expect_tx(&full[stage], 2 * L::kMainBytes);
+            uint8_t* sf = sm_sf + stage * L::kSfBytes;
+            tma_load_2d_pair(&maps.x, a, bar, kb * 128, row_a);
+            tma_load_2d_pair(&maps.w, b, bar, kb * 128, row_b);
+            tma_load_2d_pair(&maps.sx, sf, bar, 0, (row_a >> 7) * args.chunks + kb * L::kChunks);
+            tma_load_2d_pair(&maps.sw, sf + L::kChunks * 512, bar, 0, nt * 2 * args.chunks + kb * L::kChunks);
+            tma_load_2d_pair(&maps.sw, sf + 2 * L::kChunks * 512, bar, 0,
+                             (nt * 2 + 1) * args.chunks + kb * L::kChunks);
+          } else {
+            if (leader) mbar_arrive_expect_tx(&full[stage], 4 * L::kOpBytes);
+            // (the stage of zeros lies beyond the operands' columns)
+            const int t = kb - args.num_kb - args.zero_kb;
+            const bool lo = t >= args.rank_kb;
+            const int c = (t < 0 ? args.rank_kb : lo ? t - args.rank_kb : t) * 64;
+            tma_load_2d_pair(lo ? &maps.zl : &maps.zh, a, bar, c, row_a);
+            tma_load_2d_pair(&maps.b, b, bar, c, row_b);
+          }
+          if (++stage == L::kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (leader && lane == 0) {
+      int stage = 0, prev = 0;
+      uint32_t phase = 0;
+      int use = 0;  // stages used so far; scale buffer = use & 1
+      int local = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < args.num_tiles; tile += npairs, ++local) {
+        if (local > 0 && !mbar_wait_bounded(acc_free, (local - 1) & 1, abort_flag, args.err, kDevErrTimeoutAccEmpty))
+          break;
+        tc_fence_after();
+        const uint32_t d = tmem + ((local & 1) ? L::kAcc1 : 0);
+        for (int kb = 0; kb < args.num_kb + tail_kb; ++kb, ++use) {
+          if (!mbar_wait_bounded(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          // The MMAs of two uses ago read the scale buffer that is written next; those
+          // of the last base stage finish before MMAs of the other kind start.
+          const int behind = kb < args.num_kb ? 2 : (kb == args.num_kb ? 1 : 0);
+          if (behind > 0 && use >= behind) {
+            prev = use - behind;
+            if (!mbar_wait_bounded(&empty[prev % L::kStages], (prev / L::kStages) & 1, abort_flag, args.err,
+                                   kDevErrTimeoutEmpty)) {
+              ok = false;
+              break;
+            }
+          }
+          tc_fence_after();
+          const uint64_t ad = umma_desc_sw128(smem_u32(sm_a + stage * L::kOpBytes));
+          const uint64_t bd = umma_desc_sw128(smem_u32(sm_b + stage * L::kOpBytes));
+          if (kb < args.num_kb) {
+            const uint32_t sf = tmem + L::kSfBase + (use & 1) * L::kSfCols;
+            const uint32_t sfb = sf + L::kChunks * 4;
+            const uint64_t sd = mx_desc_scales(smem_u32(sm_sf + stage * L::kSfBytes));
+#pragma unroll
+            for (int j = 0; j < L::kChunks; ++j) {
+              mx_cp_scales_pair(sf + 4 * j, sd + static_cast<uint64_t>(32 * j));
+              mx_cp_scales_pair(sfb + 8 * j, sd + static_cast<uint64_t>(32 * (L::kChunks + j)));
+              mx_cp_scales_pair(sfb + 8 * j + 4, sd + static_cast<uint64_t>(32 * (2 * L::kChunks + j)));
+            }
+            const int nk = kb == args.num_kb - 1 ? args.last_k64 : 4;
+            for (int k = 0; k < nk; ++k) {
+              const int j = FMT == LORA_MXFP4 ? k >> 1 : k;
+              const uint32_t id = FMT == LORA_MXFP4 ? static_cast<uint32_t>(k & 1) * 2u : 0u;
+              mx_mma_pair<FMT>(d, ad + static_cast<uint64_t>(2 * k), bd + static_cast<uint64_t>(2 * k),
+                               kIdesc | (id << 4) | (id << 29), sf + 4 * j, sfb + 8 * j, (kb > 0 || k > 0) ? 1u : 0u);
+            }
+          } else {
+            const int t = kb - args.num_kb - args.zero_kb;
+            const int c = t >= args.rank_kb ? t - args.rank_kb : t;
+            const int nk = t < 0 ? 1 : c == args.rank_kb - 1 ? args.last_k16 : 4;
+            const int shift = t < 0 ? 15 : t == 0 ? args.dshift - 15 * args.zero_kb : 0;
+            for (int k = 0; k < nk; ++k)
+              mx_mma_f16_pair_shift(d, ad + static_cast<uint64_t>(2 * k), bd + static_cast<uint64_t>(2 * k), kIdescTail,
+                                    k == 0 ? shift : 0);
+          }
+          tc_commit_pair(&empty[stage], kBoth);
+          if (++stage == L::kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (ok) tc_commit_pair(acc_full, kBoth);
+      }
+    }
+  } else {
+    const int quad = warp & 3;
+    const bool vec = (args.ldo % 8) == 0 && (reinterpret_cast<uintptr_t>(args.out) % 16) == 0;
+    int local = 0;
+    for (int tile = pair; tile < args.num_tiles; tile += npairs, ++local) {
+      int mt, nt;
+      mx_tile_coords(tile, args, mt, nt);
+      if (!mbar_wait_bounded(acc_full, local & 1, abort_flag, args.err, kDevErrTimeoutAccFull)) break;
+      tc_fence_after();
+      const int row = mt * 256 + static_cast<int>(rank) * 128 + quad * 32 + lane;
+      T* out_row = static_cast<T*>(args.out) + static_cast<int64_t>(row) * args.ldo;
+      const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16) + ((local & 1) ? L::kAcc1 : 0);
+      // columns in the order: shared with the other accumulator, then the rest
+      const int first = (local & 1) ? 0 : L::kAcc1;
+#pragma unroll 1
+      for (int i = 0; i < 256; i += 16) {
+        const int c = (first + i) & 255;
+        uint32_t r[16];
+        tmem_ld_32x32b_x16(t_row + c, r);
+        tmem_wait_ld();
+        if (i == L::kOverlap - 16) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(acc_free), 0));
+        }
+        mx_store16<T>(args, out_row, row, nt * 256 + c, vec, r);
+      }
+    }
+  }
+
+  tc_fence_before();
+  cluster_sync_all();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+template <typename T, int FMT>
+int launch_pair(const MxLinearOperands& o, cudaStream_t stream) {
+  using L = MxSmem<FMT>;
+  const int dev = current_device();
+  if (dev < 0) return LORA_ERR_DEVICE;
+  const DeviceInfo& info = device_info(dev);
+  MxMaps maps;
+  MxGemmArgs a;
+  const int64_t pitch = mx_code_pitch(o.K, FMT);
+  a.chunks = static_cast<int>(mx_scale_chunks(o.K, FMT));
+  if (!mx_encode_map(&maps.x, o.x_codes, 1, pitch, o.M, pitch, 128, 128, true) ||
+      !mx_encode_map(&maps.w, o.w_codes, 1, pitch, o.N, pitch, 128, 128, true) ||
+      !mx_encode_map(&maps.sx, o.x_scales, 4, 128, (o.M + 127) / 128 * a.chunks, 512, 128, L::kChunks, false) ||
+      !mx_encode_map(&maps.sw, o.w_scales, 4, 128, (o.N + 127) / 128 * a.chunks, 512, 128, L::kChunks, false))
+    return LORA_ERR_CUDA;
+  if (o.R > 0) {
+    const char* z = static_cast<const char*>(o.z);
+    if (!mx_encode_map(&maps.zh, z, 2, o.R, o.M, o.ldz * 2, 64, 128, true) ||
+        !mx_encode_map(&maps.zl, z + o.z_lo * 2, 2, o.R, o.M, o.ldz * 2, 64, 128, true) ||
+        !mx_encode_map(&maps.b, o.b, 2, o.R, o.N, o.ldb * 2, 64, 128, true))
+      return LORA_ERR_CUDA;
+  } else {
+    maps.zh = maps.zl = maps.b = maps.x;
+  }
+  a.out = o.out;
+  a.bias = o.bias;
+  a.err = info.err_word;
+  a.ldo = o.ldo;
+  a.M = static_cast<int>(o.M);
+  a.N = static_cast<int>(o.N);
+  const int64_t kp = mx_padded_k(o.K);
+  a.num_kb = static_cast<int>((kp + 255) / 256);
+  a.last_k64 = static_cast<int>((kp - (a.num_kb - 1) * 256ll + 63) / 64);
+  a.rank_kb = static_cast<int>((o.R + 63) / 64);
+  a.last_k16 = a.rank_kb > 0 ? static_cast<int>((o.R - (a.rank_kb - 1) * 64ll + 15) / 16) : 0;
+  a.zero_kb = o.dshift > 15 ? 1 : 0;
+  a.num_m_tiles = static_cast<int>((o.M + 255) / 256);
+  a.num_n_tiles = static_cast<int>((o.N + 255) / 256);
+  a.num_tiles = a.num_m_tiles * a.num_n_tiles;
+  a.group_m = 8;
+  a.dshift = o.dshift;
+  a.alpha = o.alpha;
+  auto kernel = mx_gemm_pair_kernel<T, FMT>;
+  static std::once_flag once[64];
+  static cudaError_t attr_err[64];
+  static int capacity[64];
+  std::call_once(once[dev], [&] {
+    attr_err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+    int clusters = 0;
+    if (attr_err[dev] == cudaSuccess) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(2 * info.num_sms);
+      cfg.blockDim = dim3(kMxGemmThreads);
+      cfg.dynamicSmemBytes = L::kBytes;
+      if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        clusters = 0;
+      }
+    }
+    capacity[dev] = clusters > 0 ? clusters : info.num_sms / 2;
+  });
+  if (attr_err[dev] != cudaSuccess) return LORA_ERR_CUDA;
+  const int pairs = std::min(a.num_tiles, capacity[dev]);
+  kernel<<<2 * pairs, kMxGemmThreads, L::kBytes, stream>>>(maps, a);
+  return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
+}
+
+}  // namespace
+
+bool mx_encode_map(CUtensorMap* map, const void* ptr, int elem, int64_t inner, int64_t outer, int64_t pitch_bytes,
+                   int box_inner, int box_outer, bool swizzle) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (enc == nullptr) return false;
+  const CUtensorMapDataType type = elem == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_UINT32;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch_bytes)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_outer)};
+  const cuuint32_t one[2] = {1, 1};
+  return enc(map, type, 2, const_cast<void*>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int mx_gemm_launch(const MxLinearOperands& o, int fmt, int dtype, cudaStream_t stream) {
+  if (dtype == LORA_BF16)
+    return fmt == LORA_MXFP4 ? launch_pair<__nv_bfloat16, LORA_MXFP4>(o, stream)
+                             : launch_pair<__nv_bfloat16, LORA_NVFP4>(o, stream);
+  return fmt == LORA_MXFP4 ? launch_pair<__half, LORA_MXFP4>(o, stream) : launch_pair<__half, LORA_NVFP4>(o, stream);
+}
+
+}  // namespace lora

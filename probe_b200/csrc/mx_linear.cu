@@ -1,0 +1,159 @@
+// The LoRA linear with 4-bit base operands: its steps and its entry point.
+//
+//   out = q(x) W^T + s (x A^T) B^T + bias
+//
+// q(x): x quantised to W's format; the adapter sees x itself.  Steps: q(x), the
+// rank shrink z = (s / alpha) x A^T as a hi/lo pair (alpha: the fp32 factor that
+// the product's epilogue applies), the block-scaled GEMM with z B^T as its tail.
+#include <cmath>
+
+#include "mx_linear.h"
+
+namespace lora {
+namespace {
+
+// Shrinks of more ranks than this run on the 16-bit tensor-core GEMM.
+constexpr int64_t kShrinkMaxRank = 128;
+
+int64_t r16(int64_t r) { return (r + 15) / 16 * 16; }
+
+struct LinearPlan {
+  size_t shrink_bytes, x_codes, x_scales, z, b, total;
+  int split_k;
+};
+
+// Workspace: the shrink's (its ticket region first, zeroed once), then scratch.
+LinearPlan linear_plan(int64_t M, int64_t N, int64_t K, int64_t R, int fmt) {
+  LinearPlan p = {};
+  size_t at = kCounterBytes;  // never scratch: calls of other shapes find their tickets zero
+  if (R > 0) {
+    if (R <= kShrinkMaxRank) {
+      p.split_k = lora_shrink_pick_split_k(M, K, R);
+      p.shrink_bytes = lora_shrink_workspace_size(M, R, p.split_k);
+    } else {
+      p.shrink_bytes = lora_gemm_workspace_size(M, R, K, 0);
+    }
+    if (p.shrink_bytes > at) at = mx_align(p.shrink_bytes);
+  }
+  p.x_codes = at;
+  at += mx_align(lora_mx_codes_size(M, K, fmt));
+  p.x_scales = at;
+  at += mx_align(lora_mx_scales_size(M, K, fmt));
+  p.z = at;
+  if (R > 0) at += mx_align(static_cast<size_t>(M) * 2 * r16(R) * 2);
+  p.b = at;
+  if (R % 8 != 0) at += mx_align(static_cast<size_t>(N) * ((R + 7) / 8 * 8) * 2);
+  p.total = at;
+  return p;
+}
+
+// B [N, R] with rows padded to a multiple of 8 elements (TMA needs 16-byte rows).
+__global__ void mx_pad_rows_kernel(const uint16_t* __restrict__ b, int64_t ldb, uint16_t* __restrict__ out, int64_t N,
+                                   int R, int R8) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (i >= N * R8) return;
+  const int64_t n = i / R8;
+  const int j = static_cast<int>(i - n * R8);
+  out[i] = j < R ? b[n * ldb + j] : 0;
+}
+
+}  // namespace
+}  // namespace lora
+
+using namespace lora;
+
+extern "C" size_t lora_mx_linear_workspace_size(int64_t M, int64_t N, int64_t K, int64_t R, int fmt) {
+  if (M <= 0 || N <= 0 || K <= 0 || R < 0 || (fmt != LORA_MXFP4 && fmt != LORA_NVFP4)) return 0;
+  return linear_plan(M, N, K, R, fmt).total;
+}
+
+extern "C" float lora_mx_linear_z_scale(float x_global, float w_global, int fmt) {
+  float scale = 1.f;
+  int shift = 0;
+  if (fmt == LORA_NVFP4) mx_split_alpha(static_cast<double>(x_global) * w_global, &scale, &shift);
+  return scale;
+}
+
+extern "C" int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, const void* w_scales, float w_global,
+                              const void* bias, const void* a, int64_t lda, const void* b, int64_t ldb, void* out,
+                              int64_t ldo, void* z_out, int64_t M, int64_t N, int64_t K, int64_t R, float scale,
+                              float x_global, int fmt, int dtype, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  if ((fmt != LORA_MXFP4 && fmt != LORA_NVFP4) || (dtype != LORA_BF16 && dtype != LORA_F16)) return LORA_ERR_DTYPE;
+  if (M < 0 || N < 0 || K < 0 || R < 0 || R > 256 || M > 8388480 || N > 8388480 || K > (int64_t{1} << 24))
+    return LORA_ERR_SHAPE;
+  if (ldx < K || ldo < N || (R > 0 && (lda < K || ldb < R))) return LORA_ERR_SHAPE;
+  if (!mx_global_ok(w_global, fmt) || !mx_global_ok(x_global, fmt)) return LORA_ERR_ARG;
+  if (M == 0 || N == 0) return LORA_OK;
+  if (K == 0) return LORA_ERR_UNSUPPORTED;
+  if (x == nullptr || w_codes == nullptr || w_scales == nullptr || out == nullptr) return LORA_ERR_ARG;
+  if (R > 0 && (a == nullptr || b == nullptr)) return LORA_ERR_ARG;
+  if (!mx_aligned(w_codes, 16) || !mx_aligned(w_scales, 16) || !mx_aligned(workspace, 256) ||
+      (z_out != nullptr && !mx_aligned(z_out, 16)))
+    return LORA_ERR_ALIGN;
+  // the wide shrink's operands are read by TMA
+  if (R > kShrinkMaxRank && (K % 8 != 0 || ldx % 8 != 0 || lda % 8 != 0 || !mx_aligned(x, 16) || !mx_aligned(a, 16)))
+    return LORA_ERR_ALIGN;
+  const int dev = current_device();
+  if (dev < 0 || !device_info(dev).is_sm100) return LORA_ERR_DEVICE;
+  const LinearPlan p = linear_plan(M, N, K, R, fmt);
+  if (workspace == nullptr || workspace_bytes < p.total) return LORA_ERR_WORKSPACE;
+  char* ws = static_cast<char*>(workspace);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+
+  MxLinearOperands o = {};
+  o.alpha = 1.f;
+  if (fmt == LORA_NVFP4) {
+    const double alpha = static_cast<double>(x_global) * w_global;
+    if (R > 0) {
+      mx_split_alpha(alpha, &o.alpha, &o.dshift);
+    } else {
+      o.alpha = static_cast<float>(alpha);
+    }
+  }
+  int rc = mx_quantize_launch(x, ldx, ws + p.x_codes, ws + p.x_scales, M, K, fmt, x_global, dtype, s);
+  if (rc != LORA_OK) return rc;
+  if (R > 0) {
+    const int64_t rp = r16(R);
+    char* z = z_out != nullptr ? static_cast<char*>(z_out) : ws + p.z;
+    const float zs = scale / o.alpha;
+    if (R <= kShrinkMaxRank) {
+      rc = lora_shrink(x, ldx, a, lda, z, 2 * rp, dtype, rp, 1, M, K, R, zs, dtype, p.split_k, ws, p.shrink_bytes, s);
+    } else {
+      if (z_out != nullptr && rp != R &&
+          cudaMemsetAsync(z, 0, static_cast<size_t>(M) * 2 * rp * 2, s) != cudaSuccess)
+        return LORA_ERR_CUDA;
+      rc = lora_gemm_ex(x, ldx, a, lda, nullptr, 0, nullptr, 0, nullptr, z, 2 * rp, M, R, K, 0, zs, rp, dtype,
+                        p.shrink_bytes ? ws : nullptr, p.shrink_bytes, s);
+    }
+    if (rc != LORA_OK) return rc;
+    o.z = z;
+    o.ldz = 2 * rp;
+    o.z_lo = rp;
+    o.b = b;
+    o.ldb = ldb;
+    if (ldb % 8 != 0 || !mx_aligned(b, 16)) {
+      if (R % 8 == 0) return LORA_ERR_ALIGN;
+      const int r8 = static_cast<int>((R + 7) / 8 * 8);
+      const int64_t n = N * r8;
+      mx_pad_rows_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(
+          static_cast<const uint16_t*>(b), ldb, reinterpret_cast<uint16_t*>(ws + p.b), N, static_cast<int>(R),
+          r8);
+      if (cudaGetLastError() != cudaSuccess) return LORA_ERR_CUDA;
+      o.b = ws + p.b;
+      o.ldb = r8;
+    }
+  }
+  o.x_codes = ws + p.x_codes;
+  o.x_scales = ws + p.x_scales;
+  o.w_codes = w_codes;
+  o.w_scales = w_scales;
+  o.bias = bias;
+  o.out = out;
+  o.ldo = ldo;
+  o.M = M;
+  o.N = N;
+  o.K = K;
+  o.R = R;
+  return mx_gemm_launch(o, fmt, dtype, s);
+}

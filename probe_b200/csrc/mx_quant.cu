@@ -1,0 +1,357 @@
+// Quantisation to the microscaled formats and back.
+//
+// mxfp4 / mxfp8: e = max(floor(log2 amax) - top, -127) over a block of 32
+// (top: the exponent of the largest code, 2 for E2M1 and 8 for E4M3), the scale
+// byte is e + 127 and a code is x 2^-e rounded to nearest even, saturating.
+// Every step before the rounding is exact.
+// nvfp4: s = E4M3(amax / (6 g)) over a block of 16, a code is x / (s g) rounded
+// to nearest even; both quotients are correctly rounded fp32.
+// A block that holds an infinity or a NaN gets a NaN scale and zero codes: all
+// its values read back as NaN, and so does every product with it.
+//
+// Bound: HBM (2 bytes read, 0.53 to 1.03 written an element).  A CTA takes 128
+// rows x 128 columns, the extent of whole scale chunks: 8 threads a row with 16
+// elements each, all four passes of 32 rows loaded before the first is used (128
+// bytes in flight a thread); the 512 scale bytes of a chunk go through shared
+// memory and leave as 16-byte stores.
+#include "mx.cuh"
+
+namespace lora {
+namespace {
+
+constexpr int kMxTile = 128;
+constexpr int kMxThreads = 256;
+
+// 16 elements of a row from column c, zeros at and beyond k.
+template <typename T>
+LORA_DEVINL void mx_load16(const T* row, int64_t c, int64_t k, bool vec, uint32_t* w) {
+  if (vec && c + 16 <= k) {
+    const uint4 a = ldg_stream(row + c), b = ldg_stream(row + c + 8);
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+    w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+    return;
+  }
+  const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t lo = c + 2 * i < k ? p[c + 2 * i] : 0u;
+    const uint32_t hi = c + 2 * i + 1 < k ? p[c + 2 * i + 1] : 0u;
+    w[i] = lo | (hi << 16);
+  }
+}
+
+// Largest magnitude, as the 16-bit pattern without its sign: infinities and
+// NaN compare above every number.
+LORA_DEVINL uint32_t mx_amax16(const uint32_t* w) {
+  uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+  return max(m & 0xffffu, m >> 16);
+}
+
+template <typename T> LORA_DEVINL float mx_bits16_to_f32(uint32_t b);
+template <> LORA_DEVINL float mx_bits16_to_f32<__nv_bfloat16>(uint32_t b) { return __uint_as_float(b << 16); }
+template <> LORA_DEVINL float mx_bits16_to_f32<__half>(uint32_t b) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(b)));
+}
+
+// Scale byte and codes of one thread's 16 elements.
+template <typename T, int FMT>
+LORA_DEVINL uint32_t mx_encode16(const uint32_t* w, float g, float g6, uint32_t* codes) {
+  constexpr uint32_t kInf = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+  uint32_t top = mx_amax16(w);
+  if constexpr (MxFormat<FMT>::kBlock == 32) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  const bool bad = top >= kInf;
+  const float amax = mx_bits16_to_f32<T>(top);
+  uint32_t byte;
+  float v[16];
+  if constexpr (FMT == LORA_NVFP4) {
+    byte = mx_to_e4m3x2(__fdiv_rn(amax, g6), 0.f) & 0xffu;
+    const float unit = mx_e4m3(byte) * g;
+    if (bad || byte == 0) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = 0.f;
+    } else {
+      // Quotients by one divisor: with r the correctly rounded reciprocal, one
+      // residual step makes x r the correctly rounded x / unit (Markstein, 1990).
+      const float r = __frcp_rn(unit);
+      const bool far = amax * r > 1e6f;  // a saturated scale: keep the residual finite
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 x = unpack2<T>(w[i]);
+        float q0 = x.x * r, q1 = x.y * r;
+        if (far) {
+          q0 = fminf(fmaxf(q0, -1e6f), 1e6f);
+          q1 = fminf(fmaxf(q1, -1e6f), 1e6f);
+        }
+        v[2 * i] = fmaf(fmaf(-q0, unit, x.x), r, q0);
+        v[2 * i + 1] = fmaf(fmaf(-q1, unit, x.y), r, q1);
+      }
+    }
+    if (bad) byte = 0x7f;
+  } else {
+    const int e = max(static_cast<int>(__float_as_uint(amax) >> 23) - MxFormat<FMT>::kTop, 0);  // biased by 127
+    byte = bad ? 255u : static_cast<uint32_t>(e);
+    const float inv = bad ? 0.f : __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 x = unpack2<T>(bad ? 0u : w[i]);
+      v[2 * i] = x.x * inv;
+      v[2 * i + 1] = x.y * inv;
+    }
+  }
+  if constexpr (MxFormat<FMT>::kBits == 4) {
+    codes[0] = mx_to_e2m1x8(v);
+    codes[1] = mx_to_e2m1x8(v + 8);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      codes[i] = mx_to_e4m3x2(v[4 * i], v[4 * i + 1]) | (mx_to_e4m3x2(v[4 * i + 2], v[4 * i + 3]) << 16);
+  }
+  return byte;
+}
+
+template <typename T, int FMT>
+__global__ void __launch_bounds__(kMxThreads)
+    mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes,
+                       uint8_t* __restrict__ scales, int64_t M, int64_t K, int64_t Kp, int chunks, float g, float g6,
+                       bool vec) {
+  constexpr int kChunks = kMxTile / MxFormat<FMT>::kBlock / 4;  // scale chunks of this tile
+  __shared__ alignas(16) uint8_t sc[kChunks * 512];
+  const int seg = threadIdx.x & 7;   // 16-column segment of the tile
+  const int sub = threadIdx.x >> 3;  // row within a pass
+  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * kMxTile;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * kMxTile + seg * 16;
+  uint32_t w[4][8];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const int64_t row = row0 + 32 * p + sub;
+    if (row < M) {
+      mx_load16<T>(x + row * ldx, col, K, vec, w[p]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[p][i] = 0u;
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const int64_t row = row0 + 32 * p + sub;
+    uint32_t c[4];
+    uint32_t byte = mx_encode16<T, FMT>(w[p], g, g6, c);
+    if (col >= Kp || row >= M) byte = 0;
+    if (row < M && col < Kp) {
+      if constexpr (MxFormat<FMT>::kBits == 4)
+        *reinterpret_cast<uint2*>(codes + row * (Kp >> 1) + (col >> 1)) = make_uint2(c[0], c[1]);
+      else
+        *reinterpret_cast<uint4*>(codes + row * Kp + col) = make_uint4(c[0], c[1], c[2], c[3]);
+    }
+    if constexpr (MxFormat<FMT>::kBlock == 16)
+      sc[(seg >> 2) * 512 + sub * 16 + p * 4 + (seg & 3)] = static_cast<uint8_t>(byte);
+    else if ((seg & 1) == 0)
+      sc[sub * 16 + p * 4 + (seg >> 1)] = static_cast<uint8_t>(byte);
+  }
+  __syncthreads();
+  if (threadIdx.x < kChunks * 32) {
+    const int chunk = static_cast<int>(blockIdx.x) * kChunks + (threadIdx.x >> 5);
+    if (chunk < chunks)
+      reinterpret_cast<uint4*>(scales + (static_cast<int64_t>(blockIdx.y) * chunks + chunk) * 512)[threadIdx.x & 31] =
+          reinterpret_cast<const uint4*>(sc)[threadIdx.x];
+  }
+}
+
+// Values of one thread's 16 codes: (code x scale) x g, rounded once to T.
+template <typename T, int FMT>
+LORA_DEVINL void mx_decode16(const uint32_t* c, uint32_t byte, float g, uint32_t* out) {
+  const float s = FMT == LORA_NVFP4 ? mx_e4m3(byte) : mx_e8m0(byte);
+  uint32_t h[8];
+  if constexpr (MxFormat<FMT>::kBits == 4) {
+    mx_from_e2m1x8(c[0], h);
+    mx_from_e2m1x8(c[1], h + 4);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = mx_from_e4m3x2((c[i >> 1] >> (16 * (i & 1))) & 0xffffu);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 q = __half22float2(*reinterpret_cast<__half2*>(&h[i]));
+    out[i] = pack2<T>(q.x * s * g, q.y * s * g);
+  }
+}
+
+// A CTA decodes 128 x 128 values, straight (rows of 256 bytes) or transposed
+// through shared memory (column c of the tensor becomes row c of out).
+template <typename T, int FMT, bool TR>
+__global__ void __launch_bounds__(kMxThreads)
+    mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out,
+                         int64_t ldo, int64_t M, int64_t K, int64_t Kp, int chunks, float g, bool vec) {
+  constexpr int kPitch = kMxTile + 2;  // 16-bit elements: odd number of 4-byte words a row
+  __shared__ alignas(16) uint16_t tile[TR ? kMxTile * kPitch : 8];
+  const int seg = threadIdx.x & 7;
+  const int sub = threadIdx.x >> 3;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * kMxTile;
+  const int64_t col0 = static_cast<int64_t>(blockIdx.x) * kMxTile;
+  const int64_t col = col0 + seg * 16;
+  const int block = static_cast<int>(col / MxFormat<FMT>::kBlock);
+  const uint8_t* sc = scales + (static_cast<int64_t>(blockIdx.y) * chunks + (block >> 2)) * 512 + sub * 16 + (block & 3);
+  uint32_t c[4][4], byte[4];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const int64_t row = row0 + 32 * p + sub;
+    c[p][0] = c[p][1] = c[p][2] = c[p][3] = byte[p] = 0u;
+    if (row < M && col < Kp) {
+      byte[p] = sc[p * 4];
+      if constexpr (MxFormat<FMT>::kBits == 4) {
+        const uint2 v = *reinterpret_cast<const uint2*>(codes + row * (Kp >> 1) + (col >> 1));
+        c[p][0] = v.x, c[p][1] = v.y;
+      } else {
+        const uint4 v = *reinterpret_cast<const uint4*>(codes + row * Kp + col);
+        c[p][0] = v.x, c[p][1] = v.y, c[p][2] = v.z, c[p][3] = v.w;
+      }
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const int64_t row = row0 + 32 * p + sub;
+    uint32_t o[8];
+    mx_decode16<T, FMT>(c[p], byte[p], g, o);
+    if constexpr (TR) {
+      const int r = 32 * p + sub;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(&tile[r * kPitch + seg * 16 + 2 * i]) = o[i];
+    } else if (row < M && col < K) {
+      T* dst = out + row * ldo + col;
+      if (vec && col + 16 <= K) {
+        reinterpret_cast<uint4*>(dst)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+        reinterpret_cast<uint4*>(dst)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+      } else {
+        uint16_t* d = reinterpret_cast<uint16_t*>(dst);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (col + i < K) d[i] = static_cast<uint16_t>(o[i >> 1] >> (16 * (i & 1)));
+      }
+    }
+  }
+  if constexpr (TR) {
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint16_t* o16 = reinterpret_cast<uint16_t*>(out);
+    // a warp writes one output row at a time: 128 values, four a lane (two pairs)
+    for (int cc = warp; cc < kMxTile; cc += kMxThreads / 32) {
+      if (col0 + cc >= K) break;
+      uint16_t* dst = o16 + (col0 + cc) * ldo + row0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = 64 * h + 2 * lane;
+        const uint32_t lo = tile[r * kPitch + cc], hi = tile[(r + 1) * kPitch + cc];
+        if (vec && row0 + r + 2 <= M) {
+          *reinterpret_cast<uint32_t*>(dst + r) = lo | (hi << 16);
+        } else {
+          if (row0 + r < M) dst[r] = static_cast<uint16_t>(lo);
+          if (row0 + r + 1 < M) dst[r + 1] = static_cast<uint16_t>(hi);
+        }
+      }
+    }
+  }
+}
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+template <typename T, int FMT>
+int quantize_t(const void* x, int64_t ldx, void* codes, void* scales, int64_t M, int64_t K, float g,
+               cudaStream_t stream) {
+  const int64_t Kp = mx_padded_k(K);
+  const dim3 grid(static_cast<unsigned>((Kp + kMxTile - 1) / kMxTile), static_cast<unsigned>((M + kMxTile - 1) / kMxTile));
+  const bool vec = aligned(x, 16) && ldx % 8 == 0;
+  mx_quantize_kernel<T, FMT><<<grid, kMxThreads, 0, stream>>>(
+      static_cast<const T*>(x), ldx, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), M, K, Kp,
+      static_cast<int>(mx_scale_chunks(K, FMT)), g, 6.0f * g, vec);
+  return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
+}
+
+template <typename T, int FMT>
+int dequantize_t(const void* codes, const void* scales, void* out, int64_t ldo, int64_t M, int64_t K, float g,
+                 int transpose, cudaStream_t stream) {
+  const int64_t Kp = mx_padded_k(K);
+  const dim3 grid(static_cast<unsigned>((Kp + kMxTile - 1) / kMxTile), static_cast<unsigned>((M + kMxTile - 1) / kMxTile));
+  const int chunks = static_cast<int>(mx_scale_chunks(K, FMT));
+  if (transpose) {
+    const bool vec = aligned(out, 4) && ldo % 2 == 0;
+    mx_dequantize_kernel<T, FMT, true><<<grid, kMxThreads, 0, stream>>>(
+        static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<T*>(out), ldo, M, K, Kp,
+        chunks, g, vec);
+  } else {
+    const bool vec = aligned(out, 16) && ldo % 8 == 0;
+    mx_dequantize_kernel<T, FMT, false><<<grid, kMxThreads, 0, stream>>>(
+        static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<T*>(out), ldo, M, K, Kp,
+        chunks, g, vec);
+  }
+  return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
+}
+
+}  // namespace
+
+int mx_quantize_launch(const void* x, int64_t ldx, void* codes, void* scales, int64_t M, int64_t K, int fmt, float g,
+                       int dtype, cudaStream_t s) {
+#define LORA_MXQ(T)                                                                                    \
+  (fmt == LORA_MXFP4   ? quantize_t<T, LORA_MXFP4>(x, ldx, codes, scales, M, K, g, s)                  \
+   : fmt == LORA_NVFP4 ? quantize_t<T, LORA_NVFP4>(x, ldx, codes, scales, M, K, g, s)                  \
+                       : quantize_t<T, LORA_MXFP8>(x, ldx, codes, scales, M, K, g, s))
+  return dtype == LORA_BF16 ? LORA_MXQ(__nv_bfloat16) : LORA_MXQ(__half);
+#undef LORA_MXQ
+}
+
+int mx_dequantize_launch(const void* codes, const void* scales, void* out, int64_t ldo, int64_t M, int64_t K, int fmt,
+                         float g, int transpose, int dtype, cudaStream_t s) {
+#define LORA_MXD(T)                                                                                    \
+  (fmt == LORA_MXFP4   ? dequantize_t<T, LORA_MXFP4>(codes, scales, out, ldo, M, K, g, transpose, s)   \
+   : fmt == LORA_NVFP4 ? dequantize_t<T, LORA_NVFP4>(codes, scales, out, ldo, M, K, g, transpose, s)   \
+                       : dequantize_t<T, LORA_MXFP8>(codes, scales, out, ldo, M, K, g, transpose, s))
+  return dtype == LORA_BF16 ? LORA_MXD(__nv_bfloat16) : LORA_MXD(__half);
+#undef LORA_MXD
+}
+
+}  // namespace lora
+
+using namespace lora;
+
+// Sizes a CTA grid of 128 x 128 tiles can cover (grid.y <= 65535).
+static bool mx_shape_ok(int64_t M, int64_t K) {
+  return M >= 0 && K >= 0 && M <= 65535ll * 128 && K <= (int64_t{1} << 30);
+}
+
+extern "C" size_t lora_mx_codes_size(int64_t M, int64_t K, int fmt) {
+  if (!mx_format_ok(fmt) || M <= 0 || K <= 0) return 0;
+  return static_cast<size_t>(M) * static_cast<size_t>(mx_code_pitch(K, fmt));
+}
+
+extern "C" size_t lora_mx_scales_size(int64_t M, int64_t K, int fmt) {
+  if (!mx_format_ok(fmt) || M <= 0 || K <= 0) return 0;
+  return static_cast<size_t>((M + 127) / 128) * static_cast<size_t>(mx_scale_chunks(K, fmt)) * 512;
+}
+
+extern "C" int lora_mx_quantize(const void* x, int64_t ldx, void* codes, void* scales, int64_t M, int64_t K, int fmt,
+                                float global_scale, int dtype, void* stream) {
+  if (!mx_format_ok(fmt) || (dtype != LORA_BF16 && dtype != LORA_F16)) return LORA_ERR_DTYPE;
+  if (!mx_shape_ok(M, K) || ldx < K) return LORA_ERR_SHAPE;
+  if (!mx_global_ok(global_scale, fmt)) return LORA_ERR_ARG;
+  if (M == 0 || K == 0) return LORA_OK;
+  if (x == nullptr || codes == nullptr || scales == nullptr) return LORA_ERR_ARG;
+  if (!aligned(codes, 16) || !aligned(scales, 16) || !aligned(x, 2)) return LORA_ERR_ALIGN;
+  const int dev = current_device();
+  if (dev < 0 || !device_info(dev).is_sm100) return LORA_ERR_DEVICE;
+  return mx_quantize_launch(x, ldx, codes, scales, M, K, fmt, global_scale, dtype, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int lora_mx_dequantize(const void* codes, const void* scales, void* out, int64_t ldo, int64_t M, int64_t K,
+                                  int fmt, float global_scale, int transpose, int dtype, void* stream) {
+  if (!mx_format_ok(fmt) || (dtype != LORA_BF16 && dtype != LORA_F16)) return LORA_ERR_DTYPE;
+  if (!mx_shape_ok(M, K) || ldo < (transpose ? M : K)) return LORA_ERR_SHAPE;
+  if (!mx_global_ok(global_scale, fmt)) return LORA_ERR_ARG;
+  if (M == 0 || K == 0) return LORA_OK;
+  if (codes == nullptr || scales == nullptr || out == nullptr) return LORA_ERR_ARG;
+  if (!aligned(codes, 16) || !aligned(scales, 16) || !aligned(out, 2)) return LORA_ERR_ALIGN;
+  const int dev = current_device();
+  if (dev < 0 || !device_info(dev).is_sm100) return LORA_ERR_DEVICE;
+  return mx_dequantize_launch(codes, scales, out, ldo, M, K, fmt, global_scale, transpose, dtype,
+                              static_cast<cudaStream_t>(stream));
+}

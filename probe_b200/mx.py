@@ -1,0 +1,183 @@
+"""Microscaled 4- and 8-bit tensors around the LoRA linear.
+
+A frozen base weight in 4 bits, an activation kept for the backward pass in 8:
+
+``mx_quantize`` / ``mx_dequantize``
+    to and from ``mxfp4`` (E2M1 codes, a power of two per 32 values), ``nvfp4``
+    (E2M1, an E4M3 scale per 16 values and one fp32 scale a tensor) and
+    ``mxfp8`` (E4M3, a power of two per 32 values).
+
+Everything runs in the sm_100a kernels behind ``include/lora_b200.h``; CPU
+tensors raise.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+_FORMATS = {"mxfp4": _lib.LORA_MXFP4, "nvfp4": _lib.LORA_NVFP4, "mxfp8": _lib.LORA_MXFP8}
+_BLOCK = {"mxfp4": 32, "nvfp4": 16, "mxfp8": 32}
+_HALF = (torch.float16, torch.bfloat16)
+
+
+def _format(fmt: str, where: str) -> int:
+    code = _FORMATS.get(fmt)
+    if code is None:
+        raise ValueError(f"{where}: unknown format {fmt!r} (one of {', '.join(_FORMATS)})")
+    return code
+
+
+def _sizes(m: int, k: int, fmt: str) -> tuple[int, int]:
+    """Bytes of a row of codes, and of all scales, of an [m, k] tensor."""
+    kp = (k + 31) // 32 * 32
+    chunks = (kp // _BLOCK[fmt] + 3) // 4
+    return (kp if fmt == "mxfp8" else kp // 2), (m + 127) // 128 * chunks * 512
+
+
+class MXTensor:
+    """An [M, K] tensor in a microscaled format.
+
+    ``codes``: uint8 ``[M, Kp / 2]`` (4 bits, the even column in the low half of a
+    byte) or ``[M, Kp]`` (8 bits), Kp = K rounded up to 32, zeros beyond K.
+    ``scales``: uint8, flat, in 512-byte chunks of 128 rows x 4 blocks -- row r,
+    block g of a chunk at byte ``16 (r % 32) + 4 (r / 32) + g``, the chunks of 128
+    rows next to one another -- zeros beyond the tensor.  A value is
+    ``code * scale * global_scale``; ``global_scale`` is 1 except for nvfp4.
+    """
+
+    __slots__ = ("codes", "scales", "shape", "fmt", "global_scale", "_code")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, fmt: str, global_scale: float = 1.0):
+        code = _format(fmt, "MXTensor")
+        m, k = (int(v) for v in shape)
+        pitch, nscales = _sizes(m, k, fmt)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("MXTensor: codes and scales are uint8")
+        if codes.shape != (m, pitch) or scales.numel() != nscales:
+            raise ValueError(f"MXTensor: a {fmt} tensor of shape {(m, k)} has codes {(m, pitch)} and {nscales} scale "
+                             f"bytes, got {tuple(codes.shape)} and {scales.numel()}")
+        if not codes.is_contiguous() or not scales.is_contiguous():
+            raise ValueError("MXTensor: codes and scales must be contiguous")
+        if codes.device != scales.device:
+            raise ValueError("MXTensor: codes and scales lie on different devices")
+        self.codes, self.scales, self.shape, self.fmt = codes, scales, (m, k), fmt
+        self.global_scale = float(global_scale)
+        self._code = code
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def __repr__(self):
+        return f"MXTensor({self.fmt}, shape={self.shape}, global_scale={self.global_scale:g}, device={self.device})"
+
+
+def nvfp4_global_scale(amax: float) -> float:
+    """The nvfp4 tensor scale that maps ``amax`` to the largest code times the largest block scale."""
+    return float(torch.tensor(max(float(amax), 2.0 ** -50) / (448.0 * 6.0), dtype=torch.float32))
+
+
+def _rows(x: torch.Tensor, where: str) -> torch.Tensor:
+    if x.dtype not in _HALF:
+        raise TypeError(f"{where}: expected float16/bfloat16, got {x.dtype}")
+    return _lib.row_major(x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x)
+
+
+def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4", global_scale: float = 1.0) -> MXTensor:
+    """``x`` [..., K] (16-bit) in the format, as an [M, K] tensor.
+
+    mxfp4 / mxfp8: scale ``2^(floor(log2 amax) - top)`` per 32 values (top = 2 / 8);
+    nvfp4: ``E4M3(amax / (6 global_scale))`` per 16.  Codes round to nearest even
+    and saturate; a block with an infinity or a NaN reads back as NaN.
+    """
+    code = _format(fmt, "mx_quantize")
+    _lib.require_cuda(x, where="mx_quantize")
+    x = _rows(x, "mx_quantize")
+    m, k = x.shape
+    pitch, nscales = _sizes(m, k, fmt)
+    codes = torch.empty((m, pitch), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(nscales, dtype=torch.uint8, device=x.device)
+    _lib.call("lora_mx_quantize", _lib.ptr(x), _lib.ld(x), _lib.ptr(codes), _lib.ptr(scales), m, k, code,
+              float(global_scale), _lib.dtype_code(x.dtype), _lib.stream_handle(x.device))
+    return MXTensor(codes, scales, (m, k), fmt, global_scale)
+
+
+def mx_dequantize(q: MXTensor, dtype: torch.dtype = torch.bfloat16, transpose: bool = False) -> torch.Tensor:
+    """The values of ``q`` in ``dtype`` (rounded once), [M, K] or, transposed, [K, M]."""
+    _lib.require_cuda(q.codes, where="mx_dequantize")
+    if dtype not in _HALF:
+        raise TypeError(f"mx_dequantize: expected float16/bfloat16, got {dtype}")
+    m, k = q.shape
+    out = torch.empty((k, m) if transpose else (m, k), dtype=dtype, device=q.device)
+    _lib.call("lora_mx_dequantize", _lib.ptr(q.codes), _lib.ptr(q.scales), _lib.ptr(out), out.shape[1], m, k, q._code,
+              q.global_scale, int(transpose), _lib.dtype_code(dtype), _lib.stream_handle(q.device))
+    return out
+
+
+# --------------------------------------------------------------------- linear
+def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """Row-major with 16-byte rows where the width allows it (copies only when needed)."""
+    t = _lib.row_major(t)
+    if t.shape[1] % 8 == 0 and (_lib.ld(t) % 8 != 0 or t.data_ptr() % 16 != 0):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _linear(x, weight, bias, a, b, scale, x_global_scale, keep_z, where):
+    _lib.require_cuda(x, weight.codes, bias, a, b, where=where)
+    if weight.fmt not in ("mxfp4", "nvfp4"):
+        raise ValueError(f"{where}: the weight must be in a 4-bit format, got {weight.fmt}")
+    shape = x.shape
+    x = _rows(x, where)
+    n, k = weight.shape
+    if x.shape[1] != k:
+        raise ValueError(f"{where}: x {tuple(shape)} and the weight {weight.shape} disagree on K")
+    dtype = x.dtype
+    r = 0
+    if a is not None and b is not None and a.shape[0] > 0 and scale != 0:
+        r = a.shape[0]
+        if a.dtype != dtype or b.dtype != dtype:
+            raise TypeError(f"{where}: x, a and b must share one dtype")
+        if a.shape[1] != k or b.shape != (n, r):
+            raise ValueError(f"{where}: a {tuple(a.shape)} / b {tuple(b.shape)} do not match [{r}, {k}] / [{n}, {r}]")
+        if r > 256:
+            raise ValueError(f"{where}: ranks up to 256, got {r}")
+        a, b = _lib.row_major(a), _aligned_rows(b)
+        if r > 128:
+            x, a = _aligned_rows(x), _aligned_rows(a)
+    if bias is not None:
+        if bias.shape != (n,) or bias.dtype != dtype:
+            raise ValueError(f"{where}: bias must be [{n}] in x's dtype")
+        bias = bias.contiguous()
+    m = x.shape[0]
+    out = torch.empty((m, n), dtype=dtype, device=x.device)
+    z = None
+    if keep_z and r:
+        z = torch.empty((m, 2 * ((r + 15) // 16 * 16)), dtype=dtype, device=x.device)
+    if m and n:
+        lib = _lib.load()
+        nbytes = lib.lora_mx_linear_workspace_size(m, n, k, r, weight._code)
+        ws = _lib.WORKSPACE.get(nbytes, x.device, "mx_linear")
+        _lib.call("lora_mx_linear", _lib.ptr(x), _lib.ld(x), _lib.ptr(weight.codes), _lib.ptr(weight.scales),
+                  weight.global_scale, _lib.ptr(bias), _lib.ptr(a) if r else None, _lib.ld(a) if r else 0,
+                  _lib.ptr(b) if r else None, _lib.ld(b) if r else 0, _lib.ptr(out), n, _lib.ptr(z), m, n, k, r,
+                  float(scale), float(x_global_scale), weight._code, _lib.dtype_code(dtype), _lib.ptr(ws), ws.numel(),
+                  _lib.stream_handle(x.device))
+    return out.view(*shape[:-1], n), z
+
+
+def mx_lora_linear(x: torch.Tensor, weight: MXTensor, bias: torch.Tensor | None, a: torch.Tensor | None,
+                   b: torch.Tensor | None, scale: float = 1.0, x_global_scale: float = 1.0) -> torch.Tensor:
+    """``q(x) @ W.T + bias + scale * (x @ a.T) @ b.T`` with W (mxfp4 or nvfp4) and q(x) in 4 bits.
+
+    x [..., K] is quantised to the weight's format (``x_global_scale``: its nvfp4
+    tensor scale); the adapter a [r, K], b [N, r] (r <= 256) takes x itself.
+    ``a`` / ``b`` None, or scale 0, leave the adapter out.
+    """
+    return _linear(x, weight, bias, a, b, scale, x_global_scale, False, "mx_lora_linear")[0]
