@@ -398,6 +398,29 @@ LORA_API int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, con
                    int64_t ldo, void* z_out, int64_t M, int64_t N, int64_t K, int64_t R, float scale,
                    float x_global, int fmt, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Backward pass of the LoRA linear  y = x . W^T + scale * (x . a^T) . b^T  from
+ * an 8-bit checkpoint of x:
+ *   g  = scale * dy . b
+ *   da = g^T . X                  [R, K]
+ *   db = z_scale * dy^T . z       [N, R]
+ *   dx = dy . W + g . a           [M, K], where dx is not NULL
+ * dy [M, N]; X: x as an MXFP8 tensor (x_codes, x_scales); z [M, 2 r16] as
+ * lora_mx_linear's z_out, of which the hi part is read, z_scale its factor; W as
+ * an MXFP4 / NVFP4 tensor [N, K] (read for dx only).  W is frozen and rounding to
+ * 8 or 4 bits counts as the identity.  Products accumulate in fp32, z and g are
+ * rounded to dtype once, outputs are written once in dtype; token ranges are
+ * summed in a fixed order.  1 <= R <= 256; z, codes and scales 16-byte aligned.
+ * Workspace: lora_mx_backward_workspace_size bytes, 256-byte aligned, zeroed
+ * ticket region first as lora_shrink's.  No counterpart in the reference, which
+ * has no backward pass. */
+LORA_API size_t lora_mx_backward_workspace_size(int64_t M, int64_t N, int64_t K, int64_t R, int need_dx);
+LORA_API int lora_mx_backward(const void* dy, int64_t lddy, const void* x_codes, const void* x_scales, const void* z,
+                     float z_scale, const void* a, int64_t lda, const void* b, int64_t ldb,
+                     const void* w_codes, const void* w_scales, float w_global, int w_fmt, void* dx,
+                     int64_t lddx, void* da, int64_t ldda, void* db, int64_t lddb, int64_t M, int64_t N,
+                     int64_t K, int64_t R, float scale, int dtype, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -94,6 +94,9 @@ SIGNATURES = {
     "lora_mx_linear_z_scale": (_F, [_F, _F, _I]),
     "lora_mx_linear": (_I, [_P, _I64, _P, _P, _F, _P, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _F, _F,
                             _I, _I, _P, _SZ, _P]),
+    "lora_mx_backward_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _I]),
+    "lora_mx_backward": (_I, [_P, _I64, _P, _P, _P, _F, _P, _I64, _P, _I64, _P, _P, _F, _I, _P, _I64, _P, _I64, _P,
+                              _I64, _I64, _I64, _I64, _I64, _F, _I, _P, _SZ, _P]),
     "lora_mx_dequantize": (_I, [_P, _P, _P, _I64, _I64, _I64, _I, _F, _I, _I, _P]),
 }
 

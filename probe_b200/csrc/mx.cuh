@@ -94,7 +94,8 @@ LORA_DEVINL uint32_t mx_from_e4m3x2(uint32_t w) {
 }
 
 // Device entry points of the parts (host launchers), used by the C ABI and by
-// the composite operators.
+// the composite operators.  transpose: 0, 1, or 2 for [K, M rounded up to 8] with
+// zeros in the padding.
 int mx_quantize_launch(const void* x, int64_t ldx, void* codes, void* scales, int64_t M, int64_t K, int fmt,
                        float global_scale, int dtype, cudaStream_t stream);
 int mx_dequantize_launch(const void* codes, const void* scales, void* out, int64_t ldo, int64_t M, int64_t K, int fmt,

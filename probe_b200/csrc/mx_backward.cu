@@ -1,0 +1,204 @@
+// Backward pass of the LoRA linear from an 8-bit checkpoint of its input.
+//
+//   g  = s dy B                [M, R]
+//   dB = zs dy^T z             [N, R]     z: the forward pass's hi/lo pair, hi part
+//   dA = g^T X8                [R, K]
+//   dx = dy Wq + g A           [M, K]     where asked for
+//
+// The base weight is frozen; rounding to 4 or 8 bits counts as the identity
+// (straight-through).  dx needs W with N as the contraction, against the direction
+// of its scale blocks, so W is decoded once, transposed, into the workspace (its
+// values are exact in 16 bits: nvfp4's tensor scale m 2^p leaves the power of two
+// in the values and m in the GEMM's alpha) and the 16-bit CTA-pair GEMM takes
+// [g_hi | g_lo] against [A^T | A^T] as its K tail.
+#include <cmath>
+
+#include "mx_grad.h"
+
+namespace lora {
+namespace {
+
+constexpr int64_t kShrinkMaxRank = 128;
+
+int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+struct BackwardPlan {
+  size_t shrink_bytes, gemm_bytes, part, g, bt, at, dy, wt, total;
+  int split_k;
+};
+
+BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need_dx) {
+  BackwardPlan p = {};
+  const int64_t np = up(N, 8), rp = up(R, 16);
+  if (R <= kShrinkMaxRank) {
+    p.split_k = lora_shrink_pick_split_k(M, np, R);
+    p.shrink_bytes = lora_shrink_workspace_size(M, R, p.split_k);
+  } else {
+    p.shrink_bytes = lora_gemm_workspace_size(M, R, np, 0);
+  }
+  if (need_dx) p.gemm_bytes = lora_gemm_workspace_size(M, K, np, 2 * rp);
+  size_t at = kCounterBytes;  // ticket counters, never scratch; the steps' partials follow them in turn
+  at = std::max(at, mx_align(std::max(p.shrink_bytes, p.gemm_bytes)));
+  p.part = at;
+  at += mx_align(std::max(mx_grad_part_bytes(M, N, R), mx_grad_part_bytes(M, K, R)));
+  p.g = at;
+  at += mx_align(static_cast<size_t>(M) * 2 * rp * 2);
+  p.bt = at;
+  at += mx_align(static_cast<size_t>(R) * np * 2);
+  p.at = at;
+  if (need_dx) at += mx_align(static_cast<size_t>(K) * 2 * rp * 2);
+  p.dy = at;
+  at += mx_align(static_cast<size_t>(M) * np * 2);
+  p.wt = at;
+  if (need_dx) at += mx_align(static_cast<size_t>(K) * np * 2);
+  p.total = at;
+  return p;
+}
+
+// out[c, j] = in[j, c] for in [rows, cols]; rows of out beyond cols up to
+// out_rows, and columns beyond rows up to width, hold zeros; copies > 1 repeats
+// the width columns side by side.  32 x 32 a block.
+__global__ void __launch_bounds__(256)
+    mx_transpose_kernel(const uint16_t* __restrict__ in, int64_t ldi, uint16_t* __restrict__ out, int64_t ldo,
+                        int64_t rows, int64_t cols, int64_t out_rows, int64_t width, int copies) {
+  __shared__ uint16_t tile[32][34];
+  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * 32, j0 = static_cast<int64_t>(blockIdx.y) * 32;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t j = j0 + ty + 8 * i, c = c0 + tx;
+    tile[ty + 8 * i][tx] = j < rows && c < cols ? in[j * ldi + c] : 0;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t c = c0 + ty + 8 * i, j = j0 + tx;
+    if (c < out_rows && j < width)
+      for (int k = 0; k < copies; ++k) out[c * ldo + k * width + j] = tile[tx][ty + 8 * i];
+  }
+}
+
+int transpose(const void* in, int64_t ldi, void* out, int64_t ldo, int64_t rows, int64_t cols, int64_t out_rows,
+              int64_t width, int copies, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>(up(out_rows, 32) / 32), static_cast<unsigned>(up(width, 32) / 32));
+  mx_transpose_kernel<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(in), ldi, static_cast<uint16_t*>(out), ldo,
+                                           rows, cols, out_rows, width, copies);
+  return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
+}
+
+// Rows of `cols` elements copied to rows of `width` (zeros beyond).
+__global__ void __launch_bounds__(256) mx_widen_kernel(const uint16_t* __restrict__ in, int64_t ldi,
+                                                       uint16_t* __restrict__ out, int64_t rows, int64_t cols,
+                                                       int64_t width) {
+  const int64_t row = blockIdx.x;
+  for (int64_t c = threadIdx.x; c < width; c += blockDim.x) out[row * width + c] = c < cols ? in[row * ldi + c] : 0;
+}
+
+}  // namespace
+}  // namespace lora
+
+using namespace lora;
+
+extern "C" size_t lora_mx_backward_workspace_size(int64_t M, int64_t N, int64_t K, int64_t R, int need_dx) {
+  if (M <= 0 || N <= 0 || K <= 0 || R <= 0) return 0;
+  return backward_plan(M, N, K, R, need_dx != 0).total;
+}
+
+extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_codes, const void* x_scales, const void* z,
+                                float z_scale, const void* a, int64_t lda, const void* b, int64_t ldb,
+                                const void* w_codes, const void* w_scales, float w_global, int w_fmt, void* dx,
+                                int64_t lddx, void* da, int64_t ldda, void* db, int64_t lddb, int64_t M, int64_t N,
+                                int64_t K, int64_t R, float scale, int dtype, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+  if (dtype != LORA_BF16 && dtype != LORA_F16) return LORA_ERR_DTYPE;
+  if (dx != nullptr && w_fmt != LORA_MXFP4 && w_fmt != LORA_NVFP4) return LORA_ERR_DTYPE;
+  if (M < 0 || N < 0 || K < 0 || R <= 0 || R > 256 || M > 4194240 || N > 4194240 || K > 4194240) return LORA_ERR_SHAPE;
+  if (lddy < N || lda < K || ldb < R || ldda < K || lddb < R || (dx != nullptr && lddx < K)) return LORA_ERR_SHAPE;
+  if (dx != nullptr && !mx_global_ok(w_global, w_fmt)) return LORA_ERR_ARG;
+  if (N == 0 || K == 0) return LORA_OK;
+  if (dy == nullptr || x_codes == nullptr || x_scales == nullptr || z == nullptr || a == nullptr || b == nullptr ||
+      da == nullptr || db == nullptr)
+    return LORA_ERR_ARG;
+  if (dx != nullptr && (w_codes == nullptr || w_scales == nullptr)) return LORA_ERR_ARG;
+  if (!mx_aligned(x_codes, 16) || !mx_aligned(x_scales, 16) || !mx_aligned(z, 16) || !mx_aligned(workspace, 256) ||
+      (dx != nullptr && (!mx_aligned(w_codes, 16) || !mx_aligned(w_scales, 16))))
+    return LORA_ERR_ALIGN;
+  const int dev = current_device();
+  if (dev < 0 || !device_info(dev).is_sm100) return LORA_ERR_DEVICE;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (M == 0) {
+    if (cudaMemset2DAsync(da, ldda * 2, 0, K * 2, R, s) != cudaSuccess ||
+        cudaMemset2DAsync(db, lddb * 2, 0, R * 2, N, s) != cudaSuccess)
+      return LORA_ERR_CUDA;
+    return LORA_OK;
+  }
+  const BackwardPlan p = backward_plan(M, N, K, R, dx != nullptr);
+  if (workspace == nullptr || workspace_bytes < p.total) return LORA_ERR_WORKSPACE;
+  char* ws = static_cast<char*>(workspace);
+  const int64_t np = up(N, 8), rp = up(R, 16);
+
+  // factor m of the tensor scale m 2^q; 2^q goes into the decoded values
+  float m = 1.f, pow2 = 1.f;
+  if (dx != nullptr && w_fmt == LORA_NVFP4) {
+    int e = 0;
+    m = 2.f * static_cast<float>(frexp(w_global, &e));
+    pow2 = static_cast<float>(ldexp(1.0, e - 1));
+  }
+  // B^T first: the shrink may read it before its own predecessor on the stream has
+  // finished, so other launches lie between
+  int rc = transpose(b, ldb, ws + p.bt, np, N, R, R, np, 1, s);
+  if (rc != LORA_OK) return rc;
+  const void* dyp = dy;
+  int64_t ldp = lddy;
+  if (N % 8 != 0 || lddy % 8 != 0 || !mx_aligned(dy, 16)) {  // TMA needs 16-byte rows
+    mx_widen_kernel<<<static_cast<unsigned>(M), 256, 0, s>>>(static_cast<const uint16_t*>(dy), lddy,
+                                                             reinterpret_cast<uint16_t*>(ws + p.dy), M, N, np);
+    if (cudaGetLastError() != cudaSuccess) return LORA_ERR_CUDA;
+    dyp = ws + p.dy;
+    ldp = np;
+  }
+  MxGradOperands gr = {};
+  gr.v = dyp;
+  gr.ldv = ldp;
+  gr.p = z;
+  gr.ldp = 2 * rp;
+  gr.out = db;
+  gr.ldo = lddb;
+  gr.part = ws + p.part;
+  gr.M = M;
+  gr.C = N;
+  gr.R = R;
+  gr.factor = z_scale;
+  rc = mx_grad_launch(gr, dtype, s);
+  if (rc != LORA_OK) return rc;
+
+  const float gs = scale / m;
+  if (R <= kShrinkMaxRank) {
+    rc = lora_shrink(dyp, ldp, ws + p.bt, np, ws + p.g, 2 * rp, dtype, rp, 1, M, np, R, gs, dtype, p.split_k, ws,
+                     p.shrink_bytes, s);
+  } else {
+    if (rp != R && cudaMemsetAsync(ws + p.g, 0, static_cast<size_t>(M) * 2 * rp * 2, s) != cudaSuccess)
+      return LORA_ERR_CUDA;
+    rc = lora_gemm_ex(dyp, ldp, ws + p.bt, np, nullptr, 0, nullptr, 0, nullptr, ws + p.g, 2 * rp, M, R, np, 0, gs, rp,
+                      dtype, p.shrink_bytes ? ws : nullptr, p.shrink_bytes, s);
+  }
+  if (rc != LORA_OK) return rc;
+
+  gr.v = x_codes;
+  gr.v_scales = x_scales;
+  gr.p = ws + p.g;
+  gr.out = da;
+  gr.ldo = ldda;
+  gr.C = K;
+  gr.factor = m;
+  gr.transposed = true;
+  rc = mx_grad_launch(gr, dtype, s);
+  if (rc != LORA_OK || dx == nullptr) return rc;
+
+  rc = transpose(a, lda, ws + p.at, 2 * rp, R, K, K, rp, 2, s);
+  if (rc != LORA_OK) return rc;
+  rc = mx_dequantize_launch(w_codes, w_scales, ws + p.wt, np, N, K, w_fmt, pow2, 2, dtype, s);
+  if (rc != LORA_OK) return rc;
+  return lora_gemm_ex(dyp, ldp, ws + p.wt, np, ws + p.g, 2 * rp, ws + p.at, 2 * rp, nullptr, dx, lddx, M, K, np, 2 * rp,
+                      m, 0, dtype, p.gemm_bytes ? ws : nullptr, p.gemm_bytes, s);
+}

@@ -1,0 +1,365 @@
+// Adapter gradients: out[c, j] = factor * sum_t V[t, c] P[t, j], a contraction
+// over tokens.
+//
+//   dB = dy^T z    V = dy (16-bit),            P = z
+//   dA = (s dy B)^T X    V = X (mxfp8 checkpoint), P = s dy B, written transposed
+//
+// tcgen05 with both operands MN-major: TMA brings V and P as they lie in memory
+// (tokens as rows, 64-column chunks, 128-byte swizzle) and the transposition is
+// the MMA's.  A CTA owns 256 columns of V (two M = 128 accumulators, N = r) and a
+// range of tokens, so V is read once from HBM; P, r columns wide, is read once per
+// 256 columns of V through L2.  The fp32 partials of the token ranges are summed
+// in a fixed order by a second kernel (no atomics).
+//
+// An mxfp8 V arrives as codes and scale chunks; eight warps turn it into 16-bit
+// values in the MMA's swizzled layout.  E4M3 times a power of two is exact in
+// bf16: the code's exponent and mantissa moved into place, times 2^120, times the
+// scale.  Bound: HBM for small ranks (2 or 1.03 bytes an element of V), the tensor
+// pipe above r ~ 100; P is rounded once to 16 bits, whose error (2^-9 of each
+// term, independent) stays below that of the 16-bit result.
+#include <mutex>
+
+#include "mx_grad.h"
+
+namespace lora {
+namespace {
+
+constexpr int kGrTok = 64;    // tokens a stage
+constexpr int kGrCols = 256;  // columns of V a CTA
+constexpr int kGrConvWarps = 8;
+constexpr int kGrThreads = 64 + 32 * kGrConvWarps;
+constexpr int kGrChunkBytes = kGrTok * 128;          // 64 tokens x 64 16-bit columns
+constexpr int kGrVBytes = 4 * kGrChunkBytes;         // 16-bit V of a stage
+constexpr int kGrRawBytes = kGrTok * kGrCols;        // codes of a stage
+constexpr int kGrScaleBytes = 2 * 512;               // their scale chunks (128 tokens x 256 columns)
+constexpr int kGrSmemMax = 224 * 1024;
+
+struct GrMaps {
+  CUtensorMap v, p, sc;
+};
+
+struct GrArgs {
+  float* part;  // [splits][C][ldp]
+  int* err;
+  int64_t C;
+  int M, r16, p_chunks, stages, stage_bytes, steps_per_split, steps, splits, scale_gb;
+};
+
+// MN-major operand in 64-wide chunks: token rows 128 bytes apart, 8-row groups
+// 1024 bytes apart, chunks `lbo` bytes apart.
+LORA_DEVINL uint64_t gr_desc_mn(uint32_t addr, uint32_t lbo) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((addr >> 4) & 0x3FFF);
+  d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFF) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
+LORA_DEVINL uint32_t gr_mul_bf16x2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 v =
+      __hmul2_rn(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Two E4M3 codes (bytes 1 and 3 of w, bytes 0 and 2 zero) times their scale.
+template <typename T>
+LORA_DEVINL uint32_t gr_decode2(uint32_t w, uint32_t scale_byte);
+template <>
+LORA_DEVINL uint32_t gr_decode2<__nv_bfloat16>(uint32_t w, uint32_t s) {
+  const uint32_t bits = (w & 0x80008000u) | ((w >> 4) & 0x07f007f0u);  // 2^-120 of the code's value
+  const uint32_t half = s == 0 ? 0x0040u : s == 255 ? 0x7fffu : s << 7;
+  return gr_mul_bf16x2(gr_mul_bf16x2(bits, 0x7b807b80u), half | (half << 16));
+}
+template <>
+LORA_DEVINL uint32_t gr_decode2<__half>(uint32_t w, uint32_t s) {
+  const uint32_t h = mx_from_e4m3x2(((w >> 8) & 0xffu) | ((w >> 16) & 0xff00u));
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  const float scale = mx_e8m0(s);
+  return pack2<__half>(v.x * scale, v.y * scale);
+}
+
+// Shared memory: the TMA ring (stage: V or codes + scales, then P), for mxfp8 two
+// converted tiles, then the barriers.
+template <typename T, bool F8>
+__global__ void __launch_bounds__(kGrThreads, 1)
+    mx_grad_kernel(const __grid_constant__ GrMaps maps, const GrArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  constexpr int kPOffset = F8 ? kGrRawBytes + kGrScaleBytes : kGrVBytes;
+  uint8_t* conv = smem + args.stages * args.stage_bytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(conv + (F8 ? 2 * kGrVBytes : 0));
+  uint64_t* empty = full + 8;
+  uint64_t* ready = empty + 8;       // [2] converted tile written
+  uint64_t* conv_empty = ready + 2;  // [2] converted tile read by its MMAs
+  uint64_t* acc_full = conv_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t col0 = static_cast<int64_t>(blockIdx.x) * kGrCols;
+  const int step0 = static_cast<int>(blockIdx.y) * args.steps_per_split;
+  const int step1 = min(step0 + args.steps_per_split, args.steps);
+  const uint32_t tmem_cols = 2 * args.r16 <= 32 ? 32u : 2 * args.r16 <= 64 ? 64u : 2 * args.r16 <= 128 ? 128u
+                             : 2 * args.r16 <= 256 ? 256u : 512u;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < args.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&ready[s], kGrConvWarps);
+      mbar_init(&conv_empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&maps.v);
+    tma_prefetch_desc(&maps.p);
+    if (F8) tma_prefetch_desc(&maps.sc);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      const uint32_t bytes = kPOffset + args.p_chunks * kGrChunkBytes;
+      for (int st = step0; st < step1; ++st) {
+        if (!mbar_wait_bounded(&empty[stage], phase ^ 1, abort_flag, args.err, kDevErrTimeoutEmpty)) break;
+        uint8_t* base = smem + stage * args.stage_bytes;
+        mbar_arrive_expect_tx(&full[stage], bytes);
+        const int tok = st * kGrTok;
+        if constexpr (F8) {
+          tma_load_2d(&maps.v, base, &full[stage], static_cast<int>(col0), tok);
+          tma_load_2d(&maps.sc, base + kGrRawBytes, &full[stage], 0,
+                      (tok >> 7) * args.scale_gb + static_cast<int>(col0 >> 7));
+        } else {
+          for (int c = 0; c < 4; ++c)
+            tma_load_2d(&maps.v, base + c * kGrChunkBytes, &full[stage], static_cast<int>(col0) + 64 * c, tok);
+        }
+        for (int c = 0; c < args.p_chunks; ++c)
+          tma_load_2d(&maps.p, base + kPOffset + c * kGrChunkBytes, &full[stage], 64 * c, tok);
+        if (++stage == args.stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // both operands MN-major (bits 15 and 16), M = 128, N = r16
+      const uint32_t idesc = (umma_idesc_f16(128, 16, std::is_same<T, __nv_bfloat16>::value ? 1 : 0) & ~(0x3fu << 17)) |
+                             (static_cast<uint32_t>(args.r16 >> 3) << 17) | (1u << 15) | (1u << 16);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int st = step0; st < step1; ++st) {
+        const int n = st - step0;
+        if (!mbar_wait_bounded(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull) ||
+            (F8 && !mbar_wait_bounded(&ready[n & 1], (n >> 1) & 1, abort_flag, args.err, kDevErrTimeoutFull))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t base = smem_u32(smem + stage * args.stage_bytes);
+        const uint32_t v = F8 ? smem_u32(conv + (n & 1) * kGrVBytes) : base;
+        for (int k = 0; k < kGrTok / 16; ++k) {
+          const uint64_t pd = gr_desc_mn(base + kPOffset + k * 2048, kGrChunkBytes);
+          for (int m = 0; m < 2; ++m)
+            tc_mma_f16(tmem + m * args.r16, gr_desc_mn(v + m * 2 * kGrChunkBytes + k * 2048, kGrChunkBytes), pd, idesc,
+                       (n > 0 || k > 0) ? 1u : 0u);
+        }
+        tc_commit(&empty[stage]);
+        if (F8) tc_commit(&conv_empty[n & 1]);
+        if (++stage == args.stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (ok) tc_commit(acc_full);
+    }
+  } else {
+    const int cw = warp - 2;
+    if constexpr (F8) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int st = step0; st < step1; ++st) {
+        const int n = st - step0;
+        if (!mbar_wait_bounded(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull) ||
+            !mbar_wait_bounded(&conv_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag, args.err, kDevErrTimeoutEmpty))
+          break;
+        const uint8_t* raw = smem + stage * args.stage_bytes;
+        const uint8_t* sc = raw + kGrRawBytes + (lane >> 4) * 512;  // chunk of this lane's 128 columns
+        uint8_t* dst = conv + (n & 1) * kGrVBytes + (lane >> 3) * kGrChunkBytes;
+#pragma unroll
+        for (int i = 0; i < kGrTok / kGrConvWarps; ++i) {
+          const int t = cw * (kGrTok / kGrConvWarps) + i;
+          const int tr = (st * kGrTok + t) & 127;  // row within the scale chunk
+          const uint2 w = *reinterpret_cast<const uint2*>(raw + t * kGrCols + lane * 8);
+          const uint32_t s = sc[(tr & 31) * 16 + (tr >> 5) * 4 + ((lane >> 2) & 3)];
+          uint4 o;
+          o.x = gr_decode2<T>(__byte_perm(w.x, 0, 0x1404), s);
+          o.y = gr_decode2<T>(__byte_perm(w.x, 0, 0x3424), s);
+          o.z = gr_decode2<T>(__byte_perm(w.y, 0, 0x1404), s);
+          o.w = gr_decode2<T>(__byte_perm(w.y, 0, 0x3424), s);
+          *reinterpret_cast<uint4*>(dst + t * 128 + (((lane & 7) ^ (t & 7)) << 4)) = o;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ready[n & 1]);
+        if (++stage == args.stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    // epilogue: warps 0..3 of these drain the first accumulator, 4..7 the second
+    const int quad = warp & 3, m = cw >> 2;
+    if (mbar_wait_bounded(acc_full, 0, abort_flag, args.err, kDevErrTimeoutAccFull)) {
+      tc_fence_after();
+      const int64_t c = col0 + m * 128 + quad * 32 + lane;
+      float* dst = args.part + (static_cast<int64_t>(blockIdx.y) * args.C + c) * args.r16;
+      for (int j = 0; j < args.r16; j += 16) {
+        uint32_t r[16];
+        tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + m * args.r16 + j, r);
+        tmem_wait_ld();
+        if (c < args.C) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            reinterpret_cast<uint4*>(dst + j)[e] = make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, tmem_cols);
+  }
+}
+
+// Sum of the splits in order, times factor, rounded to T: out[c, j] (ldo) or,
+// transposed, out[j, c].  32 columns of V x 32 ranks a block.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    mx_grad_reduce_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t ldo, int64_t C, int r, int r16,
+                          int splits, float factor, bool transposed) {
+  __shared__ float tile[32][33];
+  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * 32;
+  const int j0 = blockIdx.y * 32;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t c = c0 + ty + 8 * i;
+    const int j = j0 + tx;
+    float v = 0.f;
+    if (c < C && j < r) {
+      const float* p = part + c * r16 + j;
+      for (int s = 0; s < splits; ++s) v += p[s * C * r16];
+      v *= factor;
+      if (!transposed) out[c * ldo + j] = from_f32<T>(v);
+    }
+    if (transposed) tile[ty + 8 * i][tx] = v;
+  }
+  if (transposed) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = j0 + ty + 8 * i;
+      const int64_t c = c0 + tx;
+      if (c < C && j < r) out[j * ldo + c] = from_f32<T>(tile[tx][ty + 8 * i]);
+    }
+  }
+}
+
+struct GrPlan {
+  int groups, steps, splits, steps_per_split;
+};
+
+GrPlan grad_plan(int64_t M, int64_t C) {
+  GrPlan p;
+  const int dev = current_device();
+  const int sms = dev >= 0 ? device_info(dev).num_sms : 148;
+  p.groups = static_cast<int>((C + kGrCols - 1) / kGrCols);
+  p.steps = static_cast<int>((M + kGrTok - 1) / kGrTok);
+  int splits = std::max(1, sms / p.groups);
+  splits = std::min(splits, p.steps);
+  p.steps_per_split = (p.steps + splits - 1) / splits;
+  p.splits = (p.steps + p.steps_per_split - 1) / p.steps_per_split;
+  return p;
+}
+
+template <typename T, bool F8>
+int launch_grad(const MxGradOperands& g, const GrPlan& pl, cudaStream_t stream) {
+  const int dev = current_device();
+  if (dev < 0) return LORA_ERR_DEVICE;
+  const DeviceInfo& info = device_info(dev);
+  GrMaps maps;
+  GrArgs a;
+  a.part = static_cast<float*>(g.part);
+  a.err = info.err_word;
+  a.C = g.C;
+  a.M = static_cast<int>(g.M);
+  a.r16 = static_cast<int>((g.R + 15) / 16 * 16);
+  a.p_chunks = (a.r16 + 63) / 64;
+  a.steps = pl.steps;
+  a.splits = pl.splits;
+  a.steps_per_split = pl.steps_per_split;
+  a.scale_gb = static_cast<int>(mx_scale_chunks(g.C, LORA_MXFP8));
+  a.stage_bytes = (F8 ? kGrRawBytes + kGrScaleBytes : kGrVBytes) + a.p_chunks * kGrChunkBytes;
+  const int fixed = (F8 ? 2 * kGrVBytes : 0) + 512 + 1024;
+  a.stages = std::min(8, (kGrSmemMax - fixed) / a.stage_bytes);
+  if (F8) {
+    const int64_t pitch = mx_padded_k(g.C);
+    if (!mx_encode_map(&maps.v, g.v, 1, pitch, g.M, pitch, kGrCols, kGrTok, false) ||
+        !mx_encode_map(&maps.sc, g.v_scales, 4, 128, (g.M + 127) / 128 * a.scale_gb, 512, 128, 2, false))
+      return LORA_ERR_CUDA;
+  } else {
+    if (!mx_encode_map(&maps.v, g.v, 2, g.C, g.M, g.ldv * 2, 64, kGrTok, true)) return LORA_ERR_CUDA;
+    maps.sc = maps.v;
+  }
+  if (!mx_encode_map(&maps.p, g.p, 2, g.R, g.M, g.ldp * 2, 64, kGrTok, true)) return LORA_ERR_CUDA;
+  auto kernel = mx_grad_kernel<T, F8>;
+  static std::once_flag once[64];
+  static cudaError_t attr_err[64];
+  std::call_once(once[dev], [&] {
+    attr_err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGrSmemMax);
+  });
+  if (attr_err[dev] != cudaSuccess) return LORA_ERR_CUDA;
+  const size_t smem = static_cast<size_t>(a.stages) * a.stage_bytes + fixed;
+  kernel<<<dim3(pl.groups, pl.splits), kGrThreads, smem, stream>>>(maps, a);
+  if (cudaGetLastError() != cudaSuccess) return LORA_ERR_CUDA;
+  mx_grad_reduce_kernel<T><<<dim3(static_cast<unsigned>((g.C + 31) / 32), (a.r16 + 31) / 32), 256, 0, stream>>>(
+      a.part, static_cast<T*>(g.out), g.ldo, g.C, static_cast<int>(g.R), a.r16, pl.splits, g.factor, g.transposed);
+  return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
+}
+
+}  // namespace
+
+size_t mx_grad_part_bytes(int64_t M, int64_t C, int64_t R) {
+  return static_cast<size_t>(grad_plan(M, C).splits) * C * ((R + 15) / 16 * 16) * sizeof(float);
+}
+
+int mx_grad_launch(const MxGradOperands& g, int dtype, cudaStream_t stream) {
+  const GrPlan pl = grad_plan(g.M, g.C);
+  const bool f8 = g.v_scales != nullptr;
+  if (dtype == LORA_BF16)
+    return f8 ? launch_grad<__nv_bfloat16, true>(g, pl, stream) : launch_grad<__nv_bfloat16, false>(g, pl, stream);
+  return f8 ? launch_grad<__half, true>(g, pl, stream) : launch_grad<__half, false>(g, pl, stream);
+}
+
+}  // namespace lora

@@ -1,0 +1,21 @@
+// Host interface of the adapter-gradient kernel (mx_grad.cu).
+#pragma once
+
+#include "mx_linear.h"
+
+namespace lora {
+
+// out[c, j] = factor * sum_t V[t, c] P[t, j]; V is 16-bit (ldv) or, with
+// v_scales, an mxfp8 tensor; transposed writes out[j, c].
+struct MxGradOperands {
+  const void *v, *v_scales, *p;
+  void *out, *part;  // part: mx_grad_part_bytes
+  int64_t ldv, ldp, ldo, M, C, R;
+  float factor;
+  bool transposed;
+};
+
+size_t mx_grad_part_bytes(int64_t M, int64_t C, int64_t R);
+int mx_grad_launch(const MxGradOperands& g, int dtype, cudaStream_t stream);
+
+}  // namespace lora

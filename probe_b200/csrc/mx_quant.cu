@@ -179,11 +179,12 @@ LORA_DEVINL void mx_decode16(const uint32_t* c, uint32_t byte, float g, uint32_t
 }
 
 // A CTA decodes 128 x 128 values, straight (rows of 256 bytes) or transposed
-// through shared memory (column c of the tensor becomes row c of out).
+// through shared memory (column c of the tensor becomes row c of out, Mw >= M
+// values wide: zeros beyond M).
 template <typename T, int FMT, bool TR>
 __global__ void __launch_bounds__(kMxThreads)
     mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out,
-                         int64_t ldo, int64_t M, int64_t K, int64_t Kp, int chunks, float g, bool vec) {
+                         int64_t ldo, int64_t M, int64_t Mw, int64_t K, int64_t Kp, int chunks, float g, bool vec) {
   constexpr int kPitch = kMxTile + 2;  // 16-bit elements: odd number of 4-byte words a row
   __shared__ alignas(16) uint16_t tile[TR ? kMxTile * kPitch : 8];
   const int seg = threadIdx.x & 7;
@@ -192,7 +193,8 @@ __global__ void __launch_bounds__(kMxThreads)
   const int64_t col0 = static_cast<int64_t>(blockIdx.x) * kMxTile;
   const int64_t col = col0 + seg * 16;
   const int block = static_cast<int>(col / MxFormat<FMT>::kBlock);
-  const uint8_t* sc = scales + (static_cast<int64_t>(blockIdx.y) * chunks + (block >> 2)) * 512 + sub * 16 + (block & 3);
+  const uint8_t* sc =
+      scales + (static_cast<int64_t>(blockIdx.y) * chunks + (block >> 2)) * 512 + sub * 16 + (block & 3);
   uint32_t c[4][4], byte[4];
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
@@ -243,11 +245,11 @@ __global__ void __launch_bounds__(kMxThreads)
       for (int h = 0; h < 2; ++h) {
         const int r = 64 * h + 2 * lane;
         const uint32_t lo = tile[r * kPitch + cc], hi = tile[(r + 1) * kPitch + cc];
-        if (vec && row0 + r + 2 <= M) {
+        if (vec && row0 + r + 2 <= Mw) {
           *reinterpret_cast<uint32_t*>(dst + r) = lo | (hi << 16);
         } else {
-          if (row0 + r < M) dst[r] = static_cast<uint16_t>(lo);
-          if (row0 + r + 1 < M) dst[r + 1] = static_cast<uint16_t>(hi);
+          if (row0 + r < Mw) dst[r] = static_cast<uint16_t>(lo);
+          if (row0 + r + 1 < Mw) dst[r + 1] = static_cast<uint16_t>(hi);
         }
       }
     }
@@ -272,18 +274,20 @@ template <typename T, int FMT>
 int dequantize_t(const void* codes, const void* scales, void* out, int64_t ldo, int64_t M, int64_t K, float g,
                  int transpose, cudaStream_t stream) {
   const int64_t Kp = mx_padded_k(K);
+  // the composite operators ask for rows padded to 16 bytes (transpose == 2)
+  const int64_t Mw = transpose == 2 ? (M + 7) / 8 * 8 : M;
   const dim3 grid(static_cast<unsigned>((Kp + kMxTile - 1) / kMxTile), static_cast<unsigned>((M + kMxTile - 1) / kMxTile));
   const int chunks = static_cast<int>(mx_scale_chunks(K, FMT));
   if (transpose) {
     const bool vec = aligned(out, 4) && ldo % 2 == 0;
     mx_dequantize_kernel<T, FMT, true><<<grid, kMxThreads, 0, stream>>>(
-        static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<T*>(out), ldo, M, K, Kp,
-        chunks, g, vec);
+        static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<T*>(out), ldo, M, Mw, K,
+        Kp, chunks, g, vec);
   } else {
     const bool vec = aligned(out, 16) && ldo % 8 == 0;
     mx_dequantize_kernel<T, FMT, false><<<grid, kMxThreads, 0, stream>>>(
-        static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<T*>(out), ldo, M, K, Kp,
-        chunks, g, vec);
+        static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<T*>(out), ldo, M, M, K,
+        Kp, chunks, g, vec);
   }
   return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
 }

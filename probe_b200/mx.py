@@ -181,3 +181,47 @@ def mx_lora_linear(x: torch.Tensor, weight: MXTensor, bias: torch.Tensor | None,
     ``a`` / ``b`` None, or scale 0, leave the adapter out.
     """
     return _linear(x, weight, bias, a, b, scale, x_global_scale, False, "mx_lora_linear")[0]
+
+
+# ------------------------------------------------------------------- training
+def mx_lora_backward(dy: torch.Tensor, x8: MXTensor, z: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+                     scale: float = 1.0, weight: MXTensor | None = None, z_scale: float = 1.0):
+    """Gradients ``(dx, da, db)`` of the LoRA linear from the 8-bit checkpoint of its input.
+
+    ``g = scale * dy @ b``;  ``da = g.T @ X`` [r, K];  ``db = z_scale * dy.T @ z`` [N, r];
+    ``dx = dy @ W + g @ a`` [..., K], or None without ``weight``.  ``x8`` is the mxfp8
+    checkpoint of x, ``z`` the [M, 2 r16] pair of the forward pass (its hi half is
+    read), W an mxfp4 / nvfp4 tensor.  W is frozen; rounding to 4 or 8 bits counts
+    as the identity.
+    """
+    where = "mx_lora_backward"
+    wc = weight.codes if weight is not None else None
+    _lib.require_cuda(dy, x8.codes, z, a, b, wc, where=where)
+    shape = dy.shape
+    dy = _rows(dy, where)
+    m, n = dy.shape
+    r, k = a.shape
+    dtype = dy.dtype
+    if x8.fmt != "mxfp8" or x8.shape != (m, k):
+        raise ValueError(f"{where}: x8 must be an mxfp8 tensor of shape {(m, k)}, got {x8.fmt} {x8.shape}")
+    if a.dtype != dtype or b.dtype != dtype or z.dtype != dtype:
+        raise TypeError(f"{where}: dy, z, a and b must share one dtype")
+    if b.shape != (n, r) or not 1 <= r <= 256:
+        raise ValueError(f"{where}: b {tuple(b.shape)} does not match [{n}, {r}] (1 <= r <= 256)")
+    if z.shape != (m, 2 * ((r + 15) // 16 * 16)) or not z.is_contiguous():
+        raise ValueError(f"{where}: z must be the contiguous [M, 2 * round_up(r, 16)] pair, got {tuple(z.shape)}")
+    if weight is not None and (weight.fmt not in ("mxfp4", "nvfp4") or weight.shape != (n, k)):
+        raise ValueError(f"{where}: the weight must be a 4-bit tensor of shape {(n, k)}, got {weight.fmt} {weight.shape}")
+    a, b = _lib.row_major(a), _lib.row_major(b)
+    da = torch.empty((r, k), dtype=dtype, device=dy.device)
+    db = torch.empty((n, r), dtype=dtype, device=dy.device)
+    dx = torch.empty((m, k), dtype=dtype, device=dy.device) if weight is not None else None
+    nbytes = _lib.load().lora_mx_backward_workspace_size(m, n, k, r, int(dx is not None))
+    ws = _lib.WORKSPACE.get(nbytes, dy.device, "mx_backward")
+    _lib.call("lora_mx_backward", _lib.ptr(dy), _lib.ld(dy), _lib.ptr(x8.codes), _lib.ptr(x8.scales), _lib.ptr(z),
+              float(z_scale), _lib.ptr(a), _lib.ld(a), _lib.ptr(b), _lib.ld(b), _lib.ptr(wc),
+              _lib.ptr(weight.scales) if weight is not None else None,
+              weight.global_scale if weight is not None else 1.0, weight._code if weight is not None else 0,
+              _lib.ptr(dx), k, _lib.ptr(da), k, _lib.ptr(db), r, m, n, k, r, float(scale), _lib.dtype_code(dtype),
+              _lib.ptr(ws), ws.numel(), _lib.stream_handle(dy.device))
+    return (None if dx is None else dx.view(*shape[:-1], k)), da, db
