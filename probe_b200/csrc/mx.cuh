@@ -45,6 +45,18 @@ inline bool mx_global_ok(float g, int fmt) {
   return fmt == LORA_NVFP4 ? (g >= 5.4210109e-20f && g <= 1.8446744e19f) : g == 1.0f;  // [2^-64, 2^64]
 }
 
+// One lane of a converged warp.
+LORA_DEVINL bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// mbar_wait_bounded by a whole warp; every lane gets the same answer.
+LORA_DEVINL bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err, int code) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort, err, code));
+}
+
 // 2^(byte - 127) of an E8M0 scale byte; 255 is NaN.
 LORA_DEVINL float mx_e8m0(uint32_t byte) {
   const uint32_t bits = byte == 0 ? 0x00400000u : (byte == 255 ? 0x7fffffffu : byte << 23);

@@ -18,7 +18,7 @@
 // tiles.  Layout: a cluster of two CTAs per 256 x 256 tile, persistent; warp 0
 // TMA (codes in 128-byte swizzled rows, scale chunks as they are stored), warp
 // 1 of the leader copies the stage's scales to TMEM (tcgen05.cp, each CTA from
-// its own shared memory) and issues the MMAs, warps 2..5 the epilogue.
+// its own shared memory) and issues the MMAs, warps 2..9 the epilogue.
 // TMEM: two 256-column accumulators and two buffers of scales do not fit 512
 // columns, so the accumulators share 48 (mxfp4) or 96 (nvfp4) columns: the
 // epilogue drains those first and only they hold up the next tile's MMAs.
@@ -32,7 +32,7 @@
 namespace lora {
 namespace {
 
-constexpr int kMxEpiWarps = 4;
+constexpr int kMxEpiWarps = 8;  // two of each TMEM lane quadrant, taking 16-column groups in turn
 constexpr int kMxGemmThreads = 64 + 32 * kMxEpiWarps;
 
 struct MxGemmArgs {
@@ -151,6 +151,8 @@ struct MxMaps {
   CUtensorMap x, w, sx, sw, zh, zl, b;
 };
 
+// 16 columns of one row: alpha, bias, rounding, one 32-byte store (vec: the row is
+// 32-byte aligned, bias 16-byte aligned).
 template <typename T>
 LORA_DEVINL void mx_store16(const MxGemmArgs& args, T* out_row, int row, int col0, bool vec, const uint32_t* r) {
   if (row >= args.M || col0 >= args.N) return;
@@ -158,22 +160,28 @@ LORA_DEVINL void mx_store16(const MxGemmArgs& args, T* out_row, int row, int col
   float v[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]) * args.alpha;
-  if (bias != nullptr) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (col0 + i < args.N) v[i] += to_f32(bias[col0 + i]);
-  }
   if (vec && col0 + 16 <= args.N) {
+    if (bias != nullptr) {
+      const uint4 b0 = __ldg(reinterpret_cast<const uint4*>(bias + col0));
+      const uint4 b1 = __ldg(reinterpret_cast<const uint4*>(bias + col0 + 8));
+      const uint32_t bw[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 f = unpack2<T>(bw[i]);
+        v[2 * i] += f.x;
+        v[2 * i + 1] += f.y;
+      }
+    }
     uint32_t w[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
-    uint4* dst = reinterpret_cast<uint4*>(out_row + col0);
-    dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out_row + col0), "r"(w[0]), "r"(w[1]),
+                 "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (col0 + i < args.N) out_row[col0 + i] = from_f32<T>(v[i]);
+      if (col0 + i < args.N) out_row[col0 + i] = from_f32<T>(v[i] + (bias != nullptr ? to_f32(bias[col0 + i]) : 0.f));
   }
 }
 
@@ -275,97 +283,149 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
       }
     }
   } else if (warp == 1) {
-    if (leader && lane == 0) {
-      int stage = 0, prev = 0;
+    // The whole warp walks the stages, so that descriptors and addresses live in
+    // uniform registers; one elected lane issues.
+    if (leader) {
+      const bool issuer = elect_one();
+      int stage = 0;
       uint32_t phase = 0;
       int use = 0;  // stages used so far; scale buffer = use & 1
       int local = 0;
       bool ok = true;
+      const uint64_t ad0 = umma_desc_sw128(smem_u32(sm_a));
+      const uint64_t bd0 = umma_desc_sw128(smem_u32(sm_b));
+      const uint64_t sd0 = mx_desc_scales(smem_u32(sm_sf));
+      // `lag` of the uses so far are not known to be complete, the first of them in
+      // stage done_stage
+      int lag = 0, done_stage = 0;
+      uint32_t done_phase = 0;
+      auto catch_up = [&](int most) {
+        while (lag > most) {
+          if (!warp_wait(&empty[done_stage], done_phase, abort_flag, args.err, kDevErrTimeoutEmpty)) return false;
+          --lag;
+          if (++done_stage == L::kStages) {
+            done_stage = 0;
+            done_phase ^= 1;
+          }
+        }
+        return true;
+      };
       for (int tile = pair; ok && tile < args.num_tiles; tile += npairs, ++local) {
-        if (local > 0 && !mbar_wait_bounded(acc_free, (local - 1) & 1, abort_flag, args.err, kDevErrTimeoutAccEmpty))
+        if (local > 0 && !warp_wait(acc_free, (local - 1) & 1, abort_flag, args.err, kDevErrTimeoutAccEmpty))
           break;
         tc_fence_after();
         const uint32_t d = tmem + ((local & 1) ? L::kAcc1 : 0);
-        for (int kb = 0; kb < args.num_kb + tail_kb; ++kb, ++use) {
-          if (!mbar_wait_bounded(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
+        for (int kb = 0; kb < args.num_kb; ++kb, ++use) {
+          // the MMAs of two uses ago read the scale buffer that is written next
+          if (!catch_up(1) || !warp_wait(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
             ok = false;
             break;
           }
-          // The MMAs of two uses ago read the scale buffer that is written next; those
-          // of the last base stage finish before MMAs of the other kind start.
-          const int behind = kb < args.num_kb ? 2 : (kb == args.num_kb ? 1 : 0);
-          if (behind > 0 && use >= behind) {
-            prev = use - behind;
-            if (!mbar_wait_bounded(&empty[prev % L::kStages], (prev / L::kStages) & 1, abort_flag, args.err,
-                                   kDevErrTimeoutEmpty)) {
-              ok = false;
-              break;
-            }
-          }
+          ++lag;
           tc_fence_after();
-          const uint64_t ad = umma_desc_sw128(smem_u32(sm_a + stage * L::kOpBytes));
-          const uint64_t bd = umma_desc_sw128(smem_u32(sm_b + stage * L::kOpBytes));
-          if (kb < args.num_kb) {
-            const uint32_t sf = tmem + L::kSfBase + (use & 1) * L::kSfCols;
-            const uint32_t sfb = sf + L::kChunks * 4;
-            const uint64_t sd = mx_desc_scales(smem_u32(sm_sf + stage * L::kSfBytes));
+          const uint64_t ad = ad0 + static_cast<uint32_t>(stage * (L::kOpBytes >> 4));
+          const uint64_t bd = bd0 + static_cast<uint32_t>(stage * (L::kOpBytes >> 4));
+          const uint64_t sd = sd0 + static_cast<uint32_t>(stage * (L::kSfBytes >> 4));
+          const uint32_t sf = tmem + L::kSfBase + (use & 1) * L::kSfCols;
+          const uint32_t sfb = sf + L::kChunks * 4;
+          const int nk = kb == args.num_kb - 1 ? args.last_k64 : 4;
+          if (issuer) {
 #pragma unroll
             for (int j = 0; j < L::kChunks; ++j) {
               mx_cp_scales_pair(sf + 4 * j, sd + static_cast<uint64_t>(32 * j));
               mx_cp_scales_pair(sfb + 8 * j, sd + static_cast<uint64_t>(32 * (L::kChunks + j)));
               mx_cp_scales_pair(sfb + 8 * j + 4, sd + static_cast<uint64_t>(32 * (2 * L::kChunks + j)));
             }
-            const int nk = kb == args.num_kb - 1 ? args.last_k64 : 4;
-            for (int k = 0; k < nk; ++k) {
-              const int j = FMT == LORA_MXFP4 ? k >> 1 : k;
-              const uint32_t id = FMT == LORA_MXFP4 ? static_cast<uint32_t>(k & 1) * 2u : 0u;
-              mx_mma_pair<FMT>(d, ad + static_cast<uint64_t>(2 * k), bd + static_cast<uint64_t>(2 * k),
-                               kIdesc | (id << 4) | (id << 29), sf + 4 * j, sfb + 8 * j, (kb > 0 || k > 0) ? 1u : 0u);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              constexpr bool kMx = FMT == LORA_MXFP4;
+              const int j = kMx ? k >> 1 : k;
+              const uint32_t id = kMx ? static_cast<uint32_t>(k & 1) * 2u : 0u;
+              if (k < nk)
+                mx_mma_pair<FMT>(d, ad + static_cast<uint64_t>(2 * k), bd + static_cast<uint64_t>(2 * k),
+                                 kIdesc | (id << 4) | (id << 29), sf + 4 * j, sfb + 8 * j, (kb > 0 || k > 0) ? 1u : 0u);
             }
-          } else {
-            const int t = kb - args.num_kb - args.zero_kb;
-            const int c = t >= args.rank_kb ? t - args.rank_kb : t;
-            const int nk = t < 0 ? 1 : c == args.rank_kb - 1 ? args.last_k16 : 4;
-            const int shift = t < 0 ? 15 : t == 0 ? args.dshift - 15 * args.zero_kb : 0;
-            for (int k = 0; k < nk; ++k)
-              mx_mma_f16_pair_shift(d, ad + static_cast<uint64_t>(2 * k), bd + static_cast<uint64_t>(2 * k), kIdescTail,
-                                    k == 0 ? shift : 0);
+            tc_commit_pair(&empty[stage], kBoth);
           }
-          tc_commit_pair(&empty[stage], kBoth);
+          __syncwarp();
           if (++stage == L::kStages) {
             stage = 0;
             phase ^= 1;
           }
         }
-        if (ok) tc_commit_pair(acc_full, kBoth);
+        for (int t = -args.zero_kb; ok && t < 2 * args.rank_kb; ++t, ++use) {
+          // the last base stage's MMAs finish before MMAs of the other kind start
+          if (!catch_up(t == -args.zero_kb ? 0 : 1) ||
+              !warp_wait(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          ++lag;
+          tc_fence_after();
+          const uint64_t ad = ad0 + static_cast<uint32_t>(stage * (L::kOpBytes >> 4));
+          const uint64_t bd = bd0 + static_cast<uint32_t>(stage * (L::kOpBytes >> 4));
+          const int c = t >= args.rank_kb ? t - args.rank_kb : t;
+          const int nk = t < 0 ? 1 : c == args.rank_kb - 1 ? args.last_k16 : 4;
+          const int shift = t < 0 ? 15 : t == 0 ? args.dshift - 15 * args.zero_kb : 0;
+          if (issuer) {
+            mx_mma_f16_pair_shift(d, ad, bd, kIdescTail, shift);
+#pragma unroll
+            for (int k = 1; k < 4; ++k)
+              if (k < nk)
+                tc_mma_f16_pair(d, ad + static_cast<uint64_t>(2 * k), bd + static_cast<uint64_t>(2 * k), kIdescTail, 1u);
+            tc_commit_pair(&empty[stage], kBoth);
+          }
+          __syncwarp();
+          if (++stage == L::kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (ok && issuer) tc_commit_pair(acc_full, kBoth);
+        __syncwarp();
       }
     }
   } else {
     const int quad = warp & 3;
-    const bool vec = (args.ldo % 8) == 0 && (reinterpret_cast<uintptr_t>(args.out) % 16) == 0;
+    const int part = (warp - 2) >> 2;  // takes the 16-column groups of this parity
+    const bool vec = (args.ldo % 16) == 0 && (reinterpret_cast<uintptr_t>(args.out) % 32) == 0 &&
+                     (reinterpret_cast<uintptr_t>(args.bias) % 16) == 0;
+    constexpr int kFirst = (L::kOverlap / 16 + 1) / 2;  // most shared groups of one warp
     int local = 0;
     for (int tile = pair; tile < args.num_tiles; tile += npairs, ++local) {
       int mt, nt;
       mx_tile_coords(tile, args, mt, nt);
-      if (!mbar_wait_bounded(acc_full, local & 1, abort_flag, args.err, kDevErrTimeoutAccFull)) break;
+      if (!warp_wait(acc_full, local & 1, abort_flag, args.err, kDevErrTimeoutAccFull)) break;
       tc_fence_after();
       const int row = mt * 256 + static_cast<int>(rank) * 128 + quad * 32 + lane;
       T* out_row = static_cast<T*>(args.out) + static_cast<int64_t>(row) * args.ldo;
       const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16) + ((local & 1) ? L::kAcc1 : 0);
-      // columns in the order: shared with the other accumulator, then the rest
+      // Groups in the order: columns shared with the other accumulator, then the
+      // rest.  The shared ones go to registers first, and the next tile may start.
       const int first = (local & 1) ? 0 : L::kAcc1;
-#pragma unroll 1
-      for (int i = 0; i < 256; i += 16) {
-        const int c = (first + i) & 255;
-        uint32_t r[16];
-        tmem_ld_32x32b_x16(t_row + c, r);
+      {
+        uint32_t r[kFirst][16];
+#pragma unroll
+        for (int q = 0; q < kFirst; ++q)
+          if (2 * q + part < L::kOverlap / 16) tmem_ld_32x32b_x16(t_row + first + (2 * q + part) * 16, r[q]);
         tmem_wait_ld();
-        if (i == L::kOverlap - 16) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(acc_free), 0));
-        }
-        mx_store16<T>(args, out_row, row, nt * 256 + c, vec, r);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(acc_free), 0));
+#pragma unroll
+        for (int q = 0; q < kFirst; ++q)
+          if (2 * q + part < L::kOverlap / 16)
+            mx_store16<T>(args, out_row, row, nt * 256 + first + (2 * q + part) * 16, vec, r[q]);
+      }
+#pragma unroll 1
+      for (int g = (L::kOverlap / 16 - part + 1) / 2 * 2 + part; g < 16; g += 4) {
+        uint32_t r[2][16];
+        const int c0 = (first + g * 16) & 255, c1 = (first + g * 16 + 32) & 255;
+        tmem_ld_32x32b_x16(t_row + c0, r[0]);
+        if (g + 2 < 16) tmem_ld_32x32b_x16(t_row + c1, r[1]);
+        tmem_wait_ld();
+        mx_store16<T>(args, out_row, row, nt * 256 + c0, vec, r[0]);
+        if (g + 2 < 16) mx_store16<T>(args, out_row, row, nt * 256 + c1, vec, r[1]);
       }
     }
   }
