@@ -52,9 +52,15 @@ LORA_DEVINL bool elect_one() {
   return p != 0;
 }
 
-// mbar_wait_bounded by a whole warp; every lane gets the same answer.
-LORA_DEVINL bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err, int code) {
-  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort, err, code));
+// mbar_wait_bounded on behalf of a whole warp: the lane that passes mine = true
+// waits (32 lanes polling one barrier are served one after another, ~200 cycles),
+// every lane gets its answer.
+LORA_DEVINL bool warp_wait(bool mine, uint64_t* bar, uint32_t parity, volatile int* abort, int* err, int code) {
+  bool ok = true;
+  if (mine) ok = mbar_wait_bounded(bar, parity, abort, err, code);
+  ok = __all_sync(0xffffffffu, ok);
+  __syncwarp();
+  return ok;
 }
 
 // 2^(byte - 127) of an E8M0 scale byte; 255 is NaN.
@@ -103,6 +109,117 @@ LORA_DEVINL uint32_t mx_from_e4m3x2(uint32_t w) {
   uint32_t h2;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(w)));
   return h2;
+}
+
+// Largest magnitude, as the 16-bit pattern without its sign: infinities and
+// NaN compare above every number.
+LORA_DEVINL uint32_t mx_amax16(const uint32_t* w) {
+  uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+  return max(m & 0xffffu, m >> 16);
+}
+
+template <typename T> LORA_DEVINL float mx_bits16_to_f32(uint32_t b);
+template <> LORA_DEVINL float mx_bits16_to_f32<__nv_bfloat16>(uint32_t b) { return __uint_as_float(b << 16); }
+template <> LORA_DEVINL float mx_bits16_to_f32<__half>(uint32_t b) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(b)));
+}
+
+// Tensor-wide constants of a quantisation: 6 g and its reciprocal, both rounded.
+struct MxGlobal {
+  float g, g6, r6;
+};
+inline MxGlobal mx_global(float g) {
+  const float g6 = 6.0f * g;
+  return MxGlobal{g, g6, 1.0f / g6};
+}
+
+// Correctly rounded quotients by one divisor: with r the correctly rounded
+// reciprocal of d, one residual step makes x r the rounded x / d (Markstein,
+// 1990).  |x r| is kept below 2^20 so that the residual stays finite; every
+// quotient that large saturates.
+LORA_DEVINL float mx_div(float x, float d, float r) {
+  const float q = x * r;
+  return fmaf(fmaf(-q, d, x), r, q);
+}
+LORA_DEVINL float mx_div_far(float x, float d, float r) {
+  const float q = fminf(fmaxf(x * r, -1048576.f), 1048576.f);
+  return fmaf(fmaf(-q, d, x), r, q);
+}
+
+// Scale of a block from its amax16: the byte to store and what turns a value
+// into units of the scale (mxfp4 / mxfp8: mul; nvfp4: divisor and reciprocal).
+template <typename T, int FMT>
+struct MxScale {
+  uint32_t byte;
+  float d, r;
+  bool far;
+  // recip: reciprocals of (E4M3 code x g) by code, 128 entries (nvfp4)
+  LORA_DEVINL MxScale(uint32_t top, const MxGlobal& gl, const float* recip) {
+    constexpr uint32_t kInf = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+    const bool bad = top >= kInf;
+    const float amax = mx_bits16_to_f32<T>(top);
+    if constexpr (FMT == LORA_NVFP4) {
+      byte = bad ? 0x7fu : mx_to_e4m3x2(mx_div_far(amax, gl.g6, gl.r6), 0.f) & 0xffu;
+      d = mx_e4m3(byte) * gl.g;
+      r = recip[byte];  // 0 for a zero or NaN scale
+      far = amax * r > 1048576.f;
+    } else {
+      const int e = max(static_cast<int>(__float_as_uint(amax) >> 23) - MxFormat<FMT>::kTop, 0);  // biased by 127
+      byte = bad ? 255u : static_cast<uint32_t>(e);
+      r = bad ? 0.f : __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+      d = 0.f;
+      far = false;
+    }
+  }
+};
+
+// Entry `code` of the reciprocals: correctly rounded, 0 for zero and NaN scales
+// (whose codes are zero).
+LORA_DEVINL float mx_recip_entry(int code, float g) {
+  return code == 0 || code >= 127 ? 0.f : __frcp_rn(mx_e4m3(static_cast<uint32_t>(code)) * g);
+}
+
+// Codes of 16 values: 8 (4-bit) or 16 bytes.
+template <typename T, int FMT>
+LORA_DEVINL void mx_codes16(const uint32_t* w, const MxScale<T, FMT>& s, uint32_t* codes) {
+  float v[16];
+  if constexpr (FMT == LORA_NVFP4) {
+    if (s.r == 0.f) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = 0.f;
+    } else if (s.far) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 x = unpack2<T>(w[i]);
+        v[2 * i] = mx_div_far(x.x, s.d, s.r);
+        v[2 * i + 1] = mx_div_far(x.y, s.d, s.r);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 x = unpack2<T>(w[i]);
+        v[2 * i] = mx_div(x.x, s.d, s.r);
+        v[2 * i + 1] = mx_div(x.y, s.d, s.r);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 x = unpack2<T>(s.byte == 255u ? 0u : w[i]);
+      v[2 * i] = x.x * s.r;
+      v[2 * i + 1] = x.y * s.r;
+    }
+  }
+  if constexpr (MxFormat<FMT>::kBits == 4) {
+    codes[0] = mx_to_e2m1x8(v);
+    codes[1] = mx_to_e2m1x8(v + 8);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      codes[i] = mx_to_e4m3x2(v[4 * i], v[4 * i + 1]) | (mx_to_e4m3x2(v[4 * i + 2], v[4 * i + 3]) << 16);
+  }
 }
 
 // Device entry points of the parts (host launchers), used by the C ABI and by

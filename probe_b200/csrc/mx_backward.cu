@@ -14,31 +14,23 @@
 #include <cmath>
 
 #include "mx_grad.h"
+#include "mx_shrink.h"
 
 namespace lora {
 namespace {
 
-constexpr int64_t kShrinkMaxRank = 128;
-
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 struct BackwardPlan {
-  size_t shrink_bytes, gemm_bytes, part, g, bt, at, dy, wt, total;
-  int split_k;
+  size_t gemm_bytes, part, g, bt, at, dy, wt, total;
 };
 
 BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need_dx) {
   BackwardPlan p = {};
   const int64_t np = up(N, 8), rp = up(R, 16);
-  if (R <= kShrinkMaxRank) {
-    p.split_k = lora_shrink_pick_split_k(M, np, R);
-    p.shrink_bytes = lora_shrink_workspace_size(M, R, p.split_k);
-  } else {
-    p.shrink_bytes = lora_gemm_workspace_size(M, R, np, 0);
-  }
   if (need_dx) p.gemm_bytes = lora_gemm_workspace_size(M, K, np, 2 * rp);
   size_t at = kCounterBytes;  // ticket counters, never scratch; the steps' partials follow them in turn
-  at = std::max(at, mx_align(std::max(p.shrink_bytes, p.gemm_bytes)));
+  at = std::max(at, mx_align(std::max(kCounterBytes + mx_shrink_part_bytes(M, np, R), p.gemm_bytes)));
   p.part = at;
   at += mx_align(std::max(mx_grad_part_bytes(M, N, R), mx_grad_part_bytes(M, K, R)));
   p.g = at;
@@ -144,10 +136,7 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
     m = 2.f * static_cast<float>(frexp(w_global, &e));
     pow2 = static_cast<float>(ldexp(1.0, e - 1));
   }
-  // B^T first: the shrink may read it before its own predecessor on the stream has
-  // finished, so other launches lie between
-  int rc = transpose(b, ldb, ws + p.bt, np, N, R, R, np, 1, s);
-  if (rc != LORA_OK) return rc;
+  int rc = LORA_OK;
   const void* dyp = dy;
   int64_t ldp = lddy;
   if (N % 8 != 0 || lddy % 8 != 0 || !mx_aligned(dy, 16)) {  // TMA needs 16-byte rows
@@ -172,16 +161,28 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   rc = mx_grad_launch(gr, dtype, s);
   if (rc != LORA_OK) return rc;
 
-  const float gs = scale / m;
-  if (R <= kShrinkMaxRank) {
-    rc = lora_shrink(dyp, ldp, ws + p.bt, np, ws + p.g, 2 * rp, dtype, rp, 1, M, np, R, gs, dtype, p.split_k, ws,
-                     p.shrink_bytes, s);
-  } else {
-    if (rp != R && cudaMemsetAsync(ws + p.g, 0, static_cast<size_t>(M) * 2 * rp * 2, s) != cudaSuccess)
-      return LORA_ERR_CUDA;
-    rc = lora_gemm_ex(dyp, ldp, ws + p.bt, np, nullptr, 0, nullptr, 0, nullptr, ws + p.g, 2 * rp, M, R, np, 0, gs, rp,
-                      dtype, p.shrink_bytes ? ws : nullptr, p.shrink_bytes, s);
+  MxShrinkOperands sh = {};
+  sh.v = dyp;
+  sh.a = b;
+  sh.a_mn = mx_shrink_serves(dyp, ldp, b, ldb);
+  sh.lda = ldb;
+  if (!sh.a_mn) {  // rows of B that TMA cannot read
+    rc = transpose(b, ldb, ws + p.bt, np, N, R, R, np, 1, s);
+    if (rc != LORA_OK) return rc;
+    sh.a = ws + p.bt;
+    sh.lda = np;
   }
+  sh.z = ws + p.g;
+  sh.tickets = ws;
+  sh.part = ws + kCounterBytes;
+  sh.ldv = ldp;
+  sh.ldz = 2 * rp;
+  sh.M = M;
+  sh.K = N;
+  sh.R = R;
+  sh.scale = scale / m;
+  sh.global_scale = 1.f;
+  rc = mx_shrink_launch(sh, -1, dtype, s);
   if (rc != LORA_OK) return rc;
 
   gr.v = x_codes;

@@ -19,9 +19,12 @@
 // TMA (codes in 128-byte swizzled rows, scale chunks as they are stored), warp
 // 1 of the leader copies the stage's scales to TMEM (tcgen05.cp, each CTA from
 // its own shared memory) and issues the MMAs, warps 2..9 the epilogue.
-// TMEM: two 256-column accumulators and two buffers of scales do not fit 512
-// columns, so the accumulators share 48 (mxfp4) or 96 (nvfp4) columns: the
-// epilogue drains those first and only they hold up the next tile's MMAs.
+// TMEM holds a buffer of scales per pipeline stage, so that a stage's full barrier
+// already says that its scale buffer is free: the MMA warp has 512 cycles a stage
+// and every further wait costs it 100 to 200.  Beside those 144 (mxfp4) or 240
+// (nvfp4) columns two 256-column accumulators do not fit: they overlap in as many,
+// the epilogue takes the shared columns to registers first and only that holds up
+// the next tile's MMAs.
 #include <cudaTypedefs.h>
 
 #include <cmath>
@@ -64,7 +67,7 @@ struct MxSmem {
   static constexpr int kBytes = kBarOffset + 256 + 1024;
   // TMEM columns
   static constexpr int kSfCols = 3 * kChunks * 4;
-  static constexpr int kSfBase = 512 - 2 * kSfCols;
+  static constexpr int kSfBase = 512 - kStages * kSfCols;
   static constexpr int kAcc1 = kSfBase - 256;  // accumulator 1; accumulator 0 starts at 0
   static constexpr int kOverlap = 256 - kAcc1;
   static_assert(kOverlap % 16 == 0 && kBytes <= 227 * 1024, "layout");
@@ -284,102 +287,84 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
     }
   } else if (warp == 1) {
     // The whole warp walks the stages, so that descriptors and addresses live in
-    // uniform registers; one elected lane issues.
+    // uniform registers; one elected lane waits and issues.
     if (leader) {
       const bool issuer = elect_one();
       int stage = 0;
       uint32_t phase = 0;
-      int use = 0;  // stages used so far; scale buffer = use & 1
       int local = 0;
-      bool ok = true;
+      bool ok = true, ready = false;
       const uint64_t ad0 = umma_desc_sw128(smem_u32(sm_a));
       const uint64_t bd0 = umma_desc_sw128(smem_u32(sm_b));
       const uint64_t sd0 = mx_desc_scales(smem_u32(sm_sf));
-      // `lag` of the uses so far are not known to be complete, the first of them in
-      // stage done_stage
-      int lag = 0, done_stage = 0;
-      uint32_t done_phase = 0;
-      auto catch_up = [&](int most) {
-        while (lag > most) {
-          if (!warp_wait(&empty[done_stage], done_phase, abort_flag, args.err, kDevErrTimeoutEmpty)) return false;
-          --lag;
-          if (++done_stage == L::kStages) {
-            done_stage = 0;
-            done_phase ^= 1;
-          }
-        }
-        return true;
-      };
       for (int tile = pair; ok && tile < args.num_tiles; tile += npairs, ++local) {
-        if (local > 0 && !warp_wait(acc_free, (local - 1) & 1, abort_flag, args.err, kDevErrTimeoutAccEmpty))
+        if (local > 0 &&
+            !warp_wait(issuer, acc_free, (local - 1) & 1, abort_flag, args.err, kDevErrTimeoutAccEmpty))
           break;
         tc_fence_after();
         const uint32_t d = tmem + ((local & 1) ? L::kAcc1 : 0);
-        for (int kb = 0; kb < args.num_kb; ++kb, ++use) {
-          // the MMAs of two uses ago read the scale buffer that is written next
-          if (!catch_up(1) || !warp_wait(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
+        for (int kb = -args.num_kb; kb < tail_kb; ++kb) {  // base stages below 0, then the tail's
+          if (!ready && !warp_wait(issuer, &full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
             ok = false;
             break;
           }
-          ++lag;
+          if (kb == 0) {  // the tile's base MMAs finish before MMAs of the other kind start
+            const int last = stage == 0 ? L::kStages - 1 : stage - 1;
+            if (!warp_wait(issuer, &empty[last], stage == 0 ? phase ^ 1 : phase, abort_flag, args.err,
+                           kDevErrTimeoutEmpty)) {
+              ok = false;
+              break;
+            }
+          }
           tc_fence_after();
           const uint64_t ad = ad0 + static_cast<uint32_t>(stage * (L::kOpBytes >> 4));
           const uint64_t bd = bd0 + static_cast<uint32_t>(stage * (L::kOpBytes >> 4));
           const uint64_t sd = sd0 + static_cast<uint32_t>(stage * (L::kSfBytes >> 4));
-          const uint32_t sf = tmem + L::kSfBase + (use & 1) * L::kSfCols;
-          const uint32_t sfb = sf + L::kChunks * 4;
-          const int nk = kb == args.num_kb - 1 ? args.last_k64 : 4;
-          if (issuer) {
+          const int next = stage + 1 == L::kStages ? 0 : stage + 1;
+          const uint32_t next_phase = next == 0 ? phase ^ 1 : phase;
+          // asked now, used after the MMAs are issued
+          ready = issuer ? mbar_try_wait(&full[next], next_phase) : true;
+          if (kb < 0) {
+            const uint32_t sf = tmem + L::kSfBase + stage * L::kSfCols;
+            const uint32_t sfb = sf + L::kChunks * 4;
+            const int nk = kb == -1 ? args.last_k64 : 4;
+            if (issuer) {
 #pragma unroll
-            for (int j = 0; j < L::kChunks; ++j) {
-              mx_cp_scales_pair(sf + 4 * j, sd + static_cast<uint64_t>(32 * j));
-              mx_cp_scales_pair(sfb + 8 * j, sd + static_cast<uint64_t>(32 * (L::kChunks + j)));
-              mx_cp_scales_pair(sfb + 8 * j + 4, sd + static_cast<uint64_t>(32 * (2 * L::kChunks + j)));
+              for (int j = 0; j < L::kChunks; ++j) {
+                mx_cp_scales_pair(sf + 4 * j, sd + static_cast<uint64_t>(32 * j));
+                mx_cp_scales_pair(sfb + 8 * j, sd + static_cast<uint64_t>(32 * (L::kChunks + j)));
+                mx_cp_scales_pair(sfb + 8 * j + 4, sd + static_cast<uint64_t>(32 * (2 * L::kChunks + j)));
+              }
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                constexpr bool kMx = FMT == LORA_MXFP4;
+                const int j = kMx ? k >> 1 : k;
+                const uint32_t id = kMx ? static_cast<uint32_t>(k & 1) * 2u : 0u;
+                if (k < nk)
+                  mx_mma_pair<FMT>(d, ad + static_cast<uint64_t>(2 * k), bd + static_cast<uint64_t>(2 * k),
+                                   kIdesc | (id << 4) | (id << 29), sf + 4 * j, sfb + 8 * j,
+                                   (kb > -args.num_kb || k > 0) ? 1u : 0u);
+              }
+              tc_commit_pair(&empty[stage], kBoth);
             }
+          } else {
+            const int t = kb - args.zero_kb;
+            const int c = t >= args.rank_kb ? t - args.rank_kb : t;
+            const int nk = t < 0 ? 1 : c == args.rank_kb - 1 ? args.last_k16 : 4;
+            const int shift = t < 0 ? 15 : t == 0 ? args.dshift - 15 * args.zero_kb : 0;
+            if (issuer) {
+              mx_mma_f16_pair_shift(d, ad, bd, kIdescTail, shift);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              constexpr bool kMx = FMT == LORA_MXFP4;
-              const int j = kMx ? k >> 1 : k;
-              const uint32_t id = kMx ? static_cast<uint32_t>(k & 1) * 2u : 0u;
-              if (k < nk)
-                mx_mma_pair<FMT>(d, ad + static_cast<uint64_t>(2 * k), bd + static_cast<uint64_t>(2 * k),
-                                 kIdesc | (id << 4) | (id << 29), sf + 4 * j, sfb + 8 * j, (kb > 0 || k > 0) ? 1u : 0u);
+              for (int k = 1; k < 4; ++k)
+                if (k < nk)
+                  tc_mma_f16_pair(d, ad + static_cast<uint64_t>(2 * k), bd + static_cast<uint64_t>(2 * k), kIdescTail,
+                                  1u);
+              tc_commit_pair(&empty[stage], kBoth);
             }
-            tc_commit_pair(&empty[stage], kBoth);
           }
-          __syncwarp();
-          if (++stage == L::kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
-        }
-        for (int t = -args.zero_kb; ok && t < 2 * args.rank_kb; ++t, ++use) {
-          // the last base stage's MMAs finish before MMAs of the other kind start
-          if (!catch_up(t == -args.zero_kb ? 0 : 1) ||
-              !warp_wait(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
-            ok = false;
-            break;
-          }
-          ++lag;
-          tc_fence_after();
-          const uint64_t ad = ad0 + static_cast<uint32_t>(stage * (L::kOpBytes >> 4));
-          const uint64_t bd = bd0 + static_cast<uint32_t>(stage * (L::kOpBytes >> 4));
-          const int c = t >= args.rank_kb ? t - args.rank_kb : t;
-          const int nk = t < 0 ? 1 : c == args.rank_kb - 1 ? args.last_k16 : 4;
-          const int shift = t < 0 ? 15 : t == 0 ? args.dshift - 15 * args.zero_kb : 0;
-          if (issuer) {
-            mx_mma_f16_pair_shift(d, ad, bd, kIdescTail, shift);
-#pragma unroll
-            for (int k = 1; k < 4; ++k)
-              if (k < nk)
-                tc_mma_f16_pair(d, ad + static_cast<uint64_t>(2 * k), bd + static_cast<uint64_t>(2 * k), kIdescTail, 1u);
-            tc_commit_pair(&empty[stage], kBoth);
-          }
-          __syncwarp();
-          if (++stage == L::kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
+          ready = __all_sync(0xffffffffu, ready);
+          stage = next;
+          phase = next_phase;
         }
         if (ok && issuer) tc_commit_pair(acc_full, kBoth);
         __syncwarp();
@@ -395,7 +380,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
     for (int tile = pair; tile < args.num_tiles; tile += npairs, ++local) {
       int mt, nt;
       mx_tile_coords(tile, args, mt, nt);
-      if (!warp_wait(acc_full, local & 1, abort_flag, args.err, kDevErrTimeoutAccFull)) break;
+      if (!warp_wait(lane == 0, acc_full, local & 1, abort_flag, args.err, kDevErrTimeoutAccFull)) break;
       tc_fence_after();
       const int row = mt * 256 + static_cast<int>(rank) * 128 + quad * 32 + lane;
       T* out_row = static_cast<T*>(args.out) + static_cast<int64_t>(row) * args.ldo;

@@ -198,8 +198,8 @@ __global__ void __launch_bounds__(kGrThreads, 1)
       uint32_t phase = 0;
       for (int st = step0; st < step1; ++st) {
         const int n = st - step0;
-        if (!mbar_wait_bounded(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull) ||
-            !mbar_wait_bounded(&conv_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag, args.err, kDevErrTimeoutEmpty))
+        if (!warp_wait(lane == 0, &full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull) ||
+            !warp_wait(lane == 0, &conv_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag, args.err, kDevErrTimeoutEmpty))
           break;
         const uint8_t* raw = smem + stage * args.stage_bytes;
         const uint8_t* sc = raw + kGrRawBytes + (lane >> 4) * 512;  // chunk of this lane's 128 columns
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     }
     // epilogue: warps 0..3 of these drain the first accumulator, 4..7 the second
     const int quad = warp & 3, m = cw >> 2;
-    if (mbar_wait_bounded(acc_full, 0, abort_flag, args.err, kDevErrTimeoutAccFull)) {
+    if (warp_wait(lane == 0, acc_full, 0, abort_flag, args.err, kDevErrTimeoutAccFull)) {
       tc_fence_after();
       const int64_t c = col0 + m * 128 + quad * 32 + lane;
       float* dst = args.part + (static_cast<int64_t>(blockIdx.y) * args.C + c) * args.r16;

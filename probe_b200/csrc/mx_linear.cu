@@ -2,12 +2,14 @@
 //
 //   out = q(x) W^T + s (x A^T) B^T + bias
 //
-// q(x): x quantised to W's format; the adapter sees x itself.  Steps: q(x), the
-// rank shrink z = (s / alpha) x A^T as a hi/lo pair (alpha: the fp32 factor that
-// the product's epilogue applies), the block-scaled GEMM with z B^T as its tail.
+// q(x): x quantised to W's format; the adapter sees x itself.  Steps: q(x) and, in
+// the same pass over x, the rank shrink z = (s / alpha) x A^T as a hi/lo pair
+// (alpha: the fp32 factor that the product's epilogue applies); the block-scaled
+// GEMM with z B^T as its tail.  Operands that TMA cannot read (rows not 16-byte
+// aligned) take the quantisation and the split-K shrink as kernels of their own.
 #include <cmath>
 
-#include "mx_linear.h"
+#include "mx_shrink.h"
 
 namespace lora {
 namespace {
@@ -27,6 +29,8 @@ LinearPlan linear_plan(int64_t M, int64_t N, int64_t K, int64_t R, int fmt) {
   LinearPlan p = {};
   size_t at = kCounterBytes;  // never scratch: calls of other shapes find their tickets zero
   if (R > 0) {
+    const size_t fused = kCounterBytes + mx_shrink_part_bytes(M, K, R);
+    if (fused > at) at = mx_align(fused);
     if (R <= kShrinkMaxRank) {
       p.split_k = lora_shrink_pick_split_k(M, K, R);
       p.shrink_bytes = lora_shrink_workspace_size(M, R, p.split_k);
@@ -111,22 +115,44 @@ extern "C" int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, c
       o.alpha = static_cast<float>(alpha);
     }
   }
-  int rc = mx_quantize_launch(x, ldx, ws + p.x_codes, ws + p.x_scales, M, K, fmt, x_global, dtype, s);
+  int rc = LORA_OK;
+  const int64_t rp = r16(R);
+  char* z = z_out != nullptr ? static_cast<char*>(z_out) : ws + p.z;
+  const float zs = scale / o.alpha;
+  if (R > 0 && mx_shrink_serves(x, ldx, a, lda)) {
+    MxShrinkOperands sh = {};
+    sh.v = x;
+    sh.a = a;
+    sh.z = z;
+    sh.codes = ws + p.x_codes;
+    sh.scales = ws + p.x_scales;
+    sh.tickets = ws;
+    sh.part = ws + kCounterBytes;
+    sh.ldv = ldx;
+    sh.lda = lda;
+    sh.ldz = 2 * rp;
+    sh.M = M;
+    sh.K = K;
+    sh.R = R;
+    sh.scale = zs;
+    sh.global_scale = x_global;
+    rc = mx_shrink_launch(sh, fmt, dtype, s);
+  } else {
+    rc = mx_quantize_launch(x, ldx, ws + p.x_codes, ws + p.x_scales, M, K, fmt, x_global, dtype, s);
+    if (rc == LORA_OK && R > 0) {
+      if (R <= kShrinkMaxRank) {
+        rc = lora_shrink(x, ldx, a, lda, z, 2 * rp, dtype, rp, 1, M, K, R, zs, dtype, p.split_k, ws, p.shrink_bytes, s);
+      } else {
+        if (z_out != nullptr && rp != R &&
+            cudaMemsetAsync(z, 0, static_cast<size_t>(M) * 2 * rp * 2, s) != cudaSuccess)
+          return LORA_ERR_CUDA;
+        rc = lora_gemm_ex(x, ldx, a, lda, nullptr, 0, nullptr, 0, nullptr, z, 2 * rp, M, R, K, 0, zs, rp, dtype,
+                          p.shrink_bytes ? ws : nullptr, p.shrink_bytes, s);
+      }
+    }
+  }
   if (rc != LORA_OK) return rc;
   if (R > 0) {
-    const int64_t rp = r16(R);
-    char* z = z_out != nullptr ? static_cast<char*>(z_out) : ws + p.z;
-    const float zs = scale / o.alpha;
-    if (R <= kShrinkMaxRank) {
-      rc = lora_shrink(x, ldx, a, lda, z, 2 * rp, dtype, rp, 1, M, K, R, zs, dtype, p.split_k, ws, p.shrink_bytes, s);
-    } else {
-      if (z_out != nullptr && rp != R &&
-          cudaMemsetAsync(z, 0, static_cast<size_t>(M) * 2 * rp * 2, s) != cudaSuccess)
-        return LORA_ERR_CUDA;
-      rc = lora_gemm_ex(x, ldx, a, lda, nullptr, 0, nullptr, 0, nullptr, z, 2 * rp, M, R, K, 0, zs, rp, dtype,
-                        p.shrink_bytes ? ws : nullptr, p.shrink_bytes, s);
-    }
-    if (rc != LORA_OK) return rc;
     o.z = z;
     o.ldz = 2 * rp;
     o.z_lo = rp;

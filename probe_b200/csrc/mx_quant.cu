@@ -40,81 +40,20 @@ LORA_DEVINL void mx_load16(const T* row, int64_t c, int64_t k, bool vec, uint32_
   }
 }
 
-// Largest magnitude, as the 16-bit pattern without its sign: infinities and
-// NaN compare above every number.
-LORA_DEVINL uint32_t mx_amax16(const uint32_t* w) {
-  uint32_t m = w[0] & 0x7fff7fffu;
-#pragma unroll
-  for (int i = 1; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
-  return max(m & 0xffffu, m >> 16);
-}
-
-template <typename T> LORA_DEVINL float mx_bits16_to_f32(uint32_t b);
-template <> LORA_DEVINL float mx_bits16_to_f32<__nv_bfloat16>(uint32_t b) { return __uint_as_float(b << 16); }
-template <> LORA_DEVINL float mx_bits16_to_f32<__half>(uint32_t b) {
-  return __half2float(__ushort_as_half(static_cast<unsigned short>(b)));
-}
-
 // Scale byte and codes of one thread's 16 elements.
 template <typename T, int FMT>
-LORA_DEVINL uint32_t mx_encode16(const uint32_t* w, float g, float g6, uint32_t* codes) {
-  constexpr uint32_t kInf = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+LORA_DEVINL uint32_t mx_encode16(const uint32_t* w, const MxGlobal& gl, const float* recip, uint32_t* codes) {
   uint32_t top = mx_amax16(w);
   if constexpr (MxFormat<FMT>::kBlock == 32) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  const bool bad = top >= kInf;
-  const float amax = mx_bits16_to_f32<T>(top);
-  uint32_t byte;
-  float v[16];
-  if constexpr (FMT == LORA_NVFP4) {
-    byte = mx_to_e4m3x2(__fdiv_rn(amax, g6), 0.f) & 0xffu;
-    const float unit = mx_e4m3(byte) * g;
-    if (bad || byte == 0) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = 0.f;
-    } else {
-      // Quotients by one divisor: with r the correctly rounded reciprocal, one
-      // residual step makes x r the correctly rounded x / unit (Markstein, 1990).
-      const float r = __frcp_rn(unit);
-      const bool far = amax * r > 1e6f;  // a saturated scale: keep the residual finite
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 x = unpack2<T>(w[i]);
-        float q0 = x.x * r, q1 = x.y * r;
-        if (far) {
-          q0 = fminf(fmaxf(q0, -1e6f), 1e6f);
-          q1 = fminf(fmaxf(q1, -1e6f), 1e6f);
-        }
-        v[2 * i] = fmaf(fmaf(-q0, unit, x.x), r, q0);
-        v[2 * i + 1] = fmaf(fmaf(-q1, unit, x.y), r, q1);
-      }
-    }
-    if (bad) byte = 0x7f;
-  } else {
-    const int e = max(static_cast<int>(__float_as_uint(amax) >> 23) - MxFormat<FMT>::kTop, 0);  // biased by 127
-    byte = bad ? 255u : static_cast<uint32_t>(e);
-    const float inv = bad ? 0.f : __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 x = unpack2<T>(bad ? 0u : w[i]);
-      v[2 * i] = x.x * inv;
-      v[2 * i + 1] = x.y * inv;
-    }
-  }
-  if constexpr (MxFormat<FMT>::kBits == 4) {
-    codes[0] = mx_to_e2m1x8(v);
-    codes[1] = mx_to_e2m1x8(v + 8);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      codes[i] = mx_to_e4m3x2(v[4 * i], v[4 * i + 1]) | (mx_to_e4m3x2(v[4 * i + 2], v[4 * i + 3]) << 16);
-  }
-  return byte;
+  const MxScale<T, FMT> s(top, gl, recip);
+  mx_codes16<T, FMT>(w, s, codes);
+  return s.byte;
 }
 
 template <typename T, int FMT>
 __global__ void __launch_bounds__(kMxThreads)
     mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes,
-                       uint8_t* __restrict__ scales, int64_t M, int64_t K, int64_t Kp, int chunks, float g, float g6,
+                       uint8_t* __restrict__ scales, int64_t M, int64_t K, int64_t Kp, int chunks, MxGlobal gl,
                        bool vec) {
   constexpr int kChunks = kMxTile / MxFormat<FMT>::kBlock / 4;  // scale chunks of this tile
   __shared__ alignas(16) uint8_t sc[kChunks * 512];
@@ -122,6 +61,7 @@ __global__ void __launch_bounds__(kMxThreads)
   const int sub = threadIdx.x >> 3;  // row within a pass
   const int64_t row0 = static_cast<int64_t>(blockIdx.y) * kMxTile;
   const int64_t col = static_cast<int64_t>(blockIdx.x) * kMxTile + seg * 16;
+  __shared__ float recip[FMT == LORA_NVFP4 ? 128 : 1];
   uint32_t w[4][8];
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
@@ -133,11 +73,15 @@ __global__ void __launch_bounds__(kMxThreads)
       for (int i = 0; i < 8; ++i) w[p][i] = 0u;
     }
   }
+  if constexpr (FMT == LORA_NVFP4) {
+    if (threadIdx.x < 128) recip[threadIdx.x] = mx_recip_entry(static_cast<int>(threadIdx.x), gl.g);
+    __syncthreads();
+  }
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     const int64_t row = row0 + 32 * p + sub;
     uint32_t c[4];
-    uint32_t byte = mx_encode16<T, FMT>(w[p], g, g6, c);
+    uint32_t byte = mx_encode16<T, FMT>(w[p], gl, recip, c);
     if (col >= Kp || row >= M) byte = 0;
     if (row < M && col < Kp) {
       if constexpr (MxFormat<FMT>::kBits == 4)
@@ -266,7 +210,7 @@ int quantize_t(const void* x, int64_t ldx, void* codes, void* scales, int64_t M,
   const bool vec = aligned(x, 16) && ldx % 8 == 0;
   mx_quantize_kernel<T, FMT><<<grid, kMxThreads, 0, stream>>>(
       static_cast<const T*>(x), ldx, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), M, K, Kp,
-      static_cast<int>(mx_scale_chunks(K, FMT)), g, 6.0f * g, vec);
+      static_cast<int>(mx_scale_chunks(K, FMT)), mx_global(g), vec);
   return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
 }
 

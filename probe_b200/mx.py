@@ -148,9 +148,7 @@ def _linear(x, weight, bias, a, b, scale, x_global_scale, keep_z, where):
             raise ValueError(f"{where}: a {tuple(a.shape)} / b {tuple(b.shape)} do not match [{r}, {k}] / [{n}, {r}]")
         if r > 256:
             raise ValueError(f"{where}: ranks up to 256, got {r}")
-        a, b = _lib.row_major(a), _aligned_rows(b)
-        if r > 128:
-            x, a = _aligned_rows(x), _aligned_rows(a)
+        x, a, b = _aligned_rows(x), _aligned_rows(a), _aligned_rows(b)
     if bias is not None:
         if bias.shape != (n,) or bias.dtype != dtype:
             raise ValueError(f"{where}: bias must be [{n}] in x's dtype")
