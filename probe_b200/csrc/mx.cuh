@@ -45,6 +45,32 @@ inline bool mx_global_ok(float g, int fmt) {
   return fmt == LORA_NVFP4 ? (g >= 5.4210109e-20f && g <= 1.8446744e19f) : g == 1.0f;  // [2^-64, 2^64]
 }
 
+// Shared-memory accesses by 32-bit address: behind the dynamic buffer's aligned
+// base the compiler only sees generic pointers, whose loads take the global path.
+LORA_DEVINL uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+LORA_DEVINL uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+LORA_DEVINL float lds_f32(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  return v;
+}
+LORA_DEVINL uint32_t lds_u8(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+LORA_DEVINL void sts128(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
 // One lane of a converged warp.
 LORA_DEVINL bool elect_one() {
   uint32_t p;
@@ -155,15 +181,15 @@ struct MxScale {
   uint32_t byte;
   float d, r;
   bool far;
-  // recip: reciprocals of (E4M3 code x g) by code, 128 entries (nvfp4)
-  LORA_DEVINL MxScale(uint32_t top, const MxGlobal& gl, const float* recip) {
+  // recip: shared address of the reciprocals of (E4M3 code x g), 128 entries (nvfp4)
+  LORA_DEVINL MxScale(uint32_t top, const MxGlobal& gl, uint32_t recip) {
     constexpr uint32_t kInf = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
     const bool bad = top >= kInf;
     const float amax = mx_bits16_to_f32<T>(top);
     if constexpr (FMT == LORA_NVFP4) {
       byte = bad ? 0x7fu : mx_to_e4m3x2(mx_div_far(amax, gl.g6, gl.r6), 0.f) & 0xffu;
       d = mx_e4m3(byte) * gl.g;
-      r = recip[byte];  // 0 for a zero or NaN scale
+      r = lds_f32(recip + byte * 4);  // 0 for a zero or NaN scale
       far = amax * r > 1048576.f;
     } else {
       const int e = max(static_cast<int>(__float_as_uint(amax) >> 23) - MxFormat<FMT>::kTop, 0);  // biased by 127

@@ -201,21 +201,22 @@ __global__ void __launch_bounds__(kGrThreads, 1)
         if (!warp_wait(lane == 0, &full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull) ||
             !warp_wait(lane == 0, &conv_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag, args.err, kDevErrTimeoutEmpty))
           break;
-        const uint8_t* raw = smem + stage * args.stage_bytes;
-        const uint8_t* sc = raw + kGrRawBytes + (lane >> 4) * 512;  // chunk of this lane's 128 columns
-        uint8_t* dst = conv + (n & 1) * kGrVBytes + (lane >> 3) * kGrChunkBytes;
+        const uint32_t raw = smem_u32(smem) + stage * args.stage_bytes;
+        // the scale chunk of this lane's 128 columns, its block
+        const uint32_t sc = raw + kGrRawBytes + (lane >> 4) * 512 + ((lane >> 2) & 3);
+        const uint32_t dst = smem_u32(conv) + (n & 1) * kGrVBytes + (lane >> 3) * kGrChunkBytes;
 #pragma unroll
         for (int i = 0; i < kGrTok / kGrConvWarps; ++i) {
           const int t = cw * (kGrTok / kGrConvWarps) + i;
           const int tr = (st * kGrTok + t) & 127;  // row within the scale chunk
-          const uint2 w = *reinterpret_cast<const uint2*>(raw + t * kGrCols + lane * 8);
-          const uint32_t s = sc[(tr & 31) * 16 + (tr >> 5) * 4 + ((lane >> 2) & 3)];
+          const uint2 w = lds64(raw + t * kGrCols + lane * 8);
+          const uint32_t s = lds_u8(sc + (tr & 31) * 16 + (tr >> 5) * 4);
           uint4 o;
           o.x = gr_decode2<T>(__byte_perm(w.x, 0, 0x1404), s);
           o.y = gr_decode2<T>(__byte_perm(w.x, 0, 0x3424), s);
           o.z = gr_decode2<T>(__byte_perm(w.y, 0, 0x1404), s);
           o.w = gr_decode2<T>(__byte_perm(w.y, 0, 0x3424), s);
-          *reinterpret_cast<uint4*>(dst + t * 128 + (((lane & 7) ^ (t & 7)) << 4)) = o;
+          sts128(dst + t * 128 + (((lane & 7) ^ (t & 7)) << 4), o);
         }
         fence_proxy_async_smem();
         __syncwarp();

@@ -42,7 +42,7 @@ LORA_DEVINL void mx_load16(const T* row, int64_t c, int64_t k, bool vec, uint32_
 
 // Scale byte and codes of one thread's 16 elements.
 template <typename T, int FMT>
-LORA_DEVINL uint32_t mx_encode16(const uint32_t* w, const MxGlobal& gl, const float* recip, uint32_t* codes) {
+LORA_DEVINL uint32_t mx_encode16(const uint32_t* w, const MxGlobal& gl, uint32_t recip, uint32_t* codes) {
   uint32_t top = mx_amax16(w);
   if constexpr (MxFormat<FMT>::kBlock == 32) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   const MxScale<T, FMT> s(top, gl, recip);
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kMxThreads)
   for (int p = 0; p < 4; ++p) {
     const int64_t row = row0 + 32 * p + sub;
     uint32_t c[4];
-    uint32_t byte = mx_encode16<T, FMT>(w[p], gl, recip, c);
+    uint32_t byte = mx_encode16<T, FMT>(w[p], gl, smem_u32(recip), c);
     if (col >= Kp || row >= M) byte = 0;
     if (row < M && col < Kp) {
       if constexpr (MxFormat<FMT>::kBits == 4)

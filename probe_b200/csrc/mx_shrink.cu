@@ -6,12 +6,12 @@
 // A is [R, K] (rows along K, an adapter's down projection) or, for gradients,
 // [K, R] (an up projection, multiplied from the other side); tcgen05 takes either
 // as the N operand, K-major or MN-major, with 128 tokens as M.  While the MMAs of
-// a 128 x 128 tile of v run, eight warps quantise the same tile from shared memory
+// a 128 x 128 tile (x 64 for ranks above 64, whose adapter tile is larger) of v run, eight warps quantise the same tile from shared memory
 // (two lanes a row: conflict-free with the 128-byte swizzle, whole 32-byte sectors
 // of codes out).
 //
 // Bound: HBM (v once, codes out), the adapter's tile through L2 for large ranks.
-// Work split: the (token block, 128-column chunk) pairs in one sequence, cut into
+// Work split: the (token block, chunk of columns) pairs in one sequence, cut into
 // equal runs, one per SM, so that any M fills the machine; a token block cut by a
 // run boundary leaves fp32 partials that its last contributor (a ticket) adds in
 // run order, so the result does not depend on timing.
@@ -22,9 +22,9 @@
 namespace lora {
 namespace {
 
-constexpr int kShWorkers = 8;
+constexpr int kShWorkers = 16;  // two groups of eight, taking stages in turn
 constexpr int kShThreads = 64 + 32 * kShWorkers;
-constexpr int kShXBytes = 128 * 128 * 2;  // 128 tokens x 128 columns
+constexpr int kShBoxBytes = 128 * 128;  // 128 tokens x 64 columns
 constexpr int kShSmemMax = 224 * 1024;
 constexpr int kNoFormat = -1;
 
@@ -39,13 +39,16 @@ struct ShArgs {
   int* tickets;  // kShWorkers per CTA, zero between calls
   int* err;
   int64_t M, K, Kp, ldz;
-  int64_t chunks_total;
+  int chunks_total;
   int kc, r16, a_boxes, a_box_bytes, stages, stage_bytes, gb;
   float scale;
   MxGlobal gl;
 };
 
-LORA_DEVINL int64_t sh_start(const ShArgs& a, int64_t cta) { return a.chunks_total * cta / gridDim.x; }
+// First chunk of a run (chunks x runs fit 31 bits).
+LORA_DEVINL int sh_start(const ShArgs& a, int cta) {
+  return static_cast<int>(static_cast<uint32_t>(a.chunks_total) * static_cast<uint32_t>(cta) / gridDim.x);
+}
 
 LORA_DEVINL uint64_t sh_desc_mn(uint32_t addr, uint32_t lbo) {
   uint64_t d = 0;
@@ -75,7 +78,7 @@ LORA_DEVINL void sh_store_pair(T* z, int r16, const float* v) {
   d[1] = make_uint4(l[4], l[5], l[6], l[7]);
 }
 
-template <typename T, int FMT, bool AMN>
+template <typename T, int FMT, bool AMN, int KB>
 __global__ void __launch_bounds__(kShThreads, 1)
     mx_shrink_kernel(const __grid_constant__ ShMaps maps, const ShArgs args) {
   extern __shared__ uint8_t smem_raw[];
@@ -90,14 +93,14 @@ __global__ void __launch_bounds__(kShThreads, 1)
   float* recip = reinterpret_cast<float*>(tmem_slot + 4);  // 128 entries (nvfp4)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t c_begin = sh_start(args, blockIdx.x), c_end = sh_start(args, blockIdx.x + 1);
+  const int c_begin = sh_start(args, blockIdx.x), c_end = sh_start(args, blockIdx.x + 1);
   const uint32_t need = 2 * args.r16;
   const uint32_t tmem_cols = need <= 32 ? 32u : need <= 64 ? 64u : need <= 128 ? 128u : need <= 256 ? 256u : 512u;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < args.stages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], FMT == kNoFormat ? 1 : 1 + kShWorkers);
+      mbar_init(&empty[s], FMT == kNoFormat ? 1 : 1 + 8);  // the MMAs, a group of workers
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&acc_full[s], 1);
@@ -127,17 +130,17 @@ __global__ void __launch_bounds__(kShThreads, 1)
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
-      const uint32_t bytes = kShXBytes + args.a_boxes * args.a_box_bytes;
-      int tb = static_cast<int>(c_begin / args.kc), kc = static_cast<int>(c_begin - static_cast<int64_t>(tb) * args.kc);
-      for (int64_t c = c_begin; c < c_end; ++c) {
+      const uint32_t bytes = KB * kShBoxBytes + args.a_boxes * args.a_box_bytes;
+      int tb = c_begin / args.kc, kc = c_begin - tb * args.kc;
+      for (int c = c_begin; c < c_end; ++c) {
         if (!mbar_wait_bounded(&empty[stage], phase ^ 1, abort_flag, args.err, kDevErrTimeoutEmpty)) break;
         uint8_t* base = smem + stage * args.stage_bytes;
         mbar_arrive_expect_tx(&full[stage], bytes);
-        for (int b = 0; b < 2; ++b)
-          tma_load_2d(&maps.v, base + b * (kShXBytes / 2), &full[stage], kc * 128 + b * 64, tb * 128);
+        for (int b = 0; b < KB; ++b)
+          tma_load_2d(&maps.v, base + b * kShBoxBytes, &full[stage], (kc * KB + b) * 64, tb * 128);
         for (int b = 0; b < args.a_boxes; ++b)
-          tma_load_2d(&maps.a, base + kShXBytes + b * args.a_box_bytes, &full[stage], AMN ? b * 64 : kc * 128 + b * 64,
-                      AMN ? kc * 128 : 0);
+          tma_load_2d(&maps.a, base + KB * kShBoxBytes + b * args.a_box_bytes, &full[stage],
+                      AMN ? b * 64 : (kc * KB + b) * 64, AMN ? kc * KB * 64 : 0);
         if (++kc == args.kc) {
           kc = 0;
           ++tb;
@@ -155,8 +158,8 @@ __global__ void __launch_bounds__(kShThreads, 1)
       int stage = 0, seg = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int64_t c = c_begin; ok && c < c_end; ++seg) {
-        const int64_t seg_end = min(c_end, (c / args.kc + 1) * args.kc);
+      for (int c = c_begin; ok && c < c_end; ++seg) {
+        const int seg_end = min(c_end, (c / args.kc + 1) * args.kc);
         if (!mbar_wait_bounded(&acc_empty[seg & 1], ((seg >> 1) & 1) ^ 1, abort_flag, args.err, kDevErrTimeoutAccEmpty))
           break;
         tc_fence_after();
@@ -168,10 +171,10 @@ __global__ void __launch_bounds__(kShThreads, 1)
           }
           tc_fence_after();
           const uint32_t xb = smem_u32(smem + stage * args.stage_bytes);
-          const uint32_t ab = xb + kShXBytes;
+          const uint32_t ab = xb + KB * kShBoxBytes;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint64_t xd = umma_desc_sw128(xb + (k >> 2) * (kShXBytes / 2)) + static_cast<uint64_t>(2 * (k & 3));
+          for (int k = 0; k < 4 * KB; ++k) {
+            const uint64_t xd = umma_desc_sw128(xb + (k >> 2) * kShBoxBytes) + static_cast<uint64_t>(2 * (k & 3));
             const uint64_t ad = AMN ? sh_desc_mn(ab + k * 2048, args.a_box_bytes)
                                     : umma_desc_sw128(ab + (k >> 2) * args.a_box_bytes) + static_cast<uint64_t>(2 * (k & 3));
             tc_mma_f16(d, xd, ad, idesc, (!first || k > 0) ? 1u : 0u);
@@ -186,73 +189,80 @@ __global__ void __launch_bounds__(kShThreads, 1)
       }
     }
   } else {
-    const int w = warp - 2, quad = warp & 3, half = w >> 2;
+    const int w = warp - 2, quad = warp & 3, part = w >> 2;
+    const uint32_t recip_addr = smem_u32(recip), smem_addr = smem_u32(smem);
     int stage = 0, seg = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int64_t c = c_begin; ok && c < c_end; ++seg) {
-      const int64_t tb = c / args.kc;
-      const int64_t seg_begin = c, seg_end = min(c_end, (tb + 1) * args.kc);
+    for (int c = c_begin; ok && c < c_end; ++seg) {
+      const int tb = c / args.kc;
+      const int seg_begin = c, seg_end = min(c_end, (tb + 1) * args.kc);
       if constexpr (FMT != kNoFormat) {
-        // rows 16 w .. 16 w + 15 of the block, 32 columns a lane
-        const int r = 16 * w + (lane >> 1);
-        const int64_t row = tb * 128 + r;
-        uint32_t* sc = reinterpret_cast<uint32_t*>(args.scales + tb * args.gb * 512 + (r & 31) * 16 + (r >> 5) * 4);
+        // rows 16 (w % 8) .. + 15 of the block, 32 columns a lane
+        const int r = 16 * (w & 7) + (lane >> 1);
+        const int64_t row = static_cast<int64_t>(tb) * 128 + r;
+        uint8_t* sc = args.scales + static_cast<int64_t>(tb) * args.gb * 512 + (r & 31) * 16 + (r >> 5) * 4;
         for (; c < seg_end; ++c) {
-          const int kc = static_cast<int>(c - tb * args.kc);
-          if (!warp_wait(lane == 0, &full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
-            ok = false;
-            break;
-          }
-          const uint8_t* xs = smem + stage * args.stage_bytes + r * 128;
-          uint32_t x[2][16];
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint4 q = *reinterpret_cast<const uint4*>(xs + b * (kShXBytes / 2) +
-                                                              ((((lane & 1) * 4 + i) ^ (r & 7)) << 4));
-              x[b][4 * i] = q.x, x[b][4 * i + 1] = q.y, x[b][4 * i + 2] = q.z, x[b][4 * i + 3] = q.w;
+          const int kc = c - tb * args.kc;
+          if ((w >> 3) == ((c - c_begin) & 1)) {
+            if (!warp_wait(lane == 0, &full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
+              ok = false;
+              break;
             }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&empty[stage]);
-          uint32_t bytes = 0;  // scale bytes of this lane, in block order
+            const uint32_t xs = smem_addr + stage * args.stage_bytes + r * 128;
+            uint32_t x[KB][16];
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const int64_t col = static_cast<int64_t>(kc) * 128 + b * 64 + (lane & 1) * 32;
-            uint32_t cd[8];
-            const uint32_t t0 = mx_amax16(x[b]), t1 = mx_amax16(x[b] + 8);
-            if constexpr (FMT == LORA_NVFP4) {
-              const MxScale<T, FMT> s0(t0, args.gl, recip), s1(t1, args.gl, recip);
-              mx_codes16<T, FMT>(x[b], s0, cd);
-              mx_codes16<T, FMT>(x[b] + 8, s1, cd + 2);
-              bytes |= (s0.byte | (s1.byte << 8)) << (16 * b);
-            } else {
-              const MxScale<T, FMT> s(max(t0, t1), args.gl, recip);
-              mx_codes16<T, FMT>(x[b], s, cd);
-              mx_codes16<T, FMT>(x[b] + 8, s, cd + (MxFormat<FMT>::kBits == 4 ? 2 : 4));
-              bytes |= s.byte << (16 * b);
-            }
-            if (row < args.M && col < args.Kp) {
-              if constexpr (MxFormat<FMT>::kBits == 4) {
-                *reinterpret_cast<uint4*>(args.codes + row * (args.Kp >> 1) + (col >> 1)) =
-                    make_uint4(cd[0], cd[1], cd[2], cd[3]);
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint4 q = lds128(xs + b * kShBoxBytes + ((((lane & 1) * 4 + i) ^ (r & 7)) << 4));
+                x[b][4 * i] = q.x, x[b][4 * i + 1] = q.y, x[b][4 * i + 2] = q.z, x[b][4 * i + 3] = q.w;
+              }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[stage]);
+            uint32_t bytes = 0;  // scale bytes of this lane, in block order
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+              const int64_t col = static_cast<int64_t>(kc * KB + b) * 64 + (lane & 1) * 32;
+              uint32_t cd[8];
+              const uint32_t t0 = mx_amax16(x[b]), t1 = mx_amax16(x[b] + 8);
+              if constexpr (FMT == LORA_NVFP4) {
+                const MxScale<T, FMT> s0(t0, args.gl, recip_addr), s1(t1, args.gl, recip_addr);
+                mx_codes16<T, FMT>(x[b], s0, cd);
+                mx_codes16<T, FMT>(x[b] + 8, s1, cd + 2);
+                bytes |= (s0.byte | (s1.byte << 8)) << (16 * b);
               } else {
-                uint4* d = reinterpret_cast<uint4*>(args.codes + row * args.Kp + col);
-                d[0] = make_uint4(cd[0], cd[1], cd[2], cd[3]);
-                d[1] = make_uint4(cd[4], cd[5], cd[6], cd[7]);
+                const MxScale<T, FMT> s(max(t0, t1), args.gl, recip_addr);
+                mx_codes16<T, FMT>(x[b], s, cd);
+                mx_codes16<T, FMT>(x[b] + 8, s, cd + (MxFormat<FMT>::kBits == 4 ? 2 : 4));
+                bytes |= s.byte << (16 * b);
+              }
+              if (row < args.M && col < args.Kp) {
+                if constexpr (MxFormat<FMT>::kBits == 4) {
+                  *reinterpret_cast<uint4*>(args.codes + row * (args.Kp >> 1) + (col >> 1)) =
+                      make_uint4(cd[0], cd[1], cd[2], cd[3]);
+                } else {
+                  uint4* d = reinterpret_cast<uint4*>(args.codes + row * args.Kp + col);
+                  d[0] = make_uint4(cd[0], cd[1], cd[2], cd[3]);
+                  d[1] = make_uint4(cd[4], cd[5], cd[6], cd[7]);
+                }
               }
             }
-          }
-          const uint32_t other = __shfl_xor_sync(0xffffffffu, bytes, 1);
-          if constexpr (FMT == LORA_NVFP4) {
-            // blocks 0, 1 of a 64-column half are the even lane's, 2, 3 the odd one's;
-            // the even lane stores the first half's chunk, the odd one the second's
-            const uint32_t word = (lane & 1) ? (other >> 16) | (bytes & 0xffff0000u) : (bytes & 0xffffu) | (other << 16);
-            const int chunk = 2 * kc + (lane & 1);
-            if (chunk < args.gb) sc[chunk * 128] = word;
-          } else if ((lane & 1) == 0) {
-            sc[kc * 128] = bytes | (other << 8);
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, bytes, 1);
+            if constexpr (FMT == LORA_NVFP4) {
+              // blocks 0, 1 of 64 columns (a chunk of scales) are the even lane's, 2, 3
+              // the odd one's; the even lane stores the first chunk, the odd one a second
+              const uint32_t word =
+                  (lane & 1) ? (other >> 16) | (bytes & 0xffff0000u) : (bytes & 0xffffu) | (other << 16);
+              const int chunk = KB * kc + (lane & 1);
+              if ((lane & 1) < KB && chunk < args.gb) *reinterpret_cast<uint32_t*>(sc + chunk * 512) = word;
+            } else if ((lane & 1) == 0) {
+              const uint32_t word = bytes | (other << 8);
+              if constexpr (KB == 2)
+                *reinterpret_cast<uint32_t*>(sc + kc * 512) = word;
+              else
+                *reinterpret_cast<uint16_t*>(sc + (kc >> 1) * 512 + (kc & 1) * 2) = static_cast<uint16_t>(word);
+            }
           }
           if (++stage == args.stages) {
             stage = 0;
@@ -262,40 +272,43 @@ __global__ void __launch_bounds__(kShThreads, 1)
         if (!ok) break;
       }
       c = seg_end;
-      // ---- the block's sum (or this run's part of it)
+      // ---- the block's sum (or this run's part of it); a warp takes its 32 rows and
+      // every fourth group of 16 columns
       if (!warp_wait(lane == 0, &acc_full[seg & 1], (seg >> 1) & 1, abort_flag, args.err, kDevErrTimeoutAccFull)) break;
       tc_fence_after();
-      const int64_t row = tb * 128 + quad * 32 + lane;
+      const int64_t row = static_cast<int64_t>(tb) * 128 + quad * 32 + lane;
       const bool whole = seg_begin == tb * args.kc && seg_end == (tb + 1) * args.kc;
       T* zrow = static_cast<T*>(args.z) + row * args.ldz;
-      float* mine = args.part +
-                    ((static_cast<int64_t>(blockIdx.x) * 2 + (seg_begin == c_begin ? 0 : 1)) * 128 + quad * 32 + lane) *
-                        args.r16;
-      for (int j = half * 16; j < args.r16; j += 32) {
+      float* slot = args.part + (static_cast<int64_t>(blockIdx.x) * 2 + (seg_begin == c_begin ? 0 : 1)) * 128 * args.r16 +
+                    (quad * 32 + lane) * args.r16;
+      for (int j = part * 16; j < args.r16; j += 64) {
         uint32_t u[16];
         tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + (seg & 1) * args.r16 + j, u);
         tmem_wait_ld();
+        if (row >= args.M) continue;
         if (whole) {
           float v[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(u[e]) * args.scale;
-          if (row < args.M) sh_store_pair<T>(zrow + j, args.r16, v);
+          sh_store_pair<T>(zrow + j, args.r16, v);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            reinterpret_cast<uint4*>(mine + j)[e] = make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
+            reinterpret_cast<uint4*>(slot + j)[e] = make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
         }
       }
-      tc_fence_before();
       __syncwarp();
+      tc_fence_before();
       if (lane == 0) mbar_arrive(&acc_empty[seg & 1]);
-      if (!whole) {
+      if (!whole && part * 16 < args.r16) {
         // first and last run with a chunk of this block
-        int64_t j0 = tb * args.kc * gridDim.x / args.chunks_total;
-        while (sh_start(args, j0 + 1) <= tb * args.kc) ++j0;
-        while (sh_start(args, j0) > tb * args.kc) --j0;
-        int64_t j1 = blockIdx.x;
-        while (sh_start(args, j1 + 1) < (tb + 1) * args.kc) ++j1;
+        const int first_chunk = tb * args.kc, end_chunk = first_chunk + args.kc;
+        int j0 = static_cast<int>(static_cast<int64_t>(first_chunk) * gridDim.x / args.chunks_total);
+        while (sh_start(args, j0 + 1) <= first_chunk) ++j0;
+        while (sh_start(args, j0) > first_chunk) --j0;
+        int j1 = static_cast<int>(static_cast<int64_t>(end_chunk - 1) * gridDim.x / args.chunks_total);
+        while (sh_start(args, j1 + 1) < end_chunk) ++j1;
+        while (sh_start(args, j1) >= end_chunk) --j1;
         // each warp has a ticket of its own for its rows and columns; j0 is the first
         // run of no other cut block
         __threadfence();
@@ -303,30 +316,44 @@ __global__ void __launch_bounds__(kShThreads, 1)
         int last = 0;
         if (lane == 0) {
           int* ticket = args.tickets + j0 * kShWorkers + w;
-          last = atomicAdd(ticket, 1) == static_cast<int>(j1 - j0);
+          last = atomicAdd(ticket, 1) == j1 - j0;
           if (last) *ticket = 0;
         }
         if (__shfl_sync(0xffffffffu, last, 0)) {
           __threadfence();
-          for (int j = half * 16; j < args.r16; j += 32) {
-            float v[16];
+          // run j0's part lies in its last slot unless the run starts with this block;
+          // every later run starts inside it
+          const int slot0 = sh_start(args, j0) >= first_chunk ? 0 : 1;
+          const float* base = args.part + (quad * 32 + lane) * args.r16;
+          const int64_t pitch = static_cast<int64_t>(2 * 128) * args.r16;
+          if (row < args.M)
+            for (int j = part * 16; j < args.r16; j += 64) {
+              float v[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = 0.f;
-            for (int64_t i = j0; i <= j1; ++i) {
-              // the block is run i's first one unless the run starts in an earlier block
-              const int slot = sh_start(args, i) / args.kc == tb ? 0 : 1;
-              const float4* p = reinterpret_cast<const float4*>(
-                  args.part + ((i * 2 + slot) * 128 + quad * 32 + lane) * args.r16 + j);
+              for (int h = 0; h < 2; ++h) {  // 8 columns at a time, four runs' loads in flight
+                float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                for (int i = j0; i <= j1; i += 4) {
+                  float4 q[4][2];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float4 q = __ldcg(p + e);
-                v[4 * e] += q.x, v[4 * e + 1] += q.y, v[4 * e + 2] += q.z, v[4 * e + 3] += q.w;
+                  for (int n = 0; n < 4; ++n)
+                    if (i + n <= j1) {
+                      const float4* p = reinterpret_cast<const float4*>(
+                          base + (i + n) * pitch + (i + n == j0 && slot0 ? 128 * args.r16 : 0) + j + 8 * h);
+                      q[n][0] = __ldcg(p);
+                      q[n][1] = __ldcg(p + 1);
+                    }
+#pragma unroll
+                  for (int n = 0; n < 4; ++n)
+                    if (i + n <= j1) {
+                      acc[0] += q[n][0].x, acc[1] += q[n][0].y, acc[2] += q[n][0].z, acc[3] += q[n][0].w;
+                      acc[4] += q[n][1].x, acc[5] += q[n][1].y, acc[6] += q[n][1].z, acc[7] += q[n][1].w;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[8 * h + e] = acc[e] * args.scale;
               }
+              sh_store_pair<T>(zrow + j, args.r16, v);
             }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] *= args.scale;
-            if (row < args.M) sh_store_pair<T>(zrow + j, args.r16, v);
-          }
         }
       }
     }
@@ -339,15 +366,18 @@ __global__ void __launch_bounds__(kShThreads, 1)
   }
 }
 
+// 64-column boxes a chunk: the adapter's part of a stage grows with the rank.
+int shrink_boxes(int64_t R) { return R > 64 ? 1 : 2; }
+
 // Runs: one per SM, but no shorter than two chunks.
-int shrink_ctas(int64_t M, int64_t K) {
+int shrink_ctas(int64_t M, int64_t K, int64_t R) {
   const int dev = current_device();
   const int sms = dev >= 0 ? device_info(dev).num_sms : 148;
-  const int64_t total = (M + 127) / 128 * ((K + 127) / 128);
+  const int64_t total = (M + 127) / 128 * ((K + 64 * shrink_boxes(R) - 1) / (64 * shrink_boxes(R)));
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms, total / 2)));
 }
 
-template <typename T, int FMT, bool AMN>
+template <typename T, int FMT, bool AMN, int KB>
 int launch_shrink(const MxShrinkOperands& o, cudaStream_t stream) {
   const int dev = current_device();
   if (dev < 0) return LORA_ERR_DEVICE;
@@ -355,10 +385,10 @@ int launch_shrink(const MxShrinkOperands& o, cudaStream_t stream) {
   ShMaps maps;
   ShArgs a;
   a.r16 = static_cast<int>((o.R + 15) / 16 * 16);
-  a.a_boxes = AMN ? (a.r16 + 63) / 64 : 2;
-  a.a_box_bytes = AMN ? 128 * 128 : a.r16 * 128;
+  a.a_boxes = AMN ? (a.r16 + 63) / 64 : KB;
+  a.a_box_bytes = AMN ? KB * 64 * 128 : a.r16 * 128;
   if (!mx_encode_map(&maps.v, o.v, 2, o.K, o.M, o.ldv * 2, 64, 128, true)) return LORA_ERR_CUDA;
-  if (AMN ? !mx_encode_map(&maps.a, o.a, 2, o.R, o.K, o.lda * 2, 64, 128, true)
+  if (AMN ? !mx_encode_map(&maps.a, o.a, 2, o.R, o.K, o.lda * 2, 64, KB * 64, true)
           : !mx_encode_map(&maps.a, o.a, 2, o.K, o.R, o.lda * 2, 64, a.r16, true))
     return LORA_ERR_CUDA;
   a.z = o.z;
@@ -371,15 +401,15 @@ int launch_shrink(const MxShrinkOperands& o, cudaStream_t stream) {
   a.K = o.K;
   a.Kp = mx_padded_k(o.K);
   a.ldz = o.ldz;
-  a.kc = static_cast<int>((o.K + 127) / 128);
-  a.chunks_total = (o.M + 127) / 128 * a.kc;
-  a.stage_bytes = kShXBytes + a.a_boxes * a.a_box_bytes;
+  a.kc = static_cast<int>((o.K + 64 * KB - 1) / (64 * KB));
+  a.chunks_total = static_cast<int>((o.M + 127) / 128 * a.kc);
+  a.stage_bytes = KB * kShBoxBytes + a.a_boxes * a.a_box_bytes;
   a.gb = FMT == kNoFormat ? 0 : static_cast<int>(mx_scale_chunks(o.K, FMT == kNoFormat ? 0 : FMT));
   a.scale = o.scale;
   a.gl = mx_global(o.global_scale);
   constexpr int kFixed = 1024 + 1024;  // alignment, barriers and reciprocals
-  a.stages = std::min(6, (kShSmemMax - kFixed) / a.stage_bytes);
-  auto kernel = mx_shrink_kernel<T, FMT, AMN>;
+  a.stages = std::min(8, (kShSmemMax - kFixed) / a.stage_bytes);
+  auto kernel = mx_shrink_kernel<T, FMT, AMN, KB>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
   std::call_once(once[dev], [&] {
@@ -387,21 +417,22 @@ int launch_shrink(const MxShrinkOperands& o, cudaStream_t stream) {
   });
   if (attr_err[dev] != cudaSuccess) return LORA_ERR_CUDA;
   const size_t smem = static_cast<size_t>(a.stages) * a.stage_bytes + kFixed;
-  kernel<<<shrink_ctas(o.M, o.K), kShThreads, smem, stream>>>(maps, a);
+  kernel<<<shrink_ctas(o.M, o.K, o.R), kShThreads, smem, stream>>>(maps, a);
   return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
 }
 
-template <typename T>
+template <typename T, int KB>
 int dispatch(const MxShrinkOperands& o, int fmt, cudaStream_t s) {
-  if (fmt == kNoFormat) return o.a_mn ? launch_shrink<T, kNoFormat, true>(o, s) : launch_shrink<T, kNoFormat, false>(o, s);
-  if (fmt == LORA_MXFP4) return launch_shrink<T, LORA_MXFP4, false>(o, s);
-  return launch_shrink<T, LORA_NVFP4, false>(o, s);
+  if (fmt == kNoFormat)
+    return o.a_mn ? launch_shrink<T, kNoFormat, true, KB>(o, s) : launch_shrink<T, kNoFormat, false, KB>(o, s);
+  if (fmt == LORA_MXFP4) return launch_shrink<T, LORA_MXFP4, false, KB>(o, s);
+  return launch_shrink<T, LORA_NVFP4, false, KB>(o, s);
 }
 
 }  // namespace
 
 size_t mx_shrink_part_bytes(int64_t M, int64_t K, int64_t R) {
-  return static_cast<size_t>(shrink_ctas(M, K)) * 2 * 128 * ((R + 15) / 16 * 16) * sizeof(float);
+  return static_cast<size_t>(shrink_ctas(M, K, R)) * 2 * 128 * ((R + 15) / 16 * 16) * sizeof(float);
 }
 
 bool mx_shrink_serves(const void* v, int64_t ldv, const void* a, int64_t lda) {
@@ -409,7 +440,9 @@ bool mx_shrink_serves(const void* v, int64_t ldv, const void* a, int64_t lda) {
 }
 
 int mx_shrink_launch(const MxShrinkOperands& o, int fmt, int dtype, cudaStream_t stream) {
-  return dtype == LORA_BF16 ? dispatch<__nv_bfloat16>(o, fmt, stream) : dispatch<__half>(o, fmt, stream);
+  if (shrink_boxes(o.R) == 1)
+    return dtype == LORA_BF16 ? dispatch<__nv_bfloat16, 1>(o, fmt, stream) : dispatch<__half, 1>(o, fmt, stream);
+  return dtype == LORA_BF16 ? dispatch<__nv_bfloat16, 2>(o, fmt, stream) : dispatch<__half, 2>(o, fmt, stream);
 }
 
 }  // namespace lora
