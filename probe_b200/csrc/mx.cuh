@@ -71,20 +71,19 @@ LORA_DEVINL void sts128(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// One lane of a converged warp.
+// One lane of a converged warp.  Asked anew in front of each block that one lane
+// executes, never kept: the code generator may repeat the election where a kept
+// answer is used, and in diverged code that elects several lanes.
 LORA_DEVINL bool elect_one() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p != 0;
 }
 
-// mbar_wait_bounded on behalf of a whole warp: the lane that passes mine = true
-// waits (32 lanes polling one barrier are served one after another, ~200 cycles),
-// every lane gets its answer.
-LORA_DEVINL bool warp_wait(bool mine, uint64_t* bar, uint32_t parity, volatile int* abort, int* err, int code) {
-  bool ok = true;
-  if (mine) ok = mbar_wait_bounded(bar, parity, abort, err, code);
-  ok = __all_sync(0xffffffffu, ok);
+// mbar_wait_bounded by a whole warp: every lane waits for itself (an elected lane
+// and a broadcast measured slower), every lane gets the same answer.
+LORA_DEVINL bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err, int code) {
+  const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort, err, code));
   __syncwarp();
   return ok;
 }

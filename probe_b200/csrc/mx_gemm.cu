@@ -289,7 +289,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
     // The whole warp walks the stages, so that descriptors and addresses live in
     // uniform registers; one elected lane waits and issues.
     if (leader) {
-      const bool issuer = elect_one();
       int stage = 0;
       uint32_t phase = 0;
       int local = 0;
@@ -299,18 +298,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
       const uint64_t sd0 = mx_desc_scales(smem_u32(sm_sf));
       for (int tile = pair; ok && tile < args.num_tiles; tile += npairs, ++local) {
         if (local > 0 &&
-            !warp_wait(issuer, acc_free, (local - 1) & 1, abort_flag, args.err, kDevErrTimeoutAccEmpty))
+            !warp_wait(acc_free, (local - 1) & 1, abort_flag, args.err, kDevErrTimeoutAccEmpty))
           break;
         tc_fence_after();
         const uint32_t d = tmem + ((local & 1) ? L::kAcc1 : 0);
         for (int kb = -args.num_kb; kb < tail_kb; ++kb) {  // base stages below 0, then the tail's
-          if (!ready && !warp_wait(issuer, &full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
+          if (!ready && !warp_wait(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
             ok = false;
             break;
           }
           if (kb == 0) {  // the tile's base MMAs finish before MMAs of the other kind start
             const int last = stage == 0 ? L::kStages - 1 : stage - 1;
-            if (!warp_wait(issuer, &empty[last], stage == 0 ? phase ^ 1 : phase, abort_flag, args.err,
+            if (!warp_wait(&empty[last], stage == 0 ? phase ^ 1 : phase, abort_flag, args.err,
                            kDevErrTimeoutEmpty)) {
               ok = false;
               break;
@@ -323,12 +322,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
           const int next = stage + 1 == L::kStages ? 0 : stage + 1;
           const uint32_t next_phase = next == 0 ? phase ^ 1 : phase;
           // asked now, used after the MMAs are issued
-          ready = issuer ? mbar_try_wait(&full[next], next_phase) : true;
+          ready = mbar_try_wait(&full[next], next_phase);
           if (kb < 0) {
             const uint32_t sf = tmem + L::kSfBase + stage * L::kSfCols;
             const uint32_t sfb = sf + L::kChunks * 4;
             const int nk = kb == -1 ? args.last_k64 : 4;
-            if (issuer) {
+            if (elect_one()) {
 #pragma unroll
               for (int j = 0; j < L::kChunks; ++j) {
                 mx_cp_scales_pair(sf + 4 * j, sd + static_cast<uint64_t>(32 * j));
@@ -352,7 +351,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
             const int c = t >= args.rank_kb ? t - args.rank_kb : t;
             const int nk = t < 0 ? 1 : c == args.rank_kb - 1 ? args.last_k16 : 4;
             const int shift = t < 0 ? 15 : t == 0 ? args.dshift - 15 * args.zero_kb : 0;
-            if (issuer) {
+            if (elect_one()) {
               mx_mma_f16_pair_shift(d, ad, bd, kIdescTail, shift);
 #pragma unroll
               for (int k = 1; k < 4; ++k)
@@ -366,7 +365,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
           stage = next;
           phase = next_phase;
         }
-        if (ok && issuer) tc_commit_pair(acc_full, kBoth);
+        if (ok && elect_one()) tc_commit_pair(acc_full, kBoth);
         __syncwarp();
       }
     }
@@ -380,7 +379,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
     for (int tile = pair; tile < args.num_tiles; tile += npairs, ++local) {
       int mt, nt;
       mx_tile_coords(tile, args, mt, nt);
-      if (!warp_wait(lane == 0, acc_full, local & 1, abort_flag, args.err, kDevErrTimeoutAccFull)) break;
+      if (!warp_wait(acc_full, local & 1, abort_flag, args.err, kDevErrTimeoutAccFull)) break;
       tc_fence_after();
       const int row = mt * 256 + static_cast<int>(rank) * 128 + quad * 32 + lane;
       T* out_row = static_cast<T*>(args.out) + static_cast<int64_t>(row) * args.ldo;

@@ -11,7 +11,7 @@
 // 256 columns of V through L2.  The fp32 partials of the token ranges are summed
 // in a fixed order by a second kernel (no atomics).
 //
-// An mxfp8 V arrives as codes and scale chunks; eight warps turn it into 16-bit
+// An mxfp8 V arrives as codes and scale chunks; sixteen warps turn it into 16-bit
 // values in the MMA's swizzled layout.  E4M3 times a power of two is exact in
 // bf16: the code's exponent and mantissa moved into place, times 2^120, times the
 // scale.  Bound: HBM for small ranks (2 or 1.03 bytes an element of V), the tensor
@@ -26,7 +26,7 @@ namespace {
 
 constexpr int kGrTok = 64;    // tokens a stage
 constexpr int kGrCols = 256;  // columns of V a CTA
-constexpr int kGrConvWarps = 8;
+constexpr int kGrConvWarps = 16;
 constexpr int kGrThreads = 64 + 32 * kGrConvWarps;
 constexpr int kGrChunkBytes = kGrTok * 128;          // 64 tokens x 64 16-bit columns
 constexpr int kGrVBytes = 4 * kGrChunkBytes;         // 16-bit V of a stage
@@ -63,21 +63,40 @@ LORA_DEVINL uint32_t gr_mul_bf16x2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Two E4M3 codes (bytes 1 and 3 of w, bytes 0 and 2 zero) times their scale.
+// Eight E4M3 codes times their scale 2^(s - 127), as 16-bit values in order.
 template <typename T>
-LORA_DEVINL uint32_t gr_decode2(uint32_t w, uint32_t scale_byte);
+LORA_DEVINL uint4 gr_decode8(uint2 w, uint32_t s);
 template <>
-LORA_DEVINL uint32_t gr_decode2<__nv_bfloat16>(uint32_t w, uint32_t s) {
-  const uint32_t bits = (w & 0x80008000u) | ((w >> 4) & 0x07f007f0u);  // 2^-120 of the code's value
-  const uint32_t half = s == 0 ? 0x0040u : s == 255 ? 0x7fffu : s << 7;
-  return gr_mul_bf16x2(gr_mul_bf16x2(bits, 0x7b807b80u), half | (half << 16));
+LORA_DEVINL uint4 gr_decode8<__nv_bfloat16>(uint2 w, uint32_t s) {
+  // two codes in the high bytes of each half: exponent and mantissa moved into
+  // bf16's place are 2^-120 of the code's value
+  const uint32_t p[4] = {__byte_perm(w.x, 0, 0x1404), __byte_perm(w.x, 0, 0x3424), __byte_perm(w.y, 0, 0x1404),
+                         __byte_perm(w.y, 0, 0x3424)};
+  uint32_t o[4];
+  if (s <= 134) {  // 2^120 and the scale in one factor: 2^(s - 7) is a normal bf16 number
+    const uint32_t f = ((s + 120) << 7) * 0x10001u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = gr_mul_bf16x2((p[i] & 0x80008000u) | ((p[i] >> 4) & 0x07f007f0u), f);
+  } else {
+    const uint32_t f = (s == 255 ? 0x7fffu : s << 7) * 0x10001u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      o[i] = gr_mul_bf16x2(gr_mul_bf16x2((p[i] & 0x80008000u) | ((p[i] >> 4) & 0x07f007f0u), 0x7b807b80u), f);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 template <>
-LORA_DEVINL uint32_t gr_decode2<__half>(uint32_t w, uint32_t s) {
-  const uint32_t h = mx_from_e4m3x2(((w >> 8) & 0xffu) | ((w >> 16) & 0xff00u));
-  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
+LORA_DEVINL uint4 gr_decode8<__half>(uint2 w, uint32_t s) {
   const float scale = mx_e8m0(s);
-  return pack2<__half>(v.x * scale, v.y * scale);
+  const uint32_t c[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t h = mx_from_e4m3x2(c[i]);
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    o[i] = pack2<__half>(v.x * scale, v.y * scale);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 // Shared memory: the TMA ring (stage: V or codes + scales, then P), for mxfp8 two
@@ -159,38 +178,44 @@ __global__ void __launch_bounds__(kGrThreads, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      // both operands MN-major (bits 15 and 16), M = 128, N = r16
-      const uint32_t idesc = (umma_idesc_f16(128, 16, std::is_same<T, __nv_bfloat16>::value ? 1 : 0) & ~(0x3fu << 17)) |
-                             (static_cast<uint32_t>(args.r16 >> 3) << 17) | (1u << 15) | (1u << 16);
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int st = step0; st < step1; ++st) {
-        const int n = st - step0;
-        if (!mbar_wait_bounded(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull) ||
-            (F8 && !mbar_wait_bounded(&ready[n & 1], (n >> 1) & 1, abort_flag, args.err, kDevErrTimeoutFull))) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t base = smem_u32(smem + stage * args.stage_bytes);
-        const uint32_t v = F8 ? smem_u32(conv + (n & 1) * kGrVBytes) : base;
-        for (int k = 0; k < kGrTok / 16; ++k) {
-          const uint64_t pd = gr_desc_mn(base + kPOffset + k * 2048, kGrChunkBytes);
+    // The whole warp walks the stages (uniform descriptors); one lane issues.  Both
+    // operands MN-major (bits 15 and 16), M = 128, N = r16.
+    const uint32_t idesc = (umma_idesc_f16(128, 16, std::is_same<T, __nv_bfloat16>::value ? 1 : 0) & ~(0x3fu << 17)) |
+                           (static_cast<uint32_t>(args.r16 >> 3) << 17) | (1u << 15) | (1u << 16);
+    const uint64_t desc0 = gr_desc_mn(smem_u32(smem), kGrChunkBytes);
+    const uint64_t conv0 = gr_desc_mn(smem_u32(conv), kGrChunkBytes);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int st = step0; st < step1; ++st) {
+      const int n = st - step0;
+      if (!warp_wait(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull) ||
+          (F8 && !warp_wait(&ready[n & 1], (n >> 1) & 1, abort_flag, args.err, kDevErrTimeoutFull))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint64_t base = desc0 + static_cast<uint32_t>((stage * args.stage_bytes) >> 4);
+      const uint64_t v = F8 ? conv0 + static_cast<uint32_t>(((n & 1) * kGrVBytes) >> 4) : base;
+      const uint64_t pd = base + static_cast<uint32_t>(kPOffset >> 4);
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < kGrTok / 16; ++k)
+#pragma unroll
           for (int m = 0; m < 2; ++m)
-            tc_mma_f16(tmem + m * args.r16, gr_desc_mn(v + m * 2 * kGrChunkBytes + k * 2048, kGrChunkBytes), pd, idesc,
-                       (n > 0 || k > 0) ? 1u : 0u);
-        }
+            tc_mma_f16(tmem + m * args.r16, v + static_cast<uint32_t>((m * 2 * kGrChunkBytes + k * 2048) >> 4),
+                       pd + static_cast<uint32_t>((k * 2048) >> 4), idesc, (n > 0 || k > 0) ? 1u : 0u);
         tc_commit(&empty[stage]);
         if (F8) tc_commit(&conv_empty[n & 1]);
-        if (++stage == args.stages) {
-          stage = 0;
-          phase ^= 1;
-        }
       }
-      if (ok) tc_commit(acc_full);
+      __syncwarp();
+      if (++stage == args.stages) {
+        stage = 0;
+        phase ^= 1;
+      }
     }
+    if (ok && elect_one()) tc_commit(acc_full);
+    __syncwarp();
   } else {
     const int cw = warp - 2;
     if constexpr (F8) {
@@ -198,8 +223,8 @@ __global__ void __launch_bounds__(kGrThreads, 1)
       uint32_t phase = 0;
       for (int st = step0; st < step1; ++st) {
         const int n = st - step0;
-        if (!warp_wait(lane == 0, &full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull) ||
-            !warp_wait(lane == 0, &conv_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag, args.err, kDevErrTimeoutEmpty))
+        if (!warp_wait(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull) ||
+            !warp_wait(&conv_empty[n & 1], ((n >> 1) & 1) ^ 1, abort_flag, args.err, kDevErrTimeoutEmpty))
           break;
         const uint32_t raw = smem_u32(smem) + stage * args.stage_bytes;
         // the scale chunk of this lane's 128 columns, its block
@@ -211,12 +236,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
           const int tr = (st * kGrTok + t) & 127;  // row within the scale chunk
           const uint2 w = lds64(raw + t * kGrCols + lane * 8);
           const uint32_t s = lds_u8(sc + (tr & 31) * 16 + (tr >> 5) * 4);
-          uint4 o;
-          o.x = gr_decode2<T>(__byte_perm(w.x, 0, 0x1404), s);
-          o.y = gr_decode2<T>(__byte_perm(w.x, 0, 0x3424), s);
-          o.z = gr_decode2<T>(__byte_perm(w.y, 0, 0x1404), s);
-          o.w = gr_decode2<T>(__byte_perm(w.y, 0, 0x3424), s);
-          sts128(dst + t * 128 + (((lane & 7) ^ (t & 7)) << 4), o);
+          sts128(dst + t * 128 + (((lane & 7) ^ (t & 7)) << 4), gr_decode8<T>(w, s));
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -227,13 +247,13 @@ __global__ void __launch_bounds__(kGrThreads, 1)
         }
       }
     }
-    // epilogue: warps 0..3 of these drain the first accumulator, 4..7 the second
-    const int quad = warp & 3, m = cw >> 2;
-    if (warp_wait(lane == 0, acc_full, 0, abort_flag, args.err, kDevErrTimeoutAccFull)) {
+    // epilogue: lane quadrant, accumulator, every other group of 16 ranks
+    const int quad = warp & 3, m = (cw >> 2) & 1;
+    if (warp_wait(acc_full, 0, abort_flag, args.err, kDevErrTimeoutAccFull)) {
       tc_fence_after();
       const int64_t c = col0 + m * 128 + quad * 32 + lane;
       float* dst = args.part + (static_cast<int64_t>(blockIdx.y) * args.C + c) * args.r16;
-      for (int j = 0; j < args.r16; j += 16) {
+      for (int j = (cw >> 3) * 16; j < args.r16; j += 32) {
         uint32_t r[16];
         tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + m * args.r16 + j, r);
         tmem_wait_ld();

@@ -152,41 +152,47 @@ __global__ void __launch_bounds__(kShThreads, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = (umma_idesc_f16(128, 16, std::is_same<T, __nv_bfloat16>::value ? 1 : 0) & ~(0x3fu << 17)) |
-                             (static_cast<uint32_t>(args.r16 >> 3) << 17) | (AMN ? 1u << 16 : 0u);
-      int stage = 0, seg = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int c = c_begin; ok && c < c_end; ++seg) {
-        const int seg_end = min(c_end, (c / args.kc + 1) * args.kc);
-        if (!mbar_wait_bounded(&acc_empty[seg & 1], ((seg >> 1) & 1) ^ 1, abort_flag, args.err, kDevErrTimeoutAccEmpty))
+    // the whole warp walks the chunks (uniform descriptors); one lane issues
+    const uint32_t idesc = (umma_idesc_f16(128, 16, std::is_same<T, __nv_bfloat16>::value ? 1 : 0) & ~(0x3fu << 17)) |
+                           (static_cast<uint32_t>(args.r16 >> 3) << 17) | (AMN ? 1u << 16 : 0u);
+    const uint64_t x0 = umma_desc_sw128(smem_u32(smem));
+    const uint64_t a0 = AMN ? sh_desc_mn(smem_u32(smem) + KB * kShBoxBytes, args.a_box_bytes)
+                            : umma_desc_sw128(smem_u32(smem) + KB * kShBoxBytes);
+    int stage = 0, seg = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int c = c_begin; ok && c < c_end; ++seg) {
+      const int seg_end = min(c_end, (c / args.kc + 1) * args.kc);
+      if (!warp_wait(&acc_empty[seg & 1], ((seg >> 1) & 1) ^ 1, abort_flag, args.err, kDevErrTimeoutAccEmpty))
+        break;
+      tc_fence_after();
+      const uint32_t d = tmem + (seg & 1) * args.r16;
+      for (bool first = true; c < seg_end; ++c, first = false) {
+        if (!warp_wait(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
+          ok = false;
           break;
+        }
         tc_fence_after();
-        const uint32_t d = tmem + (seg & 1) * args.r16;
-        for (bool first = true; c < seg_end; ++c, first = false) {
-          if (!mbar_wait_bounded(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t xb = smem_u32(smem + stage * args.stage_bytes);
-          const uint32_t ab = xb + KB * kShBoxBytes;
+        const uint32_t at = static_cast<uint32_t>((stage * args.stage_bytes) >> 4);
+        if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < 4 * KB; ++k) {
-            const uint64_t xd = umma_desc_sw128(xb + (k >> 2) * kShBoxBytes) + static_cast<uint64_t>(2 * (k & 3));
-            const uint64_t ad = AMN ? sh_desc_mn(ab + k * 2048, args.a_box_bytes)
-                                    : umma_desc_sw128(ab + (k >> 2) * args.a_box_bytes) + static_cast<uint64_t>(2 * (k & 3));
+            const uint64_t xd = x0 + (at + static_cast<uint32_t>((k >> 2) * (kShBoxBytes >> 4) + 2 * (k & 3)));
+            const uint64_t ad =
+                a0 + (at + (AMN ? static_cast<uint32_t>(k * (2048 >> 4))
+                                : static_cast<uint32_t>((k >> 2) * (args.a_box_bytes >> 4) + 2 * (k & 3))));
             tc_mma_f16(d, xd, ad, idesc, (!first || k > 0) ? 1u : 0u);
           }
           tc_commit(&empty[stage]);
-          if (++stage == args.stages) {
-            stage = 0;
-            phase ^= 1;
-          }
         }
-        if (ok) tc_commit(&acc_full[seg & 1]);
+        __syncwarp();
+        if (++stage == args.stages) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
+      if (ok && elect_one()) tc_commit(&acc_full[seg & 1]);
+      __syncwarp();
     }
   } else {
     const int w = warp - 2, quad = warp & 3, part = w >> 2;
@@ -205,7 +211,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
         for (; c < seg_end; ++c) {
           const int kc = c - tb * args.kc;
           if ((w >> 3) == ((c - c_begin) & 1)) {
-            if (!warp_wait(lane == 0, &full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
+            if (!warp_wait(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
               ok = false;
               break;
             }
@@ -274,7 +280,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
       c = seg_end;
       // ---- the block's sum (or this run's part of it); a warp takes its 32 rows and
       // every fourth group of 16 columns
-      if (!warp_wait(lane == 0, &acc_full[seg & 1], (seg >> 1) & 1, abort_flag, args.err, kDevErrTimeoutAccFull)) break;
+      if (!warp_wait(&acc_full[seg & 1], (seg >> 1) & 1, abort_flag, args.err, kDevErrTimeoutAccFull)) break;
       tc_fence_after();
       const int64_t row = static_cast<int64_t>(tb) * 128 + quad * 32 + lane;
       const bool whole = seg_begin == tb * args.kc && seg_end == (tb + 1) * args.kc;
