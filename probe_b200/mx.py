@@ -13,6 +13,8 @@ tensors raise.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -20,6 +22,43 @@ from . import _lib
 _FORMATS = {"mxfp4": _lib.LORA_MXFP4, "nvfp4": _lib.LORA_NVFP4, "mxfp8": _lib.LORA_MXFP8}
 _BLOCK = {"mxfp4": 32, "nvfp4": 16, "mxfp8": 32}
 _HALF = (torch.float16, torch.bfloat16)
+_DTYPE = {torch.float16: _lib.LORA_F16, torch.bfloat16: _lib.LORA_BF16}
+
+
+# A call of a few tokens takes the GPU a few microseconds: the wrappers below pass
+# plain integers to the C ABI, look the raw stream up directly and keep sizes by shape.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_buffers: dict[tuple, torch.Tensor] = {}
+
+
+@functools.cache
+def _entry(name: str):
+    return getattr(_lib.load(), name)
+
+
+def _workspace(slot: str, nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
+    """The zero-initialised per-stream workspace of the slot (grown by ``_lib.WORKSPACE``)."""
+    buf = _buffers.get((slot, device.index, stream))
+    if buf is None or buf.numel() < nbytes:
+        buf = _lib.WORKSPACE.get(nbytes, device, slot)
+        _buffers[(slot, device.index, stream)] = buf
+    return buf
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_bytes(m, n, k, r, code):
+    return _entry("lora_mx_linear_workspace_size")(m, n, k, r, code)
+
+
+@functools.lru_cache(maxsize=4096)
+def _backward_bytes(m, n, k, r, need_dx):
+    return _entry("lora_mx_backward_workspace_size")(m, n, k, r, need_dx)
+
+
+def _need_cuda(where, *tensors):
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            _lib.require_cuda(t, where=where)
 
 
 def _format(fmt: str, where: str) -> int:
@@ -29,6 +68,7 @@ def _format(fmt: str, where: str) -> int:
     return code
 
 
+@functools.lru_cache(maxsize=4096)
 def _sizes(m: int, k: int, fmt: str) -> tuple[int, int]:
     """Bytes of a row of codes, and of all scales, of an [m, k] tensor."""
     kp = (k + 31) // 32 * 32
@@ -66,6 +106,13 @@ class MXTensor:
         self.global_scale = float(global_scale)
         self._code = code
 
+    @classmethod
+    def _of(cls, codes, scales, shape, fmt, global_scale, code):
+        """An MXTensor of buffers that the caller has laid out itself."""
+        t = object.__new__(cls)
+        t.codes, t.scales, t.shape, t.fmt, t.global_scale, t._code = codes, scales, shape, fmt, global_scale, code
+        return t
+
     @property
     def device(self) -> torch.device:
         return self.codes.device
@@ -86,7 +133,13 @@ def nvfp4_global_scale(amax: float) -> float:
 def _rows(x: torch.Tensor, where: str) -> torch.Tensor:
     if x.dtype not in _HALF:
         raise TypeError(f"{where}: expected float16/bfloat16, got {x.dtype}")
+    if x.dim() == 2 and x.is_contiguous():
+        return x
     return _lib.row_major(x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x)
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4", global_scale: float = 1.0) -> MXTensor:
@@ -97,49 +150,60 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4", global_scale: float = 1.0) 
     and saturate; a block with an infinity or a NaN reads back as NaN.
     """
     code = _format(fmt, "mx_quantize")
-    _lib.require_cuda(x, where="mx_quantize")
+    _need_cuda("mx_quantize", x)
     x = _rows(x, "mx_quantize")
     m, k = x.shape
     pitch, nscales = _sizes(m, k, fmt)
-    codes = torch.empty((m, pitch), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(nscales, dtype=torch.uint8, device=x.device)
-    _lib.call("lora_mx_quantize", _lib.ptr(x), _lib.ld(x), _lib.ptr(codes), _lib.ptr(scales), m, k, code,
-              float(global_scale), _lib.dtype_code(x.dtype), _lib.stream_handle(x.device))
-    return MXTensor(codes, scales, (m, k), fmt, global_scale)
+    device, dtype = x.device, x.dtype
+    codes = torch.empty((m, pitch), dtype=torch.uint8, device=device)
+    scales = torch.empty(nscales, dtype=torch.uint8, device=device)
+    global_scale = float(global_scale)
+    rc = _entry("lora_mx_quantize")(x.data_ptr(), _ld(x), codes.data_ptr(), scales.data_ptr(), m, k, code, global_scale,
+                                    _DTYPE[dtype], _raw_stream(device.index))
+    if rc:
+        _lib.check(rc, "lora_mx_quantize")
+    return MXTensor._of(codes, scales, (m, k), fmt, global_scale, code)
 
 
 def mx_dequantize(q: MXTensor, dtype: torch.dtype = torch.bfloat16, transpose: bool = False) -> torch.Tensor:
     """The values of ``q`` in ``dtype`` (rounded once), [M, K] or, transposed, [K, M]."""
-    _lib.require_cuda(q.codes, where="mx_dequantize")
+    _need_cuda("mx_dequantize", q.codes)
     if dtype not in _HALF:
         raise TypeError(f"mx_dequantize: expected float16/bfloat16, got {dtype}")
     m, k = q.shape
-    out = torch.empty((k, m) if transpose else (m, k), dtype=dtype, device=q.device)
-    _lib.call("lora_mx_dequantize", _lib.ptr(q.codes), _lib.ptr(q.scales), _lib.ptr(out), out.shape[1], m, k, q._code,
-              q.global_scale, int(transpose), _lib.dtype_code(dtype), _lib.stream_handle(q.device))
+    device = q.codes.device
+    out = torch.empty((k, m) if transpose else (m, k), dtype=dtype, device=device)
+    rc = _entry("lora_mx_dequantize")(q.codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), m if transpose else k, m,
+                                      k, q._code, q.global_scale, int(transpose), _DTYPE[dtype],
+                                      _raw_stream(device.index))
+    if rc:
+        _lib.check(rc, "lora_mx_dequantize")
     return out
 
 
 # --------------------------------------------------------------------- linear
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     """Row-major with 16-byte rows where the width allows it (copies only when needed)."""
-    t = _lib.row_major(t)
-    if t.shape[1] % 8 == 0 and (_lib.ld(t) % 8 != 0 or t.data_ptr() % 16 != 0):
+    if not t.is_contiguous():
+        t = _lib.row_major(t)
+    if t.shape[1] % 8 == 0 and (_ld(t) % 8 != 0 or t.data_ptr() % 16 != 0):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _linear(x, weight, bias, a, b, scale, x_global_scale, keep_z, where):
-    _lib.require_cuda(x, weight.codes, bias, a, b, where=where)
+    _need_cuda(where, x, weight.codes, bias, a, b)
     if weight.fmt not in ("mxfp4", "nvfp4"):
         raise ValueError(f"{where}: the weight must be in a 4-bit format, got {weight.fmt}")
     shape = x.shape
     x = _rows(x, where)
     n, k = weight.shape
+    m = x.shape[0]
     if x.shape[1] != k:
         raise ValueError(f"{where}: x {tuple(shape)} and the weight {weight.shape} disagree on K")
-    dtype = x.dtype
+    device, dtype = x.device, x.dtype
     r = 0
+    ap = bp = lda = ldb = 0
     if a is not None and b is not None and a.shape[0] > 0 and scale != 0:
         r = a.shape[0]
         if a.dtype != dtype or b.dtype != dtype:
@@ -149,25 +213,28 @@ def _linear(x, weight, bias, a, b, scale, x_global_scale, keep_z, where):
         if r > 256:
             raise ValueError(f"{where}: ranks up to 256, got {r}")
         x, a, b = _aligned_rows(x), _aligned_rows(a), _aligned_rows(b)
+        ap, lda, bp, ldb = a.data_ptr(), _ld(a), b.data_ptr(), _ld(b)
+    bias_ptr = None
     if bias is not None:
         if bias.shape != (n,) or bias.dtype != dtype:
             raise ValueError(f"{where}: bias must be [{n}] in x's dtype")
         bias = bias.contiguous()
-    m = x.shape[0]
-    out = torch.empty((m, n), dtype=dtype, device=x.device)
+        bias_ptr = bias.data_ptr()
+    out = torch.empty((m, n), dtype=dtype, device=device)
     z = None
     if keep_z and r:
-        z = torch.empty((m, 2 * ((r + 15) // 16 * 16)), dtype=dtype, device=x.device)
+        z = torch.empty((m, 2 * ((r + 15) // 16 * 16)), dtype=dtype, device=device)
     if m and n:
-        lib = _lib.load()
-        nbytes = lib.lora_mx_linear_workspace_size(m, n, k, r, weight._code)
-        ws = _lib.WORKSPACE.get(nbytes, x.device, "mx_linear")
-        _lib.call("lora_mx_linear", _lib.ptr(x), _lib.ld(x), _lib.ptr(weight.codes), _lib.ptr(weight.scales),
-                  weight.global_scale, _lib.ptr(bias), _lib.ptr(a) if r else None, _lib.ld(a) if r else 0,
-                  _lib.ptr(b) if r else None, _lib.ld(b) if r else 0, _lib.ptr(out), n, _lib.ptr(z), m, n, k, r,
-                  float(scale), float(x_global_scale), weight._code, _lib.dtype_code(dtype), _lib.ptr(ws), ws.numel(),
-                  _lib.stream_handle(x.device))
-    return out.view(*shape[:-1], n), z
+        code = weight._code
+        stream = _raw_stream(device.index)
+        ws = _workspace("mx_linear", _linear_bytes(m, n, k, r, code), device, stream)
+        rc = _entry("lora_mx_linear")(x.data_ptr(), _ld(x), weight.codes.data_ptr(), weight.scales.data_ptr(),
+                                      weight.global_scale, bias_ptr, ap or None, lda, bp or None, ldb, out.data_ptr(), n,
+                                      z.data_ptr() if z is not None else None, m, n, k, r, float(scale),
+                                      float(x_global_scale), code, _DTYPE[dtype], ws.data_ptr(), ws.numel(), stream)
+        if rc:
+            _lib.check(rc, "lora_mx_linear")
+    return (out if len(shape) == 2 else out.view(*shape[:-1], n)), z
 
 
 def mx_lora_linear(x: torch.Tensor, weight: MXTensor, bias: torch.Tensor | None, a: torch.Tensor | None,
@@ -194,7 +261,7 @@ def mx_lora_backward(dy: torch.Tensor, x8: MXTensor, z: torch.Tensor, a: torch.T
     """
     where = "mx_lora_backward"
     wc = weight.codes if weight is not None else None
-    _lib.require_cuda(dy, x8.codes, z, a, b, wc, where=where)
+    _need_cuda(where, dy, x8.codes, z, a, b, wc)
     shape = dy.shape
     dy = _rows(dy, where)
     m, n = dy.shape
@@ -211,15 +278,20 @@ def mx_lora_backward(dy: torch.Tensor, x8: MXTensor, z: torch.Tensor, a: torch.T
     if weight is not None and (weight.fmt not in ("mxfp4", "nvfp4") or weight.shape != (n, k)):
         raise ValueError(f"{where}: the weight must be a 4-bit tensor of shape {(n, k)}, got {weight.fmt} {weight.shape}")
     a, b = _lib.row_major(a), _lib.row_major(b)
-    da = torch.empty((r, k), dtype=dtype, device=dy.device)
-    db = torch.empty((n, r), dtype=dtype, device=dy.device)
-    dx = torch.empty((m, k), dtype=dtype, device=dy.device) if weight is not None else None
-    nbytes = _lib.load().lora_mx_backward_workspace_size(m, n, k, r, int(dx is not None))
-    ws = _lib.WORKSPACE.get(nbytes, dy.device, "mx_backward")
-    _lib.call("lora_mx_backward", _lib.ptr(dy), _lib.ld(dy), _lib.ptr(x8.codes), _lib.ptr(x8.scales), _lib.ptr(z),
-              float(z_scale), _lib.ptr(a), _lib.ld(a), _lib.ptr(b), _lib.ld(b), _lib.ptr(wc),
-              _lib.ptr(weight.scales) if weight is not None else None,
-              weight.global_scale if weight is not None else 1.0, weight._code if weight is not None else 0,
-              _lib.ptr(dx), k, _lib.ptr(da), k, _lib.ptr(db), r, m, n, k, r, float(scale), _lib.dtype_code(dtype),
-              _lib.ptr(ws), ws.numel(), _lib.stream_handle(dy.device))
-    return (None if dx is None else dx.view(*shape[:-1], k)), da, db
+    device = dy.device
+    da = torch.empty((r, k), dtype=dtype, device=device)
+    db = torch.empty((n, r), dtype=dtype, device=device)
+    dx = wp = sp = None
+    wg, wcode = 1.0, 0
+    if weight is not None:
+        dx = torch.empty((m, k), dtype=dtype, device=device)
+        wp, sp, wg, wcode = wc.data_ptr(), weight.scales.data_ptr(), weight.global_scale, weight._code
+    stream = _raw_stream(device.index)
+    ws = _workspace("mx_backward", _backward_bytes(m, n, k, r, int(dx is not None)), device, stream)
+    rc = _entry("lora_mx_backward")(dy.data_ptr(), _ld(dy), x8.codes.data_ptr(), x8.scales.data_ptr(), z.data_ptr(),
+                                    float(z_scale), a.data_ptr(), _ld(a), b.data_ptr(), _ld(b), wp, sp, wg, wcode,
+                                    dx.data_ptr() if dx is not None else None, k, da.data_ptr(), k, db.data_ptr(), r, m,
+                                    n, k, r, float(scale), _DTYPE[dtype], ws.data_ptr(), ws.numel(), stream)
+    if rc:
+        _lib.check(rc, "lora_mx_backward")
+    return (dx if dx is None or len(shape) == 2 else dx.view(*shape[:-1], k)), da, db
