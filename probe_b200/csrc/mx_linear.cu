@@ -17,6 +17,9 @@ namespace {
 // Shrinks of more ranks than this run on the 16-bit tensor-core GEMM.
 constexpr int64_t kShrinkMaxRank = 128;
 
+// Rows up to which the W-streaming kernel runs.
+constexpr int64_t kSmallRows = 128;
+
 int64_t r16(int64_t r) { return (r + 15) / 16 * 16; }
 
 struct LinearPlan {
@@ -115,6 +118,21 @@ extern "C" int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, c
       o.alpha = static_cast<float>(alpha);
     }
   }
+  o.b = b;
+  o.ldb = ldb;
+  // ahead of the other steps: a kernel that reads B before its predecessor on the
+  // stream has finished must not have this one as its predecessor
+  if (R > 0 && (ldb % 8 != 0 || !mx_aligned(b, 16))) {
+    if (R % 8 == 0) return LORA_ERR_ALIGN;
+    const int r8 = static_cast<int>((R + 7) / 8 * 8);
+    const int64_t n = N * r8;
+    mx_pad_rows_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(
+        static_cast<const uint16_t*>(b), ldb, reinterpret_cast<uint16_t*>(ws + p.b), N, static_cast<int>(R),
+        r8);
+    if (cudaGetLastError() != cudaSuccess) return LORA_ERR_CUDA;
+    o.b = ws + p.b;
+    o.ldb = r8;
+  }
   int rc = LORA_OK;
   const int64_t rp = r16(R);
   char* z = z_out != nullptr ? static_cast<char*>(z_out) : ws + p.z;
@@ -156,19 +174,6 @@ extern "C" int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, c
     o.z = z;
     o.ldz = 2 * rp;
     o.z_lo = rp;
-    o.b = b;
-    o.ldb = ldb;
-    if (ldb % 8 != 0 || !mx_aligned(b, 16)) {
-      if (R % 8 == 0) return LORA_ERR_ALIGN;
-      const int r8 = static_cast<int>((R + 7) / 8 * 8);
-      const int64_t n = N * r8;
-      mx_pad_rows_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(
-          static_cast<const uint16_t*>(b), ldb, reinterpret_cast<uint16_t*>(ws + p.b), N, static_cast<int>(R),
-          r8);
-      if (cudaGetLastError() != cudaSuccess) return LORA_ERR_CUDA;
-      o.b = ws + p.b;
-      o.ldb = r8;
-    }
   }
   o.x_codes = ws + p.x_codes;
   o.x_scales = ws + p.x_scales;
@@ -181,5 +186,6 @@ extern "C" int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, c
   o.N = N;
   o.K = K;
   o.R = R;
+  if (M <= kSmallRows) return mx_small_launch(o, fmt, dtype, s);
   return mx_gemm_launch(o, fmt, dtype, s);
 }

@@ -17,6 +17,8 @@ struct MxLinearOperands {
   int dshift;
 };
 
+// Few tokens (mx_small.cu) and many (mx_gemm.cu).
+int mx_small_launch(const MxLinearOperands& o, int fmt, int dtype, cudaStream_t stream);
 int mx_gemm_launch(const MxLinearOperands& o, int fmt, int dtype, cudaStream_t stream);
 
 // 2-D TMA map over rows of `inner` elements of 1, 2 or 4 bytes.

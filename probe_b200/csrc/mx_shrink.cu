@@ -14,7 +14,9 @@
 // Work split: the (token block, chunk of columns) pairs in one sequence, cut into
 // equal runs, one per SM, so that any M fills the machine; a token block cut by a
 // run boundary leaves fp32 partials that its last contributor (a ticket) adds in
-// run order, so the result does not depend on timing.
+// run order, so the result does not depend on timing.  Up to about 2000 tokens a
+// cluster of up to 8 CTAs takes each token block instead, its partial sums meet in
+// shared memory: no ticket, fence and reload, whose latencies would be half the call.
 #include <mutex>
 
 #include "mx_shrink.h"
@@ -41,6 +43,7 @@ struct ShArgs {
   int64_t M, K, Kp, ldz;
   int chunks_total;
   int kc, r16, a_boxes, a_box_bytes, stages, stage_bytes, gb;
+  int cluster;  // CTAs of a token block's cluster; 0: runs
   float scale;
   MxGlobal gl;
 };
@@ -91,9 +94,13 @@ __global__ void __launch_bounds__(kShThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* recip = reinterpret_cast<float*>(tmem_slot + 4);  // 128 entries (nvfp4)
+  const uint32_t csum = smem_u32(full) + 1024;              // cluster mode: [128][r16] partial sums
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int c_begin = sh_start(args, blockIdx.x), c_end = sh_start(args, blockIdx.x + 1);
+  const int crank = args.cluster ? static_cast<int>(cluster_ctarank()) : 0;
+  const int cblock = args.cluster ? static_cast<int>(blockIdx.x) / args.cluster * args.kc : 0;  // its first chunk
+  const int c_begin = args.cluster ? cblock + args.kc * crank / args.cluster : sh_start(args, blockIdx.x);
+  const int c_end = args.cluster ? cblock + args.kc * (crank + 1) / args.cluster : sh_start(args, blockIdx.x + 1);
   const uint32_t need = 2 * args.r16;
   const uint32_t tmem_cols = need <= 32 ? 32u : need <= 64 ? 64u : need <= 128 ? 128u : need <= 256 ? 256u : 512u;
 
@@ -125,6 +132,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -291,6 +299,13 @@ __global__ void __launch_bounds__(kShThreads, 1)
         uint32_t u[16];
         tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + (seg & 1) * args.r16 + j, u);
         tmem_wait_ld();
+        if (args.cluster) {
+          const uint32_t dst = csum + ((quad * 32 + lane) * args.r16 + j) * 4;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            sts128(dst + 16 * e, make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]));
+          continue;
+        }
         if (row >= args.M) continue;
         if (whole) {
           float v[16];
@@ -306,7 +321,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
       __syncwarp();
       tc_fence_before();
       if (lane == 0) mbar_arrive(&acc_empty[seg & 1]);
-      if (!whole && part * 16 < args.r16) {
+      if (!args.cluster && !whole && part * 16 < args.r16) {
         // first and last run with a chunk of this block
         const int first_chunk = tb * args.kc, end_chunk = first_chunk + args.kc;
         int j0 = static_cast<int>(static_cast<int64_t>(first_chunk) * gridDim.x / args.chunks_total);
@@ -365,7 +380,35 @@ __global__ void __launch_bounds__(kShThreads, 1)
     }
   }
   tc_fence_before();
-  __syncthreads();
+  if (args.cluster) {
+    cluster_sync_all();  // every CTA's partial sums are in its shared memory
+    // rows are dealt to the ranks, groups of four columns to the threads
+    const int per = 128 / args.cluster, quads = args.r16 / 4;
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x / args.cluster) * 128 + crank * per;
+    for (int i = threadIdx.x; i < per * quads; i += kShThreads) {
+      const int r = i / quads, j = (i - r * quads) * 4;
+      if (row0 + r >= args.M) break;
+      const uint32_t src = csum + ((crank * per + r) * args.r16 + j) * 4;
+      float4 p[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (q < args.cluster) p[q] = ld_dsmem_f4(mapa_shared(src, q));
+      float4 v = p[0];
+#pragma unroll
+      for (int q = 1; q < 8; ++q)
+        if (q < args.cluster) v.x += p[q].x, v.y += p[q].y, v.z += p[q].z, v.w += p[q].w;
+      v.x *= args.scale, v.y *= args.scale, v.z *= args.scale, v.w *= args.scale;
+      T* z = static_cast<T*>(args.z) + (row0 + r) * args.ldz + j;
+      const uint2 h = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+      const float2 h0 = unpack2<T>(h.x), h1 = unpack2<T>(h.y);
+      *reinterpret_cast<uint2*>(z) = h;
+      *reinterpret_cast<uint2*>(z + args.r16) =
+          make_uint2(pack2<T>(v.x - h0.x, v.y - h0.y), pack2<T>(v.z - h1.x, v.w - h1.y));
+    }
+    cluster_sync_all();  // no CTA leaves while another reads its sums
+  } else {
+    __syncthreads();
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, tmem_cols);
@@ -381,6 +424,18 @@ int shrink_ctas(int64_t M, int64_t K, int64_t R) {
   const int sms = dev >= 0 ? device_info(dev).num_sms : 148;
   const int64_t total = (M + 127) / 128 * ((K + 64 * shrink_boxes(R) - 1) / (64 * shrink_boxes(R)));
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms, total / 2)));
+}
+
+// CTAs of a token block's cluster where that fills no more than the machine: a
+// power of two up to 8, each with a chunk or more.  0: equal runs over all blocks.
+int shrink_cluster(int64_t M, int64_t K, int64_t R) {
+  const int dev = current_device();
+  const int sms = dev >= 0 ? device_info(dev).num_sms : 148;
+  const int64_t blocks = (M + 127) / 128, kc = (K + 64 * shrink_boxes(R) - 1) / (64 * shrink_boxes(R));
+  if (blocks * 8 > sms) return 0;
+  int c = 8;
+  while (c > kc) c /= 2;
+  return c;
 }
 
 template <typename T, int FMT, bool AMN, int KB>
@@ -414,7 +469,9 @@ int launch_shrink(const MxShrinkOperands& o, cudaStream_t stream) {
   a.scale = o.scale;
   a.gl = mx_global(o.global_scale);
   constexpr int kFixed = 1024 + 1024;  // alignment, barriers and reciprocals
-  a.stages = std::min(8, (kShSmemMax - kFixed) / a.stage_bytes);
+  a.cluster = shrink_cluster(o.M, o.K, o.R);
+  const int sums = a.cluster ? 128 * a.r16 * 4 : 0;
+  a.stages = std::min(8, (kShSmemMax - kFixed - sums) / a.stage_bytes);
   auto kernel = mx_shrink_kernel<T, FMT, AMN, KB>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
@@ -422,9 +479,28 @@ int launch_shrink(const MxShrinkOperands& o, cudaStream_t stream) {
     attr_err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShSmemMax);
   });
   if (attr_err[dev] != cudaSuccess) return LORA_ERR_CUDA;
-  const size_t smem = static_cast<size_t>(a.stages) * a.stage_bytes + kFixed;
-  kernel<<<shrink_ctas(o.M, o.K, o.R), kShThreads, smem, stream>>>(maps, a);
-  return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
+  const size_t smem = static_cast<size_t>(a.stages) * a.stage_bytes + kFixed + sums;
+  if (!a.cluster) {
+    kernel<<<shrink_ctas(o.M, o.K, o.R), kShThreads, smem, stream>>>(maps, a);
+    return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((o.M + 127) / 128 * a.cluster));
+  cfg.blockDim = dim3(kShThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = a.cluster;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, maps, a) != cudaSuccess) {
+    cudaGetLastError();
+    return LORA_ERR_CUDA;
+  }
+  return LORA_OK;
 }
 
 template <typename T, int KB>

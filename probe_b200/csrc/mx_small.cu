@@ -1,0 +1,412 @@
+// 4-bit LoRA linear of few tokens: W streamed once through block-scaled MMAs with
+// the tokens as the narrow operand.
+//
+//   out[t, n] = alpha (2^-d sum_k wq[n,k] sw xq[t,k] sx + sum_j B[n,j] (zh + zl)[t,j]) + bias[n]
+//
+// tcgen05.mma.kind::mxf4nvf4 with 128 rows of W as M and the tokens (16..128) as N;
+// the adapter's products go to an accumulator of their own (kind::f16, B's rows as
+// M), so the two kinds never meet and the power of two is taken in the epilogue.
+// Bound: HBM, 0.53 (mxfp4) or 0.56 (nvfp4) bytes a weight; for a handful of tokens
+// the chain of launches and latencies.  So K is cut over a cluster of up to 8 CTAs
+// until about two CTAs an SM stream W; their partial tiles meet in shared memory
+// and are summed in rank order over DSMEM.  The kernel starts while its predecessor
+// (the shrink that makes xq, sx and z) still runs: W's first stages load before
+// griddepcontrol.wait.
+#include <cmath>
+#include <mutex>
+
+#include "mx_linear.h"
+
+namespace lora {
+namespace {
+
+constexpr int kSmThreads = 192;
+// Two CTAs an SM, each with at most half of TMEM, or (128 tokens) one with all of
+// it: a CTA must never wait for another's TMEM, whose cluster may wait for its own.
+template <int NB> __host__ __device__ constexpr int sm_smem_max() { return NB == 128 ? 220 * 1024 : 112 * 1024; }
+template <int NB> __host__ __device__ constexpr int sm_tmem_max() { return NB == 128 ? 512 : 256; }
+
+struct SmMaps {
+  CUtensorMap x, w, sx, sw, zh, zl, b;
+};
+
+struct SmArgs {
+  void* out;
+  const void* bias;
+  int* err;
+  int64_t ldo;
+  int M, N;
+  int num_kb, last_k64, rank_kb, last_k16, chunks, stages;
+  float alpha, base_scale;  // 2^-dshift
+};
+
+LORA_DEVINL uint64_t sm_desc_scales(uint32_t addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((addr >> 4) & 0x3FFF);
+  d |= static_cast<uint64_t>(128 >> 4) << 16;
+  d |= static_cast<uint64_t>(128 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  return d;
+}
+LORA_DEVINL void sm_cp_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+template <int FMT>
+LORA_DEVINL void sm_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                        uint32_t accumulate) {
+  if constexpr (FMT == LORA_MXFP4) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  }
+}
+
+template <int FMT, int NB>
+struct SmLayout {
+  static constexpr int kChunks = 256 / MxFormat<FMT>::kBlock / 4;
+  static constexpr int kW = 128 * 128, kX = NB * 128, kSf = kChunks * 512;
+  static constexpr int kStage = (kW + kX + 2 * kSf + 1023) / 1024 * 1024;
+  static constexpr int kXOffset = kW, kSfOffset = kW + kX;
+  static constexpr int kMainBytes = kW + kX + 2 * kSf;
+  static constexpr int kSfCols = 2 * kChunks * 4;
+  // TMEM: base accumulator, adapter accumulator, scales of every stage
+  static constexpr int kFit = (sm_tmem_max<NB>() - 2 * NB) / kSfCols;
+  static constexpr int kMaxStages = kFit < 8 ? kFit : 8;
+};
+
+template <typename T, int FMT, int NB>
+__global__ void __launch_bounds__(kSmThreads)
+    mx_small_kernel(const __grid_constant__ SmMaps maps, const SmArgs args) {
+  using L = SmLayout<FMT, NB>;
+  constexpr uint32_t kCols = 2 * NB + L::kMaxStages * L::kSfCols;
+  constexpr uint32_t kTmemCols = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+  static_assert(kTmemCols <= sm_tmem_max<NB>(), "TMEM");
+  constexpr uint32_t kIdesc = (1u << 7) | (1u << 10) | (static_cast<uint32_t>(NB >> 3) << 17) |
+                              ((FMT == LORA_MXFP4 ? 1u : 0u) << 23) | (8u << 24);
+  constexpr uint32_t kIdescTail = (1u << 4) | ((std::is_same<T, __nv_bfloat16>::value ? 1u : 0u) << 7) |
+                                  ((std::is_same<T, __nv_bfloat16>::value ? 1u : 0u) << 10) |
+                                  (static_cast<uint32_t>(NB >> 3) << 17) | (8u << 24);
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + args.stages * L::kStage);
+  uint64_t* empty = full + 8;
+  uint64_t* acc_full = empty + 8;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int splits = 1;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int n0 = static_cast<int>(blockIdx.x) / splits * 128;
+  const int t0 = static_cast<int>(blockIdx.y) * NB;
+  const int kb0 = args.num_kb * rank / splits, kb1 = args.num_kb * (rank + 1) / splits;
+  // the adapter's stages follow the first rank's base stages
+  const int tail_kb = rank == 0 ? 2 * args.rank_kb : 0;
+  const int total = kb1 - kb0 + tail_kb;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < args.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      auto weights = [&](int i, int stage) {
+        uint8_t* base = smem + stage * L::kStage;
+        if (i < kb1 - kb0) {
+          mbar_arrive_expect_tx(&full[stage], L::kMainBytes);
+          tma_load_2d(&maps.w, base, &full[stage], (kb0 + i) * 128, n0);
+          tma_load_2d(&maps.sw, base + L::kSfOffset, &full[stage], 0, (n0 >> 7) * args.chunks + (kb0 + i) * L::kChunks);
+        } else {
+          const int t = i - (kb1 - kb0);
+          mbar_arrive_expect_tx(&full[stage], L::kW + L::kX);
+          tma_load_2d(&maps.b, base, &full[stage], (t >= args.rank_kb ? t - args.rank_kb : t) * 64, n0);
+        }
+      };
+      auto tokens = [&](int i, int stage) {
+        uint8_t* base = smem + stage * L::kStage;
+        if (i < kb1 - kb0) {
+          tma_load_2d(&maps.x, base + L::kXOffset, &full[stage], (kb0 + i) * 128, t0);
+          tma_load_2d(&maps.sx, base + L::kSfOffset + L::kSf, &full[stage], 0,
+                      (t0 >> 7) * args.chunks + (kb0 + i) * L::kChunks);
+        } else {
+          const int t = i - (kb1 - kb0);
+          const bool lo = t >= args.rank_kb;
+          tma_load_2d(lo ? &maps.zl : &maps.zh, base + L::kXOffset, &full[stage], (lo ? t - args.rank_kb : t) * 64, t0);
+        }
+      };
+      const int pre = min(total, args.stages);
+      for (int i = 0; i < pre; ++i) weights(i, i);
+      pdl_wait();  // the shrink's codes, scales and z
+      for (int i = 0; i < pre; ++i) tokens(i, i);
+      int stage = pre == args.stages ? 0 : pre;
+      uint32_t phase = pre == args.stages ? 1 : 0;
+      for (int i = pre; i < total; ++i) {
+        if (!mbar_wait_bounded(&empty[stage], phase ^ 1, abort_flag, args.err, kDevErrTimeoutEmpty)) break;
+        weights(i, stage);
+        tokens(i, stage);
+        if (++stage == args.stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const uint64_t wd0 = umma_desc_sw128(smem_u32(smem));
+    const uint64_t xd0 = umma_desc_sw128(smem_u32(smem) + L::kXOffset);
+    const uint64_t sd0 = sm_desc_scales(smem_u32(smem) + L::kSfOffset);
+    for (int i = 0; i < total; ++i) {
+      if (!warp_wait(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t at = static_cast<uint32_t>(stage * (L::kStage >> 4));
+      const uint64_t wd = wd0 + at, xd = xd0 + at, sd = sd0 + at;
+      if (i < kb1 - kb0) {
+        const uint32_t sfa = tmem + 2 * NB + stage * L::kSfCols, sfb = sfa + L::kChunks * 4;
+        const int nk = kb0 + i == args.num_kb - 1 ? args.last_k64 : 4;
+        if (elect_one()) {
+#pragma unroll
+          for (int j = 0; j < L::kChunks; ++j) {
+            sm_cp_scales(sfa + 4 * j, sd + static_cast<uint32_t>(32 * j));
+            sm_cp_scales(sfb + 4 * j, sd + static_cast<uint32_t>(32 * (L::kChunks + j)));
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            constexpr bool kMx = FMT == LORA_MXFP4;
+            const int j = kMx ? k >> 1 : k;
+            const uint32_t id = kMx ? static_cast<uint32_t>(k & 1) * 2u : 0u;
+            if (k < nk)
+              sm_mma<FMT>(tmem, wd + static_cast<uint32_t>(2 * k), xd + static_cast<uint32_t>(2 * k),
+                          kIdesc | (id << 4) | (id << 29), sfa + 4 * j, sfb + 4 * j, (i > 0 || k > 0) ? 1u : 0u);
+          }
+          tc_commit(&empty[stage]);
+        }
+      } else {
+        const int t = i - (kb1 - kb0);
+        const int c = t >= args.rank_kb ? t - args.rank_kb : t;
+        const int nk = c == args.rank_kb - 1 ? args.last_k16 : 4;
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (k < nk)
+              tc_mma_f16(tmem + NB, wd + static_cast<uint32_t>(2 * k), xd + static_cast<uint32_t>(2 * k), kIdescTail,
+                         (t > 0 || k > 0) ? 1u : 0u);
+          tc_commit(&empty[stage]);
+        }
+      }
+      __syncwarp();
+      if (++stage == args.stages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+    if (ok && elect_one()) tc_commit(acc_full);
+    __syncwarp();
+  }
+
+  // ---- epilogue: warps 2..5 put the partial tile, one row of W a thread, into the
+  // drained stages as [token][128]; then a warp sums and stores one token's 128
+  // columns at a time, the ranks' parts in rank order
+  const int count = min(NB, args.M - t0);
+  float* part = reinterpret_cast<float*>(smem);
+  if (warp >= 2 && warp_wait(acc_full, 0, abort_flag, args.err, kDevErrTimeoutAccFull)) {
+    tc_fence_after();
+    const int quad = warp & 3;
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t dst = smem_u32(part) + (quad * 32 + lane) * 4;
+#pragma unroll 1
+    for (int c = 0; c < count; c += 16) {
+      uint32_t u[16], l[16];
+      tmem_ld_32x32b_x16(t_row + c, u);
+      if (tail_kb > 0) tmem_ld_32x32b_x16(t_row + NB + c, l);
+      tmem_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float v = __uint_as_float(u[e]) * args.base_scale;
+        if (tail_kb > 0) v += __uint_as_float(l[e]);
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + (c + e) * 512), "f"(v) : "memory");
+      }
+    }
+  }
+  if (splits > 1)
+    cluster_sync_all();  // every rank's partial tile is in its shared memory
+  else
+    __syncthreads();
+  {
+    const int b = count * rank / splits, e = count * (rank + 1) / splits;
+    const int n = n0 + 4 * lane;
+    const bool vec = args.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(args.out) & 7) == 0 && n + 4 <= args.N;
+    const T* bias = static_cast<const T*>(args.bias);
+    float add[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (bias != nullptr && n + i < args.N) add[i] = to_f32(bias[n + i]);
+    const uint32_t src = smem_u32(part) + lane * 16;
+    for (int t = b + warp; t < e; t += kSmThreads / 32) {
+      float4 v;
+      if (splits == 1) {
+        const uint4 u = lds128(src + t * 512);
+        v = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+      } else {
+        float4 p[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (q < splits) p[q] = ld_dsmem_f4(mapa_shared(src + t * 512, q));
+        v = p[0];
+#pragma unroll
+        for (int q = 1; q < 8; ++q)
+          if (q < splits) v.x += p[q].x, v.y += p[q].y, v.z += p[q].z, v.w += p[q].w;
+      }
+      v.x = v.x * args.alpha + add[0], v.y = v.y * args.alpha + add[1];
+      v.z = v.z * args.alpha + add[2], v.w = v.w * args.alpha + add[3];
+      T* o = static_cast<T*>(args.out) + static_cast<int64_t>(t0 + t) * args.ldo + n;
+      if (vec) {
+        *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+      } else {
+        if (n < args.N) o[0] = from_f32<T>(v.x);
+        if (n + 1 < args.N) o[1] = from_f32<T>(v.y);
+        if (n + 2 < args.N) o[2] = from_f32<T>(v.z);
+        if (n + 3 < args.N) o[3] = from_f32<T>(v.w);
+      }
+    }
+  }
+  tc_fence_before();
+  if (splits > 1)
+    cluster_sync_all();  // no CTA leaves while another reads its partial tile
+  else
+    __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+template <typename T, int FMT, int NB>
+int launch_small(const MxLinearOperands& o, cudaStream_t stream) {
+  using L = SmLayout<FMT, NB>;
+  const int dev = current_device();
+  if (dev < 0) return LORA_ERR_DEVICE;
+  const DeviceInfo& info = device_info(dev);
+  SmMaps maps;
+  SmArgs a;
+  const int64_t pitch = mx_code_pitch(o.K, FMT);
+  a.chunks = static_cast<int>(mx_scale_chunks(o.K, FMT));
+  if (!mx_encode_map(&maps.x, o.x_codes, 1, pitch, o.M, pitch, 128, NB, true) ||
+      !mx_encode_map(&maps.w, o.w_codes, 1, pitch, o.N, pitch, 128, 128, true) ||
+      !mx_encode_map(&maps.sx, o.x_scales, 4, 128, (o.M + 127) / 128 * a.chunks, 512, 128, L::kChunks, false) ||
+      !mx_encode_map(&maps.sw, o.w_scales, 4, 128, (o.N + 127) / 128 * a.chunks, 512, 128, L::kChunks, false))
+    return LORA_ERR_CUDA;
+  if (o.R > 0) {
+    const char* z = static_cast<const char*>(o.z);
+    if (!mx_encode_map(&maps.zh, z, 2, o.R, o.M, o.ldz * 2, 64, NB, true) ||
+        !mx_encode_map(&maps.zl, z + o.z_lo * 2, 2, o.R, o.M, o.ldz * 2, 64, NB, true) ||
+        !mx_encode_map(&maps.b, o.b, 2, o.R, o.N, o.ldb * 2, 64, 128, true))
+      return LORA_ERR_CUDA;
+  } else {
+    maps.zh = maps.zl = maps.b = maps.x;
+  }
+  a.out = o.out;
+  a.bias = o.bias;
+  a.err = info.err_word;
+  a.ldo = o.ldo;
+  a.M = static_cast<int>(o.M);
+  a.N = static_cast<int>(o.N);
+  const int64_t kp = mx_padded_k(o.K);
+  a.num_kb = static_cast<int>((kp + 255) / 256);
+  a.last_k64 = static_cast<int>((kp - (a.num_kb - 1) * 256ll + 63) / 64);
+  a.rank_kb = static_cast<int>((o.R + 63) / 64);
+  a.last_k16 = a.rank_kb > 0 ? static_cast<int>((o.R - (a.rank_kb - 1) * 64ll + 15) / 16) : 0;
+  a.alpha = o.alpha;
+  a.base_scale = ldexpf(1.f, -o.dshift);
+  // The partial tile (NB x 128 fp32) lies over the stages.
+  constexpr int kFixed = 1024 + 256;
+  a.stages = std::min<int>(L::kMaxStages, (sm_smem_max<NB>() - kFixed) / L::kStage);
+  const int n_tiles = static_cast<int>((o.N + 127) / 128), t_tiles = static_cast<int>((o.M + NB - 1) / NB);
+  // as many CTAs as are resident at once, each with two or more stages of K
+  const int resident = (NB == 128 ? 1 : 2) * info.num_sms;
+  int splits = 1;
+  while (splits < 8 && n_tiles * t_tiles * splits * 2 <= resident && a.num_kb >= 4 * splits) splits *= 2;
+  // over a third (NB 128: half) of an SM's shared memory: no third (second) CTA joins
+  size_t smem = static_cast<size_t>(a.stages) * L::kStage;
+  static_assert(L::kStage * 2 >= NB * 512 || NB == 128, "the partial tile lies over the stages");
+  if (smem < static_cast<size_t>(NB) * 512) return LORA_ERR_UNSUPPORTED;
+  smem = std::max<size_t>(smem + kFixed, NB == 128 ? 120 * 1024 : 80 * 1024);
+  auto kernel = mx_small_kernel<T, FMT, NB>;
+  static std::once_flag once[64];
+  static cudaError_t attr_err[64];
+  std::call_once(once[dev], [&] {
+    attr_err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sm_smem_max<NB>());
+  });
+  if (attr_err[dev] != cudaSuccess) return LORA_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(n_tiles * splits, t_tiles);
+  cfg.blockDim = dim3(kSmThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, maps, a) != cudaSuccess) {
+    cudaGetLastError();
+    return LORA_ERR_CUDA;
+  }
+  return LORA_OK;
+}
+
+template <typename T, int FMT>
+int dispatch(const MxLinearOperands& o, cudaStream_t s) {
+  if (o.M <= 16) return launch_small<T, FMT, 16>(o, s);
+  if (o.M <= 32) return launch_small<T, FMT, 32>(o, s);
+  if (o.M <= 64) return launch_small<T, FMT, 64>(o, s);
+  return launch_small<T, FMT, 128>(o, s);
+}
+
+}  // namespace
+
+int mx_small_launch(const MxLinearOperands& o, int fmt, int dtype, cudaStream_t s) {
+  if (dtype == LORA_BF16)
+    return fmt == LORA_MXFP4 ? dispatch<__nv_bfloat16, LORA_MXFP4>(o, s) : dispatch<__nv_bfloat16, LORA_NVFP4>(o, s);
+  return fmt == LORA_MXFP4 ? dispatch<__half, LORA_MXFP4>(o, s) : dispatch<__half, LORA_NVFP4>(o, s);
+}
+
+}  // namespace lora
