@@ -405,11 +405,13 @@ LORA_API int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, con
  *   db = z_scale * dy^T . z       [N, R]
  *   dx = dy . W + g . a           [M, K], where dx is not NULL
  * dy [M, N]; X: x as an MXFP8 tensor (x_codes, x_scales); z [M, 2 r16] as
- * lora_mx_linear's z_out, of which the hi part is read, z_scale its factor; W as
+ * lora_mx_linear's z_out (columns R..r16-1 of each half are not used), z_scale its
+ * factor; W as
  * an MXFP4 / NVFP4 tensor [N, K] (read for dx only).  W is frozen and rounding to
- * 8 or 4 bits counts as the identity.  Products accumulate in fp32, z and g are
- * rounded to dtype once, outputs are written once in dtype; token ranges are
- * summed in a fixed order.  1 <= R <= 256; z, codes and scales 16-byte aligned.
+ * 8 or 4 bits counts as the identity.  Products accumulate in fp32; g, like z, is
+ * held as a hi/lo pair of dtype, of which da and db take both halves up to rank 64
+ * and the hi half above; outputs are rounded once to dtype; token ranges are summed
+ * in a fixed order.  1 <= R <= 256; z, codes and scales 16-byte aligned.
  * Workspace: lora_mx_backward_workspace_size bytes, 256-byte aligned, zeroed
  * ticket region first as lora_shrink's.  No counterpart in the reference, which
  * has no backward pass. */

@@ -3,7 +3,9 @@
 A drop-in for the ``loraforge_kernels`` package of lishenghui/probe: the same
 public names (``__init__.py:1-71`` there), backed by hand-written CUDA for
 Blackwell behind the C ABI in ``include/lora_b200.h``.  The PEFT bridge is
-resolved lazily, as in the reference.
+resolved lazily, as in the reference.  ``mx`` adds what the reference lacks: base
+weights in microscaled 4-bit formats and the adapter's gradients from 8-bit
+activation checkpoints.
 """
 
 from .fused_linear import (
@@ -23,6 +25,16 @@ from .fused_linear import (
     selection_report,
 )
 from .fused_lora import classed_lora, classed_tiled_lora, fused_lora, grouped_lora, tiled_lora
+from .mx import (
+    MXLoRALinear,
+    MXTensor,
+    mx_dequantize,
+    mx_lora_backward,
+    mx_lora_forward,
+    mx_lora_linear,
+    mx_quantize,
+    nvfp4_global_scale,
+)
 from .overlapped_linear import DualStreamOverlappedLinear
 from .runtime_lora import attach_fused_lora, fused_lora_module_count, total_fused_rank
 from .splitk_lora import (
@@ -64,6 +76,14 @@ __all__ = [
     "align_to_deploy_rank",
     "DEPLOY_RANK_BUCKETS",
     "DualStreamOverlappedLinear",
+    "MXTensor",
+    "MXLoRALinear",
+    "mx_quantize",
+    "mx_dequantize",
+    "mx_lora_linear",
+    "mx_lora_forward",
+    "mx_lora_backward",
+    "nvfp4_global_scale",
 ]
 
 

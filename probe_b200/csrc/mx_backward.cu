@@ -1,7 +1,7 @@
 // Backward pass of the LoRA linear from an 8-bit checkpoint of its input.
 //
 //   g  = s dy B                [M, R]
-//   dB = zs dy^T z             [N, R]     z: the forward pass's hi/lo pair, hi part
+//   dB = zs dy^T z             [N, R]     z: the forward pass's hi/lo pair
 //   dA = g^T X8                [R, K]
 //   dx = dy Wq + g A           [M, K]     where asked for
 //

@@ -15,8 +15,10 @@
 // values in the MMA's swizzled layout.  E4M3 times a power of two is exact in
 // bf16: the code's exponent and mantissa moved into place, times 2^120, times the
 // scale.  Bound: HBM for small ranks (2 or 1.03 bytes an element of V), the tensor
-// pipe above r ~ 100; P is rounded once to 16 bits, whose error (2^-9 of each
-// term, independent) stays below that of the 16-bit result.
+// pipe above r ~ 100.  Up to rank 64 P is the whole hi/lo pair (N = 2 r, the halves
+// added in the epilogue), free while HBM is the bound; above, where it would double
+// the tensor pipe's work, the hi part alone, whose rounding (2^-9 of each term,
+// independent) stays below that of the 16-bit result.
 #include <mutex>
 
 #include "mx_grad.h"
@@ -42,7 +44,8 @@ struct GrArgs {
   float* part;  // [splits][C][ldp]
   int* err;
   int64_t C;
-  int M, r16, p_chunks, stages, stage_bytes, steps_per_split, steps, splits, scale_gb;
+  int M, r16, n, p_chunks,  // n: columns of P (2 r16 with the lo part, else r16)
+      stages, stage_bytes, steps_per_split, steps, splits, scale_gb;
 };
 
 // MN-major operand in 64-wide chunks: token rows 128 bytes apart, 8-row groups
@@ -121,8 +124,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
   const int64_t col0 = static_cast<int64_t>(blockIdx.x) * kGrCols;
   const int step0 = static_cast<int>(blockIdx.y) * args.steps_per_split;
   const int step1 = min(step0 + args.steps_per_split, args.steps);
-  const uint32_t tmem_cols = 2 * args.r16 <= 32 ? 32u : 2 * args.r16 <= 64 ? 64u : 2 * args.r16 <= 128 ? 128u
-                             : 2 * args.r16 <= 256 ? 256u : 512u;
+  const uint32_t tmem_cols = args.n <= 16 ? 32u : args.n <= 32 ? 64u : args.n <= 64 ? 128u : args.n <= 128 ? 256u : 512u;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < args.stages; ++s) {
@@ -179,9 +181,9 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     }
   } else if (warp == 1) {
     // The whole warp walks the stages (uniform descriptors); one lane issues.  Both
-    // operands MN-major (bits 15 and 16), M = 128, N = r16.
+    // operands MN-major (bits 15 and 16), M = 128.
     const uint32_t idesc = (umma_idesc_f16(128, 16, std::is_same<T, __nv_bfloat16>::value ? 1 : 0) & ~(0x3fu << 17)) |
-                           (static_cast<uint32_t>(args.r16 >> 3) << 17) | (1u << 15) | (1u << 16);
+                           (static_cast<uint32_t>(args.n >> 3) << 17) | (1u << 15) | (1u << 16);
     const uint64_t desc0 = gr_desc_mn(smem_u32(smem), kGrChunkBytes);
     const uint64_t conv0 = gr_desc_mn(smem_u32(conv), kGrChunkBytes);
     int stage = 0;
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
         for (int k = 0; k < kGrTok / 16; ++k)
 #pragma unroll
           for (int m = 0; m < 2; ++m)
-            tc_mma_f16(tmem + m * args.r16, v + static_cast<uint32_t>((m * 2 * kGrChunkBytes + k * 2048) >> 4),
+            tc_mma_f16(tmem + m * args.n, v + static_cast<uint32_t>((m * 2 * kGrChunkBytes + k * 2048) >> 4),
                        pd + static_cast<uint32_t>((k * 2048) >> 4), idesc, (n > 0 || k > 0) ? 1u : 0u);
         tc_commit(&empty[stage]);
         if (F8) tc_commit(&conv_empty[n & 1]);
@@ -254,9 +256,15 @@ __global__ void __launch_bounds__(kGrThreads, 1)
       const int64_t c = col0 + m * 128 + quad * 32 + lane;
       float* dst = args.part + (static_cast<int64_t>(blockIdx.y) * args.C + c) * args.r16;
       for (int j = (cw >> 3) * 16; j < args.r16; j += 32) {
-        uint32_t r[16];
-        tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + m * args.r16 + j, r);
+        const uint32_t src = tmem + (static_cast<uint32_t>(quad * 32) << 16) + m * args.n + j;
+        uint32_t r[16], lo[16];
+        tmem_ld_32x32b_x16(src, r);
+        if (args.n > args.r16) tmem_ld_32x32b_x16(src + args.r16, lo);
         tmem_wait_ld();
+        if (args.n > args.r16) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) + __uint_as_float(lo[e]));
+        }
         if (c < args.C) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -336,7 +344,8 @@ int launch_grad(const MxGradOperands& g, const GrPlan& pl, cudaStream_t stream) 
   a.C = g.C;
   a.M = static_cast<int>(g.M);
   a.r16 = static_cast<int>((g.R + 15) / 16 * 16);
-  a.p_chunks = (a.r16 + 63) / 64;
+  a.n = a.r16 <= 64 ? 2 * a.r16 : a.r16;
+  a.p_chunks = (a.n + 63) / 64;
   a.steps = pl.steps;
   a.splits = pl.splits;
   a.steps_per_split = pl.steps_per_split;
@@ -353,7 +362,7 @@ int launch_grad(const MxGradOperands& g, const GrPlan& pl, cudaStream_t stream) 
     if (!mx_encode_map(&maps.v, g.v, 2, g.C, g.M, g.ldv * 2, 64, kGrTok, true)) return LORA_ERR_CUDA;
     maps.sc = maps.v;
   }
-  if (!mx_encode_map(&maps.p, g.p, 2, g.R, g.M, g.ldp * 2, 64, kGrTok, true)) return LORA_ERR_CUDA;
+  if (!mx_encode_map(&maps.p, g.p, 2, a.n, g.M, g.ldp * 2, 64, kGrTok, true)) return LORA_ERR_CUDA;
   auto kernel = mx_grad_kernel<T, F8>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];

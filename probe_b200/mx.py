@@ -6,6 +6,13 @@ A frozen base weight in 4 bits, an activation kept for the backward pass in 8:
     to and from ``mxfp4`` (E2M1 codes, a power of two per 32 values), ``nvfp4``
     (E2M1, an E4M3 scale per 16 values and one fp32 scale a tensor) and
     ``mxfp8`` (E4M3, a power of two per 32 values).
+``mx_lora_linear``
+    the LoRA linear with W and the quantised input in 4 bits (block-scaled
+    tcgen05 MMAs) and the adapter in 16.
+``mx_lora_forward`` / ``mx_lora_backward``
+    the same with an 8-bit checkpoint of its input, and the gradients from it.
+``MXLoRALinear``
+    all of it as a module: a base frozen in 4 bits under a trainable adapter.
 
 Everything runs in the sm_100a kernels behind ``include/lora_b200.h``; CPU
 tensors raise.
@@ -255,8 +262,8 @@ def mx_lora_backward(dy: torch.Tensor, x8: MXTensor, z: torch.Tensor, a: torch.T
 
     ``g = scale * dy @ b``;  ``da = g.T @ X`` [r, K];  ``db = z_scale * dy.T @ z`` [N, r];
     ``dx = dy @ W + g @ a`` [..., K], or None without ``weight``.  ``x8`` is the mxfp8
-    checkpoint of x, ``z`` the [M, 2 r16] pair of the forward pass (its hi half is
-    read), W an mxfp4 / nvfp4 tensor.  W is frozen; rounding to 4 or 8 bits counts
+    checkpoint of x, ``z`` the [M, 2 r16] pair [hi | lo] of the forward pass (above
+    rank 64 its hi half alone is read), W an mxfp4 / nvfp4 tensor.  W is frozen; rounding to 4 or 8 bits counts
     as the identity.
     """
     where = "mx_lora_backward"
@@ -295,3 +302,94 @@ def mx_lora_backward(dy: torch.Tensor, x8: MXTensor, z: torch.Tensor, a: torch.T
     if rc:
         _lib.check(rc, "lora_mx_backward")
     return (dx if dx is None or len(shape) == 2 else dx.view(*shape[:-1], k)), da, db
+
+
+def mx_lora_forward(x: torch.Tensor, weight: MXTensor, bias: torch.Tensor | None, a: torch.Tensor, b: torch.Tensor,
+                    scale: float = 1.0, x_global_scale: float = 1.0):
+    """The linear with what its backward pass keeps: ``(y, x8, z, z_scale)``.
+
+    ``y`` as ``mx_lora_linear``; ``x8`` the mxfp8 checkpoint of x (half its bytes),
+    ``z`` the [M, 2 r16] pair with ``z_scale * (hi + lo) = scale * x @ a.T``.
+    """
+    if a is None or b is None or a.shape[0] == 0 or scale == 0:
+        raise ValueError("mx_lora_forward: an adapter (rank >= 1, scale != 0) is required")
+    y, z = _linear(x, weight, bias, a, b, scale, x_global_scale, True, "mx_lora_forward")
+    z_scale = _entry("lora_mx_linear_z_scale")(float(x_global_scale), weight.global_scale, weight._code)
+    return y, mx_quantize(x, "mxfp8"), z, z_scale
+
+
+class _MXLoRAFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, a, b, weight, bias, scale, x_global_scale):
+        a, b = a.detach(), b.detach()
+        y, x8, z, ctx.z_scale = mx_lora_forward(x, weight, bias, a, b, scale, x_global_scale)
+        ctx.save_for_backward(x8.codes, x8.scales, z, a, b)
+        ctx.x_shape, ctx.weight, ctx.scale = x8.shape, weight, scale
+        ctx.set_materialize_grads(False)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        if dy is None:
+            return (None,) * 7
+        codes, scales, z, a, b = ctx.saved_tensors
+        x8 = MXTensor(codes, scales, ctx.x_shape, "mxfp8")
+        need_x, need_a, need_b = ctx.needs_input_grad[:3]
+        dx, da, db = mx_lora_backward(dy, x8, z, a, b, ctx.scale, ctx.weight if need_x else None, ctx.z_scale)
+        return dx, da if need_a else None, db if need_b else None, None, None, None, None
+
+
+class MXLoRALinear(torch.nn.Module):
+    """An ``nn.Linear`` frozen in 4 bits with a trainable LoRA adapter.
+
+    ``y = q(x) @ W.T + bias + scale * (x @ lora_a.T) @ lora_b.T``.  W is quantised
+    once (``fmt`` mxfp4 or nvfp4) and frozen; ``lora_a`` [r, K] and ``lora_b`` [N, r]
+    are parameters.  While gradients are recorded the input is kept for the backward
+    pass in 8 bits (mxfp8) with the [M, r] product, and nothing else of its size;
+    without them the call is ``mx_lora_linear``.  ``x_amax``, for nvfp4: the largest
+    magnitude expected of the input (its calibration).
+    """
+
+    def __init__(self, base: torch.nn.Linear, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0,
+                 fmt: str = "mxfp4", x_amax: float = 32.0):
+        super().__init__()
+        if fmt not in ("mxfp4", "nvfp4"):
+            raise ValueError(f"MXLoRALinear: fmt must be mxfp4 or nvfp4, got {fmt!r}")
+        if a.shape[1] != base.in_features or b.shape[0] != base.out_features or a.shape[0] != b.shape[1]:
+            raise ValueError(
+                f"LoRA factors {tuple(a.shape)}/{tuple(b.shape)} do not match "
+                f"Linear({base.in_features}, {base.out_features})"
+            )
+        weight = base.weight.detach()
+        self.in_features, self.out_features = base.in_features, base.out_features
+        self.scale, self.fmt = float(scale), fmt
+        nv = fmt == "nvfp4"
+        self.w_global_scale = nvfp4_global_scale(weight.abs().max()) if nv else 1.0
+        self.x_global_scale = nvfp4_global_scale(x_amax) if nv else 1.0
+        q = mx_quantize(weight, fmt, self.w_global_scale)
+        self.register_buffer("w_codes", q.codes)
+        self.register_buffer("w_scales", q.scales)
+        self.register_buffer("bias", None if base.bias is None else base.bias.detach())
+        self.lora_a = torch.nn.Parameter(a.detach().to(weight).contiguous().clone())
+        self.lora_b = torch.nn.Parameter(b.detach().to(weight).contiguous().clone())
+
+    @property
+    def rank(self) -> int:
+        return self.lora_a.shape[0]
+
+    @property
+    def weight(self) -> MXTensor:
+        return MXTensor(self.w_codes, self.w_scales, (self.out_features, self.in_features), self.fmt,
+                        self.w_global_scale)
+
+    def extra_repr(self) -> str:
+        return (f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, "
+                f"rank={self.rank}, scale={self.scale}, fmt={self.fmt}")
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        learns = torch.is_grad_enabled() and (
+            x.requires_grad or self.lora_a.requires_grad or self.lora_b.requires_grad)
+        if learns:
+            return _MXLoRAFunction.apply(x, self.lora_a, self.lora_b, self.weight, self.bias, self.scale,
+                                         self.x_global_scale)
+        return mx_lora_linear(x, self.weight, self.bias, self.lora_a, self.lora_b, self.scale, self.x_global_scale)
