@@ -108,9 +108,8 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   if (lddy < N || lda < K || ldb < R || ldda < K || lddb < R || (dx != nullptr && lddx < K)) return LORA_ERR_SHAPE;
   if (dx != nullptr && !mx_global_ok(w_global, w_fmt)) return LORA_ERR_ARG;
   if (N == 0 || K == 0) return LORA_OK;
-  if (dy == nullptr || x_codes == nullptr || x_scales == nullptr || z == nullptr || a == nullptr || b == nullptr ||
-      da == nullptr || db == nullptr)
-    return LORA_ERR_ARG;
+  if (a == nullptr || b == nullptr || da == nullptr || db == nullptr) return LORA_ERR_ARG;
+  if (M > 0 && (dy == nullptr || x_codes == nullptr || x_scales == nullptr || z == nullptr)) return LORA_ERR_ARG;
   if (dx != nullptr && (w_codes == nullptr || w_scales == nullptr)) return LORA_ERR_ARG;
   if (!mx_aligned(x_codes, 16) || !mx_aligned(x_scales, 16) || !mx_aligned(z, 16) || !mx_aligned(workspace, 256) ||
       (dx != nullptr && (!mx_aligned(w_codes, 16) || !mx_aligned(w_scales, 16))))

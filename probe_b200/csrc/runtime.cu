@@ -27,7 +27,20 @@ int current_device() {
     cudaGetLastError();
     return -1;
   }
-  return (dev >= 0 && dev < kMaxDevices) ? dev : -1;
+  if (dev < 0 || dev >= kMaxDevices) return -1;
+  // A host thread that has made no runtime call yet (an autograd worker whose
+  // allocations all came from a cache) has no current context, and the driver's
+  // tensor-map encoder then fails: bind the device's context once per thread.
+  static thread_local uint64_t bound = 0;
+  static_assert(kMaxDevices <= 64, "one bit a device");
+  if (!(bound >> dev & 1)) {
+    if (cudaSetDevice(dev) != cudaSuccess) {
+      cudaGetLastError();
+      return -1;
+    }
+    bound |= uint64_t{1} << dev;
+  }
+  return dev;
 }
 
 const DeviceInfo& device_info(int dev) {

@@ -288,3 +288,17 @@ def test_module_refusals():
         mx.MXLoRALinear(base, a, b, fmt="mxfp8")
     with pytest.raises(ValueError, match="do not match"):
         mx.MXLoRALinear(base, a[:, :32], b)
+
+
+def test_from_a_fresh_host_thread():
+    """A thread whose first CUDA work is the call itself (its tensors come from the allocator's cache)."""
+    import threading
+
+    dy, x8, z, a, b, w = case(130, 192, 256, 12, torch.bfloat16)
+    want = mx.mx_lora_backward(dy, x8, z, a, b, 1.0, weight=w)
+    torch.cuda.synchronize()
+    got = []
+    t = threading.Thread(target=lambda: got.append(mx.mx_lora_backward(dy, x8, z, a, b, 1.0, weight=w)))
+    t.start()
+    t.join()
+    assert len(got) == 1 and all(torch.equal(p, q) for p, q in zip(got[0], want))
