@@ -22,7 +22,7 @@ namespace {
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 struct BackwardPlan {
-  size_t gemm_bytes, part, g, bt, at, dy, wt, total;
+  size_t gemm_bytes, part, part_a, g, bt, at, dy, wt, total;
 };
 
 BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need_dx) {
@@ -32,7 +32,9 @@ BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need
   size_t at = kCounterBytes;  // ticket counters, never scratch; the steps' partials follow them in turn
   at = std::max(at, mx_align(std::max(kCounterBytes + mx_shrink_part_bytes(M, np, R), p.gemm_bytes)));
   p.part = at;
-  at += mx_align(std::max(mx_grad_part_bytes(M, N, R), mx_grad_part_bytes(M, K, R)));
+  at += mx_align(mx_grad_part_bytes(M, N, R));
+  p.part_a = at;
+  at += mx_align(mx_grad_part_bytes(M, K, R));
   p.g = at;
   at += mx_align(static_cast<size_t>(M) * 2 * rp * 2);
   p.bt = at;
@@ -145,7 +147,8 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
     dyp = ws + p.dy;
     ldp = np;
   }
-  MxGradOperands gr = {};
+  MxGradOperands grads[2] = {};
+  MxGradOperands& gr = grads[0];
   gr.v = dyp;
   gr.ldv = ldp;
   gr.p = z;
@@ -184,15 +187,20 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   rc = mx_shrink_launch(sh, -1, dtype, s);
   if (rc != LORA_OK) return rc;
 
-  gr.v = x_codes;
-  gr.v_scales = x_scales;
-  gr.p = ws + p.g;
-  gr.out = da;
-  gr.ldo = ldda;
-  gr.C = K;
-  gr.factor = m;
-  gr.transposed = true;
-  rc = mx_grad_launch(gr, dtype, s);
+  MxGradOperands& ga = grads[1];
+  ga = gr;
+  ga.v = x_codes;
+  ga.v_scales = x_scales;
+  ga.p = ws + p.g;
+  ga.out = da;
+  ga.ldo = ldda;
+  ga.part = ws + p.part_a;
+  ga.C = K;
+  ga.factor = m;
+  ga.transposed = true;
+  rc = mx_grad_launch(ga, dtype, s);
+  if (rc != LORA_OK) return rc;
+  rc = mx_grad_reduce_launch(grads, 2, dtype, s);
   if (rc != LORA_OK || dx == nullptr) return rc;
 
   rc = transpose(a, lda, ws + p.at, 2 * rp, R, K, K, rp, 2, s);

@@ -282,35 +282,52 @@ __global__ void __launch_bounds__(kGrThreads, 1)
 }
 
 // Sum of the splits in order, times factor, rounded to T: out[c, j] (ldo) or,
-// transposed, out[j, c].  32 columns of V x 32 ranks a block.
+// transposed, out[j, c].  32 columns of V x 32 ranks a block; the blocks of several
+// gradients side by side.
+struct GrSum {
+  const float* part;
+  void* out;
+  int64_t ldo, C;
+  int r, r16, splits, blocks;
+  float factor;
+  bool transposed;
+};
+struct GrSums {
+  GrSum of[2];
+};
+
 template <typename T>
-__global__ void __launch_bounds__(256)
-    mx_grad_reduce_kernel(const float* __restrict__ part, T* __restrict__ out, int64_t ldo, int64_t C, int r, int r16,
-                          int splits, float factor, bool transposed) {
+__global__ void __launch_bounds__(256) mx_grad_reduce_kernel(const GrSums sums) {
   __shared__ float tile[32][33];
-  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * 32;
+  const bool second = static_cast<int>(blockIdx.x) >= sums.of[0].blocks;
+  const GrSum& g = second ? sums.of[1] : sums.of[0];
+  T* out = static_cast<T*>(g.out);
+  const int64_t c0 = static_cast<int64_t>(second ? blockIdx.x - sums.of[0].blocks : blockIdx.x) * 32;
   const int j0 = blockIdx.y * 32;
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  const int j = j0 + tx;
+  for (int s = 0; s < g.splits; ++s) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t c = c0 + ty + 8 * i;
+      if (c < g.C && j < g.r) v[i] += g.part[(s * g.C + c) * g.r16 + j];
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t c = c0 + ty + 8 * i;
-    const int j = j0 + tx;
-    float v = 0.f;
-    if (c < C && j < r) {
-      const float* p = part + c * r16 + j;
-      for (int s = 0; s < splits; ++s) v += p[s * C * r16];
-      v *= factor;
-      if (!transposed) out[c * ldo + j] = from_f32<T>(v);
-    }
-    if (transposed) tile[ty + 8 * i][tx] = v;
+    if (g.transposed)
+      tile[ty + 8 * i][tx] = v[i] * g.factor;
+    else if (c < g.C && j < g.r)
+      out[c * g.ldo + j] = from_f32<T>(v[i] * g.factor);
   }
-  if (transposed) {
+  if (g.transposed) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int j = j0 + ty + 8 * i;
       const int64_t c = c0 + tx;
-      if (c < C && j < r) out[j * ldo + c] = from_f32<T>(tile[tx][ty + 8 * i]);
+      if (c < g.C && j0 + ty + 8 * i < g.r) out[(j0 + ty + 8 * i) * g.ldo + c] = from_f32<T>(tile[tx][ty + 8 * i]);
     }
   }
 }
@@ -372,9 +389,6 @@ int launch_grad(const MxGradOperands& g, const GrPlan& pl, cudaStream_t stream) 
   if (attr_err[dev] != cudaSuccess) return LORA_ERR_CUDA;
   const size_t smem = static_cast<size_t>(a.stages) * a.stage_bytes + fixed;
   kernel<<<dim3(pl.groups, pl.splits), kGrThreads, smem, stream>>>(maps, a);
-  if (cudaGetLastError() != cudaSuccess) return LORA_ERR_CUDA;
-  mx_grad_reduce_kernel<T><<<dim3(static_cast<unsigned>((g.C + 31) / 32), (a.r16 + 31) / 32), 256, 0, stream>>>(
-      a.part, static_cast<T*>(g.out), g.ldo, g.C, static_cast<int>(g.R), a.r16, pl.splits, g.factor, g.transposed);
   return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
 }
 
@@ -390,6 +404,31 @@ int mx_grad_launch(const MxGradOperands& g, int dtype, cudaStream_t stream) {
   if (dtype == LORA_BF16)
     return f8 ? launch_grad<__nv_bfloat16, true>(g, pl, stream) : launch_grad<__nv_bfloat16, false>(g, pl, stream);
   return f8 ? launch_grad<__half, true>(g, pl, stream) : launch_grad<__half, false>(g, pl, stream);
+}
+
+int mx_grad_reduce_launch(const MxGradOperands* g, int count, int dtype, cudaStream_t stream) {
+  GrSums sums = {};
+  int blocks = 0, r32 = 0;
+  for (int i = 0; i < count; ++i) {
+    GrSum& s = sums.of[i];
+    s.part = static_cast<const float*>(g[i].part);
+    s.out = g[i].out;
+    s.ldo = g[i].ldo;
+    s.C = g[i].C;
+    s.r = static_cast<int>(g[i].R);
+    s.r16 = (s.r + 15) / 16 * 16;
+    s.splits = grad_plan(g[i].M, g[i].C).splits;
+    s.blocks = static_cast<int>((g[i].C + 31) / 32);
+    s.factor = g[i].factor;
+    s.transposed = g[i].transposed;
+    blocks += s.blocks;
+    r32 = std::max(r32, (s.r + 31) / 32);
+  }
+  if (dtype == LORA_BF16)
+    mx_grad_reduce_kernel<__nv_bfloat16><<<dim3(blocks, r32), 256, 0, stream>>>(sums);
+  else
+    mx_grad_reduce_kernel<__half><<<dim3(blocks, r32), 256, 0, stream>>>(sums);
+  return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
 }
 
 }  // namespace lora

@@ -17,6 +17,8 @@ struct MxGradOperands {
 };
 
 size_t mx_grad_part_bytes(int64_t M, int64_t C, int64_t R);
+// The partial sums of one gradient, and the sums of several in one launch.
 int mx_grad_launch(const MxGradOperands& g, int dtype, cudaStream_t stream);
+int mx_grad_reduce_launch(const MxGradOperands* g, int count, int dtype, cudaStream_t stream);
 
 }  // namespace lora

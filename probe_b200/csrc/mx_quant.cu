@@ -129,8 +129,10 @@ template <typename T, int FMT, bool TR>
 __global__ void __launch_bounds__(kMxThreads)
     mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out,
                          int64_t ldo, int64_t M, int64_t Mw, int64_t K, int64_t Kp, int chunks, float g, bool vec) {
-  constexpr int kPitch = kMxTile + 2;  // 16-bit elements: odd number of 4-byte words a row
-  __shared__ alignas(16) uint16_t tile[TR ? kMxTile * kPitch : 8];
+  // Transposed: rows of sixteen 16-byte units, unit u of row r at u ^ f(r), f(r) =
+  // 2 (r / 8 % 4) + r % 2, so that the eight rows an 8 x 8 matrix is gathered from
+  // below lie in different banks.
+  __shared__ alignas(128) uint16_t tile[TR ? kMxTile * kMxTile : 8];
   const int seg = threadIdx.x & 7;
   const int sub = threadIdx.x >> 3;
   const int64_t row0 = static_cast<int64_t>(blockIdx.y) * kMxTile;
@@ -162,8 +164,13 @@ __global__ void __launch_bounds__(kMxThreads)
     mx_decode16<T, FMT>(c[p], byte[p], g, o);
     if constexpr (TR) {
       const int r = 32 * p + sub;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(&tile[r * kPitch + seg * 16 + 2 * i]) = o[i];
+      const int f = ((r >> 3) & 3) * 2 + (r & 1);
+      const uint32_t base = smem_u32(tile) + r * 256;
+      const uint4 h0 = make_uint4(o[0], o[1], o[2], o[3]), h1 = make_uint4(o[4], o[5], o[6], o[7]);
+      // the upper segments store their second unit first: eight lanes, eight banks
+      const int swap = seg >> 2;
+      sts128(base + (((2 * seg + swap) ^ f) << 4), swap ? h1 : h0);
+      sts128(base + (((2 * seg + 1 - swap) ^ f) << 4), swap ? h0 : h1);
     } else if (row < M && col < K) {
       T* dst = out + row * ldo + col;
       if (vec && col + 16 <= K) {
@@ -181,20 +188,25 @@ __global__ void __launch_bounds__(kMxThreads)
     __syncthreads();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint16_t* o16 = reinterpret_cast<uint16_t*>(out);
-    // a warp writes one output row at a time: 128 values, four a lane (two pairs)
-    for (int cc = warp; cc < kMxTile; cc += kMxThreads / 32) {
-      if (col0 + cc >= K) break;
-      uint16_t* dst = o16 + (col0 + cc) * ldo + row0;
+    // 32 rows x 8 columns at a time: matrix i takes rows 8 q + 2 i + {0, 1} as its slots
+    // 2 q + {0, 1}, so that transposed lane (c, q) holds rows 8 q .. 8 q + 7 of column c
+    // -- 16 bytes of the output's row c
+    const int slot = lane & 7, mat = lane >> 3;
+    const int cc = lane >> 2, q = lane & 3;
+    for (int t = warp; t < 4 * (kMxTile / 8); t += kMxThreads / 32) {
+      const int rb = (t & 3) * 32, u = t >> 2;  // row block, unit of eight columns
+      const int r = rb + 8 * (slot >> 1) + 2 * mat + (slot & 1);
+      uint32_t v[4];
+      __syncwarp();
+      ldmatrix_x4_trans(v, smem_u32(tile) + r * 256 + ((u ^ (((r >> 3) & 3) * 2 + (r & 1))) << 4));
+      const int64_t c = col0 + u * 8 + cc, row = row0 + rb + 8 * q;
+      uint16_t* dst = o16 + c * ldo + row;
+      if (c < K && vec && row + 8 <= Mw) {
+        *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
+      } else if (c < K) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = 64 * h + 2 * lane;
-        const uint32_t lo = tile[r * kPitch + cc], hi = tile[(r + 1) * kPitch + cc];
-        if (vec && row0 + r + 2 <= Mw) {
-          *reinterpret_cast<uint32_t*>(dst + r) = lo | (hi << 16);
-        } else {
-          if (row0 + r < Mw) dst[r] = static_cast<uint16_t>(lo);
-          if (row0 + r + 1 < Mw) dst[r + 1] = static_cast<uint16_t>(hi);
-        }
+        for (int i = 0; i < 8; ++i)
+          if (row + i < Mw) dst[i] = static_cast<uint16_t>(v[i >> 1] >> (16 * (i & 1)));
       }
     }
   }
@@ -223,7 +235,7 @@ int dequantize_t(const void* codes, const void* scales, void* out, int64_t ldo, 
   const dim3 grid(static_cast<unsigned>((Kp + kMxTile - 1) / kMxTile), static_cast<unsigned>((M + kMxTile - 1) / kMxTile));
   const int chunks = static_cast<int>(mx_scale_chunks(K, FMT));
   if (transpose) {
-    const bool vec = aligned(out, 4) && ldo % 2 == 0;
+    const bool vec = aligned(out, 16) && ldo % 8 == 0;
     mx_dequantize_kernel<T, FMT, true><<<grid, kMxThreads, 0, stream>>>(
         static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<T*>(out), ldo, M, Mw, K,
         Kp, chunks, g, vec);

@@ -14,9 +14,10 @@
 // Work split: the (token block, chunk of columns) pairs in one sequence, cut into
 // equal runs, one per SM, so that any M fills the machine; a token block cut by a
 // run boundary leaves fp32 partials that its last contributor (a ticket) adds in
-// run order, so the result does not depend on timing.  Up to about 2000 tokens a
-// cluster of up to 8 CTAs takes each token block instead, its partial sums meet in
-// shared memory: no ticket, fence and reload, whose latencies would be half the call.
+// run order, so the result does not depend on timing.  Where token blocks are no more
+// than SMs (18944 tokens), a cluster of 8, 4, 2 or 1 CTAs takes each block instead and
+// its partial sums meet in shared memory: no ticket, fence and reload, whose latencies
+// would be half of a short call.
 #include <mutex>
 
 #include "mx_shrink.h"
@@ -432,9 +433,9 @@ int shrink_cluster(int64_t M, int64_t K, int64_t R) {
   const int dev = current_device();
   const int sms = dev >= 0 ? device_info(dev).num_sms : 148;
   const int64_t blocks = (M + 127) / 128, kc = (K + 64 * shrink_boxes(R) - 1) / (64 * shrink_boxes(R));
-  if (blocks * 8 > sms) return 0;
   int c = 8;
-  while (c > kc) c /= 2;
+  while (c > 1 && (c > kc || blocks * c > sms)) c /= 2;
+  if (blocks * c > sms) return 0;
   return c;
 }
 
