@@ -18,7 +18,7 @@
 // tiles.  Layout: a cluster of two CTAs per 256 x 256 tile, persistent; warp 0
 // TMA (codes in 128-byte swizzled rows, scale chunks as they are stored), warp
 // 1 of the leader copies the stage's scales to TMEM (tcgen05.cp, each CTA from
-// its own shared memory) and issues the MMAs, warps 2..9 the epilogue.
+// its own shared memory) and issues the MMAs, warps 2..9 the epilogue, warp 10 the scales' loads.
 // TMEM holds a buffer of scales per pipeline stage, so that a stage's full barrier
 // already says that its scale buffer is free: the MMA warp has 512 cycles a stage
 // and every further wait costs it 100 to 200.  Beside those 144 (mxfp4) or 240
@@ -36,7 +36,8 @@ namespace lora {
 namespace {
 
 constexpr int kMxEpiWarps = 8;  // two of each TMEM lane quadrant, taking 16-column groups in turn
-constexpr int kMxGemmThreads = 64 + 32 * kMxEpiWarps;
+constexpr int kMxScaleWarp = 2 + kMxEpiWarps;  // loads the scales
+constexpr int kMxGemmThreads = 64 + 32 * kMxEpiWarps + 32;
 
 struct MxGemmArgs {
   void* out;
@@ -48,6 +49,7 @@ struct MxGemmArgs {
   int last_k64;       // MMA steps of the last one
   int rank_kb;        // 64-deep tail stages of each z part (0: no adapter)
   int last_k16;       // MMA steps of the last of them
+  int fused_tail;     // 1: [zh | zl] in one stage (up to rank 32)
   int zero_kb;        // 1: a tail stage of zeros comes first
   int chunks;         // scale chunks of a block of 128 rows
   int num_m_tiles, num_n_tiles, num_tiles, group_m;
@@ -240,7 +242,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int tail_kb = 2 * args.rank_kb + args.zero_kb;
+  const int tail_kb = (args.fused_tail ? 1 : 2 * args.rank_kb) + args.zero_kb;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -262,13 +264,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
           uint8_t* b = sm_b + stage * L::kOpBytes;
           if (kb < args.num_kb) {
             if (leader) mbar_arrive_expect_tx(&full[stage], 2 * L::kMainBytes);
-            uint8_t* sf = sm_sf + stage * L::kSfBytes;
             tma_load_2d_pair(&maps.x, a, bar, kb * 128, row_a);
             tma_load_2d_pair(&maps.w, b, bar, kb * 128, row_b);
-            tma_load_2d_pair(&maps.sx, sf, bar, 0, (row_a >> 7) * args.chunks + kb * L::kChunks);
-            tma_load_2d_pair(&maps.sw, sf + L::kChunks * 512, bar, 0, nt * 2 * args.chunks + kb * L::kChunks);
-            tma_load_2d_pair(&maps.sw, sf + 2 * L::kChunks * 512, bar, 0,
-                             (nt * 2 + 1) * args.chunks + kb * L::kChunks);
           } else {
             if (leader) mbar_arrive_expect_tx(&full[stage], 4 * L::kOpBytes);
             // (the stage of zeros lies beyond the operands' columns)
@@ -277,6 +274,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
             const int c = (t < 0 ? args.rank_kb : lo ? t - args.rank_kb : t) * 64;
             tma_load_2d_pair(lo ? &maps.zl : &maps.zh, a, bar, c, row_a);
             tma_load_2d_pair(&maps.b, b, bar, c, row_b);
+          }
+          if (++stage == L::kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+    }
+  } else if (warp == kMxScaleWarp) {
+    // Five loads a stage are more than one thread issues in the stage's 512 cycles of
+    // MMAs (618 measured): the scales' two come from here.  Their bytes are part of
+    // the stage's expected ones.
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < args.num_tiles; tile += npairs) {
+        int mt, nt;
+        mx_tile_coords(tile, args, mt, nt);
+        for (int kb = 0; kb < args.num_kb + tail_kb; ++kb) {
+          // (the tail's stages are waited for too: a phase further on would read as free)
+          if (!mbar_wait_bounded(&empty[stage], phase ^ 1, abort_flag, args.err, kDevErrTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          if (kb < args.num_kb) {
+            const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);
+            uint8_t* sf = sm_sf + stage * L::kSfBytes;
+            tma_load_2d_pair(&maps.sx, sf, bar, 0,
+                             (mt * 2 + static_cast<int>(rank)) * args.chunks + kb * L::kChunks);
+            tma_load_3d_pair(&maps.sw, sf + L::kChunks * 512, bar, 0, kb * L::kChunks, nt * 2);
           }
           if (++stage == L::kStages) {
             stage = 0;
@@ -349,15 +377,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
           } else {
             const int t = kb - args.zero_kb;
             const int c = t >= args.rank_kb ? t - args.rank_kb : t;
-            const int nk = t < 0 ? 1 : c == args.rank_kb - 1 ? args.last_k16 : 4;
+            const int nk = t < 0 ? 1 : c == args.rank_kb - 1 ? args.last_k16 << args.fused_tail : 4;
             const int shift = t < 0 ? 15 : t == 0 ? args.dshift - 15 * args.zero_kb : 0;
+            // one stage of [zh | zl]: the lo part's steps meet the same columns of B
+            const int wrap = args.fused_tail ? args.last_k16 : 4;
             if (elect_one()) {
               mx_mma_f16_pair_shift(d, ad, bd, kIdescTail, shift);
 #pragma unroll
               for (int k = 1; k < 4; ++k)
                 if (k < nk)
-                  tc_mma_f16_pair(d, ad + static_cast<uint64_t>(2 * k), bd + static_cast<uint64_t>(2 * k), kIdescTail,
-                                  1u);
+                  tc_mma_f16_pair(d, ad + static_cast<uint64_t>(2 * k),
+                                  bd + static_cast<uint64_t>(2 * (k >= wrap ? k - wrap : k)), kIdescTail, 1u);
               tc_commit_pair(&empty[stage], kBoth);
             }
           }
@@ -422,6 +452,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
   }
 }
 
+// Scale chunks of two neighbouring blocks of 128 rows in one box: 128 words x
+// `box_chunks` chunks x 2 row blocks.
+bool encode_scale_pairs(CUtensorMap* map, const void* ptr, int64_t chunks, int64_t blocks, int box_chunks) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (enc == nullptr) return false;
+  const cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(chunks), static_cast<cuuint64_t>(blocks)};
+  const cuuint64_t strides[2] = {512, static_cast<cuuint64_t>(chunks) * 512};
+  const cuuint32_t box[3] = {128, static_cast<cuuint32_t>(box_chunks), 2};
+  const cuuint32_t one[3] = {1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(ptr), dims, strides, box, one,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int FMT>
 int launch_pair(const MxLinearOperands& o, cudaStream_t stream) {
   using L = MxSmem<FMT>;
@@ -435,15 +479,17 @@ int launch_pair(const MxLinearOperands& o, cudaStream_t stream) {
   if (!mx_encode_map(&maps.x, o.x_codes, 1, pitch, o.M, pitch, 128, 128, true) ||
       !mx_encode_map(&maps.w, o.w_codes, 1, pitch, o.N, pitch, 128, 128, true) ||
       !mx_encode_map(&maps.sx, o.x_scales, 4, 128, (o.M + 127) / 128 * a.chunks, 512, 128, L::kChunks, false) ||
-      !mx_encode_map(&maps.sw, o.w_scales, 4, 128, (o.N + 127) / 128 * a.chunks, 512, 128, L::kChunks, false))
+      !encode_scale_pairs(&maps.sw, o.w_scales, a.chunks, (o.N + 127) / 128, L::kChunks))
     return LORA_ERR_CUDA;
   if (o.R > 0) {
     const char* z = static_cast<const char*>(o.z);
-    if (!mx_encode_map(&maps.zh, z, 2, o.R, o.M, o.ldz * 2, 64, 128, true) ||
+    a.fused_tail = o.z_lo * 2 <= 64 ? 1 : 0;
+    if (!mx_encode_map(&maps.zh, z, 2, a.fused_tail ? 2 * o.z_lo : o.R, o.M, o.ldz * 2, 64, 128, true) ||
         !mx_encode_map(&maps.zl, z + o.z_lo * 2, 2, o.R, o.M, o.ldz * 2, 64, 128, true) ||
         !mx_encode_map(&maps.b, o.b, 2, o.R, o.N, o.ldb * 2, 64, 128, true))
       return LORA_ERR_CUDA;
   } else {
+    a.fused_tail = 0;
     maps.zh = maps.zl = maps.b = maps.x;
   }
   a.out = o.out;

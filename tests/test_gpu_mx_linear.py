@@ -53,6 +53,7 @@ SIZES = [
     (64, 1000, 2080, 16, True), (128, 256, 256, 64, False), (129, 513, 544, 20, True), (256, 512, 1024, 128, False),
     (257, 264, 288, 130, True), (600, 768, 1120, 224, True), (1025, 520, 512, 256, False), (70, 96, 64, 0, True),
     (300, 640, 768, 0, False), (2100, 2304, 320, 8, True),
+    (2560, 2304, 320, 224, False), (2500, 2400, 288, 32, True),  # more tiles than CTA pairs, long and short tails
 ]
 
 
