@@ -19,18 +19,25 @@
 namespace lora {
 namespace {
 
+// Rows up to which dx of an mxfp4 weight takes the W-streaming linear (its limit).
+constexpr int64_t kSmallDxRows = 256;
+
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 struct BackwardPlan {
-  size_t gemm_bytes, part, part_a, g, bt, at, dy, wt, total;
+  size_t gemm_bytes, small_bytes, part, part_a, g, bt, at, dy, wt, total;
 };
 
 BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need_dx) {
   BackwardPlan p = {};
   const int64_t np = up(N, 8), rp = up(R, 16);
-  if (need_dx) p.gemm_bytes = lora_gemm_workspace_size(M, K, np, 2 * rp);
+  if (need_dx) {
+    p.gemm_bytes = lora_gemm_workspace_size(M, K, np, 2 * rp);
+    if (M <= kSmallDxRows) p.small_bytes = lora_linear_small_workspace_size(M, K, R);
+  }
   size_t at = kCounterBytes;  // ticket counters, never scratch; the steps' partials follow them in turn
-  at = std::max(at, mx_align(std::max(kCounterBytes + mx_shrink_part_bytes(M, np, R), p.gemm_bytes)));
+  at = std::max(at, mx_align(std::max(kCounterBytes + std::max(mx_shrink_part_bytes(M, np, R), p.small_bytes),
+                                      p.gemm_bytes)));
   p.part = at;
   at += mx_align(mx_grad_part_bytes(M, N, R));
   p.part_a = at;
@@ -49,34 +56,52 @@ BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need
   return p;
 }
 
-// out[c, j] = in[j, c] for in [rows, cols]; rows of out beyond cols up to
-// out_rows, and columns beyond rows up to width, hold zeros; copies > 1 repeats
-// the width columns side by side.  32 x 32 a block.
-__global__ void __launch_bounds__(256)
-    mx_transpose_kernel(const uint16_t* __restrict__ in, int64_t ldi, uint16_t* __restrict__ out, int64_t ldo,
-                        int64_t rows, int64_t cols, int64_t out_rows, int64_t width, int copies) {
+// out[c, j] = in[j, c] for in [rows, cols], j < width (zeros beyond rows); `copies`
+// of the width columns side by side.  32 x 32 a block; the blocks of two matrices
+// side by side.
+struct TransposeJob {
+  const uint16_t* in;
+  uint16_t* out;
+  int64_t ldi, ldo, rows, cols, width;
+  int copies, blocks_c, blocks;
+};
+struct TransposeJobs {
+  TransposeJob of[2];
+};
+
+__global__ void __launch_bounds__(256) mx_transpose_kernel(const TransposeJobs jobs) {
   __shared__ uint16_t tile[32][34];
-  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * 32, j0 = static_cast<int64_t>(blockIdx.y) * 32;
+  const bool second = static_cast<int>(blockIdx.x) >= jobs.of[0].blocks;
+  const TransposeJob& t = second ? jobs.of[1] : jobs.of[0];
+  const int block = second ? blockIdx.x - jobs.of[0].blocks : blockIdx.x;
+  const int64_t c0 = static_cast<int64_t>(block % t.blocks_c) * 32, j0 = static_cast<int64_t>(block / t.blocks_c) * 32;
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t j = j0 + ty + 8 * i, c = c0 + tx;
-    tile[ty + 8 * i][tx] = j < rows && c < cols ? in[j * ldi + c] : 0;
+    tile[ty + 8 * i][tx] = j < t.rows && c < t.cols ? t.in[j * t.ldi + c] : 0;
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t c = c0 + ty + 8 * i, j = j0 + tx;
-    if (c < out_rows && j < width)
-      for (int k = 0; k < copies; ++k) out[c * ldo + k * width + j] = tile[tx][ty + 8 * i];
+    if (c < t.cols && j < t.width)
+      for (int k = 0; k < t.copies; ++k) t.out[c * t.ldo + k * t.width + j] = tile[tx][ty + 8 * i];
   }
 }
 
-int transpose(const void* in, int64_t ldi, void* out, int64_t ldo, int64_t rows, int64_t cols, int64_t out_rows,
-              int64_t width, int copies, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>(up(out_rows, 32) / 32), static_cast<unsigned>(up(width, 32) / 32));
-  mx_transpose_kernel<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(in), ldi, static_cast<uint16_t*>(out), ldo,
-                                           rows, cols, out_rows, width, copies);
+TransposeJob transpose_job(const void* in, int64_t ldi, void* out, int64_t ldo, int64_t rows, int64_t cols, int64_t width,
+                           int copies) {
+  TransposeJob t{static_cast<const uint16_t*>(in), static_cast<uint16_t*>(out), ldi, ldo, rows, cols, width, copies};
+  t.blocks_c = static_cast<int>(up(cols, 32) / 32);
+  t.blocks = t.blocks_c * static_cast<int>(up(width, 32) / 32);
+  return t;
+}
+
+int transpose(const TransposeJobs& jobs, cudaStream_t s) {
+  const int blocks = jobs.of[0].blocks + jobs.of[1].blocks;
+  if (blocks == 0) return LORA_OK;
+  mx_transpose_kernel<<<blocks, 256, 0, s>>>(jobs);
   return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
 }
 
@@ -137,7 +162,20 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
     m = 2.f * static_cast<float>(frexp(w_global, &e));
     pow2 = static_cast<float>(ldexp(1.0, e - 1));
   }
-  int rc = LORA_OK;
+  // What the weights give comes first: a kernel that reads it may start before its own
+  // predecessor on the stream has finished, so other launches lie between.
+  // few rows of an mxfp4 W (no fp32 factor on the product): the W-streaming linear
+  const bool small_dx = dx != nullptr && w_fmt == LORA_MXFP4 && M <= kSmallDxRows && R <= 128;
+  TransposeJobs jobs = {};
+  const bool b_rows = mx_aligned(b, 16) && ldb % 8 == 0;  // TMA can read them
+  if (!b_rows || small_dx) jobs.of[0] = transpose_job(b, ldb, ws + p.bt, np, N, R, np, 1);
+  if (dx != nullptr) jobs.of[1] = transpose_job(a, lda, ws + p.at, 2 * rp, R, K, rp, 2);
+  int rc = transpose(jobs, s);
+  if (rc != LORA_OK) return rc;
+  if (dx != nullptr) {
+    rc = mx_dequantize_launch(w_codes, w_scales, ws + p.wt, np, N, K, w_fmt, pow2, 2, dtype, s);
+    if (rc != LORA_OK) return rc;
+  }
   const void* dyp = dy;
   int64_t ldp = lddy;
   if (N % 8 != 0 || lddy % 8 != 0 || !mx_aligned(dy, 16)) {  // TMA needs 16-byte rows
@@ -166,11 +204,9 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   MxShrinkOperands sh = {};
   sh.v = dyp;
   sh.a = b;
-  sh.a_mn = mx_shrink_serves(dyp, ldp, b, ldb);
+  sh.a_mn = b_rows;
   sh.lda = ldb;
-  if (!sh.a_mn) {  // rows of B that TMA cannot read
-    rc = transpose(b, ldb, ws + p.bt, np, N, R, R, np, 1, s);
-    if (rc != LORA_OK) return rc;
+  if (!sh.a_mn) {
     sh.a = ws + p.bt;
     sh.lda = np;
   }
@@ -203,10 +239,11 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   rc = mx_grad_reduce_launch(grads, 2, dtype, s);
   if (rc != LORA_OK || dx == nullptr) return rc;
 
-  rc = transpose(a, lda, ws + p.at, 2 * rp, R, K, K, rp, 2, s);
-  if (rc != LORA_OK) return rc;
-  rc = mx_dequantize_launch(w_codes, w_scales, ws + p.wt, np, N, K, w_fmt, pow2, 2, dtype, s);
-  if (rc != LORA_OK) return rc;
+  if (small_dx) {
+    rc = lora_linear_small(dyp, ldp, ws + p.wt, np, ws + p.bt, np, ws + p.at, 2 * rp, nullptr, dx, lddx, M, K, np, R,
+                           scale, dtype, ws + kCounterBytes, p.small_bytes, s);
+    if (rc != LORA_ERR_UNSUPPORTED) return rc;
+  }
   return lora_gemm_ex(dyp, ldp, ws + p.wt, np, ws + p.g, 2 * rp, ws + p.at, 2 * rp, nullptr, dx, lddx, M, K, np, 2 * rp,
                       m, 0, dtype, p.gemm_bytes ? ws : nullptr, p.gemm_bytes, s);
 }

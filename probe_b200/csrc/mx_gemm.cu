@@ -242,6 +242,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_wait();  // the codes, scales and z of the kernels before
+  pdl_launch_dependents();
   const int tail_kb = (args.fused_tail ? 1 : 2 * args.rank_kb) + args.zero_kb;
 
   if (warp == 0) {
@@ -531,8 +533,7 @@ int launch_pair(const MxLinearOperands& o, cudaStream_t stream) {
   });
   if (attr_err[dev] != cudaSuccess) return LORA_ERR_CUDA;
   const int pairs = std::min(a.num_tiles, capacity[dev]);
-  kernel<<<2 * pairs, kMxGemmThreads, L::kBytes, stream>>>(maps, a);
-  return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
+  return mx_launch(kernel, dim3(2 * pairs), kMxGemmThreads, L::kBytes, stream, 0, maps, a);
 }
 
 }  // namespace

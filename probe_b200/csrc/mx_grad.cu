@@ -152,6 +152,8 @@ __global__ void __launch_bounds__(kGrThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -299,6 +301,8 @@ struct GrSums {
 template <typename T>
 __global__ void __launch_bounds__(256) mx_grad_reduce_kernel(const GrSums sums) {
   __shared__ float tile[32][33];
+  pdl_wait();
+  pdl_launch_dependents();
   const bool second = static_cast<int>(blockIdx.x) >= sums.of[0].blocks;
   const GrSum& g = second ? sums.of[1] : sums.of[0];
   T* out = static_cast<T*>(g.out);
@@ -388,8 +392,7 @@ int launch_grad(const MxGradOperands& g, const GrPlan& pl, cudaStream_t stream) 
   });
   if (attr_err[dev] != cudaSuccess) return LORA_ERR_CUDA;
   const size_t smem = static_cast<size_t>(a.stages) * a.stage_bytes + fixed;
-  kernel<<<dim3(pl.groups, pl.splits), kGrThreads, smem, stream>>>(maps, a);
-  return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
+  return mx_launch(kernel, dim3(pl.groups, pl.splits), kGrThreads, smem, stream, 0, maps, a);
 }
 
 }  // namespace
@@ -424,11 +427,8 @@ int mx_grad_reduce_launch(const MxGradOperands* g, int count, int dtype, cudaStr
     blocks += s.blocks;
     r32 = std::max(r32, (s.r + 31) / 32);
   }
-  if (dtype == LORA_BF16)
-    mx_grad_reduce_kernel<__nv_bfloat16><<<dim3(blocks, r32), 256, 0, stream>>>(sums);
-  else
-    mx_grad_reduce_kernel<__half><<<dim3(blocks, r32), 256, 0, stream>>>(sums);
-  return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
+  return mx_launch(dtype == LORA_BF16 ? mx_grad_reduce_kernel<__nv_bfloat16> : mx_grad_reduce_kernel<__half>,
+                   dim3(blocks, r32), 256, 0, stream, 0, sums);
 }
 
 }  // namespace lora

@@ -17,8 +17,13 @@ namespace {
 // Shrinks of more ranks than this run on the 16-bit tensor-core GEMM.
 constexpr int64_t kShrinkMaxRank = 128;
 
-// Rows up to which the W-streaming kernel runs.
-constexpr int64_t kSmallRows = 128;
+// The W-streaming kernel (mx_small.cu) runs one tile of 128 tokens, or as many 128 x
+// 128 tiles as there are SMs.  Measured whole calls, r = 16, mxfp4, against 256 x 256
+// pair tiles: N = K = 4096, 333 tokens 17.6 against 23.3 us, 512 18.8 against 23.5, 768
+// (192 tiles) 27.4 against 23.7; N = 11008, 256 (172 tiles) 26.9 against 23.5.
+bool few_tokens(int64_t M, int64_t N, int num_sms) {
+  return M <= 128 || (M + 127) / 128 * ((N + 127) / 128) <= num_sms;
+}
 
 int64_t r16(int64_t r) { return (r + 15) / 16 * 16; }
 
@@ -120,8 +125,8 @@ extern "C" int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, c
   }
   o.b = b;
   o.ldb = ldb;
-  // ahead of the other steps: a kernel that reads B before its predecessor on the
-  // stream has finished must not have this one as its predecessor
+  // two launches ahead of the kernel that reads B, which may start before its own
+  // predecessor on the stream has finished
   if (R > 0 && (ldb % 8 != 0 || !mx_aligned(b, 16))) {
     if (R % 8 == 0) return LORA_ERR_ALIGN;
     const int r8 = static_cast<int>((R + 7) / 8 * 8);
@@ -186,6 +191,6 @@ extern "C" int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, c
   o.N = N;
   o.K = K;
   o.R = R;
-  if (M <= kSmallRows) return mx_small_launch(o, fmt, dtype, s);
+  if (few_tokens(M, N, device_info(dev).num_sms)) return mx_small_launch(o, fmt, dtype, s);
   return mx_gemm_launch(o, fmt, dtype, s);
 }

@@ -25,6 +25,39 @@ int mx_gemm_launch(const MxLinearOperands& o, int fmt, int dtype, cudaStream_t s
 bool mx_encode_map(CUtensorMap* map, const void* ptr, int elem, int64_t inner, int64_t outer, int64_t pitch_bytes,
                    int box_inner, int box_outer, bool swizzle);
 
+// Launch with a thread-block cluster of `cluster` CTAs along x (0: none) and, unless
+// the process turned it off, as a programmatic dependent of the kernel before it:
+// the kernel calls pdl_wait before it touches what that one reads or writes, and
+// lets its own dependents start only after that, so that a kernel which reads
+// weights ahead of its wait finds everything up to two launches back complete.
+template <typename... P, typename... A>
+int mx_launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, int cluster, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  unsigned n = 0;
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 0) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
+    cudaGetLastError();
+    return LORA_ERR_CUDA;
+  }
+  return LORA_OK;
+}
+
 inline size_t mx_align(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 inline bool mx_aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 

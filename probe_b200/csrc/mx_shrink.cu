@@ -133,7 +133,8 @@ __global__ void __launch_bounds__(kShThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_launch_dependents();
+  pdl_wait();  // v, and the buffers that the kernels before may still read
+  pdl_launch_dependents();  // after the wait: a dependent may take what came before this kernel as done
 
   if (warp == 0) {
     if (lane == 0) {
@@ -481,27 +482,8 @@ int launch_shrink(const MxShrinkOperands& o, cudaStream_t stream) {
   });
   if (attr_err[dev] != cudaSuccess) return LORA_ERR_CUDA;
   const size_t smem = static_cast<size_t>(a.stages) * a.stage_bytes + kFixed + sums;
-  if (!a.cluster) {
-    kernel<<<shrink_ctas(o.M, o.K, o.R), kShThreads, smem, stream>>>(maps, a);
-    return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((o.M + 127) / 128 * a.cluster));
-  cfg.blockDim = dim3(kShThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = a.cluster;
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, maps, a) != cudaSuccess) {
-    cudaGetLastError();
-    return LORA_ERR_CUDA;
-  }
-  return LORA_OK;
+  const int64_t ctas = a.cluster ? (o.M + 127) / 128 * a.cluster : shrink_ctas(o.M, o.K, o.R);
+  return mx_launch(kernel, dim3(static_cast<unsigned>(ctas)), kShThreads, smem, stream, a.cluster, maps, a);
 }
 
 template <typename T, int KB>

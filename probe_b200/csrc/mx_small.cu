@@ -136,7 +136,6 @@ __global__ void __launch_bounds__(kSmThreads)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_launch_dependents();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -167,6 +166,7 @@ __global__ void __launch_bounds__(kSmThreads)
       const int pre = min(total, args.stages);
       for (int i = 0; i < pre; ++i) weights(i, i);
       pdl_wait();  // the shrink's codes, scales and z
+      pdl_launch_dependents();
       for (int i = 0; i < pre; ++i) tokens(i, i);
       int stage = pre == args.stages ? 0 : pre;
       uint32_t phase = pre == args.stages ? 1 : 0;
@@ -356,10 +356,10 @@ int launch_small(const MxLinearOperands& o, cudaStream_t stream) {
   constexpr int kFixed = 1024 + 256;
   a.stages = std::min<int>(L::kMaxStages, (sm_smem_max<NB>() - kFixed) / L::kStage);
   const int n_tiles = static_cast<int>((o.N + 127) / 128), t_tiles = static_cast<int>((o.M + NB - 1) / NB);
-  // as many CTAs as are resident at once, each with two or more stages of K
+  // as many CTAs as are resident at once, each with four or more stages of K
   const int resident = (NB == 128 ? 1 : 2) * info.num_sms;
   int splits = 1;
-  while (splits < 8 && n_tiles * t_tiles * splits * 2 <= resident && a.num_kb >= 4 * splits) splits *= 2;
+  while (splits < 8 && n_tiles * t_tiles * splits * 2 <= resident && a.num_kb >= 8 * splits) splits *= 2;
   // over a third (NB 128: half) of an SM's shared memory: no third (second) CTA joins
   size_t smem = static_cast<size_t>(a.stages) * L::kStage;
   static_assert(L::kStage * 2 >= NB * 512 || NB == 128, "the partial tile lies over the stages");
@@ -372,25 +372,7 @@ int launch_small(const MxLinearOperands& o, cudaStream_t stream) {
     attr_err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sm_smem_max<NB>());
   });
   if (attr_err[dev] != cudaSuccess) return LORA_ERR_CUDA;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(n_tiles * splits, t_tiles);
-  cfg.blockDim = dim3(kSmThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = splits;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, maps, a) != cudaSuccess) {
-    cudaGetLastError();
-    return LORA_ERR_CUDA;
-  }
-  return LORA_OK;
+  return mx_launch(kernel, dim3(n_tiles * splits, t_tiles), kSmThreads, smem, stream, splits, maps, a);
 }
 
 template <typename T, int FMT>
