@@ -71,6 +71,38 @@ LORA_DEVINL void sts128(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
+// 32-byte global accesses (32-byte aligned).
+LORA_DEVINL void ldg_stream_v8(const void* p, uint32_t* w) {
+  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p));
+}
+LORA_DEVINL void st_global_v8(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+// Two fp32 operations an instruction.
+LORA_DEVINL uint64_t f32x2(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+LORA_DEVINL void unpack_f32x2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+LORA_DEVINL uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+LORA_DEVINL uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+
 // One lane of a converged warp.  Asked anew in front of each block that one lane
 // executes, never kept: the code generator may repeat the election where a kept
 // answer is used, and in diverged code that elects several lanes.
@@ -164,10 +196,6 @@ inline MxGlobal mx_global(float g) {
 // reciprocal of d, one residual step makes x r the rounded x / d (Markstein,
 // 1990).  |x r| is kept below 2^20 so that the residual stays finite; every
 // quotient that large saturates.
-LORA_DEVINL float mx_div(float x, float d, float r) {
-  const float q = x * r;
-  return fmaf(fmaf(-q, d, x), r, q);
-}
 LORA_DEVINL float mx_div_far(float x, float d, float r) {
   const float q = fminf(fmaxf(x * r, -1048576.f), 1048576.f);
   return fmaf(fmaf(-q, d, x), r, q);
@@ -221,20 +249,21 @@ LORA_DEVINL void mx_codes16(const uint32_t* w, const MxScale<T, FMT>& s, uint32_
         v[2 * i] = mx_div_far(x.x, s.d, s.r);
         v[2 * i + 1] = mx_div_far(x.y, s.d, s.r);
       }
-    } else {
+    } else {  // mx_div_far without its clamp, on pairs
+      const uint64_t r = f32x2(s.r, s.r), nd = f32x2(-s.d, -s.d);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float2 x = unpack2<T>(w[i]);
-        v[2 * i] = mx_div(x.x, s.d, s.r);
-        v[2 * i + 1] = mx_div(x.y, s.d, s.r);
+        const uint64_t xx = f32x2(x.x, x.y);
+        const uint64_t q = mul_f32x2(xx, r);
+        unpack_f32x2(fma_f32x2(fma_f32x2(q, nd, xx), r, q), v[2 * i], v[2 * i + 1]);
       }
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float2 x = unpack2<T>(s.byte == 255u ? 0u : w[i]);
-      v[2 * i] = x.x * s.r;
-      v[2 * i + 1] = x.y * s.r;
+      unpack_f32x2(mul_f32x2(f32x2(x.x, x.y), f32x2(s.r, s.r)), v[2 * i], v[2 * i + 1]);
     }
   }
   if constexpr (MxFormat<FMT>::kBits == 4) {

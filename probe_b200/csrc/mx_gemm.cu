@@ -180,9 +180,7 @@ LORA_DEVINL void mx_store16(const MxGemmArgs& args, T* out_row, int row, int col
     uint32_t w[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out_row + col0), "r"(w[0]), "r"(w[1]),
-                 "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
+    st_global_v8(out_row + col0, w);
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
