@@ -89,7 +89,8 @@ def check(got, want):
 
 
 SIZES = [(1, 64, 32, 4), (1, 8, 256, 64), (2, 257, 96, 1), (63, 128, 130, 16), (64, 256, 256, 48), (65, 520, 288, 65),
-         (130, 1001, 544, 20), (300, 96, 1000, 224), (513, 264, 520, 256), (1030, 2304, 320, 8), (2600, 136, 264, 130)]
+         (130, 1001, 544, 20), (300, 96, 1000, 224), (513, 264, 520, 256), (1030, 2304, 320, 8), (2600, 136, 264, 130),
+         (4100, 264, 288, 200), (4097, 130, 160, 16)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
