@@ -67,6 +67,11 @@ LORA_DEVINL uint32_t lds_u8(uint32_t a) {
   asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
   return v;
 }
+LORA_DEVINL uint32_t lds_u16(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+  return v;
+}
 LORA_DEVINL void sts128(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -81,6 +86,38 @@ LORA_DEVINL void st_global_v8(void* p, const uint32_t* w) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
                "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
+}
+
+// 16 elements of 2 bytes of a row from column c, zeros at and beyond k, at any
+// 2-byte alignment: the aligned 16-byte words that hold them, funnelled into place
+// (no word is read that holds none of the 16).
+LORA_DEVINL void ldg16_any(const void* row, int64_t c, int64_t k, uint32_t* w) {
+  const uint16_t* p = static_cast<const uint16_t*>(row) + c;
+  if (c + 16 <= k) {
+    const uint32_t sh = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
+    const uint4* base = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(15));
+    const uint4 a = ldg_stream(base), b = ldg_stream(base + 1);
+    uint4 d = make_uint4(0u, 0u, 0u, 0u);
+    if (sh != 0) d = ldg_stream(base + 2);
+    uint32_t v[12] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, d.x, d.y, d.z, d.w};
+    if (sh & 8) {
+#pragma unroll
+      for (int i = 0; i < 10; ++i) v[i] = v[i + 2];
+    }
+    if (sh & 4) {
+#pragma unroll
+      for (int i = 0; i < 9; ++i) v[i] = v[i + 1];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = (sh & 2) ? __funnelshift_r(v[i], v[i + 1], 16) : v[i];
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t lo = c + 2 * i < k ? p[2 * i] : 0u;
+    const uint32_t hi = c + 2 * i + 1 < k ? p[2 * i + 1] : 0u;
+    w[i] = lo | (hi << 16);
+  }
 }
 
 // Two fp32 operations an instruction.

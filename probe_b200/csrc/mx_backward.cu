@@ -111,12 +111,17 @@ int transpose(const TransposeJobs& jobs, cudaStream_t s) {
   return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
 }
 
-// Rows of `cols` elements copied to rows of `width` (zeros beyond).
+// Rows of `cols` elements copied to 16-byte aligned rows of `width` (a multiple of 8;
+// zeros beyond cols), 16 elements a thread.
 __global__ void __launch_bounds__(256) mx_widen_kernel(const uint16_t* __restrict__ in, int64_t ldi,
-                                                       uint16_t* __restrict__ out, int64_t rows, int64_t cols,
-                                                       int64_t width) {
-  const int64_t row = blockIdx.x;
-  for (int64_t c = threadIdx.x; c < width; c += blockDim.x) out[row * width + c] = c < cols ? in[row * ldi + c] : 0;
+                                                       uint16_t* __restrict__ out, int64_t cols, int64_t width) {
+  const int64_t row = blockIdx.x, c = (static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x) * 16;
+  if (c >= width) return;
+  uint32_t w[8];
+  ldg16_any(in + row * ldi, c, cols, w);
+  uint4* dst = reinterpret_cast<uint4*>(out + row * width + c);
+  dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  if (c + 8 < width) dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
 }  // namespace
@@ -186,8 +191,9 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   const void* dyp = dy;
   int64_t ldp = lddy;
   if (N % 8 != 0 || lddy % 8 != 0 || !mx_aligned(dy, 16)) {  // TMA needs 16-byte rows
-    mx_widen_kernel<<<static_cast<unsigned>(M), 256, 0, s>>>(static_cast<const uint16_t*>(dy), lddy,
-                                                             reinterpret_cast<uint16_t*>(ws + p.dy), M, N, np);
+    const dim3 grid(static_cast<unsigned>(M), static_cast<unsigned>((np + 4095) / 4096));
+    mx_widen_kernel<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(dy), lddy, reinterpret_cast<uint16_t*>(ws + p.dy), N,
+                                         np);
     if (cudaGetLastError() != cudaSuccess) return LORA_ERR_CUDA;
     dyp = ws + p.dy;
     ldp = np;

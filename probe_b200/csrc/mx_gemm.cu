@@ -66,7 +66,8 @@ struct MxSmem {
   static constexpr int kMainBytes = 2 * kOpBytes + kSfBytes;
   static constexpr int kSfOffset = kStages * 2 * kOpBytes;
   static constexpr int kBarOffset = kSfOffset + kStages * kSfBytes;
-  static constexpr int kBytes = kBarOffset + 256 + 1024;
+  static constexpr int kEpiOffset = kBarOffset + 256;                 // 32 rows x 16 columns an epilogue warp
+  static constexpr int kBytes = kEpiOffset + kMxEpiWarps * 1024 + 1024;
   // TMEM columns
   static constexpr int kSfCols = 3 * kChunks * 4;
   static constexpr int kSfBase = 512 - kStages * kSfCols;
@@ -156,17 +157,21 @@ struct MxMaps {
   CUtensorMap x, w, sx, sw, zh, zl, b;
 };
 
-// 16 columns of one row: alpha, bias, rounding, one 32-byte store (vec: the row is
-// 32-byte aligned, bias 16-byte aligned).
-template <typename T>
-LORA_DEVINL void mx_store16(const MxGemmArgs& args, T* out_row, int row, int col0, bool vec, const uint32_t* r) {
-  if (row >= args.M || col0 >= args.N) return;
+// 16 columns of 32 rows, a row a lane: alpha, bias, rounding, then one 32-byte store
+// or two of 16 bytes (align: the rows' alignment), or (ANY), for rows of any alignment
+// and the last columns, 4-byte words through `stage` (1 KB of shared memory), eight lanes
+// a row -- 16 two-byte stores a lane made such a call five times as long.
+template <typename T, bool ANY>
+LORA_DEVINL void mx_store16(const MxGemmArgs& args, int row0, int lane, int col0, int align, uint32_t stage,
+                            const uint32_t* r) {
+  if (col0 >= args.N || row0 >= args.M) return;
   const T* bias = static_cast<const T*>(args.bias);
+  const int row = row0 + lane;
   float v[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]) * args.alpha;
-  if (vec && col0 + 16 <= args.N) {
-    if (bias != nullptr) {
+  if (bias != nullptr) {
+    if (col0 + 16 <= args.N && (reinterpret_cast<uintptr_t>(bias) & 15) == 0) {
       const uint4 b0 = __ldg(reinterpret_cast<const uint4*>(bias + col0));
       const uint4 b1 = __ldg(reinterpret_cast<const uint4*>(bias + col0 + 8));
       const uint32_t bw[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
@@ -176,19 +181,52 @@ LORA_DEVINL void mx_store16(const MxGemmArgs& args, T* out_row, int row, int col
         v[2 * i] += f.x;
         v[2 * i + 1] += f.y;
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (col0 + i < args.N) v[i] += to_f32(bias[col0 + i]);
     }
-    uint32_t w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
-    st_global_v8(out_row + col0, w);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (col0 + i < args.N) out_row[col0 + i] = from_f32<T>(v[i] + (bias != nullptr ? to_f32(bias[col0 + i]) : 0.f));
   }
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+  T* out = static_cast<T*>(args.out) + col0;
+  if (align >= 16 && col0 + 16 <= args.N) {
+    if (row >= args.M) return;
+    T* dst = out + static_cast<int64_t>(row) * args.ldo;
+    if (align == 32) {
+      st_global_v8(dst, w);
+    } else {
+      reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+    return;
+  }
+  if constexpr (!ANY) return;
+  sts128(stage + lane * 32, make_uint4(w[0], w[1], w[2], w[3]));
+  sts128(stage + lane * 32 + 16, make_uint4(w[4], w[5], w[6], w[7]));
+  __syncwarp();
+  const int n = min(16, args.N - col0), word = lane & 7;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int q = 4 * i + (lane >> 3);
+    if (row0 + q < args.M) {
+      uint16_t* dst = reinterpret_cast<uint16_t*>(out + static_cast<int64_t>(row0 + q) * args.ldo);
+      const int odd = (reinterpret_cast<uintptr_t>(dst) >> 1) & 1;  // elements ahead of the first whole word
+      const int e = odd + 2 * word;
+      const uint32_t src = stage + q * 32;
+      if (e + 1 < n)
+        *reinterpret_cast<uint32_t*>(dst + e) = lds_u16(src + 2 * e) | (lds_u16(src + 2 * e + 2) << 16);
+      else if (e < n)
+        dst[e] = static_cast<uint16_t>(lds_u16(src + 2 * e));
+      if (odd && word == 0) dst[0] = static_cast<uint16_t>(lds_u16(src));
+    }
+  }
+  __syncwarp();
 }
 
-template <typename T, int FMT>
+// ANY: rows that are not 16-byte aligned, or N no multiple of 16.
+template <typename T, int FMT, bool ANY>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
     mx_gemm_pair_kernel(const __grid_constant__ MxMaps maps, const MxGemmArgs args) {
   using L = MxSmem<FMT>;
@@ -402,8 +440,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
   } else {
     const int quad = warp & 3;
     const int part = (warp - 2) >> 2;  // takes the 16-column groups of this parity
-    const bool vec = (args.ldo % 16) == 0 && (reinterpret_cast<uintptr_t>(args.out) % 32) == 0 &&
-                     (reinterpret_cast<uintptr_t>(args.bias) % 16) == 0;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(args.out) | static_cast<uintptr_t>(args.ldo * 2);
+    const int align = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : 2;
+    const uint32_t stage = smem_u32(smem) + L::kEpiOffset + (warp - 2) * 1024;
     constexpr int kFirst = (L::kOverlap / 16 + 1) / 2;  // most shared groups of one warp
     int local = 0;
     for (int tile = pair; tile < args.num_tiles; tile += npairs, ++local) {
@@ -411,8 +450,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
       mx_tile_coords(tile, args, mt, nt);
       if (!warp_wait(acc_full, local & 1, abort_flag, args.err, kDevErrTimeoutAccFull)) break;
       tc_fence_after();
-      const int row = mt * 256 + static_cast<int>(rank) * 128 + quad * 32 + lane;
-      T* out_row = static_cast<T*>(args.out) + static_cast<int64_t>(row) * args.ldo;
+      const int row = mt * 256 + static_cast<int>(rank) * 128 + quad * 32;
       const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16) + ((local & 1) ? L::kAcc1 : 0);
       // Groups in the order: columns shared with the other accumulator, then the
       // rest.  The shared ones go to registers first, and the next tile may start.
@@ -429,7 +467,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
 #pragma unroll
         for (int q = 0; q < kFirst; ++q)
           if (2 * q + part < L::kOverlap / 16)
-            mx_store16<T>(args, out_row, row, nt * 256 + first + (2 * q + part) * 16, vec, r[q]);
+            mx_store16<T, ANY>(args, row, lane, nt * 256 + first + (2 * q + part) * 16, align, stage, r[q]);
       }
 #pragma unroll 1
       for (int g = (L::kOverlap / 16 - part + 1) / 2 * 2 + part; g < 16; g += 4) {
@@ -438,8 +476,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
         tmem_ld_32x32b_x16(t_row + c0, r[0]);
         if (g + 2 < 16) tmem_ld_32x32b_x16(t_row + c1, r[1]);
         tmem_wait_ld();
-        mx_store16<T>(args, out_row, row, nt * 256 + c0, vec, r[0]);
-        if (g + 2 < 16) mx_store16<T>(args, out_row, row, nt * 256 + c1, vec, r[1]);
+        mx_store16<T, ANY>(args, row, lane, nt * 256 + c0, align, stage, r[0]);
+        if (g + 2 < 16) mx_store16<T, ANY>(args, row, lane, nt * 256 + c1, align, stage, r[1]);
       }
     }
   }
@@ -466,7 +504,7 @@ bool encode_scale_pairs(CUtensorMap* map, const void* ptr, int64_t chunks, int64
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int FMT>
+template <typename T, int FMT, bool ANY>
 int launch_pair(const MxLinearOperands& o, cudaStream_t stream) {
   using L = MxSmem<FMT>;
   const int dev = current_device();
@@ -510,7 +548,7 @@ int launch_pair(const MxLinearOperands& o, cudaStream_t stream) {
   a.group_m = 8;
   a.dshift = o.dshift;
   a.alpha = o.alpha;
-  auto kernel = mx_gemm_pair_kernel<T, FMT>;
+  auto kernel = mx_gemm_pair_kernel<T, FMT, ANY>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
   static int capacity[64];
@@ -553,10 +591,12 @@ bool mx_encode_map(CUtensorMap* map, const void* ptr, int elem, int64_t inner, i
 }
 
 int mx_gemm_launch(const MxLinearOperands& o, int fmt, int dtype, cudaStream_t stream) {
+  const bool any = o.N % 16 != 0 || o.ldo % 8 != 0 || !mx_aligned(o.out, 16);
+#define LORA_MXG(T, F) (any ? launch_pair<T, F, true>(o, stream) : launch_pair<T, F, false>(o, stream))
   if (dtype == LORA_BF16)
-    return fmt == LORA_MXFP4 ? launch_pair<__nv_bfloat16, LORA_MXFP4>(o, stream)
-                             : launch_pair<__nv_bfloat16, LORA_NVFP4>(o, stream);
-  return fmt == LORA_MXFP4 ? launch_pair<__half, LORA_MXFP4>(o, stream) : launch_pair<__half, LORA_NVFP4>(o, stream);
+    return fmt == LORA_MXFP4 ? LORA_MXG(__nv_bfloat16, LORA_MXFP4) : LORA_MXG(__nv_bfloat16, LORA_NVFP4);
+  return fmt == LORA_MXFP4 ? LORA_MXG(__half, LORA_MXFP4) : LORA_MXG(__half, LORA_NVFP4);
+#undef LORA_MXG
 }
 
 }  // namespace lora

@@ -23,22 +23,6 @@ namespace {
 constexpr int kMxTile = 128;
 constexpr int kMxThreads = 256;
 
-// 16 elements of a row from column c, zeros at and beyond k.
-template <typename T>
-LORA_DEVINL void mx_load16(const T* row, int64_t c, int64_t k, bool vec, uint32_t* w) {
-  if (vec && c + 16 <= k) {
-    ldg_stream_v8(row + c, w);
-    return;
-  }
-  const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t lo = c + 2 * i < k ? p[c + 2 * i] : 0u;
-    const uint32_t hi = c + 2 * i + 1 < k ? p[c + 2 * i + 1] : 0u;
-    w[i] = lo | (hi << 16);
-  }
-}
-
 // Scale byte and codes of one thread's 16 elements.
 template <typename T, int FMT>
 LORA_DEVINL uint32_t mx_encode16(const uint32_t* w, const MxGlobal& gl, uint32_t recip, uint32_t* codes) {
@@ -49,11 +33,11 @@ LORA_DEVINL uint32_t mx_encode16(const uint32_t* w, const MxGlobal& gl, uint32_t
   return s.byte;
 }
 
-template <typename T, int FMT>
+// ALIGN: of the rows, in bytes (32, 16, 2).
+template <typename T, int FMT, int ALIGN>
 __global__ void __launch_bounds__(kMxThreads)
     mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes,
-                       uint8_t* __restrict__ scales, int64_t M, int64_t K, int64_t Kp, int chunks, MxGlobal gl,
-                       bool vec) {
+                       uint8_t* __restrict__ scales, int64_t M, int64_t K, int64_t Kp, int chunks, MxGlobal gl) {
   constexpr int kChunks = kMxTile / MxFormat<FMT>::kBlock / 4;  // scale chunks of this tile
   __shared__ alignas(16) uint8_t sc[kChunks * 512];
   const int seg = threadIdx.x & 7;   // 16-column segment of the tile
@@ -66,7 +50,16 @@ __global__ void __launch_bounds__(kMxThreads)
   for (int p = 0; p < 4; ++p) {
     const int64_t row = row0 + 32 * p + sub;
     if (row < M) {
-      mx_load16<T>(x + row * ldx, col, K, vec, w[p]);
+      const T* src = x + row * ldx + col;
+      if (ALIGN == 32 && col + 16 <= K) {
+        ldg_stream_v8(src, w[p]);
+      } else if (ALIGN == 16 && col + 16 <= K) {
+        const uint4 a = ldg_stream(src), b = ldg_stream(src + 8);
+        w[p][0] = a.x, w[p][1] = a.y, w[p][2] = a.z, w[p][3] = a.w;
+        w[p][4] = b.x, w[p][5] = b.y, w[p][6] = b.z, w[p][7] = b.w;
+      } else {
+        ldg16_any(x + row * ldx, col, K, w[p]);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[p][i] = 0u;
@@ -121,17 +114,20 @@ LORA_DEVINL void mx_decode16(const uint32_t* c, uint32_t byte, float g, uint32_t
   }
 }
 
-// A CTA decodes 128 x 128 values, straight (rows of 256 bytes) or transposed
-// through shared memory (column c of the tensor becomes row c of out, Mw >= M
-// values wide: zeros beyond M).
-template <typename T, int FMT, bool TR>
+// A CTA decodes 128 x 128 values: straight to rows aligned to 16 or (vec) 32 bytes; to rows of any
+// alignment, through shared memory, in 4-byte words; or transposed through shared
+// memory (column c of the tensor becomes row c of out, Mw >= M values wide: zeros
+// beyond M).
+enum { kDqRows, kDqAnyRows, kDqTransposed };
+template <typename T, int FMT, int MODE>
 __global__ void __launch_bounds__(kMxThreads)
     mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out,
                          int64_t ldo, int64_t M, int64_t Mw, int64_t K, int64_t Kp, int chunks, float g, bool vec) {
+  constexpr bool TR = MODE == kDqTransposed;
   // Transposed: rows of sixteen 16-byte units, unit u of row r at u ^ f(r), f(r) =
   // 2 (r / 8 % 4) + r % 2, so that the eight rows an 8 x 8 matrix is gathered from
   // below lie in different banks.
-  __shared__ alignas(128) uint16_t tile[TR ? kMxTile * kMxTile : 8];
+  __shared__ alignas(128) uint16_t tile[MODE != kDqRows ? kMxTile * kMxTile : 8];
   const int seg = threadIdx.x & 7;
   const int sub = threadIdx.x >> 3;
   const int64_t row0 = static_cast<int64_t>(blockIdx.y) * kMxTile;
@@ -170,16 +166,37 @@ __global__ void __launch_bounds__(kMxThreads)
       const int swap = seg >> 2;
       sts128(base + (((2 * seg + swap) ^ f) << 4), swap ? h1 : h0);
       sts128(base + (((2 * seg + 1 - swap) ^ f) << 4), swap ? h0 : h1);
+    } else if constexpr (MODE == kDqAnyRows) {
+      const uint32_t base = smem_u32(tile) + (32 * p + sub) * 256 + seg * 32;
+      sts128(base, make_uint4(o[0], o[1], o[2], o[3]));
+      sts128(base + 16, make_uint4(o[4], o[5], o[6], o[7]));
     } else if (row < M && col < K) {
       T* dst = out + row * ldo + col;
-      if (vec && col + 16 <= K) {
+      if (col + 16 <= K && vec) {
         st_global_v8(dst, o);
+      } else if (col + 16 <= K) {
+        reinterpret_cast<uint4*>(dst)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+        reinterpret_cast<uint4*>(dst)[1] = make_uint4(o[4], o[5], o[6], o[7]);
       } else {
         uint16_t* d = reinterpret_cast<uint16_t*>(dst);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (col + i < K) d[i] = static_cast<uint16_t>(o[i >> 1] >> (16 * (i & 1)));
       }
+    }
+  }
+  if constexpr (MODE == kDqAnyRows) {
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n = static_cast<int>(min(static_cast<int64_t>(kMxTile), K - col0));
+    for (int r = warp; r < kMxTile && row0 + r < M; r += kMxThreads / 32) {
+      uint16_t* dst = reinterpret_cast<uint16_t*>(out) + (row0 + r) * ldo + col0;
+      const uint16_t* src = tile + r * kMxTile;
+      const int odd = (reinterpret_cast<uintptr_t>(dst) >> 1) & 1;  // elements ahead of the first whole word
+      for (int e = odd + 2 * lane; e + 1 < n; e += 64)
+        *reinterpret_cast<uint32_t*>(dst + e) = src[e] | (static_cast<uint32_t>(src[e + 1]) << 16);
+      if (odd && lane == 0) dst[0] = src[0];
+      if (((n - odd) & 1) && n > odd && lane == 1) dst[n - 1] = src[n - 1];
     }
   }
   if constexpr (TR) {
@@ -217,10 +234,12 @@ int quantize_t(const void* x, int64_t ldx, void* codes, void* scales, int64_t M,
                cudaStream_t stream) {
   const int64_t Kp = mx_padded_k(K);
   const dim3 grid(static_cast<unsigned>((Kp + kMxTile - 1) / kMxTile), static_cast<unsigned>((M + kMxTile - 1) / kMxTile));
-  const bool vec = aligned(x, 32) && ldx % 16 == 0;
-  mx_quantize_kernel<T, FMT><<<grid, kMxThreads, 0, stream>>>(
-      static_cast<const T*>(x), ldx, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), M, K, Kp,
-      static_cast<int>(mx_scale_chunks(K, FMT)), mx_global(g), vec);
+  auto kernel = aligned(x, 32) && ldx % 16 == 0  ? mx_quantize_kernel<T, FMT, 32>
+                : aligned(x, 16) && ldx % 8 == 0 ? mx_quantize_kernel<T, FMT, 16>
+                                                 : mx_quantize_kernel<T, FMT, 2>;
+  kernel<<<grid, kMxThreads, 0, stream>>>(static_cast<const T*>(x), ldx, static_cast<uint8_t*>(codes),
+                                          static_cast<uint8_t*>(scales), M, K, Kp,
+                                          static_cast<int>(mx_scale_chunks(K, FMT)), mx_global(g));
   return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
 }
 
@@ -232,17 +251,12 @@ int dequantize_t(const void* codes, const void* scales, void* out, int64_t ldo, 
   const int64_t Mw = transpose == 2 ? (M + 7) / 8 * 8 : M;
   const dim3 grid(static_cast<unsigned>((Kp + kMxTile - 1) / kMxTile), static_cast<unsigned>((M + kMxTile - 1) / kMxTile));
   const int chunks = static_cast<int>(mx_scale_chunks(K, FMT));
-  if (transpose) {
-    const bool vec = aligned(out, 16) && ldo % 8 == 0;
-    mx_dequantize_kernel<T, FMT, true><<<grid, kMxThreads, 0, stream>>>(
-        static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<T*>(out), ldo, M, Mw, K,
-        Kp, chunks, g, vec);
-  } else {
-    const bool vec = aligned(out, 32) && ldo % 16 == 0;
-    mx_dequantize_kernel<T, FMT, false><<<grid, kMxThreads, 0, stream>>>(
-        static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<T*>(out), ldo, M, M, K,
-        Kp, chunks, g, vec);
-  }
+  const bool vec = transpose ? aligned(out, 16) && ldo % 8 == 0 : aligned(out, 32) && ldo % 16 == 0;
+  auto kernel = transpose ? mx_dequantize_kernel<T, FMT, kDqTransposed>
+                : aligned(out, 16) && ldo % 8 == 0 ? mx_dequantize_kernel<T, FMT, kDqRows>
+                                                   : mx_dequantize_kernel<T, FMT, kDqAnyRows>;
+  kernel<<<grid, kMxThreads, 0, stream>>>(static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales),
+                                          static_cast<T*>(out), ldo, M, Mw, K, Kp, chunks, g, vec);
   return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
 }
 

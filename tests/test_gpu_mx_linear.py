@@ -54,6 +54,9 @@ SIZES = [
     (257, 264, 288, 130, True), (600, 768, 1120, 224, True), (1025, 520, 512, 256, False), (70, 96, 64, 0, True),
     (300, 640, 768, 0, False), (2100, 2304, 320, 8, True),
     (2560, 2304, 320, 224, False), (2500, 2400, 288, 32, True),  # more tiles than CTA pairs, long and short tails
+    # the same for outputs and lengths that end inside a tile, rows of every alignment
+    (2000, 2313, 256, 16, True), (1300, 2050, 96, 20, True), (1500, 1976, 544, 130, False), (2100, 2304, 32, 4, True),
+    (1411, 2311, 1000, 8, False), (19000, 136, 64, 6, True),
 ]
 
 
