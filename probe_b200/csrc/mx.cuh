@@ -67,9 +67,9 @@ LORA_DEVINL uint32_t lds_u8(uint32_t a) {
   asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
   return v;
 }
-LORA_DEVINL uint32_t lds_u16(uint32_t a) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+LORA_DEVINL uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
   return v;
 }
 LORA_DEVINL void sts128(uint32_t a, uint4 v) {

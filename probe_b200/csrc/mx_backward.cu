@@ -10,7 +10,7 @@
 // of its scale blocks, so W is decoded once, transposed, into the workspace (its
 // values are exact in 16 bits: nvfp4's tensor scale m 2^p leaves the power of two
 // in the values and m in the GEMM's alpha) and the 16-bit CTA-pair GEMM takes
-// [g_hi | g_lo] against [A^T | A^T] as its K tail.
+// [g_hi | g_lo] against [A^T | A^T] as its K tail (few rows: the W-streaming kernel).
 #include <cmath>
 
 #include "mx_grad.h"
@@ -24,26 +24,19 @@ namespace {
 // against 109 us).
 constexpr int64_t kWideRank = 128, kWideRows = 4096;
 
-// Rows up to which dx of an mxfp4 weight takes the W-streaming linear (its limit).
-constexpr int64_t kSmallDxRows = 256;
-
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 struct BackwardPlan {
-  size_t gemm_bytes, small_bytes, part, part_a, g, bt, at, dy, wt, total;
+  size_t gemm_bytes, part, part_a, g, bt, at, dy, wt, total;
 };
 
 BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need_dx) {
   BackwardPlan p = {};
   const int64_t np = up(N, 8), rp = up(R, 16);
-  if (need_dx) {
-    p.gemm_bytes = lora_gemm_workspace_size(M, K, np, 2 * rp);
-    if (M <= kSmallDxRows) p.small_bytes = lora_linear_small_workspace_size(M, K, R);
-  }
+  if (need_dx) p.gemm_bytes = lora_gemm_workspace_size(M, K, np, 2 * rp);
   if (R > kWideRank && M >= kWideRows) p.gemm_bytes = std::max(p.gemm_bytes, lora_gemm_workspace_size(M, R, np, 0));
   size_t at = kCounterBytes;  // ticket counters, never scratch; the steps' partials follow them in turn
-  at = std::max(at, mx_align(std::max(kCounterBytes + std::max(mx_shrink_part_bytes(M, np, R), p.small_bytes),
-                                      p.gemm_bytes)));
+  at = std::max(at, mx_align(std::max(kCounterBytes + mx_shrink_part_bytes(M, np, R), p.gemm_bytes)));
   p.part = at;
   at += mx_align(mx_grad_part_bytes(M, N, R));
   p.part_a = at;
@@ -175,12 +168,10 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   }
   // What the weights give comes first: a kernel that reads it may start before its own
   // predecessor on the stream has finished, so other launches lie between.
-  // few rows of an mxfp4 W (no fp32 factor on the product): the W-streaming linear
-  const bool small_dx = dx != nullptr && w_fmt == LORA_MXFP4 && M <= kSmallDxRows && R <= 128;
   TransposeJobs jobs = {};
   const bool b_rows = mx_aligned(b, 16) && ldb % 8 == 0;  // TMA can read them
   const bool wide = R > kWideRank && M >= kWideRows;
-  if (!b_rows || small_dx || wide) jobs.of[0] = transpose_job(b, ldb, ws + p.bt, np, N, R, np, 1);
+  if (!b_rows || wide) jobs.of[0] = transpose_job(b, ldb, ws + p.bt, np, N, R, np, 1);
   if (dx != nullptr) jobs.of[1] = transpose_job(a, lda, ws + p.at, 2 * rp, R, K, rp, 2);
   int rc = transpose(jobs, s);
   if (rc != LORA_OK) return rc;
@@ -259,10 +250,25 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   rc = mx_grad_reduce_launch(grads, 2, dtype, s);
   if (rc != LORA_OK || dx == nullptr) return rc;
 
-  if (small_dx) {
-    rc = lora_linear_small(dyp, ldp, ws + p.wt, np, ws + p.bt, np, ws + p.at, 2 * rp, nullptr, dx, lddx, M, K, np, R,
-                           scale, dtype, ws + kCounterBytes, p.small_bytes, s);
-    if (rc != LORA_ERR_UNSUPPORTED) return rc;
+  if (mx_few_tokens(M, K, device_info(dev).num_sms)) {
+    MxLinearOperands o = {};
+    o.x_codes = dyp;
+    o.ldx = ldp;
+    o.w_codes = ws + p.wt;
+    o.ldw = np;
+    o.z = ws + p.g;
+    o.ldz = 2 * rp;
+    o.z_lo = rp;
+    o.b = ws + p.at;
+    o.ldb = 2 * rp;
+    o.out = dx;
+    o.ldo = lddx;
+    o.M = M;
+    o.N = K;
+    o.K = np;
+    o.R = R;
+    o.alpha = m;
+    return mx_small_launch(o, -1, dtype, s);
   }
   return lora_gemm_ex(dyp, ldp, ws + p.wt, np, ws + p.g, 2 * rp, ws + p.at, 2 * rp, nullptr, dx, lddx, M, K, np, 2 * rp,
                       m, 0, dtype, p.gemm_bytes ? ws : nullptr, p.gemm_bytes, s);

@@ -206,20 +206,34 @@ LORA_DEVINL void mx_store16(const MxGemmArgs& args, int row0, int lane, int col0
   sts128(stage + lane * 32, make_uint4(w[0], w[1], w[2], w[3]));
   sts128(stage + lane * 32 + 16, make_uint4(w[4], w[5], w[6], w[7]));
   __syncwarp();
+  // lane: word `lane % 8` of rows 4 i + lane / 8; where a row starts on an odd element
+  // the words lie one element on, and the eighth lane stores the two left over
   const int n = min(16, args.N - col0), word = lane & 7;
+  const uint32_t src = stage + (lane >> 3) * 32 + word * 4;
+  uint32_t lo[8], hi[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int q = 4 * i + (lane >> 3);
-    if (row0 + q < args.M) {
-      uint16_t* dst = reinterpret_cast<uint16_t*>(out + static_cast<int64_t>(row0 + q) * args.ldo);
-      const int odd = (reinterpret_cast<uintptr_t>(dst) >> 1) & 1;  // elements ahead of the first whole word
-      const int e = odd + 2 * word;
-      const uint32_t src = stage + q * 32;
-      if (e + 1 < n)
-        *reinterpret_cast<uint32_t*>(dst + e) = lds_u16(src + 2 * e) | (lds_u16(src + 2 * e + 2) << 16);
-      else if (e < n)
-        dst[e] = static_cast<uint16_t>(lds_u16(src + 2 * e));
-      if (odd && word == 0) dst[0] = static_cast<uint16_t>(lds_u16(src));
+    lo[i] = lds32(src + i * 128);
+    hi[i] = lds32(word < 7 ? src + i * 128 + 4 : src + i * 128 - 28);  // the next word; the eighth lane: the first
+  }
+  uint16_t* base = reinterpret_cast<uint16_t*>(out + static_cast<int64_t>(row0 + (lane >> 3)) * args.ldo);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint16_t* dst = base + static_cast<int64_t>(4 * i) * args.ldo;
+    if (row0 + 4 * i + (lane >> 3) >= args.M) continue;
+    if ((reinterpret_cast<uintptr_t>(dst) & 2) == 0) {
+      if (2 * word + 1 < n)
+        *reinterpret_cast<uint32_t*>(dst + 2 * word) = lo[i];
+      else if (2 * word < n)
+        dst[2 * word] = static_cast<uint16_t>(lo[i]);
+    } else if (word < 7) {
+      if (2 * word + 2 < n)
+        *reinterpret_cast<uint32_t*>(dst + 2 * word + 1) = __funnelshift_r(lo[i], hi[i], 16);
+      else if (2 * word + 1 < n)
+        dst[2 * word + 1] = static_cast<uint16_t>(lo[i] >> 16);
+    } else {
+      if (n == 16) dst[15] = static_cast<uint16_t>(lo[i] >> 16);
+      dst[0] = static_cast<uint16_t>(hi[i]);
     }
   }
   __syncwarp();

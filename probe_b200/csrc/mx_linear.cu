@@ -17,14 +17,6 @@ namespace {
 // Shrinks of more ranks than this run on the 16-bit tensor-core GEMM.
 constexpr int64_t kShrinkMaxRank = 128;
 
-// The W-streaming kernel (mx_small.cu) runs one tile of 128 tokens, or as many 128 x
-// 128 tiles as there are SMs.  Measured whole calls, r = 16, mxfp4, against 256 x 256
-// pair tiles: N = K = 4096, 333 tokens 17.6 against 23.3 us, 512 18.8 against 23.5, 768
-// (192 tiles) 27.4 against 23.7; N = 11008, 256 (172 tiles) 26.9 against 23.5.
-bool few_tokens(int64_t M, int64_t N, int num_sms) {
-  return M <= 128 || (M + 127) / 128 * ((N + 127) / 128) <= num_sms;
-}
-
 int64_t r16(int64_t r) { return (r + 15) / 16 * 16; }
 
 struct LinearPlan {
@@ -70,6 +62,14 @@ __global__ void mx_pad_rows_kernel(const uint16_t* __restrict__ b, int64_t ldb, 
 }
 
 }  // namespace
+
+// Measured whole calls, r = 16, mxfp4, against 256 x 256 pair tiles: N = K = 4096, 333
+// tokens 17.6 against 23.3 us, 512 18.8 against 23.5, 768 (192 tiles) 27.4 against 23.7;
+// N = 11008, 256 (172 tiles) 26.9 against 23.5.
+bool mx_few_tokens(int64_t M, int64_t N, int num_sms) {
+  return M <= 128 || (M + 127) / 128 * ((N + 127) / 128) <= num_sms;
+}
+
 }  // namespace lora
 
 using namespace lora;
@@ -191,6 +191,6 @@ extern "C" int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, c
   o.N = N;
   o.K = K;
   o.R = R;
-  if (few_tokens(M, N, device_info(dev).num_sms)) return mx_small_launch(o, fmt, dtype, s);
+  if (mx_few_tokens(M, N, device_info(dev).num_sms)) return mx_small_launch(o, fmt, dtype, s);
   return mx_gemm_launch(o, fmt, dtype, s);
 }

@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* recip = reinterpret_cast<float*>(tmem_slot + 4);  // 128 entries (nvfp4)
-  const uint32_t csum = smem_u32(full) + 1024;              // cluster mode: [128][r16] partial sums
+  const uint32_t csum = smem_u32(smem);  // cluster mode: [128][r16] partial sums, over the drained stages
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int crank = args.cluster ? static_cast<int>(cluster_ctarank()) : 0;
@@ -288,6 +288,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
         if (!ok) break;
       }
       c = seg_end;
+      if (args.cluster) break;  // below
       // ---- the block's sum (or this run's part of it); a warp takes its 32 rows and
       // every fourth group of 16 columns
       if (!warp_wait(&acc_full[seg & 1], (seg >> 1) & 1, abort_flag, args.err, kDevErrTimeoutAccFull)) break;
@@ -301,13 +302,6 @@ __global__ void __launch_bounds__(kShThreads, 1)
         uint32_t u[16];
         tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + (seg & 1) * args.r16 + j, u);
         tmem_wait_ld();
-        if (args.cluster) {
-          const uint32_t dst = csum + ((quad * 32 + lane) * args.r16 + j) * 4;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            sts128(dst + 16 * e, make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]));
-          continue;
-        }
         if (row >= args.M) continue;
         if (whole) {
           float v[16];
@@ -323,7 +317,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
       __syncwarp();
       tc_fence_before();
       if (lane == 0) mbar_arrive(&acc_empty[seg & 1]);
-      if (!args.cluster && !whole && part * 16 < args.r16) {
+      if (!whole && part * 16 < args.r16) {
         // first and last run with a chunk of this block
         const int first_chunk = tb * args.kc, end_chunk = first_chunk + args.kc;
         int j0 = static_cast<int>(static_cast<int64_t>(first_chunk) * gridDim.x / args.chunks_total);
@@ -378,6 +372,21 @@ __global__ void __launch_bounds__(kShThreads, 1)
               sh_store_pair<T>(zrow + j, args.r16, v);
             }
         }
+      }
+    }
+    if (args.cluster) {
+      // every worker has read its tiles, every MMA has: the sums may take their place
+      ok = warp_wait(&acc_full[0], 0, abort_flag, args.err, kDevErrTimeoutAccFull);
+      named_bar_sync(1, 32 * kShWorkers);
+      tc_fence_after();
+      for (int j = part * 16; ok && j < args.r16; j += 64) {
+        uint32_t u[16];
+        tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + j, u);
+        tmem_wait_ld();
+        const uint32_t dst = csum + ((quad * 32 + lane) * args.r16 + j) * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          sts128(dst + 16 * e, make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]));
       }
     }
   }
@@ -472,8 +481,7 @@ int launch_shrink(const MxShrinkOperands& o, cudaStream_t stream) {
   a.gl = mx_global(o.global_scale);
   constexpr int kFixed = 1024 + 1024;  // alignment, barriers and reciprocals
   a.cluster = shrink_cluster(o.M, o.K, o.R);
-  const int sums = a.cluster ? 128 * a.r16 * 4 : 0;
-  a.stages = std::min(8, (kShSmemMax - kFixed - sums) / a.stage_bytes);
+  a.stages = std::min(8, (kShSmemMax - kFixed) / a.stage_bytes);
   auto kernel = mx_shrink_kernel<T, FMT, AMN, KB>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
@@ -481,7 +489,8 @@ int launch_shrink(const MxShrinkOperands& o, cudaStream_t stream) {
     attr_err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShSmemMax);
   });
   if (attr_err[dev] != cudaSuccess) return LORA_ERR_CUDA;
-  const size_t smem = static_cast<size_t>(a.stages) * a.stage_bytes + kFixed + sums;
+  const size_t smem = static_cast<size_t>(a.stages) * a.stage_bytes + kFixed;
+  if (a.cluster && a.stages * a.stage_bytes < 128 * a.r16 * 4) return LORA_ERR_UNSUPPORTED;  // never: 167 KB and more
   const int64_t ctas = a.cluster ? (o.M + 127) / 128 * a.cluster : shrink_ctas(o.M, o.K, o.R);
   return mx_launch(kernel, dim3(static_cast<unsigned>(ctas)), kShThreads, smem, stream, a.cluster, maps, a);
 }

@@ -11,7 +11,8 @@
 // until about two CTAs an SM stream W; their partial tiles meet in shared memory
 // and are summed in rank order over DSMEM.  The kernel starts while its predecessor
 // (the shrink that makes xq, sx and z) still runs: W's first stages load before
-// griddepcontrol.wait.
+// griddepcontrol.wait.  The same kernel with W in 16 bits (64-deep stages, no scales)
+// gives dx of few rows in the backward pass.
 #include <cmath>
 #include <mutex>
 
@@ -36,7 +37,7 @@ struct SmArgs {
   int* err;
   int64_t ldo;
   int M, N;
-  int num_kb, last_k64, rank_kb, last_k16, chunks, stages;
+  int num_kb, last_step, rank_kb, last_k16, chunks, stages;
   float alpha, base_scale;  // 2^-dshift
 };
 
@@ -73,16 +74,23 @@ LORA_DEVINL void sm_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint
   }
 }
 
+constexpr int kSm16Bit = -1;  // FMT of a 16-bit W
+
+template <int FMT> __host__ __device__ constexpr int sm_chunks() { return 256 / MxFormat<FMT>::kBlock / 4; }
+template <> __host__ __device__ constexpr int sm_chunks<kSm16Bit>() { return 0; }
+
 template <int FMT, int NB>
 struct SmLayout {
-  static constexpr int kChunks = 256 / MxFormat<FMT>::kBlock / 4;
+  static constexpr int kChunks = sm_chunks<FMT>();
+  static constexpr int kDepth = FMT == kSm16Bit ? 64 : 256;  // K of a stage: 128 bytes a row
+  static constexpr int kStep = kDepth / 4;                   // K of an MMA
   static constexpr int kW = 128 * 128, kX = NB * 128, kSf = kChunks * 512;
   static constexpr int kStage = (kW + kX + 2 * kSf + 1023) / 1024 * 1024;
   static constexpr int kXOffset = kW, kSfOffset = kW + kX;
   static constexpr int kMainBytes = kW + kX + 2 * kSf;
   static constexpr int kSfCols = 2 * kChunks * 4;
   // TMEM: base accumulator, adapter accumulator, scales of every stage
-  static constexpr int kFit = (sm_tmem_max<NB>() - 2 * NB) / kSfCols;
+  static constexpr int kFit = kSfCols == 0 ? 8 : (sm_tmem_max<NB>() - 2 * NB) / (kSfCols == 0 ? 1 : kSfCols);
   static constexpr int kMaxStages = kFit < 8 ? kFit : 8;
 };
 
@@ -93,6 +101,7 @@ __global__ void __launch_bounds__(kSmThreads)
   constexpr uint32_t kCols = 2 * NB + L::kMaxStages * L::kSfCols;
   constexpr uint32_t kTmemCols = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
   static_assert(kTmemCols <= sm_tmem_max<NB>(), "TMEM");
+  constexpr int kInner = FMT == kSm16Bit ? 64 : 128;  // map elements of a stage's row
   constexpr uint32_t kIdesc = (1u << 7) | (1u << 10) | (static_cast<uint32_t>(NB >> 3) << 17) |
                               ((FMT == LORA_MXFP4 ? 1u : 0u) << 23) | (8u << 24);
   constexpr uint32_t kIdescTail = (1u << 4) | ((std::is_same<T, __nv_bfloat16>::value ? 1u : 0u) << 7) |
@@ -143,8 +152,10 @@ __global__ void __launch_bounds__(kSmThreads)
         uint8_t* base = smem + stage * L::kStage;
         if (i < kb1 - kb0) {
           mbar_arrive_expect_tx(&full[stage], L::kMainBytes);
-          tma_load_2d(&maps.w, base, &full[stage], (kb0 + i) * 128, n0);
-          tma_load_2d(&maps.sw, base + L::kSfOffset, &full[stage], 0, (n0 >> 7) * args.chunks + (kb0 + i) * L::kChunks);
+          tma_load_2d(&maps.w, base, &full[stage], (kb0 + i) * kInner, n0);
+          if constexpr (L::kChunks > 0)
+            tma_load_2d(&maps.sw, base + L::kSfOffset, &full[stage], 0,
+                        (n0 >> 7) * args.chunks + (kb0 + i) * L::kChunks);
         } else {
           const int t = i - (kb1 - kb0);
           mbar_arrive_expect_tx(&full[stage], L::kW + L::kX);
@@ -154,9 +165,10 @@ __global__ void __launch_bounds__(kSmThreads)
       auto tokens = [&](int i, int stage) {
         uint8_t* base = smem + stage * L::kStage;
         if (i < kb1 - kb0) {
-          tma_load_2d(&maps.x, base + L::kXOffset, &full[stage], (kb0 + i) * 128, t0);
-          tma_load_2d(&maps.sx, base + L::kSfOffset + L::kSf, &full[stage], 0,
-                      (t0 >> 7) * args.chunks + (kb0 + i) * L::kChunks);
+          tma_load_2d(&maps.x, base + L::kXOffset, &full[stage], (kb0 + i) * kInner, t0);
+          if constexpr (L::kChunks > 0)
+            tma_load_2d(&maps.sx, base + L::kSfOffset + L::kSf, &full[stage], 0,
+                        (t0 >> 7) * args.chunks + (kb0 + i) * L::kChunks);
         } else {
           const int t = i - (kb1 - kb0);
           const bool lo = t >= args.rank_kb;
@@ -197,7 +209,7 @@ __global__ void __launch_bounds__(kSmThreads)
       const uint64_t wd = wd0 + at, xd = xd0 + at, sd = sd0 + at;
       if (i < kb1 - kb0) {
         const uint32_t sfa = tmem + 2 * NB + stage * L::kSfCols, sfb = sfa + L::kChunks * 4;
-        const int nk = kb0 + i == args.num_kb - 1 ? args.last_k64 : 4;
+        const int nk = kb0 + i == args.num_kb - 1 ? args.last_step : 4;
         if (elect_one()) {
 #pragma unroll
           for (int j = 0; j < L::kChunks; ++j) {
@@ -206,12 +218,18 @@ __global__ void __launch_bounds__(kSmThreads)
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            constexpr bool kMx = FMT == LORA_MXFP4;
-            const int j = kMx ? k >> 1 : k;
-            const uint32_t id = kMx ? static_cast<uint32_t>(k & 1) * 2u : 0u;
-            if (k < nk)
-              sm_mma<FMT>(tmem, wd + static_cast<uint32_t>(2 * k), xd + static_cast<uint32_t>(2 * k),
-                          kIdesc | (id << 4) | (id << 29), sfa + 4 * j, sfb + 4 * j, (i > 0 || k > 0) ? 1u : 0u);
+            if constexpr (FMT == kSm16Bit) {
+              if (k < nk)
+                tc_mma_f16(tmem, wd + static_cast<uint32_t>(2 * k), xd + static_cast<uint32_t>(2 * k), kIdescTail,
+                           (i > 0 || k > 0) ? 1u : 0u);
+            } else {
+              constexpr bool kMx = FMT == LORA_MXFP4;
+              const int j = kMx ? k >> 1 : k;
+              const uint32_t id = kMx ? static_cast<uint32_t>(k & 1) * 2u : 0u;
+              if (k < nk)
+                sm_mma<FMT>(tmem, wd + static_cast<uint32_t>(2 * k), xd + static_cast<uint32_t>(2 * k),
+                            kIdesc | (id << 4) | (id << 29), sfa + 4 * j, sfb + 4 * j, (i > 0 || k > 0) ? 1u : 0u);
+            }
           }
           tc_commit(&empty[stage]);
         }
@@ -323,13 +341,21 @@ int launch_small(const MxLinearOperands& o, cudaStream_t stream) {
   const DeviceInfo& info = device_info(dev);
   SmMaps maps;
   SmArgs a;
-  const int64_t pitch = mx_code_pitch(o.K, FMT);
-  a.chunks = static_cast<int>(mx_scale_chunks(o.K, FMT));
-  if (!mx_encode_map(&maps.x, o.x_codes, 1, pitch, o.M, pitch, 128, NB, true) ||
-      !mx_encode_map(&maps.w, o.w_codes, 1, pitch, o.N, pitch, 128, 128, true) ||
-      !mx_encode_map(&maps.sx, o.x_scales, 4, 128, (o.M + 127) / 128 * a.chunks, 512, 128, L::kChunks, false) ||
-      !mx_encode_map(&maps.sw, o.w_scales, 4, 128, (o.N + 127) / 128 * a.chunks, 512, 128, L::kChunks, false))
-    return LORA_ERR_CUDA;
+  if constexpr (FMT == kSm16Bit) {
+    a.chunks = 0;
+    if (!mx_encode_map(&maps.x, o.x_codes, 2, o.K, o.M, o.ldx * 2, 64, NB, true) ||
+        !mx_encode_map(&maps.w, o.w_codes, 2, o.K, o.N, o.ldw * 2, 64, 128, true))
+      return LORA_ERR_CUDA;
+    maps.sx = maps.sw = maps.x;
+  } else {
+    const int64_t pitch = mx_code_pitch(o.K, FMT);
+    a.chunks = static_cast<int>(mx_scale_chunks(o.K, FMT));
+    if (!mx_encode_map(&maps.x, o.x_codes, 1, pitch, o.M, pitch, 128, NB, true) ||
+        !mx_encode_map(&maps.w, o.w_codes, 1, pitch, o.N, pitch, 128, 128, true) ||
+        !mx_encode_map(&maps.sx, o.x_scales, 4, 128, (o.M + 127) / 128 * a.chunks, 512, 128, L::kChunks, false) ||
+        !mx_encode_map(&maps.sw, o.w_scales, 4, 128, (o.N + 127) / 128 * a.chunks, 512, 128, L::kChunks, false))
+      return LORA_ERR_CUDA;
+  }
   if (o.R > 0) {
     const char* z = static_cast<const char*>(o.z);
     if (!mx_encode_map(&maps.zh, z, 2, o.R, o.M, o.ldz * 2, 64, NB, true) ||
@@ -345,9 +371,9 @@ int launch_small(const MxLinearOperands& o, cudaStream_t stream) {
   a.ldo = o.ldo;
   a.M = static_cast<int>(o.M);
   a.N = static_cast<int>(o.N);
-  const int64_t kp = mx_padded_k(o.K);
-  a.num_kb = static_cast<int>((kp + 255) / 256);
-  a.last_k64 = static_cast<int>((kp - (a.num_kb - 1) * 256ll + 63) / 64);
+  const int64_t kp = FMT == kSm16Bit ? o.K : mx_padded_k(o.K);
+  a.num_kb = static_cast<int>((kp + L::kDepth - 1) / L::kDepth);
+  a.last_step = static_cast<int>((kp - static_cast<int64_t>(a.num_kb - 1) * L::kDepth + L::kStep - 1) / L::kStep);
   a.rank_kb = static_cast<int>((o.R + 63) / 64);
   a.last_k16 = a.rank_kb > 0 ? static_cast<int>((o.R - (a.rank_kb - 1) * 64ll + 15) / 16) : 0;
   a.alpha = o.alpha;
@@ -386,6 +412,7 @@ int dispatch(const MxLinearOperands& o, cudaStream_t s) {
 }  // namespace
 
 int mx_small_launch(const MxLinearOperands& o, int fmt, int dtype, cudaStream_t s) {
+  if (fmt == kSm16Bit) return dtype == LORA_BF16 ? dispatch<__nv_bfloat16, kSm16Bit>(o, s) : dispatch<__half, kSm16Bit>(o, s);
   if (dtype == LORA_BF16)
     return fmt == LORA_MXFP4 ? dispatch<__nv_bfloat16, LORA_MXFP4>(o, s) : dispatch<__nv_bfloat16, LORA_NVFP4>(o, s);
   return fmt == LORA_MXFP4 ? dispatch<__half, LORA_MXFP4>(o, s) : dispatch<__half, LORA_NVFP4>(o, s);
