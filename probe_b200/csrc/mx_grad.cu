@@ -268,9 +268,8 @@ __global__ void __launch_bounds__(kGrThreads, 1)
           for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) + __uint_as_float(lo[e]));
         }
         if (c < args.C) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            reinterpret_cast<uint4*>(dst + j)[e] = make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
+          st_global_v8(dst + j, r);
+          st_global_v8(dst + j + 8, r + 8);
         }
       }
     }

@@ -309,9 +309,8 @@ __global__ void __launch_bounds__(kShThreads, 1)
           for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(u[e]) * args.scale;
           sh_store_pair<T>(zrow + j, args.r16, v);
         } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            reinterpret_cast<uint4*>(slot + j)[e] = make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
+          st_global_v8(slot + j, u);
+          st_global_v8(slot + j + 8, u + 8);
         }
       }
       __syncwarp();
