@@ -162,8 +162,8 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4", global_scale: float = 1.0) 
     m, k = x.shape
     pitch, nscales = _sizes(m, k, fmt)
     device, dtype = x.device, x.dtype
-    codes = torch.empty((m, pitch), dtype=torch.uint8, device=device)
-    scales = torch.empty(nscales, dtype=torch.uint8, device=device)
+    codes = x.new_empty((m, pitch), dtype=torch.uint8)
+    scales = x.new_empty(nscales, dtype=torch.uint8)
     global_scale = float(global_scale)
     rc = _entry("lora_mx_quantize")(x.data_ptr(), _ld(x), codes.data_ptr(), scales.data_ptr(), m, k, code, global_scale,
                                     _DTYPE[dtype], _raw_stream(device.index))
@@ -179,7 +179,7 @@ def mx_dequantize(q: MXTensor, dtype: torch.dtype = torch.bfloat16, transpose: b
         raise TypeError(f"mx_dequantize: expected float16/bfloat16, got {dtype}")
     m, k = q.shape
     device = q.codes.device
-    out = torch.empty((k, m) if transpose else (m, k), dtype=dtype, device=device)
+    out = q.codes.new_empty((k, m) if transpose else (m, k), dtype=dtype)
     rc = _entry("lora_mx_dequantize")(q.codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), m if transpose else k, m,
                                       k, q._code, q.global_scale, int(transpose), _DTYPE[dtype],
                                       _raw_stream(device.index))
@@ -198,47 +198,65 @@ def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-def _linear(x, weight, bias, a, b, scale, x_global_scale, keep_z, where):
+def _refuse_linear(x, weight, bias, a, b, where):
+    """The error of a call that ``_linear``'s one check found wrong."""
     _need_cuda(where, x, weight.codes, bias, a, b)
+    n, k = weight.shape
     if weight.fmt not in ("mxfp4", "nvfp4"):
         raise ValueError(f"{where}: the weight must be in a 4-bit format, got {weight.fmt}")
-    shape = x.shape
-    x = _rows(x, where)
+    if x.dtype not in _HALF:
+        raise TypeError(f"{where}: expected float16/bfloat16, got {x.dtype}")
+    if x.shape[-1] != k:
+        raise ValueError(f"{where}: x {tuple(x.shape)} and the weight {weight.shape} disagree on K")
+    if bias is not None and (bias.shape != (n,) or bias.dtype != x.dtype):
+        raise ValueError(f"{where}: bias must be [{n}] in x's dtype")
+    if a.dtype != x.dtype or b.dtype != x.dtype:
+        raise TypeError(f"{where}: x, a and b must share one dtype")
+    r = a.shape[0]
+    if a.shape != (r, k) or b.shape != (n, r):
+        raise ValueError(f"{where}: a {tuple(a.shape)} / b {tuple(b.shape)} do not match [{r}, {k}] / [{n}, {r}]")
+    raise ValueError(f"{where}: ranks up to 256, got {r}")
+
+
+def _linear(x, weight, bias, a, b, scale, x_global_scale, keep_z, where):
+    shape, dtype, codes, code = x.shape, x.dtype, weight.codes, weight._code
     n, k = weight.shape
+    r = 0 if a is None or b is None or scale == 0 else a.shape[0]
+    dt = _DTYPE.get(dtype)
+    if (dt is None or code == _lib.LORA_MXFP8 or not x.is_cuda or not codes.is_cuda or shape[-1] != k
+            or (bias is not None and (not bias.is_cuda or bias.dtype != dtype or bias.shape != (n,)))
+            or (r and (r > 256 or a.dtype != dtype or b.dtype != dtype or not a.is_cuda or not b.is_cuda
+                       or a.shape != (r, k) or b.shape != (n, r)))):
+        _refuse_linear(x, weight, bias, a, b, where)
+    if len(shape) != 2 or not x.is_contiguous():
+        x = _rows(x, where)
     m = x.shape[0]
-    if x.shape[1] != k:
-        raise ValueError(f"{where}: x {tuple(shape)} and the weight {weight.shape} disagree on K")
-    device, dtype = x.device, x.dtype
-    r = 0
-    ap = bp = lda = ldb = 0
-    if a is not None and b is not None and a.shape[0] > 0 and scale != 0:
-        r = a.shape[0]
-        if a.dtype != dtype or b.dtype != dtype:
-            raise TypeError(f"{where}: x, a and b must share one dtype")
-        if a.shape[1] != k or b.shape != (n, r):
-            raise ValueError(f"{where}: a {tuple(a.shape)} / b {tuple(b.shape)} do not match [{r}, {k}] / [{n}, {r}]")
-        if r > 256:
-            raise ValueError(f"{where}: ranks up to 256, got {r}")
-        x, a, b = _aligned_rows(x), _aligned_rows(a), _aligned_rows(b)
-        ap, lda, bp, ldb = a.data_ptr(), _ld(a), b.data_ptr(), _ld(b)
-    bias_ptr = None
+    xp, ap, bp, lda, ldb = x.data_ptr(), None, None, 0, 0
+    ldx = _ld(x)
+    if r:
+        # TMA reads rows of 16-byte multiples: copies only where the layout is another
+        if (xp | 2 * ldx) & 15 and k % 8 == 0:
+            x = _aligned_rows(x)
+            xp, ldx = x.data_ptr(), _ld(x)
+        ap, bp, lda, ldb = a.data_ptr(), b.data_ptr(), k, r
+        if not a.is_contiguous() or (ap | 2 * k) & 15:
+            a = _aligned_rows(a)
+            ap, lda = a.data_ptr(), _ld(a)
+        if not b.is_contiguous() or (bp | 2 * r) & 15:
+            b = _aligned_rows(b)
+            bp, ldb = b.data_ptr(), _ld(b)
     if bias is not None:
-        if bias.shape != (n,) or bias.dtype != dtype:
-            raise ValueError(f"{where}: bias must be [{n}] in x's dtype")
         bias = bias.contiguous()
-        bias_ptr = bias.data_ptr()
-    out = torch.empty((m, n), dtype=dtype, device=device)
-    z = None
-    if keep_z and r:
-        z = torch.empty((m, 2 * ((r + 15) // 16 * 16)), dtype=dtype, device=device)
+    out = x.new_empty((m, n))
+    z = x.new_empty((m, 2 * ((r + 15) // 16 * 16))) if keep_z and r else None
     if m and n:
-        code = weight._code
+        device = x.device
         stream = _raw_stream(device.index)
         ws = _workspace("mx_linear", _linear_bytes(m, n, k, r, code), device, stream)
-        rc = _entry("lora_mx_linear")(x.data_ptr(), _ld(x), weight.codes.data_ptr(), weight.scales.data_ptr(),
-                                      weight.global_scale, bias_ptr, ap or None, lda, bp or None, ldb, out.data_ptr(), n,
-                                      z.data_ptr() if z is not None else None, m, n, k, r, float(scale),
-                                      float(x_global_scale), code, _DTYPE[dtype], ws.data_ptr(), ws.numel(), stream)
+        rc = _entry("lora_mx_linear")(xp, ldx, codes.data_ptr(), weight.scales.data_ptr(), weight.global_scale,
+                                      None if bias is None else bias.data_ptr(), ap, lda, bp, ldb, out.data_ptr(), n,
+                                      None if z is None else z.data_ptr(), m, n, k, r, float(scale), float(x_global_scale),
+                                      code, dt, ws.data_ptr(), ws.numel(), stream)
         if rc:
             _lib.check(rc, "lora_mx_linear")
     return (out if len(shape) == 2 else out.view(*shape[:-1], n)), z
@@ -286,12 +304,11 @@ def mx_lora_backward(dy: torch.Tensor, x8: MXTensor, z: torch.Tensor, a: torch.T
         raise ValueError(f"{where}: the weight must be a 4-bit tensor of shape {(n, k)}, got {weight.fmt} {weight.shape}")
     a, b = _lib.row_major(a), _lib.row_major(b)
     device = dy.device
-    da = torch.empty((r, k), dtype=dtype, device=device)
-    db = torch.empty((n, r), dtype=dtype, device=device)
+    da, db = dy.new_empty((r, k)), dy.new_empty((n, r))
     dx = wp = sp = None
     wg, wcode = 1.0, 0
     if weight is not None:
-        dx = torch.empty((m, k), dtype=dtype, device=device)
+        dx = dy.new_empty((m, k))
         wp, sp, wg, wcode = wc.data_ptr(), weight.scales.data_ptr(), weight.global_scale, weight._code
     stream = _raw_stream(device.index)
     ws = _workspace("mx_backward", _backward_bytes(m, n, k, r, int(dx is not None)), device, stream)
