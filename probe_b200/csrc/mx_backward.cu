@@ -202,8 +202,6 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   gr.C = N;
   gr.R = R;
   gr.factor = z_scale;
-  rc = mx_grad_launch(gr, dtype, s);
-  if (rc != LORA_OK) return rc;
 
   MxShrinkOperands sh = {};
   sh.v = dyp;
@@ -245,9 +243,9 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   ga.C = K;
   ga.factor = m;
   ga.transposed = true;
-  rc = mx_grad_launch(ga, dtype, s);
+  rc = mx_grad_launch(grads, dtype, s);
   if (rc != LORA_OK) return rc;
-  rc = mx_grad_reduce_launch(grads, 2, dtype, s);
+  rc = mx_grad_reduce_launch(grads, dtype, s);
   if (rc != LORA_OK || dx == nullptr) return rc;
 
   if (mx_few_tokens(M, K, device_info(dev).num_sms)) {

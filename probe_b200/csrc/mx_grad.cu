@@ -105,8 +105,7 @@ LORA_DEVINL uint4 gr_decode8<__half>(uint2 w, uint32_t s) {
 // Shared memory: the TMA ring (stage: V or codes + scales, then P), for mxfp8 two
 // converted tiles, then the barriers.
 template <typename T, bool F8>
-__global__ void __launch_bounds__(kGrThreads, 1)
-    mx_grad_kernel(const __grid_constant__ GrMaps maps, const GrArgs args) {
+LORA_DEVINL void gr_job(const GrMaps& maps, const GrArgs& args, int group, int split) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -121,8 +120,8 @@ __global__ void __launch_bounds__(kGrThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t col0 = static_cast<int64_t>(blockIdx.x) * kGrCols;
-  const int step0 = static_cast<int>(blockIdx.y) * args.steps_per_split;
+  const int64_t col0 = static_cast<int64_t>(group) * kGrCols;
+  const int step0 = split * args.steps_per_split;
   const int step1 = min(step0 + args.steps_per_split, args.steps);
   const uint32_t tmem_cols = args.n <= 16 ? 32u : args.n <= 32 ? 64u : args.n <= 64 ? 128u : args.n <= 128 ? 256u : 512u;
 
@@ -256,7 +255,7 @@ __global__ void __launch_bounds__(kGrThreads, 1)
     if (warp_wait(acc_full, 0, abort_flag, args.err, kDevErrTimeoutAccFull)) {
       tc_fence_after();
       const int64_t c = col0 + m * 128 + quad * 32 + lane;
-      float* dst = args.part + (static_cast<int64_t>(blockIdx.y) * args.C + c) * args.r16;
+      float* dst = args.part + (static_cast<int64_t>(split) * args.C + c) * args.r16;
       for (int j = (cw >> 3) * 16; j < args.r16; j += 32) {
         const uint32_t src = tmem + (static_cast<uint32_t>(quad * 32) << 16) + m * args.n + j;
         uint32_t r[16], lo[16];
@@ -279,6 +278,25 @@ __global__ void __launch_bounds__(kGrThreads, 1)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, tmem_cols);
+  }
+}
+
+// Both gradients of a call in one launch: the blocks of dB, then those of dA, which
+// start as the first leave.
+struct GrJobs {
+  GrMaps maps[2];
+  GrArgs args[2];
+  int groups[2], blocks0;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kGrThreads, 1) mx_grad_kernel(const __grid_constant__ GrJobs jobs) {
+  const int b = static_cast<int>(blockIdx.x);
+  if (b < jobs.blocks0) {
+    gr_job<T, false>(jobs.maps[0], jobs.args[0], b % jobs.groups[0], b / jobs.groups[0]);
+  } else {
+    const int c = b - jobs.blocks0;
+    gr_job<T, true>(jobs.maps[1], jobs.args[1], c % jobs.groups[1], c / jobs.groups[1]);
   }
 }
 
@@ -352,46 +370,58 @@ GrPlan grad_plan(int64_t M, int64_t C) {
   return p;
 }
 
-template <typename T, bool F8>
-int launch_grad(const MxGradOperands& g, const GrPlan& pl, cudaStream_t stream) {
+// Maps and arguments of one gradient; its shared memory through `smem`.
+bool fill_job(const MxGradOperands& g, const GrPlan& pl, bool f8, int* err, GrMaps* maps, GrArgs* a, size_t* smem) {
+  a->part = static_cast<float*>(g.part);
+  a->err = err;
+  a->C = g.C;
+  a->M = static_cast<int>(g.M);
+  a->r16 = static_cast<int>((g.R + 15) / 16 * 16);
+  a->n = a->r16 <= 64 ? 2 * a->r16 : a->r16;
+  a->p_chunks = (a->n + 63) / 64;
+  a->steps = pl.steps;
+  a->splits = pl.splits;
+  a->steps_per_split = pl.steps_per_split;
+  a->scale_gb = static_cast<int>(mx_scale_chunks(g.C, LORA_MXFP8));
+  a->stage_bytes = (f8 ? kGrRawBytes + kGrScaleBytes : kGrVBytes) + a->p_chunks * kGrChunkBytes;
+  const int fixed = (f8 ? 2 * kGrVBytes : 0) + 512 + 1024;
+  a->stages = std::min(8, (kGrSmemMax - fixed) / a->stage_bytes);
+  *smem = std::max(*smem, static_cast<size_t>(a->stages) * a->stage_bytes + fixed);
+  if (f8) {
+    const int64_t pitch = mx_padded_k(g.C);
+    if (!mx_encode_map(&maps->v, g.v, 1, pitch, g.M, pitch, kGrCols, kGrTok, false) ||
+        !mx_encode_map(&maps->sc, g.v_scales, 4, 128, (g.M + 127) / 128 * a->scale_gb, 512, 128, 2, false))
+      return false;
+  } else {
+    if (!mx_encode_map(&maps->v, g.v, 2, g.C, g.M, g.ldv * 2, 64, kGrTok, true)) return false;
+    maps->sc = maps->v;
+  }
+  return mx_encode_map(&maps->p, g.p, 2, a->n, g.M, g.ldp * 2, 64, kGrTok, true);
+}
+
+template <typename T>
+int launch_grads(const MxGradOperands* g, cudaStream_t stream) {
   const int dev = current_device();
   if (dev < 0) return LORA_ERR_DEVICE;
   const DeviceInfo& info = device_info(dev);
-  GrMaps maps;
-  GrArgs a;
-  a.part = static_cast<float*>(g.part);
-  a.err = info.err_word;
-  a.C = g.C;
-  a.M = static_cast<int>(g.M);
-  a.r16 = static_cast<int>((g.R + 15) / 16 * 16);
-  a.n = a.r16 <= 64 ? 2 * a.r16 : a.r16;
-  a.p_chunks = (a.n + 63) / 64;
-  a.steps = pl.steps;
-  a.splits = pl.splits;
-  a.steps_per_split = pl.steps_per_split;
-  a.scale_gb = static_cast<int>(mx_scale_chunks(g.C, LORA_MXFP8));
-  a.stage_bytes = (F8 ? kGrRawBytes + kGrScaleBytes : kGrVBytes) + a.p_chunks * kGrChunkBytes;
-  const int fixed = (F8 ? 2 * kGrVBytes : 0) + 512 + 1024;
-  a.stages = std::min(8, (kGrSmemMax - fixed) / a.stage_bytes);
-  if (F8) {
-    const int64_t pitch = mx_padded_k(g.C);
-    if (!mx_encode_map(&maps.v, g.v, 1, pitch, g.M, pitch, kGrCols, kGrTok, false) ||
-        !mx_encode_map(&maps.sc, g.v_scales, 4, 128, (g.M + 127) / 128 * a.scale_gb, 512, 128, 2, false))
-      return LORA_ERR_CUDA;
-  } else {
-    if (!mx_encode_map(&maps.v, g.v, 2, g.C, g.M, g.ldv * 2, 64, kGrTok, true)) return LORA_ERR_CUDA;
-    maps.sc = maps.v;
+  GrJobs jobs;
+  size_t smem = 0;
+  int blocks = 0;
+  for (int i = 0; i < 2; ++i) {
+    const GrPlan pl = grad_plan(g[i].M, g[i].C);
+    if (!fill_job(g[i], pl, i == 1, info.err_word, &jobs.maps[i], &jobs.args[i], &smem)) return LORA_ERR_CUDA;
+    jobs.groups[i] = pl.groups;
+    if (i == 1) jobs.blocks0 = blocks;
+    blocks += pl.groups * pl.splits;
   }
-  if (!mx_encode_map(&maps.p, g.p, 2, a.n, g.M, g.ldp * 2, 64, kGrTok, true)) return LORA_ERR_CUDA;
-  auto kernel = mx_grad_kernel<T, F8>;
+  auto kernel = mx_grad_kernel<T>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
   std::call_once(once[dev], [&] {
     attr_err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGrSmemMax);
   });
   if (attr_err[dev] != cudaSuccess) return LORA_ERR_CUDA;
-  const size_t smem = static_cast<size_t>(a.stages) * a.stage_bytes + fixed;
-  return mx_launch(kernel, dim3(pl.groups, pl.splits), kGrThreads, smem, stream, 0, maps, a);
+  return mx_launch(kernel, dim3(blocks), kGrThreads, smem, stream, 0, jobs);
 }
 
 }  // namespace
@@ -400,18 +430,14 @@ size_t mx_grad_part_bytes(int64_t M, int64_t C, int64_t R) {
   return static_cast<size_t>(grad_plan(M, C).splits) * C * ((R + 15) / 16 * 16) * sizeof(float);
 }
 
-int mx_grad_launch(const MxGradOperands& g, int dtype, cudaStream_t stream) {
-  const GrPlan pl = grad_plan(g.M, g.C);
-  const bool f8 = g.v_scales != nullptr;
-  if (dtype == LORA_BF16)
-    return f8 ? launch_grad<__nv_bfloat16, true>(g, pl, stream) : launch_grad<__nv_bfloat16, false>(g, pl, stream);
-  return f8 ? launch_grad<__half, true>(g, pl, stream) : launch_grad<__half, false>(g, pl, stream);
+int mx_grad_launch(const MxGradOperands* g, int dtype, cudaStream_t stream) {
+  return dtype == LORA_BF16 ? launch_grads<__nv_bfloat16>(g, stream) : launch_grads<__half>(g, stream);
 }
 
-int mx_grad_reduce_launch(const MxGradOperands* g, int count, int dtype, cudaStream_t stream) {
+int mx_grad_reduce_launch(const MxGradOperands* g, int dtype, cudaStream_t stream) {
   GrSums sums = {};
   int blocks = 0, r32 = 0;
-  for (int i = 0; i < count; ++i) {
+  for (int i = 0; i < 2; ++i) {
     GrSum& s = sums.of[i];
     s.part = static_cast<const float*>(g[i].part);
     s.out = g[i].out;

@@ -17,8 +17,9 @@ struct MxGradOperands {
 };
 
 size_t mx_grad_part_bytes(int64_t M, int64_t C, int64_t R);
-// The partial sums of one gradient, and the sums of several in one launch.
-int mx_grad_launch(const MxGradOperands& g, int dtype, cudaStream_t stream);
-int mx_grad_reduce_launch(const MxGradOperands* g, int count, int dtype, cudaStream_t stream);
+// g[0]: a 16-bit V, g[1]: an mxfp8 V.  The partial sums of both in one launch, and
+// their sums in another.
+int mx_grad_launch(const MxGradOperands* g, int dtype, cudaStream_t stream);
+int mx_grad_reduce_launch(const MxGradOperands* g, int dtype, cudaStream_t stream);
 
 }  // namespace lora
