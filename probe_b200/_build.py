@@ -21,7 +21,7 @@ INCLUDE = REPO_DIR / "include"
 BUILD_DIR = PKG_DIR / "_build"
 LIB_PATH = PKG_DIR / "liblora_b200.so"
 
-SOURCES = ("runtime.cu", "gemm_tc.cu", "shrink.cu", "expand.cu", "decode.cu", "sgmv.cu", "sgmv_block.cu", "sgmv_tc.cu", "sgmv_unit.cu", "sgmv_linear.cu", "skinny_tc.cu", "gemm_split.cu", "mx_quant.cu", "mx_gemm.cu", "mx_small.cu", "mx_linear.cu", "mx_shrink.cu", "mx_grad.cu", "mx_backward.cu")
+SOURCES = ("runtime.cu", "gemm_tc.cu", "shrink.cu", "expand.cu", "decode.cu", "sgmv.cu", "sgmv_block.cu", "sgmv_tc.cu", "sgmv_unit.cu", "sgmv_linear.cu", "skinny_tc.cu", "gemm_split.cu", "mx_quant.cu", "mx_gemm.cu", "mx_small.cu", "mx_linear.cu", "mx_shrink.cu", "mx_grad.cu", "mx_dx.cu", "mx_backward.cu")
 ARCH_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a")
 NVCC_FLAGS = ("-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden")
 

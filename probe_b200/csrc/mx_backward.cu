@@ -7,12 +7,14 @@
 //
 // The base weight is frozen; rounding to 4 or 8 bits counts as the identity
 // (straight-through).  dx needs W with N as the contraction, against the direction
-// of its scale blocks, so W is decoded once, transposed, into the workspace (its
-// values are exact in 16 bits: nvfp4's tensor scale m 2^p leaves the power of two
-// in the values and m in the GEMM's alpha) and the 16-bit CTA-pair GEMM takes
-// [g_hi | g_lo] against [A^T | A^T] as its K tail (few rows: the W-streaming kernel).
+// of its scale blocks.  Few rows (mx_few_tokens): W is decoded on its way into the MMAs
+// (mx_dx.cu).  Many: W is decoded once, transposed, into the workspace and the 16-bit
+// CTA-pair GEMM takes [g_hi | g_lo] against [A^T | A^T] as its K tail.  Either way W's
+// values are exact in 16 bits: nvfp4's tensor scale m 2^p leaves the power of two in the
+// values and m in the product's alpha.
 #include <cmath>
 
+#include "mx_dx.h"
 #include "mx_grad.h"
 #include "mx_shrink.h"
 
@@ -27,13 +29,16 @@ constexpr int64_t kWideRank = 128, kWideRows = 4096;
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 struct BackwardPlan {
+  bool few;  // dx of few rows
   size_t gemm_bytes, part, part_a, g, bt, at, dy, wt, total;
 };
 
 BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need_dx) {
   BackwardPlan p = {};
   const int64_t np = up(N, 8), rp = up(R, 16);
-  if (need_dx) p.gemm_bytes = lora_gemm_workspace_size(M, K, np, 2 * rp);
+  const int dev = current_device();
+  p.few = need_dx && mx_few_tokens(M, K, dev >= 0 ? device_info(dev).num_sms : 148);
+  if (need_dx && !p.few) p.gemm_bytes = lora_gemm_workspace_size(M, K, np, 2 * rp);
   if (R > kWideRank && M >= kWideRows) p.gemm_bytes = std::max(p.gemm_bytes, lora_gemm_workspace_size(M, R, np, 0));
   size_t at = kCounterBytes;  // ticket counters, never scratch; the steps' partials follow them in turn
   at = std::max(at, mx_align(std::max(kCounterBytes + mx_shrink_part_bytes(M, np, R), p.gemm_bytes)));
@@ -46,11 +51,11 @@ BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need
   p.bt = at;
   at += mx_align(static_cast<size_t>(R) * np * 2);
   p.at = at;
-  if (need_dx) at += mx_align(static_cast<size_t>(K) * 2 * rp * 2);
+  if (need_dx) at += mx_align(p.few ? static_cast<size_t>(R) * up(K, 8) * 2 : static_cast<size_t>(K) * 2 * rp * 2);
   p.dy = at;
   at += mx_align(static_cast<size_t>(M) * np * 2);
   p.wt = at;
-  if (need_dx) at += mx_align(static_cast<size_t>(K) * np * 2);
+  if (need_dx && !p.few) at += mx_align(static_cast<size_t>(K) * np * 2);
   p.total = at;
   return p;
 }
@@ -117,6 +122,12 @@ __global__ void __launch_bounds__(256) mx_widen_kernel(const uint16_t* __restric
   if (c + 8 < width) dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
+int widen(const void* in, int64_t ldi, void* out, int64_t rows, int64_t cols, int64_t width, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>((width + 4095) / 4096));
+  mx_widen_kernel<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(in), ldi, static_cast<uint16_t*>(out), cols, width);
+  return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
+}
+
 }  // namespace
 }  // namespace lora
 
@@ -172,20 +183,26 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   const bool b_rows = mx_aligned(b, 16) && ldb % 8 == 0;  // TMA can read them
   const bool wide = R > kWideRank && M >= kWideRows;
   if (!b_rows || wide) jobs.of[0] = transpose_job(b, ldb, ws + p.bt, np, N, R, np, 1);
-  if (dx != nullptr) jobs.of[1] = transpose_job(a, lda, ws + p.at, 2 * rp, R, K, rp, 2);
+  if (dx != nullptr && !p.few) jobs.of[1] = transpose_job(a, lda, ws + p.at, 2 * rp, R, K, rp, 2);
   int rc = transpose(jobs, s);
   if (rc != LORA_OK) return rc;
-  if (dx != nullptr) {
+  const void* ap = a;
+  int64_t lda_p = lda;
+  if (p.few && (lda % 8 != 0 || !mx_aligned(a, 16))) {
+    lda_p = up(K, 8);
+    ap = ws + p.at;
+    rc = widen(a, lda, ws + p.at, R, K, lda_p, s);
+    if (rc != LORA_OK) return rc;
+  }
+  if (dx != nullptr && !p.few) {
     rc = mx_dequantize_launch(w_codes, w_scales, ws + p.wt, np, N, K, w_fmt, pow2, 2, dtype, s);
     if (rc != LORA_OK) return rc;
   }
   const void* dyp = dy;
   int64_t ldp = lddy;
   if (N % 8 != 0 || lddy % 8 != 0 || !mx_aligned(dy, 16)) {  // TMA needs 16-byte rows
-    const dim3 grid(static_cast<unsigned>(M), static_cast<unsigned>((np + 4095) / 4096));
-    mx_widen_kernel<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(dy), lddy, reinterpret_cast<uint16_t*>(ws + p.dy), N,
-                                         np);
-    if (cudaGetLastError() != cudaSuccess) return LORA_ERR_CUDA;
+    rc = widen(dy, lddy, ws + p.dy, M, N, np, s);
+    if (rc != LORA_OK) return rc;
     dyp = ws + p.dy;
     ldp = np;
   }
@@ -248,25 +265,26 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   rc = mx_grad_reduce_launch(grads, dtype, s);
   if (rc != LORA_OK || dx == nullptr) return rc;
 
-  if (mx_few_tokens(M, K, device_info(dev).num_sms)) {
-    MxLinearOperands o = {};
-    o.x_codes = dyp;
-    o.ldx = ldp;
-    o.w_codes = ws + p.wt;
-    o.ldw = np;
-    o.z = ws + p.g;
-    o.ldz = 2 * rp;
-    o.z_lo = rp;
-    o.b = ws + p.at;
-    o.ldb = 2 * rp;
-    o.out = dx;
-    o.ldo = lddx;
+  if (p.few) {
+    MxDxOperands o = {};
+    o.dy = dyp;
+    o.lddy = ldp;
+    o.w_codes = w_codes;
+    o.w_scales = w_scales;
+    o.g = ws + p.g;
+    o.ldg = 2 * rp;
+    o.g_lo = rp;
+    o.a = ap;
+    o.lda = lda_p;
+    o.dx = dx;
+    o.lddx = lddx;
     o.M = M;
-    o.N = K;
-    o.K = np;
+    o.N = N;
+    o.K = K;
     o.R = R;
     o.alpha = m;
-    return mx_small_launch(o, -1, dtype, s);
+    o.pow2 = pow2;
+    return mx_dx_launch(o, w_fmt, dtype, s);
   }
   return lora_gemm_ex(dyp, ldp, ws + p.wt, np, ws + p.g, 2 * rp, ws + p.at, 2 * rp, nullptr, dx, lddx, M, K, np, 2 * rp,
                       m, 0, dtype, p.gemm_bytes ? ws : nullptr, p.gemm_bytes, s);

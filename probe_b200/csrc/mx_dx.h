@@ -1,0 +1,19 @@
+// Host interface of the input gradient of few rows (mx_dx.cu).
+#pragma once
+
+#include "mx_linear.h"
+
+namespace lora {
+
+// dx[t, k] = alpha (sum_n dy[t, n] Wv[n, k] + sum_j (gh + gl)[t, j] A[j, k]), Wv the
+// values of the 4-bit W [N, K] times pow2.
+struct MxDxOperands {
+  const void *dy, *w_codes, *w_scales, *g, *a;  // dy [M, lddy], rows of 16 bytes; a [R, lda], likewise
+  void* dx;
+  int64_t lddy, ldg, g_lo, lda, lddx, M, N, K, R;
+  float alpha, pow2;
+};
+
+int mx_dx_launch(const MxDxOperands& o, int fmt, int dtype, cudaStream_t stream);
+
+}  // namespace lora

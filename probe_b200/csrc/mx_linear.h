@@ -15,11 +15,10 @@ struct MxLinearOperands {
   int64_t ldz, z_lo, ldb, ldo, M, N, K, R;
   float alpha;
   int dshift;
-  int64_t ldx, ldw;  // 16-bit operands (in x_codes, w_codes) only
 };
 
-// Few tokens (mx_small.cu; fmt -1: x and W in 16 bits) and many (mx_gemm.cu).  Few: one
-// tile of 128 tokens, or as many 128 x 128 tiles as there are SMs.
+// Few tokens (mx_small.cu) and many (mx_gemm.cu).  Few: one tile of 128 tokens, or as
+// many 128 x 128 tiles as there are SMs.
 bool mx_few_tokens(int64_t M, int64_t N, int num_sms);
 int mx_small_launch(const MxLinearOperands& o, int fmt, int dtype, cudaStream_t stream);
 int mx_gemm_launch(const MxLinearOperands& o, int fmt, int dtype, cudaStream_t stream);

@@ -11,12 +11,11 @@
 // until about two CTAs an SM stream W; their partial tiles meet in shared memory
 // and are summed in rank order over DSMEM.  The kernel starts while its predecessor
 // (the shrink that makes xq, sx and z) still runs: W's first stages load before
-// griddepcontrol.wait.  The same kernel with W in 16 bits (64-deep stages, no scales)
-// gives dx of few rows in the backward pass.
+// griddepcontrol.wait.
 #include <cmath>
 #include <mutex>
 
-#include "mx_linear.h"
+#include "mx_tile.cuh"
 
 namespace lora {
 namespace {
@@ -32,13 +31,9 @@ struct SmMaps {
 };
 
 struct SmArgs {
-  void* out;
-  const void* bias;
+  MxTileOut tile;
   int* err;
-  int64_t ldo;
-  int M, N;
   int num_kb, last_step, rank_kb, last_k16, chunks, stages;
-  float alpha, base_scale;  // 2^-dshift
 };
 
 LORA_DEVINL uint64_t sm_desc_scales(uint32_t addr) {
@@ -74,23 +69,16 @@ LORA_DEVINL void sm_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint
   }
 }
 
-constexpr int kSm16Bit = -1;  // FMT of a 16-bit W
-
-template <int FMT> __host__ __device__ constexpr int sm_chunks() { return 256 / MxFormat<FMT>::kBlock / 4; }
-template <> __host__ __device__ constexpr int sm_chunks<kSm16Bit>() { return 0; }
-
 template <int FMT, int NB>
 struct SmLayout {
-  static constexpr int kChunks = sm_chunks<FMT>();
-  static constexpr int kDepth = FMT == kSm16Bit ? 64 : 256;  // K of a stage: 128 bytes a row
-  static constexpr int kStep = kDepth / 4;                   // K of an MMA
+  static constexpr int kChunks = 256 / MxFormat<FMT>::kBlock / 4;
   static constexpr int kW = 128 * 128, kX = NB * 128, kSf = kChunks * 512;
   static constexpr int kStage = (kW + kX + 2 * kSf + 1023) / 1024 * 1024;
   static constexpr int kXOffset = kW, kSfOffset = kW + kX;
   static constexpr int kMainBytes = kW + kX + 2 * kSf;
   static constexpr int kSfCols = 2 * kChunks * 4;
   // TMEM: base accumulator, adapter accumulator, scales of every stage
-  static constexpr int kFit = kSfCols == 0 ? 8 : (sm_tmem_max<NB>() - 2 * NB) / (kSfCols == 0 ? 1 : kSfCols);
+  static constexpr int kFit = (sm_tmem_max<NB>() - 2 * NB) / kSfCols;
   static constexpr int kMaxStages = kFit < 8 ? kFit : 8;
 };
 
@@ -101,7 +89,6 @@ __global__ void __launch_bounds__(kSmThreads)
   constexpr uint32_t kCols = 2 * NB + L::kMaxStages * L::kSfCols;
   constexpr uint32_t kTmemCols = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
   static_assert(kTmemCols <= sm_tmem_max<NB>(), "TMEM");
-  constexpr int kInner = FMT == kSm16Bit ? 64 : 128;  // map elements of a stage's row
   constexpr uint32_t kIdesc = (1u << 7) | (1u << 10) | (static_cast<uint32_t>(NB >> 3) << 17) |
                               ((FMT == LORA_MXFP4 ? 1u : 0u) << 23) | (8u << 24);
   constexpr uint32_t kIdescTail = (1u << 4) | ((std::is_same<T, __nv_bfloat16>::value ? 1u : 0u) << 7) |
@@ -152,10 +139,9 @@ __global__ void __launch_bounds__(kSmThreads)
         uint8_t* base = smem + stage * L::kStage;
         if (i < kb1 - kb0) {
           mbar_arrive_expect_tx(&full[stage], L::kMainBytes);
-          tma_load_2d(&maps.w, base, &full[stage], (kb0 + i) * kInner, n0);
-          if constexpr (L::kChunks > 0)
-            tma_load_2d(&maps.sw, base + L::kSfOffset, &full[stage], 0,
-                        (n0 >> 7) * args.chunks + (kb0 + i) * L::kChunks);
+          tma_load_2d(&maps.w, base, &full[stage], (kb0 + i) * 128, n0);
+          tma_load_2d(&maps.sw, base + L::kSfOffset, &full[stage], 0,
+                      (n0 >> 7) * args.chunks + (kb0 + i) * L::kChunks);
         } else {
           const int t = i - (kb1 - kb0);
           mbar_arrive_expect_tx(&full[stage], L::kW + L::kX);
@@ -165,10 +151,9 @@ __global__ void __launch_bounds__(kSmThreads)
       auto tokens = [&](int i, int stage) {
         uint8_t* base = smem + stage * L::kStage;
         if (i < kb1 - kb0) {
-          tma_load_2d(&maps.x, base + L::kXOffset, &full[stage], (kb0 + i) * kInner, t0);
-          if constexpr (L::kChunks > 0)
-            tma_load_2d(&maps.sx, base + L::kSfOffset + L::kSf, &full[stage], 0,
-                        (t0 >> 7) * args.chunks + (kb0 + i) * L::kChunks);
+          tma_load_2d(&maps.x, base + L::kXOffset, &full[stage], (kb0 + i) * 128, t0);
+          tma_load_2d(&maps.sx, base + L::kSfOffset + L::kSf, &full[stage], 0,
+                      (t0 >> 7) * args.chunks + (kb0 + i) * L::kChunks);
         } else {
           const int t = i - (kb1 - kb0);
           const bool lo = t >= args.rank_kb;
@@ -218,18 +203,12 @@ __global__ void __launch_bounds__(kSmThreads)
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            if constexpr (FMT == kSm16Bit) {
-              if (k < nk)
-                tc_mma_f16(tmem, wd + static_cast<uint32_t>(2 * k), xd + static_cast<uint32_t>(2 * k), kIdescTail,
-                           (i > 0 || k > 0) ? 1u : 0u);
-            } else {
-              constexpr bool kMx = FMT == LORA_MXFP4;
-              const int j = kMx ? k >> 1 : k;
-              const uint32_t id = kMx ? static_cast<uint32_t>(k & 1) * 2u : 0u;
-              if (k < nk)
-                sm_mma<FMT>(tmem, wd + static_cast<uint32_t>(2 * k), xd + static_cast<uint32_t>(2 * k),
-                            kIdesc | (id << 4) | (id << 29), sfa + 4 * j, sfb + 4 * j, (i > 0 || k > 0) ? 1u : 0u);
-            }
+            constexpr bool kMx = FMT == LORA_MXFP4;
+            const int j = kMx ? k >> 1 : k;
+            const uint32_t id = kMx ? static_cast<uint32_t>(k & 1) * 2u : 0u;
+            if (k < nk)
+              sm_mma<FMT>(tmem, wd + static_cast<uint32_t>(2 * k), xd + static_cast<uint32_t>(2 * k),
+                          kIdesc | (id << 4) | (id << 29), sfa + 4 * j, sfb + 4 * j, (i > 0 || k > 0) ? 1u : 0u);
           }
           tc_commit(&empty[stage]);
         }
@@ -256,72 +235,8 @@ __global__ void __launch_bounds__(kSmThreads)
     __syncwarp();
   }
 
-  // ---- epilogue: warps 2..5 put the partial tile, one row of W a thread, into the
-  // drained stages as [token][128]; then a warp sums and stores one token's 128
-  // columns at a time, the ranks' parts in rank order
-  const int count = min(NB, args.M - t0);
-  float* part = reinterpret_cast<float*>(smem);
-  if (warp >= 2 && warp_wait(acc_full, 0, abort_flag, args.err, kDevErrTimeoutAccFull)) {
-    tc_fence_after();
-    const int quad = warp & 3;
-    const uint32_t t_row = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t dst = smem_u32(part) + (quad * 32 + lane) * 4;
-#pragma unroll 1
-    for (int c = 0; c < count; c += 16) {
-      uint32_t u[16], l[16];
-      tmem_ld_32x32b_x16(t_row + c, u);
-      if (tail_kb > 0) tmem_ld_32x32b_x16(t_row + NB + c, l);
-      tmem_wait_ld();
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        float v = __uint_as_float(u[e]) * args.base_scale;
-        if (tail_kb > 0) v += __uint_as_float(l[e]);
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + (c + e) * 512), "f"(v) : "memory");
-      }
-    }
-  }
-  if (splits > 1)
-    cluster_sync_all();  // every rank's partial tile is in its shared memory
-  else
-    __syncthreads();
-  {
-    const int b = count * rank / splits, e = count * (rank + 1) / splits;
-    const int n = n0 + 4 * lane;
-    const bool vec = args.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(args.out) & 7) == 0 && n + 4 <= args.N;
-    const T* bias = static_cast<const T*>(args.bias);
-    float add[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (bias != nullptr && n + i < args.N) add[i] = to_f32(bias[n + i]);
-    const uint32_t src = smem_u32(part) + lane * 16;
-    for (int t = b + warp; t < e; t += kSmThreads / 32) {
-      float4 v;
-      if (splits == 1) {
-        const uint4 u = lds128(src + t * 512);
-        v = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
-      } else {
-        float4 p[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          if (q < splits) p[q] = ld_dsmem_f4(mapa_shared(src + t * 512, q));
-        v = p[0];
-#pragma unroll
-        for (int q = 1; q < 8; ++q)
-          if (q < splits) v.x += p[q].x, v.y += p[q].y, v.z += p[q].z, v.w += p[q].w;
-      }
-      v.x = v.x * args.alpha + add[0], v.y = v.y * args.alpha + add[1];
-      v.z = v.z * args.alpha + add[2], v.w = v.w * args.alpha + add[3];
-      T* o = static_cast<T*>(args.out) + static_cast<int64_t>(t0 + t) * args.ldo + n;
-      if (vec) {
-        *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
-      } else {
-        if (n < args.N) o[0] = from_f32<T>(v.x);
-        if (n + 1 < args.N) o[1] = from_f32<T>(v.y);
-        if (n + 2 < args.N) o[2] = from_f32<T>(v.z);
-        if (n + 3 < args.N) o[3] = from_f32<T>(v.w);
-      }
-    }
-  }
+  mx_tile_out<T, NB, kSmThreads, 2, 4>(args.tile, reinterpret_cast<float*>(smem), tmem, tail_kb > 0 ? NB : 0, acc_full,
+                                       abort_flag, args.err, splits, rank, n0, t0);
   tc_fence_before();
   if (splits > 1)
     cluster_sync_all();  // no CTA leaves while another reads its partial tile
@@ -341,21 +256,13 @@ int launch_small(const MxLinearOperands& o, cudaStream_t stream) {
   const DeviceInfo& info = device_info(dev);
   SmMaps maps;
   SmArgs a;
-  if constexpr (FMT == kSm16Bit) {
-    a.chunks = 0;
-    if (!mx_encode_map(&maps.x, o.x_codes, 2, o.K, o.M, o.ldx * 2, 64, NB, true) ||
-        !mx_encode_map(&maps.w, o.w_codes, 2, o.K, o.N, o.ldw * 2, 64, 128, true))
-      return LORA_ERR_CUDA;
-    maps.sx = maps.sw = maps.x;
-  } else {
-    const int64_t pitch = mx_code_pitch(o.K, FMT);
-    a.chunks = static_cast<int>(mx_scale_chunks(o.K, FMT));
-    if (!mx_encode_map(&maps.x, o.x_codes, 1, pitch, o.M, pitch, 128, NB, true) ||
-        !mx_encode_map(&maps.w, o.w_codes, 1, pitch, o.N, pitch, 128, 128, true) ||
-        !mx_encode_map(&maps.sx, o.x_scales, 4, 128, (o.M + 127) / 128 * a.chunks, 512, 128, L::kChunks, false) ||
-        !mx_encode_map(&maps.sw, o.w_scales, 4, 128, (o.N + 127) / 128 * a.chunks, 512, 128, L::kChunks, false))
-      return LORA_ERR_CUDA;
-  }
+  const int64_t pitch = mx_code_pitch(o.K, FMT);
+  a.chunks = static_cast<int>(mx_scale_chunks(o.K, FMT));
+  if (!mx_encode_map(&maps.x, o.x_codes, 1, pitch, o.M, pitch, 128, NB, true) ||
+      !mx_encode_map(&maps.w, o.w_codes, 1, pitch, o.N, pitch, 128, 128, true) ||
+      !mx_encode_map(&maps.sx, o.x_scales, 4, 128, (o.M + 127) / 128 * a.chunks, 512, 128, L::kChunks, false) ||
+      !mx_encode_map(&maps.sw, o.w_scales, 4, 128, (o.N + 127) / 128 * a.chunks, 512, 128, L::kChunks, false))
+    return LORA_ERR_CUDA;
   if (o.R > 0) {
     const char* z = static_cast<const char*>(o.z);
     if (!mx_encode_map(&maps.zh, z, 2, o.R, o.M, o.ldz * 2, 64, NB, true) ||
@@ -365,19 +272,13 @@ int launch_small(const MxLinearOperands& o, cudaStream_t stream) {
   } else {
     maps.zh = maps.zl = maps.b = maps.x;
   }
-  a.out = o.out;
-  a.bias = o.bias;
+  a.tile = {o.out, o.bias, o.ldo, static_cast<int>(o.M), static_cast<int>(o.N), o.alpha, ldexpf(1.f, -o.dshift)};
   a.err = info.err_word;
-  a.ldo = o.ldo;
-  a.M = static_cast<int>(o.M);
-  a.N = static_cast<int>(o.N);
-  const int64_t kp = FMT == kSm16Bit ? o.K : mx_padded_k(o.K);
-  a.num_kb = static_cast<int>((kp + L::kDepth - 1) / L::kDepth);
-  a.last_step = static_cast<int>((kp - static_cast<int64_t>(a.num_kb - 1) * L::kDepth + L::kStep - 1) / L::kStep);
+  const int64_t kp = mx_padded_k(o.K);
+  a.num_kb = static_cast<int>((kp + 255) / 256);
+  a.last_step = static_cast<int>((kp - static_cast<int64_t>(a.num_kb - 1) * 256 + 63) / 64);
   a.rank_kb = static_cast<int>((o.R + 63) / 64);
   a.last_k16 = a.rank_kb > 0 ? static_cast<int>((o.R - (a.rank_kb - 1) * 64ll + 15) / 16) : 0;
-  a.alpha = o.alpha;
-  a.base_scale = ldexpf(1.f, -o.dshift);
   // The partial tile (NB x 128 fp32) lies over the stages.
   constexpr int kFixed = 1024 + 256;
   a.stages = std::min<int>(L::kMaxStages, (sm_smem_max<NB>() - kFixed) / L::kStage);
@@ -412,7 +313,6 @@ int dispatch(const MxLinearOperands& o, cudaStream_t s) {
 }  // namespace
 
 int mx_small_launch(const MxLinearOperands& o, int fmt, int dtype, cudaStream_t s) {
-  if (fmt == kSm16Bit) return dtype == LORA_BF16 ? dispatch<__nv_bfloat16, kSm16Bit>(o, s) : dispatch<__half, kSm16Bit>(o, s);
   if (dtype == LORA_BF16)
     return fmt == LORA_MXFP4 ? dispatch<__nv_bfloat16, LORA_MXFP4>(o, s) : dispatch<__nv_bfloat16, LORA_NVFP4>(o, s);
   return fmt == LORA_MXFP4 ? dispatch<__half, LORA_MXFP4>(o, s) : dispatch<__half, LORA_NVFP4>(o, s);
