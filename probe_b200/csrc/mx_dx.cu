@@ -8,7 +8,7 @@
 // on its way into the MMA: TMA brings the codes of 64 rows x 128 columns and their
 // scale chunks, eight warps turn them into 16-bit values in the MN-major layout of
 // the MMA's 128-wide operand -- 64-column chunks, token rows 128 bytes apart, the
-// 128-byte swizzle -- so the transposition is the MMA's; dy's tile, 16..128 tokens, is
+// 128-byte swizzle -- so the transposition is the MMA's; dy's tile, 16..256 tokens, is
 // the other operand.  A's rows, as they lie in memory, have that layout by TMA alone:
 // they follow as the last stages, against gh and then gl.
 //
@@ -29,14 +29,17 @@
 namespace lora {
 namespace {
 
-constexpr int kDxConvWarps = 8;
-constexpr int kDxThreads = 64 + 32 * kDxConvWarps;
+constexpr int kDxGroupWarps = 8;                 // decode a stage
 constexpr int kDxRows = 64;                      // of W (or A) a stage
 constexpr int kDxHalf = kDxRows * 128;           // 64 rows x 64 16-bit columns
 constexpr int kDxW = 2 * kDxHalf;                // the operand tile
 constexpr int kDxRaw = kDxRows * 64;             // codes of a stage
-// Two CTAs an SM, or (128 tokens) one.
-template <int NB> __host__ __device__ constexpr int dx_smem_max() { return NB == 128 ? 220 * 1024 : 112 * 1024; }
+// Two CTAs an SM, or (128 tokens and more) one, with two groups of decoding warps that
+// take stages in turn.
+template <int NB> __host__ __device__ constexpr int dx_ctas() { return NB >= 128 ? 1 : 2; }
+template <int NB> __host__ __device__ constexpr int dx_smem_max() { return NB >= 128 ? 220 * 1024 : 112 * 1024; }
+template <int NB> __host__ __device__ constexpr int dx_groups() { return NB >= 128 ? 2 : 1; }
+template <int NB> __host__ __device__ constexpr int dx_threads() { return 64 + 32 * kDxGroupWarps * dx_groups<NB>(); }
 
 struct DxMaps {
   CUtensorMap x, w, sw, gh, gl, a;
@@ -120,7 +123,7 @@ LORA_DEVINL uint4 dx_decode8_any(uint32_t w, float f) {
 }
 
 template <typename T, int FMT, int NB>
-__global__ void __launch_bounds__(kDxThreads)
+__global__ void __launch_bounds__(dx_threads<NB>(), dx_ctas<NB>())
     mx_dx_kernel(const __grid_constant__ DxMaps maps, const DxArgs args) {
   using L = DxLayout<FMT, NB>;
   constexpr uint32_t kTmemCols = NB <= 32 ? 32 : NB;
@@ -154,7 +157,7 @@ __global__ void __launch_bounds__(kDxThreads)
     for (int s = 0; s < args.stages; ++s) {
       mbar_init(&full_w[s], 1);
       mbar_init(&full_x[s], 1);
-      mbar_init(&ready[s], kDxConvWarps);
+      mbar_init(&ready[s], kDxGroupWarps);
       mbar_init(&empty[s], 1);
     }
     mbar_init(acc_full, 1);
@@ -251,7 +254,8 @@ __global__ void __launch_bounds__(kDxThreads)
   } else {
     // a thread decodes 32 columns of a row; the upper 64 columns' threads take their
     // 16-byte units in another order, so that eight lanes' stores meet eight banks
-    const int id = threadIdx.x - 64, r = id >> 2, seg = id & 3, swap = seg >> 1;
+    const int group = (warp - 2) / kDxGroupWarps, id = (threadIdx.x - 64) % (32 * kDxGroupWarps);
+    const int r = id >> 2, seg = id & 3, swap = seg >> 1;
     const uint32_t src = smem_u32(smem) + L::kRawOffset + id * 16;
     const uint32_t dst = smem_u32(smem) + swap * kDxHalf + r * 128;
     const uint32_t sf = smem_u32(smem) + L::kSfOffset + (r & 31) * 16 + (r >> 5) * 4 +
@@ -259,34 +263,36 @@ __global__ void __launch_bounds__(kDxThreads)
     int stage = 0;
     uint32_t phase = 0;
     for (int i = 0; i < total; ++i) {
-      if (!warp_wait(&full_w[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) break;
-      if (i < base) {
-        const uint32_t at = static_cast<uint32_t>(stage * L::kStage);
-        const uint32_t sa = sf + at + ((kb0 + i) & 1) * 8;  // odd stages: rows 64..127 of their scale chunk
-        const uint4 q = lds128(src + at);
-        const uint32_t w[4] = {swap ? q.z : q.x, swap ? q.w : q.y, swap ? q.x : q.z, swap ? q.y : q.w};
-        float f[2];
-        if constexpr (FMT == LORA_NVFP4) {
-          f[0] = mx_e4m3(lds_u8(sa + swap)) * args.pow2;
-          f[1] = mx_e4m3(lds_u8(sa + 1 - swap)) * args.pow2;
-        } else {
-          f[0] = f[1] = mx_e8m0(lds_u8(sa)) * args.pow2;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t pair;
-          const bool exact = dx_factor<T>(f[h], pair);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int j = 2 * h + e;  // unit j ^ (2 swap) of this thread's four
-            const uint4 v = exact ? dx_decode8<T>(w[j], pair) : dx_decode8_any<T>(w[j], f[h]);
-            sts128(dst + at + (((((seg & 1) << 2) + (j ^ (2 * swap))) ^ (r & 7)) << 4), v);
+      if (i % dx_groups<NB>() == group) {
+        if (!warp_wait(&full_w[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) break;
+        if (i < base) {
+          const uint32_t at = static_cast<uint32_t>(stage * L::kStage);
+          const uint32_t sa = sf + at + ((kb0 + i) & 1) * 8;  // odd stages: rows 64..127 of their scale chunk
+          const uint4 q = lds128(src + at);
+          const uint32_t w[4] = {swap ? q.z : q.x, swap ? q.w : q.y, swap ? q.x : q.z, swap ? q.y : q.w};
+          float f[2];
+          if constexpr (FMT == LORA_NVFP4) {
+            f[0] = mx_e4m3(lds_u8(sa + swap)) * args.pow2;
+            f[1] = mx_e4m3(lds_u8(sa + 1 - swap)) * args.pow2;
+          } else {
+            f[0] = f[1] = mx_e8m0(lds_u8(sa)) * args.pow2;
           }
+  #pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t pair;
+            const bool exact = dx_factor<T>(f[h], pair);
+  #pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int j = 2 * h + e;  // unit j ^ (2 swap) of this thread's four
+              const uint4 v = exact ? dx_decode8<T>(w[j], pair) : dx_decode8_any<T>(w[j], f[h]);
+              sts128(dst + at + (((((seg & 1) << 2) + (j ^ (2 * swap))) ^ (r & 7)) << 4), v);
+            }
+          }
+          fence_proxy_async_smem();
         }
-        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ready[stage]);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ready[stage]);
       if (++stage == args.stages) {
         stage = 0;
         phase ^= 1;
@@ -294,8 +300,8 @@ __global__ void __launch_bounds__(kDxThreads)
     }
   }
 
-  mx_tile_out<T, NB, kDxThreads, 2, kDxConvWarps>(args.tile, reinterpret_cast<float*>(smem), tmem, 0, acc_full, abort_flag,
-                                                  args.err, splits, rank, k0, t0);
+  mx_tile_out<T, NB, dx_threads<NB>(), 2, kDxGroupWarps * dx_groups<NB>()>(
+      args.tile, reinterpret_cast<float*>(smem), tmem, 0, acc_full, abort_flag, args.err, splits, rank, k0, t0);
   tc_fence_before();
   if (splits > 1)
     cluster_sync_all();  // no CTA leaves while another reads its partial tile
@@ -337,7 +343,7 @@ int launch_dx(const MxDxOperands& o, cudaStream_t stream) {
   static_assert((dx_smem_max<NB>() - kFixed) / L::kStage * L::kStage >= NB * 512, "the partial tile lies over the stages");
   const int k_tiles = static_cast<int>((o.K + 127) / 128), t_tiles = static_cast<int>((o.M + NB - 1) / NB);
   // as many CTAs as are resident at once, each with eight or more stages
-  const int resident = (NB == 128 ? 1 : 2) * info.num_sms;
+  const int resident = dx_ctas<NB>() * info.num_sms;
   int splits = 1;
   while (splits < 8 && k_tiles * t_tiles * splits * 2 <= resident && a.num_kb >= 16 * splits) splits *= 2;
   const size_t smem = static_cast<size_t>(a.stages) * L::kStage + kFixed;
@@ -348,7 +354,7 @@ int launch_dx(const MxDxOperands& o, cudaStream_t stream) {
     attr_err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, dx_smem_max<NB>());
   });
   if (attr_err[dev] != cudaSuccess) return LORA_ERR_CUDA;
-  return mx_launch(kernel, dim3(k_tiles * splits, t_tiles), kDxThreads, smem, stream, splits, maps, a);
+  return mx_launch(kernel, dim3(k_tiles * splits, t_tiles), dx_threads<NB>(), smem, stream, splits, maps, a);
 }
 
 template <typename T, int FMT>
@@ -356,7 +362,7 @@ int dispatch(const MxDxOperands& o, cudaStream_t s) {
   if (o.M <= 16) return launch_dx<T, FMT, 16>(o, s);
   if (o.M <= 32) return launch_dx<T, FMT, 32>(o, s);
   if (o.M <= 64) return launch_dx<T, FMT, 64>(o, s);
-  return launch_dx<T, FMT, 128>(o, s);
+  return o.M <= 128 ? launch_dx<T, FMT, 128>(o, s) : launch_dx<T, FMT, 256>(o, s);
 }
 
 }  // namespace
