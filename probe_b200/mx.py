@@ -97,8 +97,9 @@ class MXTensor:
     __slots__ = ("codes", "scales", "shape", "fmt", "global_scale", "_code")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, fmt: str, global_scale: float = 1.0):
-        code = _format(fmt, "MXTensor")
-        m, k = (int(v) for v in shape)
+        self._code = _format(fmt, "MXTensor")
+        m, k = shape
+        m, k = int(m), int(k)
         pitch, nscales = _sizes(m, k, fmt)
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise TypeError("MXTensor: codes and scales are uint8")
@@ -111,7 +112,6 @@ class MXTensor:
             raise ValueError("MXTensor: codes and scales lie on different devices")
         self.codes, self.scales, self.shape, self.fmt = codes, scales, (m, k), fmt
         self.global_scale = float(global_scale)
-        self._code = code
 
     @classmethod
     def _of(cls, codes, scales, shape, fmt, global_scale, code):
@@ -274,6 +274,24 @@ def mx_lora_linear(x: torch.Tensor, weight: MXTensor, bias: torch.Tensor | None,
 
 
 # ------------------------------------------------------------------- training
+def _refuse_backward(dy, x8, z, a, b, weight, where):
+    """The error of a call that ``mx_lora_backward``'s one check found wrong."""
+    _need_cuda(where, dy, x8.codes, z, a, b, weight.codes if weight is not None else None)
+    m, n = dy.shape
+    r, k = a.shape
+    if dy.dtype not in _HALF:
+        raise TypeError(f"{where}: expected float16/bfloat16, got {dy.dtype}")
+    if x8.fmt != "mxfp8" or x8.shape != (m, k):
+        raise ValueError(f"{where}: x8 must be an mxfp8 tensor of shape {(m, k)}, got {x8.fmt} {x8.shape}")
+    if a.dtype != dy.dtype or b.dtype != dy.dtype or z.dtype != dy.dtype:
+        raise TypeError(f"{where}: dy, z, a and b must share one dtype")
+    if b.shape != (n, r) or not 1 <= r <= 256:
+        raise ValueError(f"{where}: b {tuple(b.shape)} does not match [{n}, {r}] (1 <= r <= 256)")
+    if z.shape != (m, 2 * ((r + 15) // 16 * 16)) or not z.is_contiguous():
+        raise ValueError(f"{where}: z must be the contiguous [M, 2 * round_up(r, 16)] pair, got {tuple(z.shape)}")
+    raise ValueError(f"{where}: the weight must be a 4-bit tensor of shape {(n, k)}, got {weight.fmt} {weight.shape}")
+
+
 def mx_lora_backward(dy: torch.Tensor, x8: MXTensor, z: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
                      scale: float = 1.0, weight: MXTensor | None = None, z_scale: float = 1.0):
     """Gradients ``(dx, da, db)`` of the LoRA linear from the 8-bit checkpoint of its input.
@@ -284,38 +302,38 @@ def mx_lora_backward(dy: torch.Tensor, x8: MXTensor, z: torch.Tensor, a: torch.T
     rank 64 its hi half alone is read), W an mxfp4 / nvfp4 tensor.  W is frozen; rounding to 4 or 8 bits counts
     as the identity.
     """
-    where = "mx_lora_backward"
+    shape, dtype = dy.shape, dy.dtype
     wc = weight.codes if weight is not None else None
-    _need_cuda(where, dy, x8.codes, z, a, b, wc)
-    shape = dy.shape
-    dy = _rows(dy, where)
+    if len(shape) != 2 or not dy.is_contiguous():
+        _need_cuda("mx_lora_backward", dy)
+        dy = _rows(dy, "mx_lora_backward")
     m, n = dy.shape
     r, k = a.shape
-    dtype = dy.dtype
-    if x8.fmt != "mxfp8" or x8.shape != (m, k):
-        raise ValueError(f"{where}: x8 must be an mxfp8 tensor of shape {(m, k)}, got {x8.fmt} {x8.shape}")
-    if a.dtype != dtype or b.dtype != dtype or z.dtype != dtype:
-        raise TypeError(f"{where}: dy, z, a and b must share one dtype")
-    if b.shape != (n, r) or not 1 <= r <= 256:
-        raise ValueError(f"{where}: b {tuple(b.shape)} does not match [{n}, {r}] (1 <= r <= 256)")
-    if z.shape != (m, 2 * ((r + 15) // 16 * 16)) or not z.is_contiguous():
-        raise ValueError(f"{where}: z must be the contiguous [M, 2 * round_up(r, 16)] pair, got {tuple(z.shape)}")
-    if weight is not None and (weight.fmt not in ("mxfp4", "nvfp4") or weight.shape != (n, k)):
-        raise ValueError(f"{where}: the weight must be a 4-bit tensor of shape {(n, k)}, got {weight.fmt} {weight.shape}")
-    a, b = _lib.row_major(a), _lib.row_major(b)
+    dt = _DTYPE.get(dtype)
+    if (dt is None or x8.fmt != "mxfp8" or x8.shape != (m, k) or a.dtype != dtype or b.dtype != dtype
+            or z.dtype != dtype or b.shape != (n, r) or not 1 <= r <= 256
+            or z.shape != (m, 2 * ((r + 15) // 16 * 16)) or not z.is_contiguous()
+            or not (dy.is_cuda and x8.codes.is_cuda and z.is_cuda and a.is_cuda and b.is_cuda)
+            or (weight is not None and (weight._code == _lib.LORA_MXFP8 or weight.shape != (n, k) or not wc.is_cuda))):
+        _refuse_backward(dy, x8, z, a, b, weight, "mx_lora_backward")
+    if not a.is_contiguous():
+        a = _lib.row_major(a)
+    if not b.is_contiguous():
+        b = _lib.row_major(b)
     device = dy.device
     da, db = dy.new_empty((r, k)), dy.new_empty((n, r))
-    dx = wp = sp = None
+    dx = wp = sp = dxp = None
     wg, wcode = 1.0, 0
     if weight is not None:
         dx = dy.new_empty((m, k))
+        dxp = dx.data_ptr()
         wp, sp, wg, wcode = wc.data_ptr(), weight.scales.data_ptr(), weight.global_scale, weight._code
     stream = _raw_stream(device.index)
     ws = _workspace("mx_backward", _backward_bytes(m, n, k, r, int(dx is not None)), device, stream)
     rc = _entry("lora_mx_backward")(dy.data_ptr(), _ld(dy), x8.codes.data_ptr(), x8.scales.data_ptr(), z.data_ptr(),
                                     float(z_scale), a.data_ptr(), _ld(a), b.data_ptr(), _ld(b), wp, sp, wg, wcode,
-                                    dx.data_ptr() if dx is not None else None, k, da.data_ptr(), k, db.data_ptr(), r, m,
-                                    n, k, r, float(scale), _DTYPE[dtype], ws.data_ptr(), ws.numel(), stream)
+                                    dxp, k, da.data_ptr(), k, db.data_ptr(), r, m, n, k, r, float(scale), dt,
+                                    ws.data_ptr(), ws.numel(), stream)
     if rc:
         _lib.check(rc, "lora_mx_backward")
     return (dx if dx is None or len(shape) == 2 else dx.view(*shape[:-1], k)), da, db
