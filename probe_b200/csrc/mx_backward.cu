@@ -7,7 +7,7 @@
 //
 // The base weight is frozen; rounding to 4 or 8 bits counts as the identity
 // (straight-through).  dx needs W with N as the contraction, against the direction
-// of its scale blocks.  Few rows (mx_few_tokens): W is decoded on its way into the MMAs
+// of its scale blocks.  Few rows (mx_dx_few): W is decoded on its way into the MMAs
 // (mx_dx.cu).  Many: W is decoded once, transposed, into the workspace and the 16-bit
 // CTA-pair GEMM takes [g_hi | g_lo] against [A^T | A^T] as its K tail.  Either way W's
 // values are exact in 16 bits: nvfp4's tensor scale m 2^p leaves the power of two in the
@@ -37,7 +37,7 @@ BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need
   BackwardPlan p = {};
   const int64_t np = up(N, 8), rp = up(R, 16);
   const int dev = current_device();
-  p.few = need_dx && mx_few_tokens(M, K, dev >= 0 ? device_info(dev).num_sms : 148);
+  p.few = need_dx && mx_dx_few(M, K, dev >= 0 ? device_info(dev).num_sms : 148);
   if (need_dx && !p.few) p.gemm_bytes = lora_gemm_workspace_size(M, K, np, 2 * rp);
   if (R > kWideRank && M >= kWideRows) p.gemm_bytes = std::max(p.gemm_bytes, lora_gemm_workspace_size(M, R, np, 0));
   size_t at = kCounterBytes;  // ticket counters, never scratch; the steps' partials follow them in turn

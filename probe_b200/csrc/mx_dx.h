@@ -14,6 +14,8 @@ struct MxDxOperands {
   float alpha, pow2;
 };
 
+// Few rows: one tile of 256, or as many 256 x 128 tiles as there are SMs.
+bool mx_dx_few(int64_t M, int64_t K, int num_sms);
 int mx_dx_launch(const MxDxOperands& o, int fmt, int dtype, cudaStream_t stream);
 
 }  // namespace lora

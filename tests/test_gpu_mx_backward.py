@@ -303,3 +303,55 @@ def test_from_a_fresh_host_thread():
     t.start()
     t.join()
     assert len(got) == 1 and all(torch.equal(p, q) for p, q in zip(got[0], want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("m,n,k,r", [(300, 72, 9608, 20), (4097, 136, 1288, 224), (260, 65, 9601, 5)])
+def test_many_output_tiles(m, n, k, r, fmt, dtype):
+    """dx of more tiles than the kernel that decodes W on the way takes."""
+    dy, x8, z, a, b, w = case(m, n, k, r, dtype, fmt, seed=3)
+    got = mx.mx_lora_backward(dy, x8, z, a, b, 0.7, weight=w, z_scale=1.25)
+    check(got, formulas(dy, x8, z, a, b, w, 0.7, 1.25, dtype))
+
+
+@pytest.mark.parametrize("m", [15, 16, 17, 32, 33, 64, 65, 128, 129, 256, 257, 600])
+@pytest.mark.parametrize("fmt,n,k,r", [("mxfp4", 63, 96, 16), ("nvfp4", 1090, 200, 72)])
+def test_row_tiles(m, fmt, n, k, r):
+    dy, x8, z, a, b, w = case(m, n, k, r, torch.bfloat16, fmt, seed=7)
+    got = mx.mx_lora_backward(dy, x8, z, a, b, 1.0, weight=w)
+    check(got, formulas(dy, x8, z, a, b, w, 1.0, 1.0, torch.bfloat16))
+
+
+@pytest.mark.parametrize("m", [20, 300])
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_weight_scales_far_from_one(m, fmt):
+    """Blocks of W whose scale is huge, tiny or zero, side by side; tensor scales likewise."""
+    n, k, r = 136, 256, 16
+    dy, x8, z, a, b, _ = case(m, n, k, r, torch.bfloat16, fmt, seed=11)
+    wf = randn((n, k), k ** -0.5, torch.bfloat16, 21)
+    if fmt == "mxfp4":
+        wf[:, :32] *= 2.0 ** 90
+        wf[:, 32:64] *= 2.0 ** -100
+        wf[:, 64:96] = 0
+        weights = [mx.mx_quantize(wf, fmt)]
+    else:
+        weights = [mx.mx_quantize(wf * 2.0 ** e, fmt, GW[fmt] * 2.0 ** e) for e in (50, -40)]
+    for w in weights:
+        got = mx.mx_lora_backward(dy, x8, z, a, b, 1.0, weight=w)
+        check(got, formulas(dy, x8, z, a, b, w, 1.0, 1.0, torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_a_nan_block_of_the_weight_reaches_its_columns_only(fmt, dtype):
+    m, n, k, r = 70, 200, 256, 8
+    dy, x8, z, a, b, w = case(m, n, k, r, dtype, fmt, seed=5)
+    wf = randn((n, k), k ** -0.5, dtype, 10)
+    wf[77, 101] = float("inf")
+    bad = mx.mx_quantize(wf, fmt, GW[fmt])
+    dx, _, _ = mx.mx_lora_backward(dy, x8, z, a, b, 1.0, weight=bad)
+    size = mo.BLOCK[fmt]
+    hit = torch.zeros(k, dtype=torch.bool, device=DEV)
+    hit[101 // size * size:101 // size * size + size] = True
+    assert torch.isnan(dx[:, hit]).all() and torch.isfinite(dx[:, ~hit]).all()
