@@ -11,10 +11,12 @@
 //
 // Bound: HBM (2 bytes read, 0.53 to 1.03 written an element).  A CTA takes 128
 // rows x 128 columns, the extent of whole scale chunks: 8 threads a row with 16
-// elements each, all four passes of 32 rows loaded before the first is used (128
-// bytes in flight a thread); the 512 scale bytes of a chunk go through shared
-// memory and leave as 16-byte stores.  A thread's 32 bytes are one access: as two
-// 16-byte stores, half a sector each, decoding 32760 x 5120 mxfp8 took 93 us, not 77.
+// elements each, in four passes of 32 rows, two of them loaded ahead: 48 registers, so
+// five CTAs an SM, whose 80 KB in flight cover the latency (all four ahead and four
+// CTAs: 13824 x 5120 nvfp4 39.1 us, not 37.2; one ahead and six 39.6); the 512 scale
+// bytes of a chunk go through shared memory and leave as 16-byte stores.  A thread's 32
+// bytes are one access: as two 16-byte stores, half a sector each, decoding
+// 32760 x 5120 mxfp8 took 93 us, not 77.
 #include "mx.cuh"
 
 namespace lora {
@@ -22,6 +24,7 @@ namespace {
 
 constexpr int kMxTile = 128;
 constexpr int kMxThreads = 256;
+constexpr int kMxAhead = 2;  // passes of 32 rows loaded ahead
 
 // Scale byte and codes of one thread's 16 elements.
 template <typename T, int FMT>
@@ -35,7 +38,7 @@ LORA_DEVINL uint32_t mx_encode16(const uint32_t* w, const MxGlobal& gl, uint32_t
 
 // ALIGN: of the rows, in bytes (32, 16, 2).
 template <typename T, int FMT, int ALIGN>
-__global__ void __launch_bounds__(kMxThreads)
+__global__ void __launch_bounds__(kMxThreads, 5)
     mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes,
                        uint8_t* __restrict__ scales, int64_t M, int64_t K, int64_t Kp, int chunks, MxGlobal gl) {
   constexpr int kChunks = kMxTile / MxFormat<FMT>::kBlock / 4;  // scale chunks of this tile
@@ -45,26 +48,28 @@ __global__ void __launch_bounds__(kMxThreads)
   const int64_t row0 = static_cast<int64_t>(blockIdx.y) * kMxTile;
   const int64_t col = static_cast<int64_t>(blockIdx.x) * kMxTile + seg * 16;
   __shared__ float recip[FMT == LORA_NVFP4 ? 128 : 1];
-  uint32_t w[4][8];
-#pragma unroll
-  for (int p = 0; p < 4; ++p) {
+  uint32_t w[kMxAhead][8];
+  auto load = [&](int p) {
+    uint32_t* v = w[p % kMxAhead];
     const int64_t row = row0 + 32 * p + sub;
     if (row < M) {
       const T* src = x + row * ldx + col;
       if (ALIGN == 32 && col + 16 <= K) {
-        ldg_stream_v8(src, w[p]);
+        ldg_stream_v8(src, v);
       } else if (ALIGN == 16 && col + 16 <= K) {
         const uint4 a = ldg_stream(src), b = ldg_stream(src + 8);
-        w[p][0] = a.x, w[p][1] = a.y, w[p][2] = a.z, w[p][3] = a.w;
-        w[p][4] = b.x, w[p][5] = b.y, w[p][6] = b.z, w[p][7] = b.w;
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
       } else {
-        ldg16_any(x + row * ldx, col, K, w[p]);
+        ldg16_any(x + row * ldx, col, K, v);
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[p][i] = 0u;
+      for (int i = 0; i < 8; ++i) v[i] = 0u;
     }
-  }
+  };
+#pragma unroll
+  for (int p = 0; p < kMxAhead; ++p) load(p);
   if constexpr (FMT == LORA_NVFP4) {
     if (threadIdx.x < 128) recip[threadIdx.x] = mx_recip_entry(static_cast<int>(threadIdx.x), gl.g);
     __syncthreads();
@@ -73,7 +78,8 @@ __global__ void __launch_bounds__(kMxThreads)
   for (int p = 0; p < 4; ++p) {
     const int64_t row = row0 + 32 * p + sub;
     uint32_t c[4];
-    uint32_t byte = mx_encode16<T, FMT>(w[p], gl, smem_u32(recip), c);
+    uint32_t byte = mx_encode16<T, FMT>(w[p % kMxAhead], gl, smem_u32(recip), c);
+    if (p + kMxAhead < 4) load(p + kMxAhead);
     if (col >= Kp || row >= M) byte = 0;
     if (row < M && col < Kp) {
       if constexpr (MxFormat<FMT>::kBits == 4)
