@@ -226,31 +226,31 @@ __global__ void __launch_bounds__(kShThreads, 1)
               break;
             }
             const uint32_t xs = smem_addr + stage * args.stage_bytes + r * 128;
-            uint32_t x[KB][16];
-#pragma unroll
-            for (int b = 0; b < KB; ++b)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint4 q = lds128(xs + b * kShBoxBytes + ((((lane & 1) * 4 + i) ^ (r & 7)) << 4));
-                x[b][4 * i] = q.x, x[b][4 * i + 1] = q.y, x[b][4 * i + 2] = q.z, x[b][4 * i + 3] = q.w;
-              }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&empty[stage]);
             uint32_t bytes = 0;  // scale bytes of this lane, in block order
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
+              uint32_t x[16];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint4 q = lds128(xs + b * kShBoxBytes + ((((lane & 1) * 4 + i) ^ (r & 7)) << 4));
+                x[4 * i] = q.x, x[4 * i + 1] = q.y, x[4 * i + 2] = q.z, x[4 * i + 3] = q.w;
+              }
+              if (b == KB - 1) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[stage]);
+              }
               const int64_t col = static_cast<int64_t>(kc * KB + b) * 64 + (lane & 1) * 32;
               uint32_t cd[8];
-              const uint32_t t0 = mx_amax16(x[b]), t1 = mx_amax16(x[b] + 8);
+              const uint32_t t0 = mx_amax16(x), t1 = mx_amax16(x + 8);
               if constexpr (FMT == LORA_NVFP4) {
                 const MxScale<T, FMT> s0(t0, args.gl, recip_addr), s1(t1, args.gl, recip_addr);
-                mx_codes16<T, FMT>(x[b], s0, cd);
-                mx_codes16<T, FMT>(x[b] + 8, s1, cd + 2);
+                mx_codes16<T, FMT>(x, s0, cd);
+                mx_codes16<T, FMT>(x + 8, s1, cd + 2);
                 bytes |= (s0.byte | (s1.byte << 8)) << (16 * b);
               } else {
                 const MxScale<T, FMT> s(max(t0, t1), args.gl, recip_addr);
-                mx_codes16<T, FMT>(x[b], s, cd);
-                mx_codes16<T, FMT>(x[b] + 8, s, cd + (MxFormat<FMT>::kBits == 4 ? 2 : 4));
+                mx_codes16<T, FMT>(x, s, cd);
+                mx_codes16<T, FMT>(x + 8, s, cd + (MxFormat<FMT>::kBits == 4 ? 2 : 4));
                 bytes |= s.byte << (16 * b);
               }
               if (row < args.M && col < args.Kp) {
