@@ -17,9 +17,16 @@
 // packed multiplication by the scale.  Codes have two significant bits and scales at
 // most four, so the product is exact wherever it is a normal number of the type.
 //
-// Bound: shared memory (a stage's codes decoded, written, read by the MMAs); for a
-// few rows HBM, 0.53 or 0.56 bytes a weight.  The contraction is cut over a cluster
-// as in the few-token linear, and W's first stages are loaded and decoded before
+// Bound: the chain load -> decode -> MMA of a stage over a ring of three to eight, then
+// the decode's ALU work.  64 rows of 13824 x 5120 (nvfp4, r = 16) take 44 us, of which
+// 11 are the decode's and 6 the MMAs' (each left out in turn); 256 rows of 4096 x 4096
+// 18.  HBM's share is small, 0.53 or 0.56 bytes a weight.  So a tile takes up to 256
+// tokens, whose decode is then paid once (256 rows, whole backward pass: two tiles of 128
+// 33.8 us, one of 256 28.3; 512 rows 52.8 and 39.5); from 128 tokens on, where one CTA
+// fills an SM, two groups of eight warps decode stages in turn (128 rows, 4096 x 11008:
+// 53.3 to 49.3), below, two CTAs of one group each share it (64 rows, 13824 x 5120: 55.8
+// against 58.5 for a CTA of two groups).  The contraction is cut over a cluster as in the
+// few-token linear, and W's first stages are loaded and decoded before
 // griddepcontrol.wait.
 #include <mutex>
 
@@ -29,11 +36,11 @@
 namespace lora {
 namespace {
 
-constexpr int kDxGroupWarps = 8;                 // decode a stage
-constexpr int kDxRows = 64;                      // of W (or A) a stage
-constexpr int kDxHalf = kDxRows * 128;           // 64 rows x 64 16-bit columns
-constexpr int kDxW = 2 * kDxHalf;                // the operand tile
-constexpr int kDxRaw = kDxRows * 64;             // codes of a stage
+constexpr int kDxGroupWarps = 8;       // decode a stage
+constexpr int kDxRows = 64;            // of W (or A) a stage
+constexpr int kDxHalf = kDxRows * 128;  // 64 rows x 64 16-bit columns
+constexpr int kDxW = 2 * kDxHalf;      // the operand tile
+constexpr int kDxRaw = kDxRows * 64;   // codes of a stage
 // Two CTAs an SM, or (128 tokens and more) one, with two groups of decoding warps that
 // take stages in turn.
 template <int NB> __host__ __device__ constexpr int dx_ctas() { return NB >= 128 ? 1 : 2; }

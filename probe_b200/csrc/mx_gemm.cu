@@ -18,13 +18,15 @@
 // tiles.  Layout: a cluster of two CTAs per 256 x 256 tile, persistent; warp 0
 // TMA (codes in 128-byte swizzled rows, scale chunks as they are stored), warp
 // 1 of the leader copies the stage's scales to TMEM (tcgen05.cp, each CTA from
-// its own shared memory) and issues the MMAs, warps 2..9 the epilogue, warp 10 the scales' loads.
+// its own shared memory) and issues the MMAs, warps 2..9 the epilogue, warp 10 the
+// scales' loads.
 // TMEM holds a buffer of scales per pipeline stage, so that a stage's full barrier
 // already says that its scale buffer is free: the MMA warp has 512 cycles a stage
 // and every further wait costs it 100 to 200.  Beside those 144 (mxfp4) or 240
 // (nvfp4) columns two 256-column accumulators do not fit: they overlap in as many,
 // the epilogue takes the shared columns to registers first and only that holds up
-// the next tile's MMAs.
+// the next tile's MMAs.  Measured: 4095 tokens, 5120 -> 13824, mxfp4, r = 16: 5.5 PFLOP/s;
+// 32760 tokens, 5120 -> 5120, nvfp4, r = 224: 417 us.
 #include <cudaTypedefs.h>
 
 #include <cmath>

