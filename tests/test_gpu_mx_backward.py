@@ -355,3 +355,18 @@ def test_a_nan_block_of_the_weight_reaches_its_columns_only(fmt, dtype):
     hit = torch.zeros(k, dtype=torch.bool, device=DEV)
     hit[101 // size * size:101 // size * size + size] = True
     assert torch.isnan(dx[:, hit]).all() and torch.isfinite(dx[:, ~hit]).all()
+
+
+@pytest.mark.parametrize("m", [20, 300])
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("e", [-12, 9])
+def test_weight_values_at_the_ends_of_fp16(m, fmt, e):
+    """Scales below fp16's normal numbers (values that it still holds exactly) and large ones."""
+    n, k, r = 136, 256, 16
+    dy, x8, z, a, b, _ = case(m, n, k, r, torch.float16, fmt, seed=13)
+    dy, a = dy * 2.0 ** -e, torch.zeros_like(a)
+    wf = randn((n, k), k ** -0.5, torch.float16, 23) * 2.0 ** e
+    w = mx.mx_quantize(wf, fmt, 1.0 if fmt == "mxfp4" else 2.0 ** (e - 11))
+    got = mx.mx_lora_backward(dy, x8, z, a, b, 2.0 ** -6, weight=w)
+    want = formulas(dy, x8, z, a, b, w, 2.0 ** -6, 1.0, torch.float16)
+    check((got[0],), {"dx": want["dx"]})
