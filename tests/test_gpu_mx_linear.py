@@ -178,3 +178,15 @@ def test_refusals():
         mx.mx_lora_linear(x, wq, None, big, torch.zeros(64, 300, dtype=x.dtype, device=DEV))
     with pytest.raises(_lib.LoraValueError):
         mx.mx_lora_linear(x, wq, bi, a, b, 1.0, x_global_scale=2.0)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("m", [1, 16, 17, 33, 64, 65, 300, 2100])
+def test_another_call_leaves_nothing_behind(m, fmt):
+    """Quantised rows beyond the tokens hold what an earlier call left there: here NaN."""
+    n, k, r = 2304, 320, 8
+    x, wq, bias, a, b, w = case(m, n, k, r, torch.bfloat16, fmt, seed=31)
+    spoilt = torch.full(((m + 127) // 128 * 128, k), float("inf"), dtype=torch.bfloat16, device=DEV)
+    assert torch.isnan(mx.mx_lora_linear(spoilt, wq, bias, a, b, 1.7, x_global_scale=G[fmt][0])).all()
+    y = mx.mx_lora_linear(x, wq, bias, a, b, 1.7, x_global_scale=G[fmt][0])
+    check(y, *want(x, w, bias, a, b, 1.7, fmt, torch.bfloat16))
