@@ -346,8 +346,10 @@ int launch_dx(const MxDxOperands& o, cudaStream_t stream) {
   a.last_k16 = static_cast<int>((o.R - (a.rank_kb - 1) * 64ll + 15) / 16);
   a.pow2 = o.pow2;
   constexpr int kFixed = 1024 + 512;
-  a.stages = std::min<int>(8, (dx_smem_max<NB>() - kFixed) / L::kStage);
-  static_assert((dx_smem_max<NB>() - kFixed) / L::kStage * L::kStage >= NB * 512, "the partial tile lies over the stages");
+  // a stage always goes to the same group: a warp that waits for a stage's next tile has
+  // seen its last one, and a barrier's parity says no more than that
+  a.stages = std::min<int>(8, (dx_smem_max<NB>() - kFixed) / L::kStage) / dx_groups<NB>() * dx_groups<NB>();
+  static_assert((dx_smem_max<NB>() - kFixed) / L::kStage / 2 * 2 * L::kStage >= NB * 512, "the partial tile lies over the stages");
   const int k_tiles = static_cast<int>((o.K + 127) / 128), t_tiles = static_cast<int>((o.M + NB - 1) / NB);
   // as many CTAs as are resident at once, each with eight or more stages
   const int resident = dx_ctas<NB>() * info.num_sms;

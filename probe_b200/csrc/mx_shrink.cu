@@ -9,9 +9,9 @@
 // a 128 x 128 tile of v run (x 64 for ranks above 64, whose adapter tile is larger),
 // eight warps quantise the same tile from shared memory (two lanes a row: conflict-free
 // with the 128-byte swizzle, whole 32-byte sectors of codes out).  A second group of
-// eight takes every other tile (a block of 64, 32, 16 rows has 4, 8, 16 smaller groups); a
-// third made it slower (4095 x 5120 mxfp4, r = 16: 26.7
-// against 25.9 us; r = 224 of 32760 tokens, nvfp4: 219 against 176).
+// eight takes every other tile; a third made it slower (4095 x 5120 mxfp4, r = 16: 26.7
+// against 25.9 us; r = 224 of 32760 tokens, nvfp4: 219 against 176).  Up to 64 tokens
+// there are four groups of four (a call of 64 tokens 17.6 to 16.4 us).
 //
 // Bound: the floor is HBM (v once, codes out); what is measured is the ALU pipe of the
 // quantisation -- 4095 x 5120 mxfp4 with r = 16, 53 MB, takes 18 to 25 us, issue slots
@@ -31,7 +31,7 @@
 namespace lora {
 namespace {
 
-constexpr int kShWorkers = 16;  // groups of eight and fewer, taking stages in turn
+constexpr int kShWorkers = 16;  // two groups of eight (or four of four), taking stages in turn
 constexpr int kShThreads = 64 + 32 * kShWorkers;
 constexpr int kShBoxBytes = 128 * 128;  // 128 tokens x 64 columns
 constexpr int kShSmemMax = 224 * 1024;
@@ -51,6 +51,7 @@ struct ShArgs {
   int chunks_total;
   int kc, r16, a_boxes, a_box_bytes, stages, stage_bytes, gb;
   int cluster;  // CTAs of a token block's cluster; 0: runs
+  int group_shift;  // log2 of the warps of a group, which takes 16 rows a warp
   float scale;
   MxGlobal gl;
 };
@@ -105,20 +106,16 @@ __global__ void __launch_bounds__(kShThreads, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int crank = args.cluster ? static_cast<int>(cluster_ctarank()) : 0;
-  const int block = args.cluster ? static_cast<int>(blockIdx.x) / args.cluster : 0;
-  const int cblock = block * args.kc;  // its first chunk
+  const int cblock = args.cluster ? static_cast<int>(blockIdx.x) / args.cluster * args.kc : 0;  // its first chunk
   const int c_begin = args.cluster ? cblock + args.kc * crank / args.cluster : sh_start(args, blockIdx.x);
   const int c_end = args.cluster ? cblock + args.kc * (crank + 1) / args.cluster : sh_start(args, blockIdx.x + 1);
-  // a group's warps take 16 rows each; a cluster's block of few rows has smaller groups, more of them
-  const int rows = args.cluster ? static_cast<int>(args.M) - block * 128 : 128;
-  const int group_shift = (rows > 16) + (rows > 32) + (rows > 64);
   const uint32_t need = 2 * args.r16;
   const uint32_t tmem_cols = need <= 32 ? 32u : need <= 64 ? 64u : need <= 128 ? 128u : need <= 256 ? 256u : 512u;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < args.stages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], FMT == kNoFormat ? 1 : 1 + (1 << group_shift));  // the MMAs, a group of workers
+      mbar_init(&empty[s], FMT == kNoFormat ? 1 : 1 + (1 << args.group_shift));  // the MMAs, a group of workers
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&acc_full[s], 1);
@@ -217,7 +214,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
   } else {
     const int w = warp - 2, quad = warp & 3, part = w >> 2;
     const uint32_t recip_addr = smem_u32(recip), smem_addr = smem_u32(smem);
-    int stage = 0, seg = 0, turn = w >> group_shift;
+    int stage = 0, seg = 0, turn = w >> args.group_shift;
     uint32_t phase = 0;
     bool ok = true;
     for (int c = c_begin; ok && c < c_end; ++seg) {
@@ -226,13 +223,13 @@ __global__ void __launch_bounds__(kShThreads, 1)
       if constexpr (FMT != kNoFormat) {
         // rows 16 (w % group) .. + 15 of the block, 32 columns a lane; rows that no warp takes
         // are beyond M, where codes read as zeros and no result is stored
-        const int r = 16 * (w & ((1 << group_shift) - 1)) + (lane >> 1);
+        const int r = 16 * (w & ((1 << args.group_shift) - 1)) + (lane >> 1);
         const int64_t row = static_cast<int64_t>(tb) * 128 + r;
         uint8_t* sc = args.scales + static_cast<int64_t>(tb) * args.gb * 512 + (r & 31) * 16 + (r >> 5) * 4;
         for (; c < seg_end; ++c) {
           const int kc = c - tb * args.kc;
           if (turn-- == 0) {
-            turn = (kShWorkers >> group_shift) - 1;
+            turn = (kShWorkers >> args.group_shift) - 1;
             if (!warp_wait(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
               ok = false;
               break;
@@ -493,6 +490,17 @@ int launch_shrink(const MxShrinkOperands& o, cudaStream_t stream) {
   constexpr int kFixed = 1024 + 1024;  // alignment, barriers and reciprocals
   a.cluster = shrink_cluster(o.M, o.K, o.R);
   a.stages = std::min(8, (kShSmemMax - kFixed) / a.stage_bytes);
+  a.group_shift = 3;
+  if (FMT != kNoFormat) {
+    // A stage always goes to the same group -- the groups divide the ring -- so that a
+    // warp which waits for a stage's next tile has seen its last one: a barrier's parity
+    // says no more than that.
+    a.stages &= ~1;
+    if (o.M <= 64) {
+      a.group_shift = 2;
+      a.stages &= ~3;
+    }
+  }
   auto kernel = mx_shrink_kernel<T, FMT, AMN, KB>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];

@@ -190,3 +190,14 @@ def test_another_call_leaves_nothing_behind(m, fmt):
     assert torch.isnan(mx.mx_lora_linear(spoilt, wq, bias, a, b, 1.7, x_global_scale=G[fmt][0])).all()
     y = mx.mx_lora_linear(x, wq, bias, a, b, 1.7, x_global_scale=G[fmt][0])
     check(y, *want(x, w, bias, a, b, 1.7, fmt, torch.bfloat16))
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("m,k,r", [(1, 13824, 64), (23, 13824, 16), (60, 6912, 200), (8343, 1184, 64), (4119, 2048, 40)])
+def test_long_rows_of_few_tokens(m, k, r, fmt):
+    """Many more tiles along K than stages, in blocks of few rows among others."""
+    n = 136
+    x, wq, bias, a, b, w = case(m, n, k, r, torch.bfloat16, fmt, seed=41)
+    for _ in range(3):
+        y = mx.mx_lora_linear(x, wq, bias, a, b, 0.8, x_global_scale=G[fmt][0])
+    check(y, *want(x, w, bias, a, b, 0.8, fmt, torch.bfloat16))
