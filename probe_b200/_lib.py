@@ -222,15 +222,20 @@ class _Workspace:
     so a buffer stays valid for every later call on the same stream.  Calls on
     one stream are ordered, so they never share a buffer concurrently.  A
     buffer only grows (by allocating a new zeroed one); warm the shapes you
-    will capture before capturing a CUDA graph.
+    will capture before capturing a CUDA graph.  A graph keeps the addresses it
+    was captured with: a buffer that a capture has taken stays allocated when a
+    larger one replaces it.
     """
 
     def __init__(self):
         self._bufs: dict[tuple, torch.Tensor] = {}
+        self._captured: set[tuple] = set()  # keys whose present buffer some graph may hold
+        self._retained: list[torch.Tensor] = []  # replaced buffers that some graph may hold
         self._lock = threading.Lock()
 
-    def get(self, nbytes: int, device: torch.device, slot: str) -> torch.Tensor:
-        stream = torch.cuda.current_stream(device).cuda_stream
+    def get(self, nbytes: int, device: torch.device, slot: str, stream: int | None = None) -> torch.Tensor:
+        if stream is None:
+            stream = torch.cuda.current_stream(device).cuda_stream
         key = (device.index, stream, slot)
         with self._lock:
             buf = self._bufs.get(key)
@@ -238,8 +243,13 @@ class _Workspace:
                 size = max(int(nbytes), 1 << 12)
                 if buf is not None:
                     size = max(size, buf.numel() * 2)
+                    if key in self._captured:
+                        self._captured.discard(key)
+                        self._retained.append(buf)
                 buf = torch.zeros(size, dtype=torch.uint8, device=device)
                 self._bufs[key] = buf
+            if torch.cuda.is_current_stream_capturing():
+                self._captured.add(key)
             return buf
 
 

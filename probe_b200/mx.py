@@ -35,21 +35,11 @@ _DTYPE = {torch.float16: _lib.LORA_F16, torch.bfloat16: _lib.LORA_BF16}
 # A call of a few tokens takes the GPU a few microseconds: the wrappers below pass
 # plain integers to the C ABI, look the raw stream up directly and keep sizes by shape.
 _raw_stream = torch._C._cuda_getCurrentRawStream
-_buffers: dict[tuple, torch.Tensor] = {}
 
 
 @functools.cache
 def _entry(name: str):
     return getattr(_lib.load(), name)
-
-
-def _workspace(slot: str, nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
-    """The zero-initialised per-stream workspace of the slot (grown by ``_lib.WORKSPACE``)."""
-    buf = _buffers.get((slot, device.index, stream))
-    if buf is None or buf.numel() < nbytes:
-        buf = _lib.WORKSPACE.get(nbytes, device, slot)
-        _buffers[(slot, device.index, stream)] = buf
-    return buf
 
 
 @functools.lru_cache(maxsize=4096)
@@ -252,7 +242,7 @@ def _linear(x, weight, bias, a, b, scale, x_global_scale, keep_z, where):
     if m and n:
         device = x.device
         stream = _raw_stream(device.index)
-        ws = _workspace("mx_linear", _linear_bytes(m, n, k, r, code), device, stream)
+        ws = _lib.WORKSPACE.get(_linear_bytes(m, n, k, r, code), device, "mx_linear", stream)
         rc = _entry("lora_mx_linear")(xp, ldx, codes.data_ptr(), weight.scales.data_ptr(), weight.global_scale,
                                       None if bias is None else bias.data_ptr(), ap, lda, bp, ldb, out.data_ptr(), n,
                                       None if z is None else z.data_ptr(), m, n, k, r, float(scale), float(x_global_scale),
@@ -329,7 +319,7 @@ def mx_lora_backward(dy: torch.Tensor, x8: MXTensor, z: torch.Tensor, a: torch.T
         dxp = dx.data_ptr()
         wp, sp, wg, wcode = wc.data_ptr(), weight.scales.data_ptr(), weight.global_scale, weight._code
     stream = _raw_stream(device.index)
-    ws = _workspace("mx_backward", _backward_bytes(m, n, k, r, int(dx is not None)), device, stream)
+    ws = _lib.WORKSPACE.get(_backward_bytes(m, n, k, r, int(dx is not None)), device, "mx_backward", stream)
     rc = _entry("lora_mx_backward")(dy.data_ptr(), _ld(dy), x8.codes.data_ptr(), x8.scales.data_ptr(), z.data_ptr(),
                                     float(z_scale), a.data_ptr(), _ld(a), b.data_ptr(), _ld(b), wp, sp, wg, wcode,
                                     dxp, k, da.data_ptr(), k, db.data_ptr(), r, m, n, k, r, float(scale), dt,

@@ -1,0 +1,52 @@
+"""Who holds a workspace, and for how long (CPU only: the stream and its capture are stand-ins)."""
+
+import gc
+import types
+import weakref
+
+import pytest
+import torch
+
+from probe_b200 import _lib
+
+CPU = torch.device("cpu")
+
+
+@pytest.fixture
+def gpu(monkeypatch):
+    """One stream, capturing when told to."""
+    state = types.SimpleNamespace(capturing=False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: types.SimpleNamespace(cuda_stream=7))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state.capturing)
+    return state
+
+
+def test_a_captured_buffer_outlives_its_replacement(gpu):
+    """A graph replays with the address it was captured with."""
+    ws = _lib._Workspace()
+    ws.get(5000, CPU, "linear")
+    gpu.capturing = True
+    taken = weakref.ref(ws.get(5000, CPU, "linear"))
+    gpu.capturing = False
+    assert ws.get(4_000_000, CPU, "linear").numel() >= 4_000_000
+    gc.collect()
+    assert taken() is not None
+
+
+def test_what_no_capture_took_is_given_back(gpu):
+    ws = _lib._Workspace()
+    first = weakref.ref(ws.get(5000, CPU, "linear"))
+    gpu.capturing = True
+    ws.get(100, CPU, "backward")
+    gpu.capturing = False
+    ws.get(4_000_000, CPU, "linear")
+    gc.collect()
+    assert first() is None
+
+
+def test_a_buffer_serves_every_smaller_call(gpu):
+    ws = _lib._Workspace()
+    buf = ws.get(9000, CPU, "linear")
+    assert ws.get(9000, CPU, "linear") is buf and ws.get(1, CPU, "linear") is buf
+    assert ws.get(1, CPU, "linear", stream=7) is buf and ws.get(1, CPU, "linear", stream=8) is not buf
+    assert ws.get(1, CPU, "backward") is not buf and not buf.any()
