@@ -372,7 +372,8 @@ class MXLoRALinear(torch.nn.Module):
     are parameters.  While gradients are recorded the input is kept for the backward
     pass in 8 bits (mxfp8) with the [M, r] product, and nothing else of its size;
     without them the call is ``mx_lora_linear``.  ``x_amax``, for nvfp4: the largest
-    magnitude expected of the input (its calibration).
+    magnitude expected of the input (its calibration).  ``state_dict`` holds codes, scales,
+    both tensor-wide scales and the format; a state of the other format is refused.
     """
 
     def __init__(self, base: torch.nn.Linear, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0,
@@ -397,6 +398,25 @@ class MXLoRALinear(torch.nn.Module):
         self.register_buffer("bias", None if base.bias is None else base.bias.detach())
         self.lora_a = torch.nn.Parameter(a.detach().to(weight).contiguous().clone())
         self.lora_b = torch.nn.Parameter(b.detach().to(weight).contiguous().clone())
+
+    # The codes mean nothing without the tensor-wide scales, which stay on the host (a call
+    # passes them by value): they travel in the state as one small CPU tensor.
+    def get_extra_state(self) -> torch.Tensor:
+        return torch.tensor([_FORMATS[self.fmt], self.w_global_scale, self.x_global_scale], dtype=torch.float64)
+
+    def set_extra_state(self, state: torch.Tensor) -> None:
+        code, w_global_scale, x_global_scale = state.tolist()
+        if code != _FORMATS[self.fmt]:
+            names = {v: k for k, v in _FORMATS.items()}
+            raise RuntimeError(f"MXLoRALinear: the state is of a {names.get(int(code), code)} layer, this one is {self.fmt}")
+        self.w_global_scale, self.x_global_scale = w_global_scale, x_global_scale
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        key = prefix + "_extra_state"
+        if self.fmt == "mxfp4" and key not in state_dict:  # nothing to restore: both scales are 1
+            state_dict = {**state_dict, key: self.get_extra_state()}
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
+                                      error_msgs)
 
     @property
     def rank(self) -> int:
