@@ -221,10 +221,11 @@ class _Workspace:
     The split-K kernels leave their ticket counters at zero when they finish,
     so a buffer stays valid for every later call on the same stream.  Calls on
     one stream are ordered, so they never share a buffer concurrently.  A
-    buffer only grows (by allocating a new zeroed one); warm the shapes you
-    will capture before capturing a CUDA graph.  A graph keeps the addresses it
-    was captured with: a buffer that a capture has taken stays allocated when a
-    larger one replaces it.
+    buffer only grows (by allocating a new zeroed one).  A CUDA graph keeps the
+    addresses it was captured with: a buffer that a capture has taken stays
+    allocated when a larger one replaces it.  Warm the shapes you will capture on
+    the stream that captures them: a buffer allocated during a capture is zeroed
+    by the graph's replays alone, so it serves that one call of that graph.
     """
 
     def __init__(self):
@@ -237,19 +238,22 @@ class _Workspace:
         if stream is None:
             stream = torch.cuda.current_stream(device).cuda_stream
         key = (device.index, stream, slot)
+        capturing = torch.cuda.is_current_stream_capturing()
         with self._lock:
             buf = self._bufs.get(key)
-            if buf is None or buf.numel() < nbytes:
-                size = max(int(nbytes), 1 << 12)
-                if buf is not None:
-                    size = max(size, buf.numel() * 2)
-                    if key in self._captured:
-                        self._captured.discard(key)
-                        self._retained.append(buf)
-                buf = torch.zeros(size, dtype=torch.uint8, device=device)
-                self._bufs[key] = buf
-            if torch.cuda.is_current_stream_capturing():
-                self._captured.add(key)
+            if buf is not None and buf.numel() >= nbytes:
+                if capturing:
+                    self._captured.add(key)
+                return buf
+            size = max(int(nbytes), 1 << 12)
+            if capturing:  # of the graph's own pool, which holds it
+                return torch.zeros(size, dtype=torch.uint8, device=device)
+            if buf is not None:
+                size = max(size, buf.numel() * 2)
+                if key in self._captured:
+                    self._captured.discard(key)
+                    self._retained.append(buf)
+            buf = self._bufs[key] = torch.zeros(size, dtype=torch.uint8, device=device)
             return buf
 
 

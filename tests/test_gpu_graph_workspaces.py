@@ -57,3 +57,28 @@ def test_a_larger_call_after_the_capture(make, small, large):
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(got, want))
         assert all(bool((t == 0xA5).all()) for t in others)
+
+
+@pytest.mark.parametrize("make,few", [(linear, 16), (linear, 700), (backward, 40), (shrink, 64)])
+def test_captures_without_a_warm_call(make, few):
+    """Two graphs captured on one stream that had no workspace yet, replayed in the other order, then eagerly."""
+    first, second = make(few), make(few + 8)
+    want = [[t.clone() for t in f()] for f in (first, second)]  # on another stream: the kernels are loaded
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    graphs, outs = [], []
+    for f in (first, second):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(f())
+        graphs.append(g)
+    for i in (1, 0, 1, 1, 0):
+        for t in outs[i]:
+            t.zero_()
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(outs[i], want[i]))
+    with torch.cuda.stream(s):
+        again = first()
+    s.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(again, want[0]))

@@ -50,3 +50,18 @@ def test_a_buffer_serves_every_smaller_call(gpu):
     assert ws.get(9000, CPU, "linear") is buf and ws.get(1, CPU, "linear") is buf
     assert ws.get(1, CPU, "linear", stream=7) is buf and ws.get(1, CPU, "linear", stream=8) is not buf
     assert ws.get(1, CPU, "backward") is not buf and not buf.any()
+
+
+def test_a_buffer_of_a_capture_serves_that_call_alone(gpu):
+    """Its zeros are written when the graph is replayed: not before another call, and not for another graph."""
+    ws = _lib._Workspace()
+    gpu.capturing = True
+    first, second = ws.get(5000, CPU, "linear"), ws.get(5000, CPU, "linear")
+    gpu.capturing = False
+    eager = ws.get(5000, CPU, "linear")
+    assert len({t.data_ptr() for t in (first, second, eager)}) == 3
+    gpu.capturing = True
+    assert ws.get(5000, CPU, "linear") is eager  # warmed now
+    assert ws.get(9000, CPU, "linear") is not eager
+    gpu.capturing = False
+    assert ws.get(5000, CPU, "linear") is eager
