@@ -149,19 +149,23 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   if (M < 0 || N < 0 || K < 0 || R <= 0 || R > 256 || M > 4194240 || N > 4194240 || K > 4194240) return LORA_ERR_SHAPE;
   if (lddy < N || lda < K || ldb < R || ldda < K || lddb < R || (dx != nullptr && lddx < K)) return LORA_ERR_SHAPE;
   if (dx != nullptr && !mx_global_ok(w_global, w_fmt)) return LORA_ERR_ARG;
-  if (N == 0 || K == 0) return LORA_OK;
-  if (a == nullptr || b == nullptr || da == nullptr || db == nullptr) return LORA_ERR_ARG;
-  if (M > 0 && (dy == nullptr || x_codes == nullptr || x_scales == nullptr || z == nullptr)) return LORA_ERR_ARG;
-  if (dx != nullptr && (w_codes == nullptr || w_scales == nullptr)) return LORA_ERR_ARG;
+  if (K == 0) return LORA_ERR_UNSUPPORTED;
+  // an empty sum leaves zeros: no operand is read
+  const bool empty = M == 0 || N == 0;
+  if (da == nullptr || (N > 0 && db == nullptr)) return LORA_ERR_ARG;
+  if (!empty && (a == nullptr || b == nullptr || dy == nullptr || x_codes == nullptr || x_scales == nullptr ||
+                 z == nullptr || (dx != nullptr && (w_codes == nullptr || w_scales == nullptr))))
+    return LORA_ERR_ARG;
   if (!mx_aligned(x_codes, 16) || !mx_aligned(x_scales, 16) || !mx_aligned(z, 16) || !mx_aligned(workspace, 256) ||
       (dx != nullptr && (!mx_aligned(w_codes, 16) || !mx_aligned(w_scales, 16))))
     return LORA_ERR_ALIGN;
   const int dev = current_device();
   if (dev < 0 || !device_info(dev).is_sm100) return LORA_ERR_DEVICE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (M == 0) {
+  if (empty) {
     if (cudaMemset2DAsync(da, ldda * 2, 0, K * 2, R, s) != cudaSuccess ||
-        cudaMemset2DAsync(db, lddb * 2, 0, R * 2, N, s) != cudaSuccess)
+        (N > 0 && cudaMemset2DAsync(db, lddb * 2, 0, R * 2, N, s) != cudaSuccess) ||
+        (M > 0 && dx != nullptr && cudaMemset2DAsync(dx, lddx * 2, 0, K * 2, M, s) != cudaSuccess))
       return LORA_ERR_CUDA;
     return LORA_OK;
   }
