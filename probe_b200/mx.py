@@ -23,6 +23,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -354,6 +355,7 @@ class _MXLoRAFunction(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         if dy is None:
             return (None,) * 7
