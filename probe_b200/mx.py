@@ -212,7 +212,7 @@ def _refuse_linear(x, weight, bias, a, b, where):
 def _linear(x, weight, bias, a, b, scale, x_global_scale, keep_z, where):
     shape, dtype, codes, code = x.shape, x.dtype, weight.codes, weight._code
     n, k = weight.shape
-    r = 0 if a is None or b is None or scale == 0 else a.shape[0]
+    r = 0 if a is None or b is None or (scale == 0 and not keep_z) else a.shape[0]
     dt = _DTYPE.get(dtype)
     if (dt is None or code == _lib.LORA_MXFP8 or not x.is_cuda or not codes.is_cuda or shape[-1] != k
             or (bias is not None and (not bias.is_cuda or bias.dtype != dtype or bias.shape != (n,)))
@@ -337,8 +337,8 @@ def mx_lora_forward(x: torch.Tensor, weight: MXTensor, bias: torch.Tensor | None
     ``y`` as ``mx_lora_linear``; ``x8`` the mxfp8 checkpoint of x (half its bytes),
     ``z`` the [M, 2 r16] pair with ``z_scale * (hi + lo) = scale * x @ a.T``.
     """
-    if a is None or b is None or a.shape[0] == 0 or scale == 0:
-        raise ValueError("mx_lora_forward: an adapter (rank >= 1, scale != 0) is required")
+    if a is None or b is None or a.shape[0] == 0:
+        raise ValueError("mx_lora_forward: an adapter (rank >= 1) is required")
     y, z = _linear(x, weight, bias, a, b, scale, x_global_scale, True, "mx_lora_forward")
     z_scale = _entry("lora_mx_linear_z_scale")(float(x_global_scale), weight.global_scale, weight._code)
     return y, mx_quantize(x, "mxfp8"), z, z_scale

@@ -1,4 +1,4 @@
-"""MXLoRALinear under autograd: second derivatives."""
+"""MXLoRALinear under autograd: second derivatives, scale 0."""
 
 import pytest
 import torch
@@ -26,3 +26,23 @@ def test_second_derivatives_raise():
     (dx,) = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         (y.float().sum() + dx.float().square().sum()).backward()
+
+
+@pytest.mark.parametrize("m", [3, 300])
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_scale_zero_trains_as_it_serves(fmt, m):
+    """The adapter is off: its gradients are zeros, y and dx are the base's."""
+    mod = module(0.0, fmt)
+    x = randn((m, 96), 1.0, torch.bfloat16, 4).requires_grad_()
+    dy = randn((m, 64), 1.0, torch.bfloat16, 5)
+    with torch.no_grad():
+        served = mod(x)
+    y = mod(x)
+    assert torch.equal(y, served)
+    y.backward(dy)
+    assert not mod.lora_a.grad.any() and not mod.lora_b.grad.any()
+    x8 = mx.mx_quantize(x.detach(), "mxfp8")
+    off = torch.zeros_like(mod.lora_b)
+    want, _, _ = mx.mx_lora_backward(dy, x8, torch.zeros(m, 32, dtype=dy.dtype, device=DEV), mod.lora_a.detach(), off,
+                                     1.0, weight=mod.weight)
+    assert torch.equal(x.grad, want)
