@@ -389,8 +389,9 @@ LORA_API int lora_mx_dequantize(const void* codes, const void* scales, void* out
  * Workspace: lora_mx_linear_workspace_size bytes, 256-byte aligned, with a
  * zeroed ticket region first as lora_shrink's; calls that share one must not
  * overlap on the GPU.  Rows of b: 16-byte aligned (any layout when R is not a
- * multiple of 8: it is copied); R > 128 also needs K, ldx, lda multiples of 8
- * and x, a 16-byte aligned.  No counterpart in the reference. */
+ * multiple of 8: it is copied).  x and a: any layout, except that R > 128 with K a
+ * multiple of 8 needs ldx, lda multiples of 8 and x, a 16-byte aligned (with K no
+ * multiple of 8 they are copied where need be).  No counterpart in the reference. */
 LORA_API size_t lora_mx_linear_workspace_size(int64_t M, int64_t N, int64_t K, int64_t R, int fmt);
 LORA_API float lora_mx_linear_z_scale(float x_global, float w_global, int fmt);
 LORA_API int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, const void* w_scales, float w_global,

@@ -109,25 +109,6 @@ int transpose(const TransposeJobs& jobs, cudaStream_t s) {
   return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
 }
 
-// Rows of `cols` elements copied to 16-byte aligned rows of `width` (a multiple of 8;
-// zeros beyond cols), 16 elements a thread.
-__global__ void __launch_bounds__(256) mx_widen_kernel(const uint16_t* __restrict__ in, int64_t ldi,
-                                                       uint16_t* __restrict__ out, int64_t cols, int64_t width) {
-  const int64_t row = blockIdx.x, c = (static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x) * 16;
-  if (c >= width) return;
-  uint32_t w[8];
-  ldg16_any(in + row * ldi, c, cols, w);
-  uint4* dst = reinterpret_cast<uint4*>(out + row * width + c);
-  dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  if (c + 8 < width) dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
-}
-
-int widen(const void* in, int64_t ldi, void* out, int64_t rows, int64_t cols, int64_t width, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>((width + 4095) / 4096));
-  mx_widen_kernel<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(in), ldi, static_cast<uint16_t*>(out), cols, width);
-  return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
-}
-
 }  // namespace
 }  // namespace lora
 
@@ -195,7 +176,7 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   if (p.few && (lda % 8 != 0 || !mx_aligned(a, 16))) {
     lda_p = up(K, 8);
     ap = ws + p.at;
-    rc = widen(a, lda, ws + p.at, R, K, lda_p, s);
+    rc = mx_widen_launch(a, lda, ws + p.at, R, K, lda_p, s);
     if (rc != LORA_OK) return rc;
   }
   if (dx != nullptr && !p.few) {
@@ -205,7 +186,7 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   const void* dyp = dy;
   int64_t ldp = lddy;
   if (N % 8 != 0 || lddy % 8 != 0 || !mx_aligned(dy, 16)) {  // TMA needs 16-byte rows
-    rc = widen(dy, lddy, ws + p.dy, M, N, np, s);
+    rc = mx_widen_launch(dy, lddy, ws + p.dy, M, N, np, s);
     if (rc != LORA_OK) return rc;
     dyp = ws + p.dy;
     ldp = np;

@@ -6,7 +6,8 @@
 // the same pass over x, the rank shrink z = (s / alpha) x A^T as a hi/lo pair
 // (alpha: the fp32 factor that the product's epilogue applies); the block-scaled
 // GEMM with z B^T as its tail.  Operands that TMA cannot read (rows not 16-byte
-// aligned) take the quantisation and the split-K shrink as kernels of their own.
+// aligned) take the quantisation and the split-K shrink as kernels of their own or,
+// at ranks beyond that shrink's, are copied to aligned rows first.
 #include <cmath>
 
 #include "mx_shrink.h"
@@ -14,13 +15,13 @@
 namespace lora {
 namespace {
 
-// Shrinks of more ranks than this run on the 16-bit tensor-core GEMM.
+// The most ranks that lora_shrink takes.
 constexpr int64_t kShrinkMaxRank = 128;
 
 int64_t r16(int64_t r) { return (r + 15) / 16 * 16; }
 
 struct LinearPlan {
-  size_t shrink_bytes, x_codes, x_scales, z, b, total;
+  size_t shrink_bytes, x_codes, x_scales, z, b, x, a, total;
   int split_k;
 };
 
@@ -34,8 +35,6 @@ LinearPlan linear_plan(int64_t M, int64_t N, int64_t K, int64_t R, int fmt) {
     if (R <= kShrinkMaxRank) {
       p.split_k = lora_shrink_pick_split_k(M, K, R);
       p.shrink_bytes = lora_shrink_workspace_size(M, R, p.split_k);
-    } else {
-      p.shrink_bytes = lora_gemm_workspace_size(M, R, K, 0);
     }
     if (p.shrink_bytes > at) at = mx_align(p.shrink_bytes);
   }
@@ -47,8 +46,27 @@ LinearPlan linear_plan(int64_t M, int64_t N, int64_t K, int64_t R, int fmt) {
   if (R > 0) at += mx_align(static_cast<size_t>(M) * 2 * r16(R) * 2);
   p.b = at;
   if (R % 8 != 0) at += mx_align(static_cast<size_t>(N) * ((R + 7) / 8 * 8) * 2);
+  // x and A, where rows of a wide adapter's operands may need a copy
+  const int64_t k8 = (K + 7) / 8 * 8;
+  const bool copies = R > kShrinkMaxRank && K % 8 != 0;
+  p.x = at;
+  if (copies) at += mx_align(static_cast<size_t>(M) * k8 * 2);
+  p.a = at;
+  if (copies) at += mx_align(static_cast<size_t>(R) * k8 * 2);
   p.total = at;
   return p;
+}
+
+// Rows of `cols` elements to 16-byte aligned rows of `width`, 16 elements a thread.
+__global__ void __launch_bounds__(256) mx_widen_kernel(const uint16_t* __restrict__ in, int64_t ldi,
+                                                       uint16_t* __restrict__ out, int64_t cols, int64_t width) {
+  const int64_t row = blockIdx.x, c = (static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x) * 16;
+  if (c >= width) return;
+  uint32_t w[8];
+  ldg16_any(in + row * ldi, c, cols, w);
+  uint4* dst = reinterpret_cast<uint4*>(out + row * width + c);
+  dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  if (c + 8 < width) dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
 // B [N, R] with rows padded to a multiple of 8 elements (TMA needs 16-byte rows).
@@ -68,6 +86,12 @@ __global__ void mx_pad_rows_kernel(const uint16_t* __restrict__ b, int64_t ldb, 
 // N = 11008, 256 (172 tiles) 26.9 against 23.5.
 bool mx_few_tokens(int64_t M, int64_t N, int num_sms) {
   return M <= 128 || (M + 127) / 128 * ((N + 127) / 128) <= num_sms;
+}
+
+int mx_widen_launch(const void* in, int64_t ldi, void* out, int64_t rows, int64_t cols, int64_t width, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>((width + 4095) / 4096));
+  mx_widen_kernel<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(in), ldi, static_cast<uint16_t*>(out), cols, width);
+  return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
 }
 
 }  // namespace lora
@@ -103,9 +127,9 @@ extern "C" int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, c
   if (!mx_aligned(w_codes, 16) || !mx_aligned(w_scales, 16) || !mx_aligned(workspace, 256) ||
       (z_out != nullptr && !mx_aligned(z_out, 16)))
     return LORA_ERR_ALIGN;
-  // the wide shrink's operands are read by TMA
-  if (R > kShrinkMaxRank && (K % 8 != 0 || ldx % 8 != 0 || lda % 8 != 0 || !mx_aligned(x, 16) || !mx_aligned(a, 16)))
-    return LORA_ERR_ALIGN;
+  const bool served = R > 0 && mx_shrink_serves(x, ldx, a, lda);
+  const bool copies = R > kShrinkMaxRank && !served;
+  if (copies && K % 8 == 0) return LORA_ERR_ALIGN;  // the workspace has no room for copies
   const int dev = current_device();
   if (dev < 0 || !device_info(dev).is_sm100) return LORA_ERR_DEVICE;
   const LinearPlan p = linear_plan(M, N, K, R, fmt);
@@ -142,7 +166,16 @@ extern "C" int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, c
   const int64_t rp = r16(R);
   char* z = z_out != nullptr ? static_cast<char*>(z_out) : ws + p.z;
   const float zs = scale / o.alpha;
-  if (R > 0 && mx_shrink_serves(x, ldx, a, lda)) {
+  if (copies) {
+    const int64_t k8 = (K + 7) / 8 * 8;
+    rc = mx_widen_launch(x, ldx, ws + p.x, M, K, k8, s);
+    if (rc == LORA_OK) rc = mx_widen_launch(a, lda, ws + p.a, R, K, k8, s);
+    if (rc != LORA_OK) return rc;
+    x = ws + p.x;
+    a = ws + p.a;
+    ldx = lda = k8;
+  }
+  if (served || copies) {
     MxShrinkOperands sh = {};
     sh.v = x;
     sh.a = a;
@@ -162,17 +195,8 @@ extern "C" int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, c
     rc = mx_shrink_launch(sh, fmt, dtype, s);
   } else {
     rc = mx_quantize_launch(x, ldx, ws + p.x_codes, ws + p.x_scales, M, K, fmt, x_global, dtype, s);
-    if (rc == LORA_OK && R > 0) {
-      if (R <= kShrinkMaxRank) {
-        rc = lora_shrink(x, ldx, a, lda, z, 2 * rp, dtype, rp, 1, M, K, R, zs, dtype, p.split_k, ws, p.shrink_bytes, s);
-      } else {
-        if (z_out != nullptr && rp != R &&
-            cudaMemsetAsync(z, 0, static_cast<size_t>(M) * 2 * rp * 2, s) != cudaSuccess)
-          return LORA_ERR_CUDA;
-        rc = lora_gemm_ex(x, ldx, a, lda, nullptr, 0, nullptr, 0, nullptr, z, 2 * rp, M, R, K, 0, zs, rp, dtype,
-                          p.shrink_bytes ? ws : nullptr, p.shrink_bytes, s);
-      }
-    }
+    if (rc == LORA_OK && R > 0)
+      rc = lora_shrink(x, ldx, a, lda, z, 2 * rp, dtype, rp, 1, M, K, R, zs, dtype, p.split_k, ws, p.shrink_bytes, s);
   }
   if (rc != LORA_OK) return rc;
   if (R > 0) {

@@ -23,6 +23,10 @@ bool mx_few_tokens(int64_t M, int64_t N, int num_sms);
 int mx_small_launch(const MxLinearOperands& o, int fmt, int dtype, cudaStream_t stream);
 int mx_gemm_launch(const MxLinearOperands& o, int fmt, int dtype, cudaStream_t stream);
 
+// Copies rows of `cols` elements of 2 bytes, of any alignment, to 16-byte aligned rows of
+// `width` (a multiple of 8; zeros beyond cols).  Rows <= 2^31 - 1, width <= 2^28.
+int mx_widen_launch(const void* in, int64_t ldi, void* out, int64_t rows, int64_t cols, int64_t width, cudaStream_t s);
+
 // 2-D TMA map over rows of `inner` elements of 1, 2 or 4 bytes.
 bool mx_encode_map(CUtensorMap* map, const void* ptr, int elem, int64_t inner, int64_t outer, int64_t pitch_bytes,
                    int box_inner, int box_outer, bool swizzle);
