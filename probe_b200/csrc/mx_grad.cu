@@ -14,15 +14,16 @@
 // An mxfp8 V arrives as codes and scale chunks; sixteen warps turn it into 16-bit
 // values in the MMA's swizzled layout.  E4M3 times a power of two is exact in
 // bf16: the code's exponent and mantissa moved into place, times 2^120, times the
-// scale.  Bound: HBM for small ranks (2 or 1.03 bytes an element of V), the tensor
-// pipe above r ~ 100 (MMAs of N = r with both operands in shared memory).  Both gradients
-// of 4097 tokens, 4096 -> 11008, r = 16, 107 MB: 45 us with the partials; of 32760 tokens,
-// 5120 -> 5120, r = 224: 145.  They are one launch: the second's blocks start as the
-// first's leave, and few tokens' blocks run side by side (256 tokens, 4096 -> 4096: 4.6 us
-// instead of 4.0 + 7.8 with waits).  Up to rank 64 P is the whole hi/lo pair (N = 2 r, the halves
-// added in the epilogue), free while HBM is the bound; above, where it would double
-// the tensor pipe's work, the hi part alone, whose rounding (2^-9 of each term,
-// independent) stays below that of the 16-bit result.
+// scale.  Bound: HBM for small ranks (2 or 1.03 bytes an element of V), the MMAs, both of
+// whose operands come from shared memory, for large ones.  Both gradients
+// of 4097 tokens, 4096 -> 11008, r = 16, 107 MB: 46 us with the partials; of 32760 tokens,
+// 5120 -> 5120: 129 at r = 64, 162 at r = 128, 300 at r = 224 (300 GFLOP).  They are one launch: the second's blocks start as the
+// first's leave, and few tokens' blocks run side by side (256 tokens, 4096 -> 4096: 4.7 us
+// instead of 4.0 + 7.8 with waits).
+// P is the whole hi/lo pair.  Up to rank 128 its halves lie side by side in one MMA (N = 2 r)
+// and are added in the epilogue; above, they meet V one after the other in the same
+// accumulator, from stages of half as many tokens.  The hi half alone would take 145 us at
+// r = 224, but its rounding is as large as that of the 16-bit result.
 #include <mutex>
 
 #include "mx_grad.h"
@@ -30,15 +31,19 @@
 namespace lora {
 namespace {
 
-constexpr int kGrTok = 64;    // tokens a stage
 constexpr int kGrCols = 256;  // columns of V a CTA
 constexpr int kGrConvWarps = 16;
 constexpr int kGrThreads = 64 + 32 * kGrConvWarps;
-constexpr int kGrChunkBytes = kGrTok * 128;          // 64 tokens x 64 16-bit columns
-constexpr int kGrVBytes = 4 * kGrChunkBytes;         // 16-bit V of a stage
-constexpr int kGrRawBytes = kGrTok * kGrCols;        // codes of a stage
-constexpr int kGrScaleBytes = 2 * 512;               // their scale chunks (128 tokens x 256 columns)
+constexpr int kGrScaleBytes = 2 * 512;  // scale chunks of a stage (128 tokens x 256 columns)
 constexpr int kGrSmemMax = 224 * 1024;
+constexpr int kGrMaxN = 256;  // columns of one MMA
+// TOK tokens a stage.
+template <int TOK>
+struct GrStage {
+  static constexpr int kChunk = TOK * 128;      // TOK tokens x 64 16-bit columns
+  static constexpr int kV = 4 * kChunk;         // 16-bit V
+  static constexpr int kRaw = TOK * kGrCols;    // codes
+};
 
 struct GrMaps {
   CUtensorMap v, p, sc;
@@ -48,8 +53,9 @@ struct GrArgs {
   float* part;  // [splits][C][ldp]
   int* err;
   int64_t C;
-  int M, r16, n, p_chunks,  // n: columns of P (2 r16 with the lo part, else r16)
-      stages, stage_bytes, steps_per_split, steps, splits, scale_gb;
+  int M, r16;
+  int n, passes, p_chunks;  // N of an MMA; the runs of P that meet V in turn, 64-column chunks of each
+  int stages, stage_bytes, steps_per_split, steps, splits, scale_gb;
 };
 
 // MN-major operand in 64-wide chunks: token rows 128 bytes apart, 8-row groups
@@ -108,14 +114,15 @@ LORA_DEVINL uint4 gr_decode8<__half>(uint2 w, uint32_t s) {
 
 // Shared memory: the TMA ring (stage: V or codes + scales, then P), for mxfp8 two
 // converted tiles, then the barriers.
-template <typename T, bool F8>
+template <typename T, bool F8, int TOK>
 LORA_DEVINL void gr_job(const GrMaps& maps, const GrArgs& args, int group, int split) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  constexpr int kPOffset = F8 ? kGrRawBytes + kGrScaleBytes : kGrVBytes;
+  using S = GrStage<TOK>;
+  constexpr int kPOffset = F8 ? S::kRaw + kGrScaleBytes : S::kV;
   uint8_t* conv = smem + args.stages * args.stage_bytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(conv + (F8 ? 2 * kGrVBytes : 0));
+  uint64_t* full = reinterpret_cast<uint64_t*>(conv + (F8 ? 2 * S::kV : 0));
   uint64_t* empty = full + 8;
   uint64_t* ready = empty + 8;       // [2] converted tile written
   uint64_t* conv_empty = ready + 2;  // [2] converted tile read by its MMAs
@@ -162,22 +169,24 @@ LORA_DEVINL void gr_job(const GrMaps& maps, const GrArgs& args, int group, int s
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
-      const uint32_t bytes = kPOffset + args.p_chunks * kGrChunkBytes;
+      const uint32_t bytes = kPOffset + args.passes * args.p_chunks * S::kChunk;
       for (int st = step0; st < step1; ++st) {
         if (!mbar_wait_bounded(&empty[stage], phase ^ 1, abort_flag, args.err, kDevErrTimeoutEmpty)) break;
         uint8_t* base = smem + stage * args.stage_bytes;
         mbar_arrive_expect_tx(&full[stage], bytes);
-        const int tok = st * kGrTok;
+        const int tok = st * TOK;
         if constexpr (F8) {
           tma_load_2d(&maps.v, base, &full[stage], static_cast<int>(col0), tok);
-          tma_load_2d(&maps.sc, base + kGrRawBytes, &full[stage], 0,
+          tma_load_2d(&maps.sc, base + S::kRaw, &full[stage], 0,
                       (tok >> 7) * args.scale_gb + static_cast<int>(col0 >> 7));
         } else {
           for (int c = 0; c < 4; ++c)
-            tma_load_2d(&maps.v, base + c * kGrChunkBytes, &full[stage], static_cast<int>(col0) + 64 * c, tok);
+            tma_load_2d(&maps.v, base + c * S::kChunk, &full[stage], static_cast<int>(col0) + 64 * c, tok);
         }
-        for (int c = 0; c < args.p_chunks; ++c)
-          tma_load_2d(&maps.p, base + kPOffset + c * kGrChunkBytes, &full[stage], 64 * c, tok);
+        uint8_t* p = base + kPOffset;
+        for (int i = 0; i < args.passes; ++i)
+          for (int c = 0; c < args.p_chunks; ++c, p += S::kChunk)
+            tma_load_2d(&maps.p, p, &full[stage], i * args.r16 + 64 * c, tok);
         if (++stage == args.stages) {
           stage = 0;
           phase ^= 1;
@@ -189,8 +198,8 @@ LORA_DEVINL void gr_job(const GrMaps& maps, const GrArgs& args, int group, int s
     // operands MN-major (bits 15 and 16), M = 128.
     const uint32_t idesc = (umma_idesc_f16(128, 16, std::is_same<T, __nv_bfloat16>::value ? 1 : 0) & ~(0x3fu << 17)) |
                            (static_cast<uint32_t>(args.n >> 3) << 17) | (1u << 15) | (1u << 16);
-    const uint64_t desc0 = gr_desc_mn(smem_u32(smem), kGrChunkBytes);
-    const uint64_t conv0 = gr_desc_mn(smem_u32(conv), kGrChunkBytes);
+    const uint64_t desc0 = gr_desc_mn(smem_u32(smem), S::kChunk);
+    const uint64_t conv0 = gr_desc_mn(smem_u32(conv), S::kChunk);
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -203,15 +212,17 @@ LORA_DEVINL void gr_job(const GrMaps& maps, const GrArgs& args, int group, int s
       }
       tc_fence_after();
       const uint64_t base = desc0 + static_cast<uint32_t>((stage * args.stage_bytes) >> 4);
-      const uint64_t v = F8 ? conv0 + static_cast<uint32_t>(((n & 1) * kGrVBytes) >> 4) : base;
-      const uint64_t pd = base + static_cast<uint32_t>(kPOffset >> 4);
+      const uint64_t v = F8 ? conv0 + static_cast<uint32_t>(((n & 1) * S::kV) >> 4) : base;
       if (elect_one()) {
+        uint64_t pd = base + static_cast<uint32_t>(kPOffset >> 4);
+        for (int i = 0; i < args.passes; ++i, pd += static_cast<uint32_t>((args.p_chunks * S::kChunk) >> 4)) {
 #pragma unroll
-        for (int k = 0; k < kGrTok / 16; ++k)
+          for (int k = 0; k < TOK / 16; ++k)
 #pragma unroll
-          for (int m = 0; m < 2; ++m)
-            tc_mma_f16(tmem + m * args.n, v + static_cast<uint32_t>((m * 2 * kGrChunkBytes + k * 2048) >> 4),
-                       pd + static_cast<uint32_t>((k * 2048) >> 4), idesc, (n > 0 || k > 0) ? 1u : 0u);
+            for (int m = 0; m < 2; ++m)
+              tc_mma_f16(tmem + m * args.n, v + static_cast<uint32_t>((m * 2 * S::kChunk + k * 2048) >> 4),
+                         pd + static_cast<uint32_t>((k * 2048) >> 4), idesc, (n > 0 || i > 0 || k > 0) ? 1u : 0u);
+        }
         tc_commit(&empty[stage]);
         if (F8) tc_commit(&conv_empty[n & 1]);
       }
@@ -235,12 +246,12 @@ LORA_DEVINL void gr_job(const GrMaps& maps, const GrArgs& args, int group, int s
           break;
         const uint32_t raw = smem_u32(smem) + stage * args.stage_bytes;
         // the scale chunk of this lane's 128 columns, its block
-        const uint32_t sc = raw + kGrRawBytes + (lane >> 4) * 512 + ((lane >> 2) & 3);
-        const uint32_t dst = smem_u32(conv) + (n & 1) * kGrVBytes + (lane >> 3) * kGrChunkBytes;
+        const uint32_t sc = raw + S::kRaw + (lane >> 4) * 512 + ((lane >> 2) & 3);
+        const uint32_t dst = smem_u32(conv) + (n & 1) * S::kV + (lane >> 3) * S::kChunk;
 #pragma unroll
-        for (int i = 0; i < kGrTok / kGrConvWarps; ++i) {
-          const int t = cw * (kGrTok / kGrConvWarps) + i;
-          const int tr = (st * kGrTok + t) & 127;  // row within the scale chunk
+        for (int i = 0; i < TOK / kGrConvWarps; ++i) {
+          const int t = cw * (TOK / kGrConvWarps) + i;
+          const int tr = (st * TOK + t) & 127;  // row within the scale chunk
           const uint2 w = lds64(raw + t * kGrCols + lane * 8);
           const uint32_t s = lds_u8(sc + (tr & 31) * 16 + (tr >> 5) * 4);
           sts128(dst + t * 128 + (((lane & 7) ^ (t & 7)) << 4), gr_decode8<T>(w, s));
@@ -264,9 +275,9 @@ LORA_DEVINL void gr_job(const GrMaps& maps, const GrArgs& args, int group, int s
         const uint32_t src = tmem + (static_cast<uint32_t>(quad * 32) << 16) + m * args.n + j;
         uint32_t r[16], lo[16];
         tmem_ld_32x32b_x16(src, r);
-        if (args.n > args.r16) tmem_ld_32x32b_x16(src + args.r16, lo);
+        if (args.passes == 1) tmem_ld_32x32b_x16(src + args.r16, lo);
         tmem_wait_ld();
-        if (args.n > args.r16) {
+        if (args.passes == 1) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) + __uint_as_float(lo[e]));
         }
@@ -293,14 +304,14 @@ struct GrJobs {
   int groups[2], blocks0;
 };
 
-template <typename T>
+template <typename T, int TOK>
 __global__ void __launch_bounds__(kGrThreads, 1) mx_grad_kernel(const __grid_constant__ GrJobs jobs) {
   const int b = static_cast<int>(blockIdx.x);
   if (b < jobs.blocks0) {
-    gr_job<T, false>(jobs.maps[0], jobs.args[0], b % jobs.groups[0], b / jobs.groups[0]);
+    gr_job<T, false, TOK>(jobs.maps[0], jobs.args[0], b % jobs.groups[0], b / jobs.groups[0]);
   } else {
     const int c = b - jobs.blocks0;
-    gr_job<T, true>(jobs.maps[1], jobs.args[1], c % jobs.groups[1], c / jobs.groups[1]);
+    gr_job<T, true, TOK>(jobs.maps[1], jobs.args[1], c % jobs.groups[1], c / jobs.groups[1]);
   }
 }
 
@@ -361,12 +372,17 @@ struct GrPlan {
   int groups, steps, splits, steps_per_split;
 };
 
-GrPlan grad_plan(int64_t M, int64_t C) {
+// Tokens a stage: half of the usual ones where both halves of P do not fit one MMA, so
+// that three stages or more of them fit beside the decoded tiles.
+int grad_tokens(int64_t R) { return 2 * ((R + 15) / 16 * 16) > kGrMaxN ? 32 : 64; }
+
+GrPlan grad_plan(int64_t M, int64_t C, int64_t R) {
+  const int tok = grad_tokens(R);
   GrPlan p;
   const int dev = current_device();
   const int sms = dev >= 0 ? device_info(dev).num_sms : 148;
   p.groups = static_cast<int>((C + kGrCols - 1) / kGrCols);
-  p.steps = static_cast<int>((M + kGrTok - 1) / kGrTok);
+  p.steps = static_cast<int>((M + tok - 1) / tok);
   int splits = std::max(1, sms / p.groups);
   splits = std::min(splits, p.steps);
   p.steps_per_split = (p.steps + splits - 1) / splits;
@@ -375,35 +391,39 @@ GrPlan grad_plan(int64_t M, int64_t C) {
 }
 
 // Maps and arguments of one gradient; its shared memory through `smem`.
+template <int TOK>
 bool fill_job(const MxGradOperands& g, const GrPlan& pl, bool f8, int* err, GrMaps* maps, GrArgs* a, size_t* smem) {
   a->part = static_cast<float*>(g.part);
   a->err = err;
   a->C = g.C;
   a->M = static_cast<int>(g.M);
   a->r16 = static_cast<int>((g.R + 15) / 16 * 16);
-  a->n = a->r16 <= 64 ? 2 * a->r16 : a->r16;
+  // [hi | lo] side by side in one MMA, or one after the other
+  a->passes = 2 * a->r16 > kGrMaxN ? 2 : 1;
+  a->n = a->passes == 1 ? 2 * a->r16 : a->r16;
   a->p_chunks = (a->n + 63) / 64;
   a->steps = pl.steps;
   a->splits = pl.splits;
   a->steps_per_split = pl.steps_per_split;
   a->scale_gb = static_cast<int>(mx_scale_chunks(g.C, LORA_MXFP8));
-  a->stage_bytes = (f8 ? kGrRawBytes + kGrScaleBytes : kGrVBytes) + a->p_chunks * kGrChunkBytes;
-  const int fixed = (f8 ? 2 * kGrVBytes : 0) + 512 + 1024;
+  using S = GrStage<TOK>;
+  a->stage_bytes = (f8 ? S::kRaw + kGrScaleBytes : S::kV) + a->passes * a->p_chunks * S::kChunk;
+  const int fixed = (f8 ? 2 * S::kV : 0) + 512 + 1024;
   a->stages = std::min(8, (kGrSmemMax - fixed) / a->stage_bytes);
   *smem = std::max(*smem, static_cast<size_t>(a->stages) * a->stage_bytes + fixed);
   if (f8) {
     const int64_t pitch = mx_padded_k(g.C);
-    if (!mx_encode_map(&maps->v, g.v, 1, pitch, g.M, pitch, kGrCols, kGrTok, false) ||
+    if (!mx_encode_map(&maps->v, g.v, 1, pitch, g.M, pitch, kGrCols, TOK, false) ||
         !mx_encode_map(&maps->sc, g.v_scales, 4, 128, (g.M + 127) / 128 * a->scale_gb, 512, 128, 2, false))
       return false;
   } else {
-    if (!mx_encode_map(&maps->v, g.v, 2, g.C, g.M, g.ldv * 2, 64, kGrTok, true)) return false;
+    if (!mx_encode_map(&maps->v, g.v, 2, g.C, g.M, g.ldv * 2, 64, TOK, true)) return false;
     maps->sc = maps->v;
   }
-  return mx_encode_map(&maps->p, g.p, 2, a->n, g.M, g.ldp * 2, 64, kGrTok, true);
+  return mx_encode_map(&maps->p, g.p, 2, 2 * a->r16, g.M, g.ldp * 2, 64, TOK, true);
 }
 
-template <typename T>
+template <typename T, int TOK>
 int launch_grads(const MxGradOperands* g, cudaStream_t stream) {
   const int dev = current_device();
   if (dev < 0) return LORA_ERR_DEVICE;
@@ -412,13 +432,13 @@ int launch_grads(const MxGradOperands* g, cudaStream_t stream) {
   size_t smem = 0;
   int blocks = 0;
   for (int i = 0; i < 2; ++i) {
-    const GrPlan pl = grad_plan(g[i].M, g[i].C);
-    if (!fill_job(g[i], pl, i == 1, info.err_word, &jobs.maps[i], &jobs.args[i], &smem)) return LORA_ERR_CUDA;
+    const GrPlan pl = grad_plan(g[i].M, g[i].C, g[i].R);
+    if (!fill_job<TOK>(g[i], pl, i == 1, info.err_word, &jobs.maps[i], &jobs.args[i], &smem)) return LORA_ERR_CUDA;
     jobs.groups[i] = pl.groups;
     if (i == 1) jobs.blocks0 = blocks;
     blocks += pl.groups * pl.splits;
   }
-  auto kernel = mx_grad_kernel<T>;
+  auto kernel = mx_grad_kernel<T, TOK>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
   std::call_once(once[dev], [&] {
@@ -431,11 +451,13 @@ int launch_grads(const MxGradOperands* g, cudaStream_t stream) {
 }  // namespace
 
 size_t mx_grad_part_bytes(int64_t M, int64_t C, int64_t R) {
-  return static_cast<size_t>(grad_plan(M, C).splits) * C * ((R + 15) / 16 * 16) * sizeof(float);
+  return static_cast<size_t>(grad_plan(M, C, R).splits) * C * ((R + 15) / 16 * 16) * sizeof(float);
 }
 
 int mx_grad_launch(const MxGradOperands* g, int dtype, cudaStream_t stream) {
-  return dtype == LORA_BF16 ? launch_grads<__nv_bfloat16>(g, stream) : launch_grads<__half>(g, stream);
+  if (grad_tokens(g[0].R) == 32)
+    return dtype == LORA_BF16 ? launch_grads<__nv_bfloat16, 32>(g, stream) : launch_grads<__half, 32>(g, stream);
+  return dtype == LORA_BF16 ? launch_grads<__nv_bfloat16, 64>(g, stream) : launch_grads<__half, 64>(g, stream);
 }
 
 int mx_grad_reduce_launch(const MxGradOperands* g, int dtype, cudaStream_t stream) {
@@ -449,7 +471,7 @@ int mx_grad_reduce_launch(const MxGradOperands* g, int dtype, cudaStream_t strea
     s.C = g[i].C;
     s.r = static_cast<int>(g[i].R);
     s.r16 = (s.r + 15) / 16 * 16;
-    s.splits = grad_plan(g[i].M, g[i].C).splits;
+    s.splits = grad_plan(g[i].M, g[i].C, g[i].R).splits;
     s.blocks = static_cast<int>((g[i].C + 31) / 32);
     s.factor = g[i].factor;
     s.transposed = g[i].transposed;

@@ -6,7 +6,7 @@
 namespace lora {
 
 // out[c, j] = factor * sum_t V[t, c] P[t, j]; P is the pair [hi | lo], R16 columns
-// each (the lo part is read up to rank 64); V is 16-bit (ldv) or, with
+// each; V is 16-bit (ldv) or, with
 // v_scales, an mxfp8 tensor; transposed writes out[j, c].
 struct MxGradOperands {
   const void *v, *v_scales, *p;

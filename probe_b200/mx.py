@@ -289,9 +289,8 @@ def mx_lora_backward(dy: torch.Tensor, x8: MXTensor, z: torch.Tensor, a: torch.T
 
     ``g = scale * dy @ b``;  ``da = g.T @ X`` [r, K];  ``db = z_scale * dy.T @ z`` [N, r];
     ``dx = dy @ W + g @ a`` [..., K], or None without ``weight``.  ``x8`` is the mxfp8
-    checkpoint of x, ``z`` the [M, 2 r16] pair [hi | lo] of the forward pass (above
-    rank 64 its hi half alone is read), W an mxfp4 / nvfp4 tensor.  W is frozen; rounding to 4 or 8 bits counts
-    as the identity.
+    checkpoint of x, ``z`` the [M, 2 r16] pair [hi | lo] of the forward pass, W an mxfp4 /
+    nvfp4 tensor.  W is frozen; rounding to 4 or 8 bits counts as the identity.
     """
     shape, dtype = dy.shape, dy.dtype
     wc = weight.codes if weight is not None else None
