@@ -409,8 +409,8 @@ LORA_API int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, con
  * lora_mx_linear's z_out (columns R..r16-1 of each half are not used), z_scale its
  * factor; W as
  * an MXFP4 / NVFP4 tensor [N, K] (read for dx only).  W is frozen and rounding to
- * 8 or 4 bits counts as the identity.  Products accumulate in fp32; g, like z, is
- * held as a hi/lo pair of dtype; outputs are rounded once to dtype; token ranges are summed
+ * 8 or 4 bits counts as the identity.  Products accumulate in fp32; g is held
+ * as a sum of bf16 parts (two, for fp16 three: its range is fp32's); outputs are rounded once to dtype; token ranges are summed
  * in a fixed order.  1 <= R <= 256; z, codes and scales 16-byte aligned.  M or N 0:
  * the outputs are zeros; K 0: LORA_ERR_UNSUPPORTED, as the forward pass.
  * Workspace: lora_mx_backward_workspace_size bytes, 256-byte aligned, zeroed

@@ -154,10 +154,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const uint64_t bdesc = umma_desc_sw128(smem_u32(sm_b + stage * L::kBBytes));
           // The last tail block only holds ceil(R%64 / 16) non-zero K16 steps.
           const int nk = (kb == num_kb - 1 && args.num_kb_tail > 0) ? args.tail_last_k16 : 4;
+          const uint32_t idesc = kb < args.num_kb_main ? kIdesc : kIdesc ^ args.tail_flip;
           for (int k = 0; k < nk; ++k) {
             // +32 bytes per K16 step inside the 128B swizzle atom (>>4 => +2).
             tc_mma_f16(d_tmem, adesc + static_cast<uint64_t>(2 * k), bdesc + static_cast<uint64_t>(2 * k),
-                       kIdesc, (kb > 0 || k > 0) ? 1u : 0u);
+                       idesc, (kb > 0 || k > 0) ? 1u : 0u);
           }
           tc_commit(&empty[stage]);
           if (++stage == STAGES) {
@@ -409,9 +410,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * EW, 1)
           const uint64_t adesc = umma_desc_sw128(smem_u32(sm_a + stage * L::kABytes));
           const uint64_t bdesc = umma_desc_sw128(smem_u32(sm_b + stage * L::kBBytes));
           const int nk = (kb == num_kb - 1 && args.num_kb_tail > 0) ? args.tail_last_k16 : 4;
+          const uint32_t idesc = kb < args.num_kb_main ? kIdesc : kIdesc ^ args.tail_flip;
           for (int k = 0; k < nk; ++k)
             tc_mma_f16_pair(d_tmem, adesc + static_cast<uint64_t>(2 * k), bdesc + static_cast<uint64_t>(2 * k),
-                            kIdesc, (kb > kb0 || k > 0) ? 1u : 0u);
+                            idesc, (kb > kb0 || k > 0) ? 1u : 0u);
           if constexpr (NW == 2) {
             if (kb == kb0) {  // the second half of the accumulator: free once the epilogue has drained it
               if (!mbar_wait_bounded(&acc_empty[1], acc_phase ^ 1, abort_flag, args.err, kDevErrTimeoutAccEmpty)) {
@@ -423,7 +425,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * EW, 1)
             const uint64_t bdesc1 = umma_desc_sw128(smem_u32(sm_b + stage * L::kBBytes + 128 * kGemmBK * 2));
             for (int k = 0; k < nk; ++k)
               tc_mma_f16_pair(tmem_base + 256, adesc + static_cast<uint64_t>(2 * k),
-                              bdesc1 + static_cast<uint64_t>(2 * k), kIdesc, (kb > kb0 || k > 0) ? 1u : 0u);
+                              bdesc1 + static_cast<uint64_t>(2 * k), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
           }
           tc_commit_pair(&empty[stage], kBoth);
           if (++stage == STAGES) {
@@ -544,7 +546,8 @@ namespace {
 template <int BN, int STAGES, typename T>
 int launch_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* z, int64_t ldz,
                 const void* bw, int64_t ldbw, const void* bias, void* out, int64_t ldo, int64_t M,
-                int64_t N, int64_t K, int64_t R, float alpha, int64_t lo_offset, int dtype, cudaStream_t stream) {
+                int64_t N, int64_t K, int64_t R, float alpha, int64_t lo_offset, int dtype, uint32_t tail_flip,
+                cudaStream_t stream) {
   using L = GemmSmem<BN, STAGES, T>;
   const int dev = current_device();
   if (dev < 0) return LORA_ERR_DEVICE;
@@ -577,6 +580,7 @@ int launch_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, const vo
   a.num_kb_tail = static_cast<int>((R + kGemmBK - 1) / kGemmBK);
   const int tail_rem = static_cast<int>(R - static_cast<int64_t>(a.num_kb_tail - 1) * kGemmBK);
   a.tail_last_k16 = a.num_kb_tail > 0 ? (tail_rem + 15) / 16 : 4;
+  a.tail_flip = tail_flip;
   a.num_m_tiles = static_cast<int>((M + kGemmBM - 1) / kGemmBM);
   a.num_n_tiles = static_cast<int>((N + BN - 1) / BN);
   a.num_tiles = a.num_m_tiles * a.num_n_tiles;
@@ -603,17 +607,17 @@ int launch_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, const vo
 template <typename T>
 int dispatch_gemm(int bn, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* z, int64_t ldz,
                   const void* bw, int64_t ldbw, const void* bias, void* out, int64_t ldo, int64_t M, int64_t N,
-                  int64_t K, int64_t R, float alpha, int64_t lo, int dtype, cudaStream_t stream) {
+                  int64_t K, int64_t R, float alpha, int64_t lo, int dtype, uint32_t tail_flip, cudaStream_t stream) {
   switch (bn) {
     case 64:
       return launch_gemm<64, 8, T>(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo, dtype,
-                                   stream);
+                                   tail_flip, stream);
     case 128:
       return launch_gemm<128, 6, T>(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo, dtype,
-                                    stream);
+                                    tail_flip, stream);
     default:
       return launch_gemm<256, 4, T>(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo, dtype,
-                                    stream);
+                                    tail_flip, stream);
   }
 }
 
@@ -693,8 +697,8 @@ int pair_capacity(int dev, const DeviceInfo& info, cudaError_t* attr_status) {
 template <int STAGES, int NW, int EW, typename T>
 int launch_gemm_pair(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* z, int64_t ldz,
                      const void* bw, int64_t ldbw, const void* bias, void* out, int64_t ldo, int64_t M, int64_t N,
-                     int64_t K, int64_t R, float alpha, int64_t lo_offset, int dtype, void* ws, size_t ws_bytes,
-                     cudaStream_t stream) {
+                     int64_t K, int64_t R, float alpha, int64_t lo_offset, int dtype, uint32_t tail_flip, void* ws,
+                     size_t ws_bytes, cudaStream_t stream) {
   using L = PairSmem<STAGES, NW>;
   const int dev = current_device();
   if (dev < 0) return LORA_ERR_DEVICE;
@@ -723,6 +727,7 @@ int launch_gemm_pair(const void* x, int64_t ldx, const void* w, int64_t ldw, con
   a.num_kb_tail = static_cast<int>((R + kGemmBK - 1) / kGemmBK);
   const int tail_rem = static_cast<int>(R - static_cast<int64_t>(a.num_kb_tail - 1) * kGemmBK);
   a.tail_last_k16 = a.num_kb_tail > 0 ? (tail_rem + 15) / 16 : 4;
+  a.tail_flip = tail_flip;
   a.num_m_tiles = static_cast<int>((M + 255) / 256);
   a.num_n_tiles = static_cast<int>((N + 256 * NW - 1) / (256 * NW));
   a.num_tiles = a.num_m_tiles * a.num_n_tiles;
@@ -845,7 +850,7 @@ namespace {
 
 int gemm_impl(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* z, int64_t ldz, const void* bw,
               int64_t ldbw, const void* bias, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K, int64_t R,
-              float alpha, int64_t lo_offset, int dtype, void* ws, size_t ws_bytes, void* stream) {
+              float alpha, int64_t lo_offset, int dtype, uint32_t tail_flip, void* ws, size_t ws_bytes, void* stream) {
   if (x == nullptr || w == nullptr || out == nullptr) return LORA_ERR_ARG;
   if (dtype != LORA_BF16 && dtype != LORA_F16) return LORA_ERR_DTYPE;
   if (M < 0 || N < 0 || K < 0 || R < 0) return LORA_ERR_SHAPE;
@@ -873,27 +878,37 @@ int gemm_impl(const void* x, int64_t ldx, const void* w, int64_t ldw, const void
 #define LORA_PAIR(ST, NWV)                                                                                        \
   (dtype == LORA_BF16                                                                                              \
        ? launch_gemm_pair<ST, NWV, kPairEpiWarps, __nv_bfloat16>(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, \
-                                                                 N, K, R, alpha, lo_offset, dtype, ws, ws_bytes, s)   \
+                                                                 N, K, R, alpha, lo_offset, dtype, tail_flip, ws,     \
+                                                                 ws_bytes, s)                                         \
        : launch_gemm_pair<ST, NWV, kPairEpiWarps, __half>(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, \
-                                                          R, alpha, lo_offset, dtype, ws, ws_bytes, s))
+                                                          R, alpha, lo_offset, dtype, tail_flip, ws, ws_bytes, s))
     return nw == 2 ? LORA_PAIR(4, 2) : LORA_PAIR(6, 1);
 #undef LORA_PAIR
   }
   if (dtype == LORA_BF16)
     return dispatch_gemm<__nv_bfloat16>(bn, x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha,
-                                        lo_offset, dtype, s);
+                                        lo_offset, dtype, tail_flip, s);
   return dispatch_gemm<__half>(bn, x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo_offset,
-                               dtype, s);
+                               dtype, tail_flip, s);
 }
 
 }  // namespace
+
+int gemm_mixed_tail(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* z, int64_t ldz, const void* bw,
+                    int64_t ldbw, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K, int64_t R, float alpha,
+                    int dtype, int z_dtype, void* ws, size_t ws_bytes, void* stream) {
+  constexpr uint32_t kOther = umma_idesc_f16(128, 256, 0) ^ umma_idesc_f16(128, 256, 1);
+  return gemm_impl(x, ldx, w, ldw, z, ldz, bw, ldbw, nullptr, out, ldo, M, N, K, R, alpha, 0, dtype,
+                   dtype == z_dtype ? 0 : kOther, ws, ws_bytes, stream);
+}
+
 }  // namespace lora
 
 extern "C" int lora_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* z, int64_t ldz,
                          const void* bw, int64_t ldbw, const void* bias, void* out, int64_t ldo, int64_t M,
                          int64_t N, int64_t K, int64_t R, float alpha, int64_t lo_offset, int dtype, void* stream) {
   return lora::gemm_impl(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo_offset, dtype,
-                         nullptr, 0, stream);
+                         0, nullptr, 0, stream);
 }
 
 extern "C" size_t lora_gemm_workspace_size(int64_t M, int64_t N, int64_t K, int64_t R) {
@@ -918,5 +933,5 @@ extern "C" int lora_gemm_ex(const void* x, int64_t ldx, const void* w, int64_t l
                             int64_t N, int64_t K, int64_t R, float alpha, int64_t lo_offset, int dtype,
                             void* workspace, size_t workspace_bytes, void* stream) {
   return lora::gemm_impl(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo_offset, dtype,
-                         workspace, workspace_bytes, stream);
+                         0, workspace, workspace_bytes, stream);
 }

@@ -14,6 +14,7 @@
 // values and m in the product's alpha.
 #include <cmath>
 
+#include "gemm_pair.cuh"
 #include "mx_dx.h"
 #include "mx_grad.h"
 #include "mx_shrink.h"
@@ -26,48 +27,69 @@ namespace {
 // against 109 us).
 constexpr int64_t kWideRank = 128, kWideRows = 4096;
 
+// g of fp16 activations is kept in three bf16 parts, which never leave its range; beside
+// A = Ah + Al the tail of dx takes [gh gm gl gh gm] against [Ah Ah Ah Al Al].
+constexpr int kTailHigh = 3, kTailLow = 2, kTailGroups = kTailHigh + kTailLow;
+
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 struct BackwardPlan {
-  bool few;  // dx of few rows
+  bool few;    // dx of few rows
+  bool wide;   // g from the pair GEMM
+  int parts;   // of g, side by side
+  int groups;  // of r16 columns of g: its parts, some of them again for the tail of dx
   size_t gemm_bytes, part, part_a, g, bt, at, dy, wt, total;
 };
 
-BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need_dx) {
+BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need_dx, bool half) {
   BackwardPlan p = {};
   const int64_t np = up(N, 8), rp = up(R, 16);
   const int dev = current_device();
   p.few = need_dx && mx_dx_few(M, K, dev >= 0 ? device_info(dev).num_sms : 148);
-  if (need_dx && !p.few) p.gemm_bytes = lora_gemm_workspace_size(M, K, np, 2 * rp);
-  if (R > kWideRank && M >= kWideRows) p.gemm_bytes = std::max(p.gemm_bytes, lora_gemm_workspace_size(M, R, np, 0));
+  const bool many = need_dx && !p.few;
+  p.parts = half ? kTailHigh : 2;
+  p.groups = half && many ? kTailGroups : p.parts;
+  p.wide = !half && R > kWideRank && M >= kWideRows;
+  const int64_t tail = p.groups * rp;
+  if (many) p.gemm_bytes = lora_gemm_workspace_size(M, K, np, tail);
+  if (p.wide) p.gemm_bytes = std::max(p.gemm_bytes, lora_gemm_workspace_size(M, R, np, 0));
   size_t at = kCounterBytes;  // ticket counters, never scratch; the steps' partials follow them in turn
   at = std::max(at, mx_align(std::max(kCounterBytes + mx_shrink_part_bytes(M, np, R), p.gemm_bytes)));
   p.part = at;
-  at += mx_align(mx_grad_part_bytes(M, N, R));
+  at += mx_align(mx_grad_part_bytes(M, N, R, p.parts));
   p.part_a = at;
-  at += mx_align(mx_grad_part_bytes(M, K, R));
+  at += mx_align(mx_grad_part_bytes(M, K, R, p.parts));
   p.g = at;
-  at += mx_align(static_cast<size_t>(M) * 2 * rp * 2);
+  at += mx_align(static_cast<size_t>(M) * tail * 2);
   p.bt = at;
   at += mx_align(static_cast<size_t>(R) * np * 2);
   p.at = at;
-  if (need_dx) at += mx_align(p.few ? static_cast<size_t>(R) * up(K, 8) * 2 : static_cast<size_t>(K) * 2 * rp * 2);
+  if (many) at += mx_align(static_cast<size_t>(K) * tail * 2);
+  if (p.few) at += mx_align(static_cast<size_t>(R) * up(K, 8) * (half ? 4 : 2));
   p.dy = at;
   at += mx_align(static_cast<size_t>(M) * np * 2);
   p.wt = at;
-  if (need_dx && !p.few) at += mx_align(static_cast<size_t>(K) * np * 2);
+  if (many) at += mx_align(static_cast<size_t>(K) * np * 2);
   p.total = at;
   return p;
 }
 
+// An fp16 value as the sum of two bf16 values (exact: 11 bits).
+LORA_DEVINL void split_half(uint16_t v, uint16_t& hi, uint16_t& lo) {
+  const float f = __half2float(__ushort_as_half(v));
+  const __nv_bfloat16 h = __float2bfloat16_rn(f);
+  hi = __bfloat16_as_ushort(h);
+  lo = __bfloat16_as_ushort(__float2bfloat16_rn(f - __bfloat162float(h)));
+}
+
 // out[c, j] = in[j, c] for in [rows, cols], j < width (zeros beyond rows); `copies`
-// of the width columns side by side.  32 x 32 a block; the blocks of two matrices
-// side by side.
+// of the width columns side by side and, of fp16 values in two bf16 parts, `lows` of the
+// low part after them.  32 x 32 a block; the blocks of two matrices side by side.
 struct TransposeJob {
   const uint16_t* in;
   uint16_t* out;
   int64_t ldi, ldo, rows, cols, width;
-  int copies, blocks_c, blocks;
+  int copies, lows, blocks_c, blocks;
 };
 struct TransposeJobs {
   TransposeJob of[2];
@@ -89,14 +111,17 @@ __global__ void __launch_bounds__(256) mx_transpose_kernel(const TransposeJobs j
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t c = c0 + ty + 8 * i, j = j0 + tx;
-    if (c < t.cols && j < t.width)
-      for (int k = 0; k < t.copies; ++k) t.out[c * t.ldo + k * t.width + j] = tile[tx][ty + 8 * i];
+    if (c < t.cols && j < t.width) {
+      uint16_t hi = tile[tx][ty + 8 * i], lo = 0;
+      if (t.lows > 0) split_half(hi, hi, lo);
+      for (int k = 0; k < t.copies + t.lows; ++k) t.out[c * t.ldo + k * t.width + j] = k < t.copies ? hi : lo;
+    }
   }
 }
 
 TransposeJob transpose_job(const void* in, int64_t ldi, void* out, int64_t ldo, int64_t rows, int64_t cols, int64_t width,
-                           int copies) {
-  TransposeJob t{static_cast<const uint16_t*>(in), static_cast<uint16_t*>(out), ldi, ldo, rows, cols, width, copies};
+                           int copies, int lows) {
+  TransposeJob t{static_cast<const uint16_t*>(in), static_cast<uint16_t*>(out), ldi, ldo, rows, cols, width, copies, lows};
   t.blocks_c = static_cast<int>(up(cols, 32) / 32);
   t.blocks = t.blocks_c * static_cast<int>(up(width, 32) / 32);
   return t;
@@ -109,6 +134,28 @@ int transpose(const TransposeJobs& jobs, cudaStream_t s) {
   return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
 }
 
+// fp16 rows of `cols` elements as two bf16 parts, hi [rows, width] and then lo (zeros
+// beyond cols), 8 elements a thread.
+__global__ void __launch_bounds__(256) mx_split_rows_kernel(const uint16_t* __restrict__ in, int64_t ldi,
+                                                            uint16_t* __restrict__ out, int64_t rows, int64_t cols,
+                                                            int64_t width) {
+  const int64_t row = blockIdx.x, c = (static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x) * 8;
+  if (c >= width) return;
+  uint16_t h[8], l[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) split_half(c + i < cols ? in[row * ldi + c + i] : uint16_t{0}, h[i], l[i]);
+  auto word = [](const uint16_t* v) { return v[0] | (static_cast<uint32_t>(v[1]) << 16); };
+  *reinterpret_cast<uint4*>(out + row * width + c) = make_uint4(word(h), word(h + 2), word(h + 4), word(h + 6));
+  *reinterpret_cast<uint4*>(out + (rows + row) * width + c) = make_uint4(word(l), word(l + 2), word(l + 4), word(l + 6));
+}
+
+int split_rows(const void* in, int64_t ldi, void* out, int64_t rows, int64_t cols, int64_t width, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>((width + 2047) / 2048));
+  mx_split_rows_kernel<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(in), ldi, static_cast<uint16_t*>(out), rows, cols,
+                                            width);
+  return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
+}
+
 }  // namespace
 }  // namespace lora
 
@@ -116,7 +163,8 @@ using namespace lora;
 
 extern "C" size_t lora_mx_backward_workspace_size(int64_t M, int64_t N, int64_t K, int64_t R, int need_dx) {
   if (M <= 0 || N <= 0 || K <= 0 || R <= 0) return 0;
-  return backward_plan(M, N, K, R, need_dx != 0).total;
+  return std::max(backward_plan(M, N, K, R, need_dx != 0, false).total,
+                  backward_plan(M, N, K, R, need_dx != 0, true).total);
 }
 
 extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_codes, const void* x_scales, const void* z,
@@ -150,7 +198,8 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
       return LORA_ERR_CUDA;
     return LORA_OK;
   }
-  const BackwardPlan p = backward_plan(M, N, K, R, dx != nullptr);
+  const bool half = dtype == LORA_F16;
+  const BackwardPlan p = backward_plan(M, N, K, R, dx != nullptr, half);
   if (workspace == nullptr || workspace_bytes < p.total) return LORA_ERR_WORKSPACE;
   char* ws = static_cast<char*>(workspace);
   const int64_t np = up(N, 8), rp = up(R, 16);
@@ -166,20 +215,22 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   // predecessor on the stream has finished, so other launches lie between.
   TransposeJobs jobs = {};
   const bool b_rows = mx_aligned(b, 16) && ldb % 8 == 0;  // TMA can read them
-  const bool wide = R > kWideRank && M >= kWideRows;
-  if (!b_rows || wide) jobs.of[0] = transpose_job(b, ldb, ws + p.bt, np, N, R, np, 1);
-  if (dx != nullptr && !p.few) jobs.of[1] = transpose_job(a, lda, ws + p.at, 2 * rp, R, K, rp, 2);
+  const bool many = dx != nullptr && !p.few;
+  const int groups = p.groups;
+  if (!b_rows || p.wide) jobs.of[0] = transpose_job(b, ldb, ws + p.bt, np, N, R, np, 1, 0);
+  if (many)
+    jobs.of[1] = transpose_job(a, lda, ws + p.at, groups * rp, R, K, rp, half ? kTailHigh : 2, half ? kTailLow : 0);
   int rc = transpose(jobs, s);
   if (rc != LORA_OK) return rc;
   const void* ap = a;
   int64_t lda_p = lda;
-  if (p.few && (lda % 8 != 0 || !mx_aligned(a, 16))) {
+  if (p.few && (half || lda % 8 != 0 || !mx_aligned(a, 16))) {
     lda_p = up(K, 8);
     ap = ws + p.at;
-    rc = mx_widen_launch(a, lda, ws + p.at, R, K, lda_p, s);
+    rc = half ? split_rows(a, lda, ws + p.at, R, K, lda_p, s) : mx_widen_launch(a, lda, ws + p.at, R, K, lda_p, s);
     if (rc != LORA_OK) return rc;
   }
-  if (dx != nullptr && !p.few) {
+  if (many) {
     rc = mx_dequantize_launch(w_codes, w_scales, ws + p.wt, np, N, K, w_fmt, pow2, 2, dtype, s);
     if (rc != LORA_OK) return rc;
   }
@@ -204,6 +255,7 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   gr.C = N;
   gr.R = R;
   gr.factor = z_scale;
+  gr.parts = 2;
 
   MxShrinkOperands sh = {};
   sh.v = dyp;
@@ -218,13 +270,14 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   sh.tickets = ws;
   sh.part = ws + kCounterBytes;
   sh.ldv = ldp;
-  sh.ldz = 2 * rp;
+  sh.ldz = groups * rp;
+  sh.groups = groups;
   sh.M = M;
   sh.K = N;
   sh.R = R;
   sh.scale = scale / m;
   sh.global_scale = 1.f;
-  if (wide) {
+  if (p.wide) {
     if (rp != R && cudaMemsetAsync(ws + p.g, 0, static_cast<size_t>(M) * 2 * rp * 2, s) != cudaSuccess)
       return LORA_ERR_CUDA;
     rc = lora_gemm_ex(dyp, ldp, ws + p.bt, np, nullptr, 0, nullptr, 0, nullptr, ws + p.g, 2 * rp, M, R, np, 0, scale / m,
@@ -239,6 +292,8 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   ga.v = x_codes;
   ga.v_scales = x_scales;
   ga.p = ws + p.g;
+  ga.ldp = groups * rp;
+  ga.parts = p.parts;
   ga.out = da;
   ga.ldo = ldda;
   ga.part = ws + p.part_a;
@@ -257,9 +312,10 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
     o.w_codes = w_codes;
     o.w_scales = w_scales;
     o.g = ws + p.g;
-    o.ldg = 2 * rp;
-    o.g_lo = rp;
+    o.ldg = groups * rp;
+    o.r16 = rp;
     o.a = ap;
+    if (half) o.a_lo = ws + p.at + R * lda_p * 2;
     o.lda = lda_p;
     o.dx = dx;
     o.lddx = lddx;
@@ -271,6 +327,7 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
     o.pow2 = pow2;
     return mx_dx_launch(o, w_fmt, dtype, s);
   }
-  return lora_gemm_ex(dyp, ldp, ws + p.wt, np, ws + p.g, 2 * rp, ws + p.at, 2 * rp, nullptr, dx, lddx, M, K, np, 2 * rp,
-                      m, 0, dtype, p.gemm_bytes ? ws : nullptr, p.gemm_bytes, s);
+  const int64_t tail = groups * rp;
+  return gemm_mixed_tail(dyp, ldp, ws + p.wt, np, ws + p.g, tail, ws + p.at, tail, dx, lddx, M, K, np, tail, m, dtype,
+                         LORA_BF16, p.gemm_bytes ? ws : nullptr, p.gemm_bytes, s);
 }

@@ -1,6 +1,6 @@
 // Input gradient of the 4-bit LoRA linear for few rows of dy.
 //
-//   dx[t, k] = alpha (sum_n dy[t,n] Wv[n,k] + sum_j (gh + gl)[t,j] A[j,k])
+//   dx[t, k] = alpha (sum_n dy[t,n] Wv[n,k] + sum_j g[t,j] A[j,k])
 //
 // The contraction runs down W's rows, against the direction of its scale blocks, so
 // the block-scaled MMAs do not apply; nor does a decoded copy of W pay for few rows
@@ -10,7 +10,9 @@
 // the MMA's 128-wide operand -- 64-column chunks, token rows 128 bytes apart, the
 // 128-byte swizzle -- so the transposition is the MMA's; dy's tile, 16..256 tokens, is
 // the other operand.  A's rows, as they lie in memory, have that layout by TMA alone:
-// they follow as the last stages, against gh and then gl.
+// they follow as the last stages, against the hi and then the lo part of g.  For fp16
+// these stages are bf16 (g may lie outside fp16's range): A = Ah + Al exactly, g in three
+// parts, and the products gh Ah, gm Ah, gl Ah, gh Al, gm Al; gl Al is below 2^-24 of g A.
 //
 // A code becomes a value in four instructions a pair: E2M1 to f16 by the converter,
 // f16's exponent moved into bf16's place (a factor 2^-112, folded into the scale), one
@@ -49,13 +51,13 @@ template <int NB> __host__ __device__ constexpr int dx_groups() { return NB >= 1
 template <int NB> __host__ __device__ constexpr int dx_threads() { return 64 + 32 * kDxGroupWarps * dx_groups<NB>(); }
 
 struct DxMaps {
-  CUtensorMap x, w, sw, gh, gl, a;
+  CUtensorMap x, w, sw, g, a, al;
 };
 
 struct DxArgs {
   MxTileOut tile;
   int* err;
-  int num_kb, last_step, rank_kb, last_k16, gb, stages;
+  int num_kb, last_step, rank_kb, last_k16, r16, gb, stages;
   float pow2;
 };
 
@@ -138,6 +140,8 @@ __global__ void __launch_bounds__(dx_threads<NB>(), dx_ctas<NB>())
   // M = 128, W's operand MN-major (bit 15)
   constexpr uint32_t kIdesc =
       (1u << 4) | (kAb << 7) | (kAb << 10) | (1u << 15) | (static_cast<uint32_t>(NB >> 3) << 17) | (8u << 24);
+  constexpr uint32_t kIdescTail = kIdesc | (1u << 7) | (1u << 10);
+  constexpr int kTails = kAb ? 2 : 5;  // products of g's parts and A's
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -158,7 +162,7 @@ __global__ void __launch_bounds__(dx_threads<NB>(), dx_ctas<NB>())
   const int t0 = static_cast<int>(blockIdx.y) * NB;
   const int kb0 = args.num_kb * rank / splits, base = args.num_kb * (rank + 1) / splits - kb0;
   // the adapter's stages follow the first rank's
-  const int total = base + (rank == 0 ? 2 * args.rank_kb : 0);
+  const int total = base + (rank == 0 ? kTails * args.rank_kb : 0);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < args.stages; ++s) {
@@ -190,10 +194,11 @@ __global__ void __launch_bounds__(dx_threads<NB>(), dx_ctas<NB>())
           tma_load_2d(&maps.w, at + L::kRawOffset, &full_w[stage], k0 / 2, n);
           tma_load_2d(&maps.sw, at + L::kSfOffset, &full_w[stage], 0, (n >> 7) * args.gb + (k0 >> 7) * L::kChunks);
         } else {
-          const int t = i - base, j = (t >= args.rank_kb ? t - args.rank_kb : t) * kDxRows;
+          const int tail = (i - base) / args.rank_kb, j = ((i - base) % args.rank_kb) * kDxRows;
+          const CUtensorMap* a = tail < 3 ? &maps.a : &maps.al;
           mbar_arrive_expect_tx(&full_w[stage], kDxW);
-          tma_load_2d(&maps.a, at, &full_w[stage], k0, j);
-          tma_load_2d(&maps.a, at + kDxHalf, &full_w[stage], k0 + 64, j);
+          tma_load_2d(a, at, &full_w[stage], k0, j);
+          tma_load_2d(a, at + kDxHalf, &full_w[stage], k0 + 64, j);
         }
       };
       auto rows = [&](int i, int stage) {
@@ -202,9 +207,9 @@ __global__ void __launch_bounds__(dx_threads<NB>(), dx_ctas<NB>())
         if (i < base) {
           tma_load_2d(&maps.x, at, &full_x[stage], (kb0 + i) * kDxRows, t0);
         } else {
-          const int t = i - base;
-          const bool lo = t >= args.rank_kb;
-          tma_load_2d(lo ? &maps.gl : &maps.gh, at, &full_x[stage], (lo ? t - args.rank_kb : t) * 64, t0);
+          // (columns beyond a part's, the next part's, meet rows of zeros)
+          const int tail = (i - base) / args.rank_kb, c = (i - base) % args.rank_kb;
+          tma_load_2d(&maps.g, at, &full_x[stage], (tail < 3 ? tail : tail - 3) * args.r16 + c * 64, t0);
         }
       };
       const int pre = min(total, args.stages);
@@ -239,15 +244,15 @@ __global__ void __launch_bounds__(dx_threads<NB>(), dx_ctas<NB>())
       }
       tc_fence_after();
       const uint32_t at = static_cast<uint32_t>(stage * (L::kStage >> 4));
-      const int t = i - base;
       const int nk = i < base ? (kb0 + i == args.num_kb - 1 ? args.last_step : 4)
-                              : ((t >= args.rank_kb ? t - args.rank_kb : t) == args.rank_kb - 1 ? args.last_k16 : 4);
+                              : ((i - base) % args.rank_kb == args.rank_kb - 1 ? args.last_k16 : 4);
+      const uint32_t idesc = i < base ? kIdesc : kIdescTail;
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           if (k < nk)
             tc_mma_f16(tmem, wd0 + at + static_cast<uint32_t>((k * 16 * 128) >> 4), xd0 + at + static_cast<uint32_t>(2 * k),
-                       kIdesc, (i > 0 || k > 0) ? 1u : 0u);
+                       idesc, (i > 0 || k > 0) ? 1u : 0u);
         tc_commit(&empty[stage]);
       }
       __syncwarp();
@@ -329,14 +334,15 @@ int launch_dx(const MxDxOperands& o, cudaStream_t stream) {
   DxMaps maps;
   DxArgs a;
   const int64_t pitch = mx_code_pitch(o.K, FMT);
-  const char* g = static_cast<const char*>(o.g);
   a.gb = static_cast<int>(mx_scale_chunks(o.K, FMT));
   if (!mx_encode_map(&maps.x, o.dy, 2, o.N, o.M, o.lddy * 2, 64, NB, true) ||
       !mx_encode_map(&maps.w, o.w_codes, 1, pitch, o.N, pitch, 64, kDxRows, false) ||
       !mx_encode_map(&maps.sw, o.w_scales, 4, 128, (o.N + 127) / 128 * a.gb, 512, 128, L::kChunks, false) ||
-      !mx_encode_map(&maps.gh, g, 2, o.R, o.M, o.ldg * 2, 64, NB, true) ||
-      !mx_encode_map(&maps.gl, g + o.g_lo * 2, 2, o.R, o.M, o.ldg * 2, 64, NB, true) ||
+      !mx_encode_map(&maps.g, o.g, 2, o.ldg, o.M, o.ldg * 2, 64, NB, true) ||
       !mx_encode_map(&maps.a, o.a, 2, o.K, o.R, o.lda * 2, 64, kDxRows, true))
+    return LORA_ERR_CUDA;
+  maps.al = maps.a;
+  if (o.a_lo != nullptr && !mx_encode_map(&maps.al, o.a_lo, 2, o.K, o.R, o.lda * 2, 64, kDxRows, true))
     return LORA_ERR_CUDA;
   a.tile = {o.dx, nullptr, o.lddx, static_cast<int>(o.M), static_cast<int>(o.K), o.alpha, 1.f};
   a.err = info.err_word;
@@ -344,6 +350,7 @@ int launch_dx(const MxDxOperands& o, cudaStream_t stream) {
   a.last_step = static_cast<int>((o.N - (a.num_kb - 1) * 64ll + 15) / 16);
   a.rank_kb = static_cast<int>((o.R + 63) / 64);
   a.last_k16 = static_cast<int>((o.R - (a.rank_kb - 1) * 64ll + 15) / 16);
+  a.r16 = static_cast<int>(o.r16);
   a.pow2 = o.pow2;
   constexpr int kFixed = 1024 + 512;
   // a stage always goes to the same group: a warp that waits for a stage's next tile has

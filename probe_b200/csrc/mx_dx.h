@@ -5,12 +5,13 @@
 
 namespace lora {
 
-// dx[t, k] = alpha (sum_n dy[t, n] Wv[n, k] + sum_j (gh + gl)[t, j] A[j, k]), Wv the
-// values of the 4-bit W [N, K] times pow2.
+// dx[t, k] = alpha (sum_n dy[t, n] Wv[n, k] + sum_j g[t, j] A[j, k]), Wv the values of the
+// 4-bit W [N, K] times pow2.  bf16: g is the pair [hi | lo].  fp16: g [hi | mid | lo] and
+// A = a + a_lo are sums of bf16 parts.
 struct MxDxOperands {
-  const void *dy, *w_codes, *w_scales, *g, *a;  // dy [M, lddy], rows of 16 bytes; a [R, lda], likewise
+  const void *dy, *w_codes, *w_scales, *g, *a, *a_lo;  // dy [M, lddy], rows of 16 bytes; a [R, lda], likewise
   void* dx;
-  int64_t lddy, ldg, g_lo, lda, lddx, M, N, K, R;
+  int64_t lddy, ldg, r16, lda, lddx, M, N, K, R;
   float alpha, pow2;
 };
 

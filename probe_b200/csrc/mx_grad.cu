@@ -22,7 +22,9 @@
 // instead of 4.0 + 7.8 with waits).
 // P is the whole hi/lo pair.  Up to rank 128 its halves lie side by side in one MMA (N = 2 r)
 // and are added in the epilogue; above, they meet V one after the other in the same
-// accumulator, from stages of half as many tokens.  The hi half alone would take 145 us at
+// accumulator, from stages of half as many tokens.  dA of fp16 activations is computed in
+// bf16, where X is exact too, with g in three parts: a gradient beside a B that has just
+// left zero lies below fp16's range, a scaled loss's beyond it.  The hi half alone would take 145 us at
 // r = 224, but its rounding is as large as that of the 16-bit result.
 #include <mutex>
 
@@ -53,7 +55,7 @@ struct GrArgs {
   float* part;  // [splits][C][ldp]
   int* err;
   int64_t C;
-  int M, r16;
+  int M, r16, parts;
   int n, passes, p_chunks;  // N of an MMA; the runs of P that meet V in turn, 64-column chunks of each
   int stages, stage_bytes, steps_per_split, steps, splits, scale_gb;
 };
@@ -76,11 +78,8 @@ LORA_DEVINL uint32_t gr_mul_bf16x2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Eight E4M3 codes times their scale 2^(s - 127), as 16-bit values in order.
-template <typename T>
-LORA_DEVINL uint4 gr_decode8(uint2 w, uint32_t s);
-template <>
-LORA_DEVINL uint4 gr_decode8<__nv_bfloat16>(uint2 w, uint32_t s) {
+// Eight E4M3 codes times their scale 2^(s - 127), as bf16 values in order.
+LORA_DEVINL uint4 gr_decode8(uint2 w, uint32_t s) {
   // two codes in the high bytes of each half: exponent and mantissa moved into
   // bf16's place are 2^-120 of the code's value
   const uint32_t p[4] = {__byte_perm(w.x, 0, 0x1404), __byte_perm(w.x, 0, 0x3424), __byte_perm(w.y, 0, 0x1404),
@@ -95,19 +94,6 @@ LORA_DEVINL uint4 gr_decode8<__nv_bfloat16>(uint2 w, uint32_t s) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       o[i] = gr_mul_bf16x2(gr_mul_bf16x2((p[i] & 0x80008000u) | ((p[i] >> 4) & 0x07f007f0u), 0x7b807b80u), f);
-  }
-  return make_uint4(o[0], o[1], o[2], o[3]);
-}
-template <>
-LORA_DEVINL uint4 gr_decode8<__half>(uint2 w, uint32_t s) {
-  const float scale = mx_e8m0(s);
-  const uint32_t c[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
-  uint32_t o[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t h = mx_from_e4m3x2(c[i]);
-    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    o[i] = pack2<__half>(v.x * scale, v.y * scale);
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
@@ -254,7 +240,7 @@ LORA_DEVINL void gr_job(const GrMaps& maps, const GrArgs& args, int group, int s
           const int tr = (st * TOK + t) & 127;  // row within the scale chunk
           const uint2 w = lds64(raw + t * kGrCols + lane * 8);
           const uint32_t s = lds_u8(sc + (tr & 31) * 16 + (tr >> 5) * 4);
-          sts128(dst + t * 128 + (((lane & 7) ^ (t & 7)) << 4), gr_decode8<T>(w, s));
+          sts128(dst + t * 128 + (((lane & 7) ^ (t & 7)) << 4), gr_decode8(w, s));
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -275,9 +261,10 @@ LORA_DEVINL void gr_job(const GrMaps& maps, const GrArgs& args, int group, int s
         const uint32_t src = tmem + (static_cast<uint32_t>(quad * 32) << 16) + m * args.n + j;
         uint32_t r[16], lo[16];
         tmem_ld_32x32b_x16(src, r);
-        if (args.passes == 1) tmem_ld_32x32b_x16(src + args.r16, lo);
         tmem_wait_ld();
-        if (args.passes == 1) {
+        for (int i = args.passes; i < args.parts; ++i) {  // (passes is 1 or parts)
+          tmem_ld_32x32b_x16(src + i * args.r16, lo);
+          tmem_wait_ld();
 #pragma unroll
           for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) + __uint_as_float(lo[e]));
         }
@@ -311,7 +298,7 @@ __global__ void __launch_bounds__(kGrThreads, 1) mx_grad_kernel(const __grid_con
     gr_job<T, false, TOK>(jobs.maps[0], jobs.args[0], b % jobs.groups[0], b / jobs.groups[0]);
   } else {
     const int c = b - jobs.blocks0;
-    gr_job<T, true, TOK>(jobs.maps[1], jobs.args[1], c % jobs.groups[1], c / jobs.groups[1]);
+    gr_job<__nv_bfloat16, true, TOK>(jobs.maps[1], jobs.args[1], c % jobs.groups[1], c / jobs.groups[1]);
   }
 }
 
@@ -372,12 +359,11 @@ struct GrPlan {
   int groups, steps, splits, steps_per_split;
 };
 
-// Tokens a stage: half of the usual ones where both halves of P do not fit one MMA, so
+// Tokens a stage: half of the usual ones where dA's parts of P do not fit one MMA, so
 // that three stages or more of them fit beside the decoded tiles.
-int grad_tokens(int64_t R) { return 2 * ((R + 15) / 16 * 16) > kGrMaxN ? 32 : 64; }
+int grad_tokens(int64_t R, int parts) { return parts * ((R + 15) / 16 * 16) > kGrMaxN ? 32 : 64; }
 
-GrPlan grad_plan(int64_t M, int64_t C, int64_t R) {
-  const int tok = grad_tokens(R);
+GrPlan grad_plan(int64_t M, int64_t C, int tok) {
   GrPlan p;
   const int dev = current_device();
   const int sms = dev >= 0 ? device_info(dev).num_sms : 148;
@@ -398,9 +384,10 @@ bool fill_job(const MxGradOperands& g, const GrPlan& pl, bool f8, int* err, GrMa
   a->C = g.C;
   a->M = static_cast<int>(g.M);
   a->r16 = static_cast<int>((g.R + 15) / 16 * 16);
-  // [hi | lo] side by side in one MMA, or one after the other
-  a->passes = 2 * a->r16 > kGrMaxN ? 2 : 1;
-  a->n = a->passes == 1 ? 2 * a->r16 : a->r16;
+  // the parts side by side in one MMA, or one after the other
+  a->parts = g.parts;
+  a->passes = g.parts * a->r16 > kGrMaxN ? g.parts : 1;
+  a->n = a->passes == 1 ? g.parts * a->r16 : a->r16;
   a->p_chunks = (a->n + 63) / 64;
   a->steps = pl.steps;
   a->splits = pl.splits;
@@ -420,7 +407,7 @@ bool fill_job(const MxGradOperands& g, const GrPlan& pl, bool f8, int* err, GrMa
     if (!mx_encode_map(&maps->v, g.v, 2, g.C, g.M, g.ldv * 2, 64, TOK, true)) return false;
     maps->sc = maps->v;
   }
-  return mx_encode_map(&maps->p, g.p, 2, 2 * a->r16, g.M, g.ldp * 2, 64, TOK, true);
+  return mx_encode_map(&maps->p, g.p, 2, g.parts * a->r16, g.M, g.ldp * 2, 64, TOK, true);
 }
 
 template <typename T, int TOK>
@@ -432,7 +419,7 @@ int launch_grads(const MxGradOperands* g, cudaStream_t stream) {
   size_t smem = 0;
   int blocks = 0;
   for (int i = 0; i < 2; ++i) {
-    const GrPlan pl = grad_plan(g[i].M, g[i].C, g[i].R);
+    const GrPlan pl = grad_plan(g[i].M, g[i].C, TOK);
     if (!fill_job<TOK>(g[i], pl, i == 1, info.err_word, &jobs.maps[i], &jobs.args[i], &smem)) return LORA_ERR_CUDA;
     jobs.groups[i] = pl.groups;
     if (i == 1) jobs.blocks0 = blocks;
@@ -450,17 +437,18 @@ int launch_grads(const MxGradOperands* g, cudaStream_t stream) {
 
 }  // namespace
 
-size_t mx_grad_part_bytes(int64_t M, int64_t C, int64_t R) {
-  return static_cast<size_t>(grad_plan(M, C, R).splits) * C * ((R + 15) / 16 * 16) * sizeof(float);
+size_t mx_grad_part_bytes(int64_t M, int64_t C, int64_t R, int parts) {
+  return static_cast<size_t>(grad_plan(M, C, grad_tokens(R, parts)).splits) * C * ((R + 15) / 16 * 16) * sizeof(float);
 }
 
 int mx_grad_launch(const MxGradOperands* g, int dtype, cudaStream_t stream) {
-  if (grad_tokens(g[0].R) == 32)
+  if (grad_tokens(g[1].R, g[1].parts) == 32)
     return dtype == LORA_BF16 ? launch_grads<__nv_bfloat16, 32>(g, stream) : launch_grads<__half, 32>(g, stream);
   return dtype == LORA_BF16 ? launch_grads<__nv_bfloat16, 64>(g, stream) : launch_grads<__half, 64>(g, stream);
 }
 
 int mx_grad_reduce_launch(const MxGradOperands* g, int dtype, cudaStream_t stream) {
+  const int tok = grad_tokens(g[1].R, g[1].parts);
   GrSums sums = {};
   int blocks = 0, r32 = 0;
   for (int i = 0; i < 2; ++i) {
@@ -471,7 +459,7 @@ int mx_grad_reduce_launch(const MxGradOperands* g, int dtype, cudaStream_t strea
     s.C = g[i].C;
     s.r = static_cast<int>(g[i].R);
     s.r16 = (s.r + 15) / 16 * 16;
-    s.splits = grad_plan(g[i].M, g[i].C, g[i].R).splits;
+    s.splits = grad_plan(g[i].M, g[i].C, tok).splits;
     s.blocks = static_cast<int>((g[i].C + 31) / 32);
     s.factor = g[i].factor;
     s.transposed = g[i].transposed;

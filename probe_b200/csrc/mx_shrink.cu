@@ -3,6 +3,8 @@
 //
 //   z [M, 2 r16] = [hi | lo], hi = round(z), lo = round(z - hi)
 //
+// (without a format, of fp16 operands: bf16 parts [hi | mid | lo], whose range is fp32's)
+//
 // A is [R, K] (rows along K, an adapter's down projection) or, for gradients,
 // [K, R] (an up projection, multiplied from the other side); tcgen05 takes either
 // as the N operand, K-major or MN-major, with 128 tokens as M.  While the MMAs of
@@ -50,6 +52,7 @@ struct ShArgs {
   int64_t M, K, Kp, ldz;
   int chunks_total;
   int kc, r16, a_boxes, a_box_bytes, stages, stage_bytes, gb;
+  int groups;   // of r16 columns of a three-part result
   int cluster;  // CTAs of a token block's cluster; 0: runs
   int group_shift;  // log2 of the warps of a group, which takes 16 rows a warp
   float scale;
@@ -89,9 +92,46 @@ LORA_DEVINL void sh_store_pair(T* z, int r16, const float* v) {
   d[1] = make_uint4(l[4], l[5], l[6], l[7]);
 }
 
+// N values as bf16 parts, v = hi + mid + lo to 24 bits, `groups` groups of columns.
+template <int N>
+LORA_DEVINL void sh_store_three(uint16_t* z, int r16, int groups, const float* v) {
+  using B = __nv_bfloat16;
+  uint32_t p[3][N / 2];
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    float2 rest = make_float2(v[2 * i], v[2 * i + 1]);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      p[k][i] = pack2<B>(rest.x, rest.y);
+      const float2 f = unpack2<B>(p[k][i]);
+      rest.x -= f.x, rest.y -= f.y;
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < 5; ++g) {
+    if (g >= groups) break;
+    const uint32_t* w = p[g % 3];
+    if constexpr (N == 4) {
+      *reinterpret_cast<uint2*>(z + g * r16) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 8; ++i)
+        reinterpret_cast<uint4*>(z + g * r16)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    }
+  }
+}
+
 template <typename T, int FMT, bool AMN, int KB>
 __global__ void __launch_bounds__(kShThreads, 1)
     mx_shrink_kernel(const __grid_constant__ ShMaps maps, const ShArgs args) {
+  // the gradient g of fp16 activations, which leaves fp16's range on either side
+  constexpr bool kThree = FMT == kNoFormat && std::is_same<T, __half>::value;
+  auto store16 = [&](T* z, const float* v) {
+    if constexpr (kThree)
+      sh_store_three<16>(reinterpret_cast<uint16_t*>(z), args.r16, args.groups, v);
+    else
+      sh_store_pair<T>(z, args.r16, v);
+  };
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -316,7 +356,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
           float v[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(u[e]) * args.scale;
-          sh_store_pair<T>(zrow + j, args.r16, v);
+          store16(zrow + j, v);
         } else {
           st_global_v8(slot + j, u);
           st_global_v8(slot + j + 8, u + 8);
@@ -377,7 +417,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[8 * h + e] = acc[e] * args.scale;
               }
-              sh_store_pair<T>(zrow + j, args.r16, v);
+              store16(zrow + j, v);
             }
         }
       }
@@ -418,6 +458,11 @@ __global__ void __launch_bounds__(kShThreads, 1)
         if (q < args.cluster) v.x += p[q].x, v.y += p[q].y, v.z += p[q].z, v.w += p[q].w;
       v.x *= args.scale, v.y *= args.scale, v.z *= args.scale, v.w *= args.scale;
       T* z = static_cast<T*>(args.z) + (row0 + r) * args.ldz + j;
+      if constexpr (kThree) {
+        const float f[4] = {v.x, v.y, v.z, v.w};
+        sh_store_three<4>(reinterpret_cast<uint16_t*>(z), args.r16, args.groups, f);
+        continue;
+      }
       const uint2 h = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
       const float2 h0 = unpack2<T>(h.x), h1 = unpack2<T>(h.y);
       *reinterpret_cast<uint2*>(z) = h;
@@ -481,6 +526,7 @@ int launch_shrink(const MxShrinkOperands& o, cudaStream_t stream) {
   a.K = o.K;
   a.Kp = mx_padded_k(o.K);
   a.ldz = o.ldz;
+  a.groups = o.groups;
   a.kc = static_cast<int>((o.K + 64 * KB - 1) / (64 * KB));
   a.chunks_total = static_cast<int>((o.M + 127) / 128 * a.kc);
   a.stage_bytes = KB * kShBoxBytes + a.a_boxes * a.a_box_bytes;

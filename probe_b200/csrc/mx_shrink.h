@@ -9,7 +9,10 @@ struct MxShrinkOperands {
   const void* v;  // [M, K], ldv
   const void* a;  // [R, K] or, a_mn, [K, R]
   bool a_mn;
-  void* z;                // [M, ldz]: hi at column 0, lo at r16
+  // [M, ldz]: hi at column 0, lo at r16.  fmt -1 of fp16 operands: `groups` columns groups of
+  // bf16, r16 wide, the parts of an exact sum of three (3) and the first two again (5)
+  void* z;
+  int groups;
   void *codes, *scales;   // of v in the format, where one is asked for
   void *part, *tickets;   // mx_shrink_part_bytes; the zeroed ticket region
   int64_t ldv, lda, ldz, M, K, R;
