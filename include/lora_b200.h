@@ -414,9 +414,17 @@ LORA_API int lora_mx_linear(const void* x, int64_t ldx, const void* w_codes, con
  * in a fixed order.  1 <= R <= 256; z, codes and scales 16-byte aligned.  M or N 0:
  * the outputs are zeros; K 0: LORA_ERR_UNSUPPORTED, as the forward pass.
  * Workspace: lora_mx_backward_workspace_size bytes, 256-byte aligned, zeroed
- * ticket region first as lora_shrink's.  No counterpart in the reference, which
+ * ticket region first as lora_shrink's.  Its flags: LORA_MX_NEED_DX where dx is
+ * asked for; the others, each a promise, leave out room that the call then does not
+ * need (a copy of dy, M x N, or of b).  No counterpart in the reference, which
  * has no backward pass. */
-LORA_API size_t lora_mx_backward_workspace_size(int64_t M, int64_t N, int64_t K, int64_t R, int need_dx);
+enum lora_mx_backward_flags {
+  LORA_MX_NEED_DX = 1,
+  LORA_MX_DY_ALIGNED = 2, /* dy starts on 16 bytes, lddy is a multiple of 8 */
+  LORA_MX_B_ALIGNED = 4,  /* b and ldb likewise                             */
+  LORA_MX_ONLY_BF16 = 8   /* dtype is LORA_BF16                             */
+};
+LORA_API size_t lora_mx_backward_workspace_size(int64_t M, int64_t N, int64_t K, int64_t R, int flags);
 LORA_API int lora_mx_backward(const void* dy, int64_t lddy, const void* x_codes, const void* x_scales, const void* z,
                      float z_scale, const void* a, int64_t lda, const void* b, int64_t ldb,
                      const void* w_codes, const void* w_scales, float w_global, int w_fmt, void* dx,

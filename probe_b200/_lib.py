@@ -39,6 +39,11 @@ LORA_MXFP4 = 0
 LORA_NVFP4 = 1
 LORA_MXFP8 = 2
 
+LORA_MX_NEED_DX = 1
+LORA_MX_DY_ALIGNED = 2
+LORA_MX_B_ALIGNED = 4
+LORA_MX_ONLY_BF16 = 8
+
 LORA_B_PEFT = 0
 LORA_B_RANK_MAJOR = 1
 

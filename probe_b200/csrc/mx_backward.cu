@@ -41,7 +41,8 @@ struct BackwardPlan {
   size_t gemm_bytes, part, part_a, g, bt, at, dy, wt, total;
 };
 
-BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need_dx, bool half) {
+// dy_rows, b_rows: TMA can read dy, b where they lie.
+BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need_dx, bool half, bool dy_rows, bool b_rows) {
   BackwardPlan p = {};
   const int64_t np = up(N, 8), rp = up(R, 16);
   const int dev = current_device();
@@ -62,12 +63,12 @@ BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need
   p.g = at;
   at += mx_align(static_cast<size_t>(M) * tail * 2);
   p.bt = at;
-  at += mx_align(static_cast<size_t>(R) * np * 2);
+  if (p.wide || !b_rows) at += mx_align(static_cast<size_t>(R) * np * 2);
   p.at = at;
   if (many) at += mx_align(static_cast<size_t>(K) * tail * 2);
   if (p.few) at += mx_align(static_cast<size_t>(R) * up(K, 8) * (half ? 4 : 2));
   p.dy = at;
-  at += mx_align(static_cast<size_t>(M) * np * 2);
+  if (!dy_rows) at += mx_align(static_cast<size_t>(M) * np * 2);
   p.wt = at;
   if (many) at += mx_align(static_cast<size_t>(K) * np * 2);
   p.total = at;
@@ -161,10 +162,13 @@ int split_rows(const void* in, int64_t ldi, void* out, int64_t rows, int64_t col
 
 using namespace lora;
 
-extern "C" size_t lora_mx_backward_workspace_size(int64_t M, int64_t N, int64_t K, int64_t R, int need_dx) {
+extern "C" size_t lora_mx_backward_workspace_size(int64_t M, int64_t N, int64_t K, int64_t R, int flags) {
   if (M <= 0 || N <= 0 || K <= 0 || R <= 0) return 0;
-  return std::max(backward_plan(M, N, K, R, need_dx != 0, false).total,
-                  backward_plan(M, N, K, R, need_dx != 0, true).total);
+  const bool dx = (flags & LORA_MX_NEED_DX) != 0;
+  const bool dy_rows = (flags & LORA_MX_DY_ALIGNED) != 0 && N % 8 == 0, b_rows = (flags & LORA_MX_B_ALIGNED) != 0;
+  const size_t bf16 = backward_plan(M, N, K, R, dx, false, dy_rows, b_rows).total;
+  if (flags & LORA_MX_ONLY_BF16) return bf16;
+  return std::max(bf16, backward_plan(M, N, K, R, dx, true, dy_rows, b_rows).total);
 }
 
 extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_codes, const void* x_scales, const void* z,
@@ -199,7 +203,9 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
     return LORA_OK;
   }
   const bool half = dtype == LORA_F16;
-  const BackwardPlan p = backward_plan(M, N, K, R, dx != nullptr, half);
+  const bool dy_rows = N % 8 == 0 && lddy % 8 == 0 && mx_aligned(dy, 16);
+  const bool b_rows = mx_aligned(b, 16) && ldb % 8 == 0;
+  const BackwardPlan p = backward_plan(M, N, K, R, dx != nullptr, half, dy_rows, b_rows);
   if (workspace == nullptr || workspace_bytes < p.total) return LORA_ERR_WORKSPACE;
   char* ws = static_cast<char*>(workspace);
   const int64_t np = up(N, 8), rp = up(R, 16);
@@ -214,7 +220,6 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   // What the weights give comes first: a kernel that reads it may start before its own
   // predecessor on the stream has finished, so other launches lie between.
   TransposeJobs jobs = {};
-  const bool b_rows = mx_aligned(b, 16) && ldb % 8 == 0;  // TMA can read them
   const bool many = dx != nullptr && !p.few;
   const int groups = p.groups;
   if (!b_rows || p.wide) jobs.of[0] = transpose_job(b, ldb, ws + p.bt, np, N, R, np, 1, 0);
@@ -236,7 +241,7 @@ extern "C" int lora_mx_backward(const void* dy, int64_t lddy, const void* x_code
   }
   const void* dyp = dy;
   int64_t ldp = lddy;
-  if (N % 8 != 0 || lddy % 8 != 0 || !mx_aligned(dy, 16)) {  // TMA needs 16-byte rows
+  if (!dy_rows) {
     rc = mx_widen_launch(dy, lddy, ws + p.dy, M, N, np, s);
     if (rc != LORA_OK) return rc;
     dyp = ws + p.dy;

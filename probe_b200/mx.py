@@ -49,8 +49,8 @@ def _linear_bytes(m, n, k, r, code):
 
 
 @functools.lru_cache(maxsize=4096)
-def _backward_bytes(m, n, k, r, need_dx):
-    return _entry("lora_mx_backward_workspace_size")(m, n, k, r, need_dx)
+def _backward_bytes(m, n, k, r, flags):
+    return _entry("lora_mx_backward_workspace_size")(m, n, k, r, flags)
 
 
 def _need_cuda(where, *tensors):
@@ -314,14 +314,21 @@ def mx_lora_backward(dy: torch.Tensor, x8: MXTensor, z: torch.Tensor, a: torch.T
     da, db = dy.new_empty((r, k)), dy.new_empty((n, r))
     dx = wp = sp = dxp = None
     wg, wcode = 1.0, 0
+    dyp, lddy, bp, ldb = dy.data_ptr(), _ld(dy), b.data_ptr(), _ld(b)
+    flags = _lib.LORA_MX_ONLY_BF16 if dtype == torch.bfloat16 else 0
+    if (dyp | 2 * lddy) & 15 == 0:
+        flags |= _lib.LORA_MX_DY_ALIGNED
+    if (bp | 2 * ldb) & 15 == 0:
+        flags |= _lib.LORA_MX_B_ALIGNED
     if weight is not None:
+        flags |= _lib.LORA_MX_NEED_DX
         dx = dy.new_empty((m, k))
         dxp = dx.data_ptr()
         wp, sp, wg, wcode = wc.data_ptr(), weight.scales.data_ptr(), weight.global_scale, weight._code
     stream = _raw_stream(device.index)
-    ws = _lib.WORKSPACE.get(_backward_bytes(m, n, k, r, int(dx is not None)), device, "mx_backward", stream)
-    rc = _entry("lora_mx_backward")(dy.data_ptr(), _ld(dy), x8.codes.data_ptr(), x8.scales.data_ptr(), z.data_ptr(),
-                                    float(z_scale), a.data_ptr(), _ld(a), b.data_ptr(), _ld(b), wp, sp, wg, wcode,
+    ws = _lib.WORKSPACE.get(_backward_bytes(m, n, k, r, flags), device, "mx_backward", stream)
+    rc = _entry("lora_mx_backward")(dyp, lddy, x8.codes.data_ptr(), x8.scales.data_ptr(), z.data_ptr(),
+                                    float(z_scale), a.data_ptr(), _ld(a), bp, ldb, wp, sp, wg, wcode,
                                     dxp, k, da.data_ptr(), k, db.data_ptr(), r, m, n, k, r, float(scale), dt,
                                     ws.data_ptr(), ws.numel(), stream)
     if rc:

@@ -60,3 +60,21 @@ def test_cpu_tensors_raise():
 
 def test_global_scale_of_a_zero_tensor_is_usable():
     assert mx.nvfp4_global_scale(0.0) > 2.0 ** -64
+
+
+@pytest.mark.parametrize("m,n,k,r", [(32760, 5120, 5120, 224), (256, 4096, 4096, 16), (4097, 11008, 4096, 20)])
+def test_backward_workspace_has_no_copies_of_rows_read_in_place(lib, m, n, k, r):
+    size = lambda flags: lib.lora_mx_backward_workspace_size(m, n, k, r, flags)  # noqa: E731
+    dy, b = (-(-m * n * 2 // 256) * 256), (-(-r * n * 2 // 256) * 256)
+    for dx in (0, _lib.LORA_MX_NEED_DX):
+        bf16 = dx | _lib.LORA_MX_ONLY_BF16
+        assert size(bf16) - size(bf16 | _lib.LORA_MX_DY_ALIGNED) == dy
+        wide = r > 128 and m >= 4096  # such an adapter's g comes from B transposed
+        assert size(bf16) - size(bf16 | _lib.LORA_MX_B_ALIGNED) == (0 if wide else b)
+        assert size(dx) >= size(bf16)
+
+
+def test_backward_workspace_keeps_the_copy_of_odd_rows(lib):
+    """N no multiple of 8 is copied whatever the alignment of its first row."""
+    size = lambda flags: lib.lora_mx_backward_workspace_size(512, 4097, 256, 16, flags)  # noqa: E731
+    assert size(_lib.LORA_MX_DY_ALIGNED) == size(0)
