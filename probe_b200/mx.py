@@ -35,7 +35,8 @@ _DTYPE = {torch.float16: _lib.LORA_F16, torch.bfloat16: _lib.LORA_BF16}
 
 # A call of a few tokens takes the GPU a few microseconds: the wrappers below pass
 # plain integers to the C ABI, look the raw stream up directly and keep sizes by shape.
-_raw_stream = torch._C._cuda_getCurrentRawStream
+def _raw_stream(device_index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device_index)  # (not there in builds without CUDA)
 
 
 @functools.cache
