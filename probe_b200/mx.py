@@ -60,6 +60,18 @@ def _need_cuda(where, *tensors):
             _lib.require_cuda(t, where=where)
 
 
+def _need_one_device(where, *tensors):
+    _need_cuda(where, *tensors)
+    devices = {str(t.device) for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"{where}: operands lie on different devices ({', '.join(sorted(devices))})")
+
+
+def _elsewhere(t: torch.Tensor) -> bool:
+    """Whether the tensor lies on a GPU that is not the current one, on which kernels launch."""
+    return t.is_cuda and t.get_device() != torch._C._cuda_getDevice()
+
+
 def _format(fmt: str, where: str) -> int:
     code = _FORMATS.get(fmt)
     if code is None:
@@ -149,6 +161,9 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4", global_scale: float = 1.0) 
     and saturate; a block with an infinity or a NaN reads back as NaN.
     """
     code = _format(fmt, "mx_quantize")
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return mx_quantize(x, fmt, global_scale)
     _need_cuda("mx_quantize", x)
     x = _rows(x, "mx_quantize")
     m, k = x.shape
@@ -166,6 +181,9 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4", global_scale: float = 1.0) 
 
 def mx_dequantize(q: MXTensor, dtype: torch.dtype = torch.bfloat16, transpose: bool = False) -> torch.Tensor:
     """The values of ``q`` in ``dtype`` (rounded once), [M, K] or, transposed, [K, M]."""
+    if _elsewhere(q.codes):
+        with torch.cuda.device(q.codes.device):
+            return mx_dequantize(q, dtype, transpose)
     _need_cuda("mx_dequantize", q.codes)
     if dtype not in _HALF:
         raise TypeError(f"mx_dequantize: expected float16/bfloat16, got {dtype}")
@@ -192,7 +210,7 @@ def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
 
 def _refuse_linear(x, weight, bias, a, b, where):
     """The error of a call that ``_linear``'s one check found wrong."""
-    _need_cuda(where, x, weight.codes, bias, a, b)
+    _need_one_device(where, x, weight.codes, bias, a, b)
     n, k = weight.shape
     if weight.fmt not in ("mxfp4", "nvfp4"):
         raise ValueError(f"{where}: the weight must be in a 4-bit format, got {weight.fmt}")
@@ -211,13 +229,16 @@ def _refuse_linear(x, weight, bias, a, b, where):
 
 
 def _linear(x, weight, bias, a, b, scale, x_global_scale, keep_z, where):
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return _linear(x, weight, bias, a, b, scale, x_global_scale, keep_z, where)
     shape, dtype, codes, code = x.shape, x.dtype, weight.codes, weight._code
     n, k = weight.shape
     r = 0 if a is None or b is None or (scale == 0 and not keep_z) else a.shape[0]
-    dt = _DTYPE.get(dtype)
-    if (dt is None or code == _lib.LORA_MXFP8 or not x.is_cuda or not codes.is_cuda or shape[-1] != k
-            or (bias is not None and (not bias.is_cuda or bias.dtype != dtype or bias.shape != (n,)))
-            or (r and (r > 256 or a.dtype != dtype or b.dtype != dtype or not a.is_cuda or not b.is_cuda
+    dt, dev = _DTYPE.get(dtype), x.get_device()  # (-1: not on a GPU)
+    if (dt is None or code == _lib.LORA_MXFP8 or dev < 0 or codes.get_device() != dev or shape[-1] != k
+            or (bias is not None and (bias.get_device() != dev or bias.dtype != dtype or bias.shape != (n,)))
+            or (r and (r > 256 or a.dtype != dtype or b.dtype != dtype or a.get_device() != dev or b.get_device() != dev
                        or a.shape != (r, k) or b.shape != (n, r)))):
         _refuse_linear(x, weight, bias, a, b, where)
     if len(shape) != 2 or not x.is_contiguous():
@@ -268,7 +289,7 @@ def mx_lora_linear(x: torch.Tensor, weight: MXTensor, bias: torch.Tensor | None,
 # ------------------------------------------------------------------- training
 def _refuse_backward(dy, x8, z, a, b, weight, where):
     """The error of a call that ``mx_lora_backward``'s one check found wrong."""
-    _need_cuda(where, dy, x8.codes, z, a, b, weight.codes if weight is not None else None)
+    _need_one_device(where, dy, x8.codes, z, a, b, weight.codes if weight is not None else None)
     m, n = dy.shape
     r, k = a.shape
     if dy.dtype not in _HALF:
@@ -293,6 +314,9 @@ def mx_lora_backward(dy: torch.Tensor, x8: MXTensor, z: torch.Tensor, a: torch.T
     checkpoint of x, ``z`` the [M, 2 r16] pair [hi | lo] of the forward pass, W an mxfp4 /
     nvfp4 tensor.  W is frozen; rounding to 4 or 8 bits counts as the identity.
     """
+    if _elsewhere(dy):
+        with torch.cuda.device(dy.device):
+            return mx_lora_backward(dy, x8, z, a, b, scale, weight, z_scale)
     shape, dtype = dy.shape, dy.dtype
     wc = weight.codes if weight is not None else None
     if len(shape) != 2 or not dy.is_contiguous():
@@ -300,12 +324,14 @@ def mx_lora_backward(dy: torch.Tensor, x8: MXTensor, z: torch.Tensor, a: torch.T
         dy = _rows(dy, "mx_lora_backward")
     m, n = dy.shape
     r, k = a.shape
-    dt = _DTYPE.get(dtype)
+    dt, dev = _DTYPE.get(dtype), dy.get_device()  # (-1: not on a GPU)
     if (dt is None or x8.fmt != "mxfp8" or x8.shape != (m, k) or a.dtype != dtype or b.dtype != dtype
             or z.dtype != dtype or b.shape != (n, r) or not 1 <= r <= 256
             or z.shape != (m, 2 * ((r + 15) // 16 * 16)) or not z.is_contiguous()
-            or not (dy.is_cuda and x8.codes.is_cuda and z.is_cuda and a.is_cuda and b.is_cuda)
-            or (weight is not None and (weight._code == _lib.LORA_MXFP8 or weight.shape != (n, k) or not wc.is_cuda))):
+            or dev < 0 or x8.codes.get_device() != dev or z.get_device() != dev or a.get_device() != dev
+            or b.get_device() != dev
+            or (weight is not None and (weight._code == _lib.LORA_MXFP8 or weight.shape != (n, k)
+                                        or wc.get_device() != dev))):
         _refuse_backward(dy, x8, z, a, b, weight, "mx_lora_backward")
     if not a.is_contiguous():
         a = _lib.row_major(a)
@@ -417,10 +443,12 @@ class MXLoRALinear(torch.nn.Module):
         code, w_global_scale, x_global_scale = state.tolist()
         if code != _FORMATS[self.fmt]:
             names = {v: k for k, v in _FORMATS.items()}
-            raise RuntimeError(f"MXLoRALinear: the state is of a {names.get(int(code), code)} layer, this one is {self.fmt}")
+            raise RuntimeError(
+                f"MXLoRALinear: the state is of a {names.get(int(code), code)} layer, this one is {self.fmt}")
         self.w_global_scale, self.x_global_scale = w_global_scale, x_global_scale
 
-    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
+                              error_msgs):
         key = prefix + "_extra_state"
         if self.fmt == "mxfp4" and key not in state_dict:  # nothing to restore: both scales are 1
             state_dict = {**state_dict, key: self.get_extra_state()}
