@@ -21,6 +21,22 @@ bool pdl_enabled() {
   return on;
 }
 
+namespace {
+PFN_cuCtxGetCurrent_v4000 context_getter() {
+  static PFN_cuCtxGetCurrent_v4000 fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      return static_cast<PFN_cuCtxGetCurrent_v4000>(nullptr);
+    }
+    return reinterpret_cast<PFN_cuCtxGetCurrent_v4000>(p);
+  }();
+  return fn;
+}
+}  // namespace
+
 int current_device() {
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess) {
@@ -30,15 +46,14 @@ int current_device() {
   if (dev < 0 || dev >= kMaxDevices) return -1;
   // A host thread that has made no runtime call yet (an autograd worker whose
   // allocations all came from a cache) has no current context, and the driver's
-  // tensor-map encoder then fails: bind the device's context once per thread.
-  static thread_local uint64_t bound = 0;
-  static_assert(kMaxDevices <= 64, "one bit a device");
-  if (!(bound >> dev & 1)) {
-    if (cudaSetDevice(dev) != cudaSuccess) {
-      cudaGetLastError();
-      return -1;
-    }
-    bound |= uint64_t{1} << dev;
+  // tensor-map encoder then fails: bind the device's primary one.  A context that the
+  // caller has made current stays.
+  CUcontext ctx = nullptr;
+  const auto get = context_getter();
+  if (get == nullptr || get(&ctx) != CUDA_SUCCESS) ctx = nullptr;
+  if (ctx == nullptr && cudaSetDevice(dev) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
   }
   return dev;
 }
