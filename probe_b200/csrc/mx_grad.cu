@@ -55,7 +55,7 @@ struct GrArgs {
   float* part;  // [splits][C][ldp]
   int* err;
   int64_t C;
-  int M, r16, parts;
+  int r16, parts;
   int n, passes, p_chunks;  // N of an MMA; the runs of P that meet V in turn, 64-column chunks of each
   int stages, stage_bytes, steps_per_split, steps, splits, scale_gb;
 };
@@ -382,7 +382,6 @@ bool fill_job(const MxGradOperands& g, const GrPlan& pl, bool f8, int* err, GrMa
   a->part = static_cast<float*>(g.part);
   a->err = err;
   a->C = g.C;
-  a->M = static_cast<int>(g.M);
   a->r16 = static_cast<int>((g.R + 15) / 16 * 16);
   // the parts side by side in one MMA, or one after the other
   a->parts = g.parts;

@@ -1,5 +1,5 @@
 // Rank shrink  z = s v A^T  with, in the same pass over v, v's quantisation to a
-// microscaled format.
+// 4-bit format.
 //
 //   z [M, 2 r16] = [hi | lo], hi = round(z), lo = round(z - hi)
 //
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
                 if (lane == 0) mbar_arrive(&empty[stage]);
               }
               const int64_t col = static_cast<int64_t>(kc * KB + b) * 64 + (lane & 1) * 32;
-              uint32_t cd[8];
+              uint32_t cd[4];
               const uint32_t t0 = mx_amax16(x), t1 = mx_amax16(x + 8);
               if constexpr (FMT == LORA_NVFP4) {
                 const MxScale<T, FMT> s0(t0, args.gl, recip_addr), s1(t1, args.gl, recip_addr);
@@ -299,19 +299,12 @@ __global__ void __launch_bounds__(kShThreads, 1)
               } else {
                 const MxScale<T, FMT> s(max(t0, t1), args.gl, recip_addr);
                 mx_codes16<T, FMT>(x, s, cd);
-                mx_codes16<T, FMT>(x + 8, s, cd + (MxFormat<FMT>::kBits == 4 ? 2 : 4));
+                mx_codes16<T, FMT>(x + 8, s, cd + 2);
                 bytes |= s.byte << (16 * b);
               }
-              if (row < args.M && col < args.Kp) {
-                if constexpr (MxFormat<FMT>::kBits == 4) {
-                  *reinterpret_cast<uint4*>(args.codes + row * (args.Kp >> 1) + (col >> 1)) =
-                      make_uint4(cd[0], cd[1], cd[2], cd[3]);
-                } else {
-                  uint4* d = reinterpret_cast<uint4*>(args.codes + row * args.Kp + col);
-                  d[0] = make_uint4(cd[0], cd[1], cd[2], cd[3]);
-                  d[1] = make_uint4(cd[4], cd[5], cd[6], cd[7]);
-                }
-              }
+              if (row < args.M && col < args.Kp)
+                *reinterpret_cast<uint4*>(args.codes + row * (args.Kp >> 1) + (col >> 1)) =
+                    make_uint4(cd[0], cd[1], cd[2], cd[3]);
             }
             const uint32_t other = __shfl_xor_sync(0xffffffffu, bytes, 1);
             if constexpr (FMT == LORA_NVFP4) {
