@@ -19,8 +19,8 @@
 // packed multiplication by the scale.  Codes have two significant bits and scales at
 // most four, so the product is exact wherever it is a normal number of the type.
 //
-// Bound: the chain load -> decode -> MMA of a stage over a ring of three to eight, then
-// the decode's ALU work.  64 rows of 13824 x 5120 (nvfp4, r = 16) take 44 us, of which
+// Bound: the chain load -> decode -> MMA of a stage over a ring of four (64 tokens: three),
+// whose 16-bit tiles fill the shared memory, then the decode's ALU work.  64 rows of 13824 x 5120 (nvfp4, r = 16) take 44 us, of which
 // 11 are the decode's and 6 the MMAs' (each left out in turn); 256 rows of 4096 x 4096
 // 18.  HBM's share is small, 0.53 or 0.56 bytes a weight.  So a tile takes up to 256
 // tokens, whose decode is then paid once (256 rows, whole backward pass: two tiles of 128
@@ -57,7 +57,7 @@ struct DxMaps {
 struct DxArgs {
   MxTileOut tile;
   int* err;
-  int num_kb, last_step, rank_kb, last_k16, r16, gb, stages;
+  int num_kb, last_step, rank_kb, last_k16, r16, gb;
   float pow2;
 };
 
@@ -68,6 +68,14 @@ struct DxLayout {
   static constexpr int kX = NB * 128;
   static constexpr int kXOffset = kDxW, kRawOffset = kDxW + kX, kSfOffset = kRawOffset + kDxRaw;
   static constexpr int kStage = (kSfOffset + kSf + 1023) / 1024 * 1024;
+  static constexpr int kFixed = 1024 + 512;  // alignment, barriers
+  // As many as fit, divided by the groups: a stage always goes to the same group, so that
+  // a warp which waits for a stage's next tile has seen its last one -- a barrier's
+  // parity says no more than that.
+  static constexpr int kStages = (dx_smem_max<NB>() - kFixed) / kStage / dx_groups<NB>() * dx_groups<NB>();
+  static constexpr size_t kBytes = static_cast<size_t>(kStages) * kStage + kFixed;
+  static_assert(kStages == (NB == 64 ? 3 : 4), "the depth that the measurements are of");
+  static_assert(kStages * kStage >= NB * 512, "the partial tile lies over the stages");
 };
 
 // MN-major operand in two 64-wide chunks.
@@ -146,7 +154,7 @@ __global__ void __launch_bounds__(dx_threads<NB>(), dx_ctas<NB>())
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint64_t* full_w = reinterpret_cast<uint64_t*>(smem + args.stages * L::kStage);
+  uint64_t* full_w = reinterpret_cast<uint64_t*>(smem + L::kStages * L::kStage);
   uint64_t* full_x = full_w + 8;
   uint64_t* ready = full_x + 8;  // W decoded
   uint64_t* empty = ready + 8;
@@ -165,7 +173,7 @@ __global__ void __launch_bounds__(dx_threads<NB>(), dx_ctas<NB>())
   const int total = base + (rank == 0 ? kTails * args.rank_kb : 0);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < args.stages; ++s) {
+    for (int s = 0; s < L::kStages; ++s) {
       mbar_init(&full_w[s], 1);
       mbar_init(&full_x[s], 1);
       mbar_init(&ready[s], kDxGroupWarps);
@@ -212,18 +220,18 @@ __global__ void __launch_bounds__(dx_threads<NB>(), dx_ctas<NB>())
           tma_load_2d(&maps.g, at, &full_x[stage], (tail < 3 ? tail : tail - 3) * args.r16 + c * 64, t0);
         }
       };
-      const int pre = min(total, args.stages);
+      const int pre = min(total, L::kStages);
       for (int i = 0; i < pre; ++i) weights(i, i);
       pdl_wait();  // g
       pdl_launch_dependents();
       for (int i = 0; i < pre; ++i) rows(i, i);
-      int stage = pre == args.stages ? 0 : pre;
-      uint32_t phase = pre == args.stages ? 1 : 0;
+      int stage = pre == L::kStages ? 0 : pre;
+      uint32_t phase = pre == L::kStages ? 1 : 0;
       for (int i = pre; i < total; ++i) {
         if (!mbar_wait_bounded(&empty[stage], phase ^ 1, abort_flag, args.err, kDevErrTimeoutEmpty)) break;
         weights(i, stage);
         rows(i, stage);
-        if (++stage == args.stages) {
+        if (++stage == L::kStages) {
           stage = 0;
           phase ^= 1;
         }
@@ -256,7 +264,7 @@ __global__ void __launch_bounds__(dx_threads<NB>(), dx_ctas<NB>())
         tc_commit(&empty[stage]);
       }
       __syncwarp();
-      if (++stage == args.stages) {
+      if (++stage == L::kStages) {
         stage = 0;
         phase ^= 1;
       }
@@ -305,7 +313,7 @@ __global__ void __launch_bounds__(dx_threads<NB>(), dx_ctas<NB>())
         __syncwarp();
         if (lane == 0) mbar_arrive(&ready[stage]);
       }
-      if (++stage == args.stages) {
+      if (++stage == L::kStages) {
         stage = 0;
         phase ^= 1;
       }
@@ -352,25 +360,20 @@ int launch_dx(const MxDxOperands& o, cudaStream_t stream) {
   a.last_k16 = static_cast<int>((o.R - (a.rank_kb - 1) * 64ll + 15) / 16);
   a.r16 = static_cast<int>(o.r16);
   a.pow2 = o.pow2;
-  constexpr int kFixed = 1024 + 512;
-  // a stage always goes to the same group: a warp that waits for a stage's next tile has
-  // seen its last one, and a barrier's parity says no more than that
-  a.stages = std::min<int>(8, (dx_smem_max<NB>() - kFixed) / L::kStage) / dx_groups<NB>() * dx_groups<NB>();
-  static_assert((dx_smem_max<NB>() - kFixed) / L::kStage / 2 * 2 * L::kStage >= NB * 512, "the partial tile lies over the stages");
   const int k_tiles = static_cast<int>((o.K + 127) / 128), t_tiles = static_cast<int>((o.M + NB - 1) / NB);
   // as many CTAs as are resident at once, each with eight or more stages
   const int resident = dx_ctas<NB>() * info.num_sms;
   int splits = 1;
   while (splits < 8 && k_tiles * t_tiles * splits * 2 <= resident && a.num_kb >= 16 * splits) splits *= 2;
-  const size_t smem = static_cast<size_t>(a.stages) * L::kStage + kFixed;
   auto kernel = mx_dx_kernel<T, FMT, NB>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
   std::call_once(once[dev], [&] {
-    attr_err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, dx_smem_max<NB>());
+    attr_err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(L::kBytes));
   });
   if (attr_err[dev] != cudaSuccess) return LORA_ERR_CUDA;
-  return mx_launch(kernel, dim3(k_tiles * splits, t_tiles), dx_threads<NB>(), smem, stream, splits, maps, a);
+  return mx_launch(kernel, dim3(k_tiles * splits, t_tiles), dx_threads<NB>(), L::kBytes, stream, splits, maps, a);
 }
 
 template <typename T, int FMT>
