@@ -26,7 +26,6 @@ struct GemmArgs {
   int64_t lo_offset;  // > 0: also write lo = v - round(v) at column + lo_offset
   int M, N, K, R;
   int num_kb_main, num_kb_tail, tail_last_k16;
-  uint32_t tail_flip = 0;  // instruction descriptor bits of a tail of the other 16-bit type
   int num_m_tiles, num_n_tiles, num_tiles, group_m;
   int l2_hints;  // bit 0: W / B_dup evict_last; bit 1: x / z evict_first; bit 2: out evict_first
   float alpha;
@@ -127,7 +126,7 @@ LORA_DEVINL void epilogue_store16(const GemmArgs& args, T* out_row, const T* bia
   }
 }
 
-// lora_gemm_ex with [z, bw] in z_dtype (either 16-bit type), x and w in dtype.
+// lora_gemm_ex with [z, bw] in z_dtype: dtype, or bf16 beside x and w in fp16.
 int gemm_mixed_tail(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* z, int64_t ldz, const void* bw,
                     int64_t ldbw, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K, int64_t R, float alpha,
                     int dtype, int z_dtype, void* ws, size_t ws_bytes, void* stream);

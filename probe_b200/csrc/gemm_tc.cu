@@ -44,7 +44,8 @@ struct GemmSmem {
   static constexpr int kBytes = kBarOffset + 256 + 1024;  // barriers + alignment slack
 };
 
-template <int BN, int STAGES, typename T>
+// TZ: type of the tail's operands z and bw.
+template <int BN, int STAGES, typename T, typename TZ>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                    const __grid_constant__ CUtensorMap tm_z, const __grid_constant__ CUtensorMap tm_b,
@@ -52,6 +53,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   using L = GemmSmem<BN, STAGES, T>;
   constexpr uint32_t kTmemCols = 2 * BN;  // 128, 256 or 512: a power of two >= 32
   constexpr uint32_t kIdesc = umma_idesc_f16(kGemmBM, BN, std::is_same<T, __nv_bfloat16>::value ? 1 : 0);
+  constexpr uint32_t kIdescTail = umma_idesc_f16(kGemmBM, BN, std::is_same<TZ, __nv_bfloat16>::value ? 1 : 0);
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -154,7 +156,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const uint64_t bdesc = umma_desc_sw128(smem_u32(sm_b + stage * L::kBBytes));
           // The last tail block only holds ceil(R%64 / 16) non-zero K16 steps.
           const int nk = (kb == num_kb - 1 && args.num_kb_tail > 0) ? args.tail_last_k16 : 4;
-          const uint32_t idesc = kb < args.num_kb_main ? kIdesc : kIdesc ^ args.tail_flip;
+          const uint32_t idesc = std::is_same<T, TZ>::value || kb < args.num_kb_main ? kIdesc : kIdescTail;
           for (int k = 0; k < nk; ++k) {
             // +32 bytes per K16 step inside the 128B swizzle atom (>>4 => +2).
             tc_mma_f16(d_tmem, adesc + static_cast<uint64_t>(2 * k), bdesc + static_cast<uint64_t>(2 * k),
@@ -277,7 +279,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 // ingest per SM, not the tensor pipe, bounds the NW = 1 form on B200).  Both
 // accumulator halves belong to the one tile; the epilogue frees them one at a
 // time and the next tile's first MMAs into each half wait only for that half.
-template <int STAGES, int NW, int EW, typename T>
+template <int STAGES, int NW, int EW, typename T, typename TZ>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * EW, 1)
     gemm_tc2_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                     const __grid_constant__ CUtensorMap tm_z, const __grid_constant__ CUtensorMap tm_b,
@@ -286,6 +288,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * EW, 1)
   constexpr uint32_t kTmemCols = 512;  // two 256-column fp32 accumulators
   constexpr int kTileN = 256 * NW;
   constexpr uint32_t kIdesc = umma_idesc_f16(256, 256, std::is_same<T, __nv_bfloat16>::value ? 1 : 0);
+  constexpr uint32_t kIdescTail = umma_idesc_f16(256, 256, std::is_same<TZ, __nv_bfloat16>::value ? 1 : 0);
   constexpr uint16_t kBoth = 0x3;
 
   extern __shared__ uint8_t smem_raw[];
@@ -410,7 +413,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * EW, 1)
           const uint64_t adesc = umma_desc_sw128(smem_u32(sm_a + stage * L::kABytes));
           const uint64_t bdesc = umma_desc_sw128(smem_u32(sm_b + stage * L::kBBytes));
           const int nk = (kb == num_kb - 1 && args.num_kb_tail > 0) ? args.tail_last_k16 : 4;
-          const uint32_t idesc = kb < args.num_kb_main ? kIdesc : kIdesc ^ args.tail_flip;
+          const uint32_t idesc = std::is_same<T, TZ>::value || kb < args.num_kb_main ? kIdesc : kIdescTail;
           for (int k = 0; k < nk; ++k)
             tc_mma_f16_pair(d_tmem, adesc + static_cast<uint64_t>(2 * k), bdesc + static_cast<uint64_t>(2 * k),
                             idesc, (kb > kb0 || k > 0) ? 1u : 0u);
@@ -543,11 +546,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * EW, 1)
 namespace {
 
 
-template <int BN, int STAGES, typename T>
+template <int BN, int STAGES, typename T, typename TZ>
 int launch_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* z, int64_t ldz,
                 const void* bw, int64_t ldbw, const void* bias, void* out, int64_t ldo, int64_t M,
-                int64_t N, int64_t K, int64_t R, float alpha, int64_t lo_offset, int dtype, uint32_t tail_flip,
-                cudaStream_t stream) {
+                int64_t N, int64_t K, int64_t R, float alpha, int64_t lo_offset, int dtype, cudaStream_t stream) {
   using L = GemmSmem<BN, STAGES, T>;
   const int dev = current_device();
   if (dev < 0) return LORA_ERR_DEVICE;
@@ -580,7 +582,6 @@ int launch_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, const vo
   a.num_kb_tail = static_cast<int>((R + kGemmBK - 1) / kGemmBK);
   const int tail_rem = static_cast<int>(R - static_cast<int64_t>(a.num_kb_tail - 1) * kGemmBK);
   a.tail_last_k16 = a.num_kb_tail > 0 ? (tail_rem + 15) / 16 : 4;
-  a.tail_flip = tail_flip;
   a.num_m_tiles = static_cast<int>((M + kGemmBM - 1) / kGemmBM);
   a.num_n_tiles = static_cast<int>((N + BN - 1) / BN);
   a.num_tiles = a.num_m_tiles * a.num_n_tiles;
@@ -592,7 +593,7 @@ int launch_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, const vo
   a.tail_tickets = nullptr;
   a.alpha = alpha;
 
-  auto kernel = gemm_tc_kernel<BN, STAGES, T>;
+  auto kernel = gemm_tc_kernel<BN, STAGES, T, TZ>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
   std::call_once(once[dev & 63], [&] {
@@ -604,20 +605,20 @@ int launch_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw, const vo
   return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
 }
 
-template <typename T>
+template <typename T, typename TZ>
 int dispatch_gemm(int bn, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* z, int64_t ldz,
                   const void* bw, int64_t ldbw, const void* bias, void* out, int64_t ldo, int64_t M, int64_t N,
-                  int64_t K, int64_t R, float alpha, int64_t lo, int dtype, uint32_t tail_flip, cudaStream_t stream) {
+                  int64_t K, int64_t R, float alpha, int64_t lo, int dtype, cudaStream_t stream) {
   switch (bn) {
     case 64:
-      return launch_gemm<64, 8, T>(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo, dtype,
-                                   tail_flip, stream);
+      return launch_gemm<64, 8, T, TZ>(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo, dtype,
+                                   stream);
     case 128:
-      return launch_gemm<128, 6, T>(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo, dtype,
-                                    tail_flip, stream);
+      return launch_gemm<128, 6, T, TZ>(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo, dtype,
+                                    stream);
     default:
-      return launch_gemm<256, 4, T>(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo, dtype,
-                                    tail_flip, stream);
+      return launch_gemm<256, 4, T, TZ>(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo, dtype,
+                                    stream);
   }
 }
 
@@ -668,10 +669,10 @@ PairSplit pair_split_plan(int64_t tiles, int pairs, int num_kb, int tile_n) {
 }
 
 // Resident CTA pairs of gemm_tc2_kernel<STAGES, NW, EW> on this device (cached).
-template <int STAGES, int NW, int EW, typename T>
+template <int STAGES, int NW, int EW, typename T, typename TZ>
 int pair_capacity(int dev, const DeviceInfo& info, cudaError_t* attr_status) {
   using L = PairSmem<STAGES, NW>;
-  auto kernel = gemm_tc2_kernel<STAGES, NW, EW, T>;
+  auto kernel = gemm_tc2_kernel<STAGES, NW, EW, T, TZ>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
   static int max_clusters[64];
@@ -694,11 +695,11 @@ int pair_capacity(int dev, const DeviceInfo& info, cudaError_t* attr_status) {
   return max_clusters[dev & 63];
 }
 
-template <int STAGES, int NW, int EW, typename T>
+template <int STAGES, int NW, int EW, typename T, typename TZ>
 int launch_gemm_pair(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* z, int64_t ldz,
                      const void* bw, int64_t ldbw, const void* bias, void* out, int64_t ldo, int64_t M, int64_t N,
-                     int64_t K, int64_t R, float alpha, int64_t lo_offset, int dtype, uint32_t tail_flip, void* ws,
-                     size_t ws_bytes, cudaStream_t stream) {
+                     int64_t K, int64_t R, float alpha, int64_t lo_offset, int dtype, void* ws, size_t ws_bytes,
+                     cudaStream_t stream) {
   using L = PairSmem<STAGES, NW>;
   const int dev = current_device();
   if (dev < 0) return LORA_ERR_DEVICE;
@@ -727,7 +728,6 @@ int launch_gemm_pair(const void* x, int64_t ldx, const void* w, int64_t ldw, con
   a.num_kb_tail = static_cast<int>((R + kGemmBK - 1) / kGemmBK);
   const int tail_rem = static_cast<int>(R - static_cast<int64_t>(a.num_kb_tail - 1) * kGemmBK);
   a.tail_last_k16 = a.num_kb_tail > 0 ? (tail_rem + 15) / 16 : 4;
-  a.tail_flip = tail_flip;
   a.num_m_tiles = static_cast<int>((M + 255) / 256);
   a.num_n_tiles = static_cast<int>((N + 256 * NW - 1) / (256 * NW));
   a.num_tiles = a.num_m_tiles * a.num_n_tiles;
@@ -742,9 +742,9 @@ int launch_gemm_pair(const void* x, int64_t ldx, const void* w, int64_t ldw, con
   a.l2_hints = env_int("LORA_B200_L2_HINTS", w_bytes >= (int64_t{48} << 20) ? 1 : 0);
   a.alpha = alpha;
 
-  auto kernel = gemm_tc2_kernel<STAGES, NW, EW, T>;
+  auto kernel = gemm_tc2_kernel<STAGES, NW, EW, T, TZ>;
   cudaError_t attr_status = cudaSuccess;
-  const int capacity = pair_capacity<STAGES, NW, EW, T>(dev, info, &attr_status);
+  const int capacity = pair_capacity<STAGES, NW, EW, T, TZ>(dev, info, &attr_status);
   if (attr_status != cudaSuccess) return LORA_ERR_CUDA;
   a.full_tiles = a.num_tiles;
   a.split = 1;
@@ -848,9 +848,24 @@ int gemm_pick_bn(int64_t M, int64_t N, int num_sms) {
 namespace lora {
 namespace {
 
+// nw: width of the pair tiles, 0 for single-CTA tiles of bn columns.
+template <typename T, typename TZ>
+int gemm_run(int nw, int bn, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* z, int64_t ldz,
+             const void* bw, int64_t ldbw, const void* bias, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K,
+             int64_t R, float alpha, int64_t lo_offset, int dtype, void* ws, size_t ws_bytes, cudaStream_t s) {
+  if (nw == 2)
+    return launch_gemm_pair<4, 2, kPairEpiWarps, T, TZ>(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R,
+                                                        alpha, lo_offset, dtype, ws, ws_bytes, s);
+  if (nw == 1)
+    return launch_gemm_pair<6, 1, kPairEpiWarps, T, TZ>(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R,
+                                                        alpha, lo_offset, dtype, ws, ws_bytes, s);
+  return dispatch_gemm<T, TZ>(bn, x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo_offset, dtype,
+                              s);
+}
+
 int gemm_impl(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* z, int64_t ldz, const void* bw,
               int64_t ldbw, const void* bias, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K, int64_t R,
-              float alpha, int64_t lo_offset, int dtype, uint32_t tail_flip, void* ws, size_t ws_bytes, void* stream) {
+              float alpha, int64_t lo_offset, int dtype, int z_dtype, void* ws, size_t ws_bytes, void* stream) {
   if (x == nullptr || w == nullptr || out == nullptr) return LORA_ERR_ARG;
   if (dtype != LORA_BF16 && dtype != LORA_F16) return LORA_ERR_DTYPE;
   if (M < 0 || N < 0 || K < 0 || R < 0) return LORA_ERR_SHAPE;
@@ -873,23 +888,15 @@ int gemm_impl(const void* x, int64_t ldx, const void* w, int64_t ldw, const void
   if (!info.is_sm100) return LORA_ERR_DEVICE;
   const int bn = gemm_pick_bn(M, N, info.num_sms);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (use_pair_tiles(M, N, K, R, info.num_sms, ws != nullptr)) {
-    const int nw = pair_tile_width(M, N, K, R, info.num_sms / 2, ws != nullptr);
-#define LORA_PAIR(ST, NWV)                                                                                        \
-  (dtype == LORA_BF16                                                                                              \
-       ? launch_gemm_pair<ST, NWV, kPairEpiWarps, __nv_bfloat16>(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, \
-                                                                 N, K, R, alpha, lo_offset, dtype, tail_flip, ws,     \
-                                                                 ws_bytes, s)                                         \
-       : launch_gemm_pair<ST, NWV, kPairEpiWarps, __half>(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, \
-                                                          R, alpha, lo_offset, dtype, tail_flip, ws, ws_bytes, s))
-    return nw == 2 ? LORA_PAIR(4, 2) : LORA_PAIR(6, 1);
-#undef LORA_PAIR
-  }
-  if (dtype == LORA_BF16)
-    return dispatch_gemm<__nv_bfloat16>(bn, x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha,
-                                        lo_offset, dtype, tail_flip, s);
-  return dispatch_gemm<__half>(bn, x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo_offset,
-                               dtype, tail_flip, s);
+  const int nw = use_pair_tiles(M, N, K, R, info.num_sms, ws != nullptr)
+                     ? pair_tile_width(M, N, K, R, info.num_sms / 2, ws != nullptr)
+                     : 0;
+#define LORA_GEMM_RUN(T, TZ)                                                                                       \
+  gemm_run<T, TZ>(nw, bn, x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo_offset, dtype, ws, \
+                  ws_bytes, s)
+  if (dtype == LORA_BF16) return LORA_GEMM_RUN(__nv_bfloat16, __nv_bfloat16);
+  return z_dtype == LORA_BF16 ? LORA_GEMM_RUN(__half, __nv_bfloat16) : LORA_GEMM_RUN(__half, __half);
+#undef LORA_GEMM_RUN
 }
 
 }  // namespace
@@ -897,9 +904,8 @@ int gemm_impl(const void* x, int64_t ldx, const void* w, int64_t ldw, const void
 int gemm_mixed_tail(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* z, int64_t ldz, const void* bw,
                     int64_t ldbw, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K, int64_t R, float alpha,
                     int dtype, int z_dtype, void* ws, size_t ws_bytes, void* stream) {
-  constexpr uint32_t kOther = umma_idesc_f16(128, 256, 0) ^ umma_idesc_f16(128, 256, 1);
-  return gemm_impl(x, ldx, w, ldw, z, ldz, bw, ldbw, nullptr, out, ldo, M, N, K, R, alpha, 0, dtype,
-                   dtype == z_dtype ? 0 : kOther, ws, ws_bytes, stream);
+  return gemm_impl(x, ldx, w, ldw, z, ldz, bw, ldbw, nullptr, out, ldo, M, N, K, R, alpha, 0, dtype, z_dtype, ws, ws_bytes,
+                   stream);
 }
 
 }  // namespace lora
@@ -908,7 +914,7 @@ extern "C" int lora_gemm(const void* x, int64_t ldx, const void* w, int64_t ldw,
                          const void* bw, int64_t ldbw, const void* bias, void* out, int64_t ldo, int64_t M,
                          int64_t N, int64_t K, int64_t R, float alpha, int64_t lo_offset, int dtype, void* stream) {
   return lora::gemm_impl(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo_offset, dtype,
-                         0, nullptr, 0, stream);
+                         dtype, nullptr, 0, stream);
 }
 
 extern "C" size_t lora_gemm_workspace_size(int64_t M, int64_t N, int64_t K, int64_t R) {
@@ -920,8 +926,8 @@ extern "C" size_t lora_gemm_workspace_size(int64_t M, int64_t N, int64_t K, int6
   if (!info.is_sm100 || !use_pair_tiles(M, N, K, R, info.num_sms, true)) return 0;
   const int nw = pair_tile_width(M, N, K, R, info.num_sms / 2, true);
   cudaError_t st = cudaSuccess;
-  const int capacity = nw == 2 ? pair_capacity<4, 2, kPairEpiWarps, __nv_bfloat16>(dev, info, &st)
-                               : pair_capacity<6, 1, kPairEpiWarps, __nv_bfloat16>(dev, info, &st);
+  const int capacity = nw == 2 ? pair_capacity<4, 2, kPairEpiWarps, __nv_bfloat16, __nv_bfloat16>(dev, info, &st)
+                               : pair_capacity<6, 1, kPairEpiWarps, __nv_bfloat16, __nv_bfloat16>(dev, info, &st);
   if (st != cudaSuccess) return 0;
   const int64_t tiles = ((M + 255) / 256) * ((N + 256 * nw - 1) / (256 * nw));
   const int num_kb = static_cast<int>((K + kGemmBK - 1) / kGemmBK + (R + kGemmBK - 1) / kGemmBK);
@@ -933,5 +939,5 @@ extern "C" int lora_gemm_ex(const void* x, int64_t ldx, const void* w, int64_t l
                             int64_t N, int64_t K, int64_t R, float alpha, int64_t lo_offset, int dtype,
                             void* workspace, size_t workspace_bytes, void* stream) {
   return lora::gemm_impl(x, ldx, w, ldw, z, ldz, bw, ldbw, bias, out, ldo, M, N, K, R, alpha, lo_offset, dtype,
-                         0, workspace, workspace_bytes, stream);
+                         dtype, workspace, workspace_bytes, stream);
 }
