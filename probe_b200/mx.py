@@ -35,8 +35,9 @@ _DTYPE = {torch.float16: _lib.LORA_F16, torch.bfloat16: _lib.LORA_BF16}
 
 # A call of a few tokens takes the GPU a few microseconds: the wrappers below pass
 # plain integers to the C ABI, look the raw stream up directly and keep sizes by shape.
-def _raw_stream(device_index: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(device_index)  # (not there in builds without CUDA)
+# (None in builds of PyTorch without CUDA, where no tensor gets that far)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 @functools.cache
@@ -67,9 +68,9 @@ def _need_one_device(where, *tensors):
         raise ValueError(f"{where}: operands lie on different devices ({', '.join(sorted(devices))})")
 
 
-def _elsewhere(t: torch.Tensor) -> bool:
-    """Whether the tensor lies on a GPU that is not the current one, on which kernels launch."""
-    return t.is_cuda and t.get_device() != torch._C._cuda_getDevice()
+def _elsewhere(device_index: int) -> bool:
+    """Whether that GPU (-1: none) is not the current one, on which kernels launch."""
+    return device_index >= 0 and device_index != _current_device()
 
 
 def _format(fmt: str, where: str) -> int:
@@ -161,7 +162,7 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4", global_scale: float = 1.0) 
     and saturate; a block with an infinity or a NaN reads back as NaN.
     """
     code = _format(fmt, "mx_quantize")
-    if _elsewhere(x):
+    if _elsewhere(x.get_device()):
         with torch.cuda.device(x.device):
             return mx_quantize(x, fmt, global_scale)
     _need_cuda("mx_quantize", x)
@@ -181,7 +182,7 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp4", global_scale: float = 1.0) 
 
 def mx_dequantize(q: MXTensor, dtype: torch.dtype = torch.bfloat16, transpose: bool = False) -> torch.Tensor:
     """The values of ``q`` in ``dtype`` (rounded once), [M, K] or, transposed, [K, M]."""
-    if _elsewhere(q.codes):
+    if _elsewhere(q.codes.get_device()):
         with torch.cuda.device(q.codes.device):
             return mx_dequantize(q, dtype, transpose)
     _need_cuda("mx_dequantize", q.codes)
@@ -229,13 +230,14 @@ def _refuse_linear(x, weight, bias, a, b, where):
 
 
 def _linear(x, weight, bias, a, b, scale, x_global_scale, keep_z, where):
-    if _elsewhere(x):
+    dev = x.get_device()  # (-1: not on a GPU)
+    if _elsewhere(dev):
         with torch.cuda.device(x.device):
             return _linear(x, weight, bias, a, b, scale, x_global_scale, keep_z, where)
     shape, dtype, codes, code = x.shape, x.dtype, weight.codes, weight._code
     n, k = weight.shape
     r = 0 if a is None or b is None or (scale == 0 and not keep_z) else a.shape[0]
-    dt, dev = _DTYPE.get(dtype), x.get_device()  # (-1: not on a GPU)
+    dt = _DTYPE.get(dtype)
     if (dt is None or code == _lib.LORA_MXFP8 or dev < 0 or codes.get_device() != dev or shape[-1] != k
             or (bias is not None and (bias.get_device() != dev or bias.dtype != dtype or bias.shape != (n,)))
             or (r and (r > 256 or a.dtype != dtype or b.dtype != dtype or a.get_device() != dev or b.get_device() != dev
@@ -314,7 +316,8 @@ def mx_lora_backward(dy: torch.Tensor, x8: MXTensor, z: torch.Tensor, a: torch.T
     checkpoint of x, ``z`` the [M, 2 r16] pair [hi | lo] of the forward pass, W an mxfp4 /
     nvfp4 tensor.  W is frozen; rounding to 4 or 8 bits counts as the identity.
     """
-    if _elsewhere(dy):
+    dev = dy.get_device()  # (-1: not on a GPU)
+    if _elsewhere(dev):
         with torch.cuda.device(dy.device):
             return mx_lora_backward(dy, x8, z, a, b, scale, weight, z_scale)
     shape, dtype = dy.shape, dy.dtype
@@ -324,7 +327,7 @@ def mx_lora_backward(dy: torch.Tensor, x8: MXTensor, z: torch.Tensor, a: torch.T
         dy = _rows(dy, "mx_lora_backward")
     m, n = dy.shape
     r, k = a.shape
-    dt, dev = _DTYPE.get(dtype), dy.get_device()  # (-1: not on a GPU)
+    dt = _DTYPE.get(dtype)
     if (dt is None or x8.fmt != "mxfp8" or x8.shape != (m, k) or a.dtype != dtype or b.dtype != dtype
             or z.dtype != dtype or b.shape != (n, r) or not 1 <= r <= 256
             or z.shape != (m, 2 * ((r + 15) // 16 * 16)) or not z.is_contiguous()

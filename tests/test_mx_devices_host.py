@@ -36,7 +36,7 @@ def current(monkeypatch):
             state.index = before
 
     monkeypatch.setattr(torch.cuda, "device", device)
-    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: state.index, raising=False)
+    monkeypatch.setattr(mx, "_current_device", lambda: state.index)
     return state
 
 
