@@ -23,9 +23,12 @@ namespace lora {
 namespace {
 
 // Ranks above this, of enough rows, take g = s dy B from the 16-bit CTA-pair GEMM,
-// which halves the shared-memory reads of so wide an adapter (r = 224, 32760 x 5120: 83
-// against 109 us).
-constexpr int64_t kWideRank = 128, kWideRows = 4096;
+// which halves the shared-memory reads of so wide an adapter; below, its few tiles leave
+// SMs idle.  Whole passes without dx, us, GEMM and shrink: 5120 -> 5120, r = 224: 8192 rows
+// 149 and 135, 16384 245 and 221, 20000 284 and 277, 24576 319 and 325, 32760 388 and 409;
+// r = 256, 24576 rows 325 and 330; r = 192 288 and 282, 32760 348 and 357; r = 144 no gain
+// (334 and 337); 4096 -> 11008, r = 224, 4096 rows 159 and 122.
+constexpr int64_t kWideRank = 144, kWideRows = 24576;
 
 // g of fp16 activations is kept in three bf16 parts, which never leave its range; beside
 // A = Ah + Al the tail of dx takes [gh gm gl gh gm] against [Ah Ah Ah Al Al].

@@ -13,7 +13,9 @@
 // with the 128-byte swizzle, whole 32-byte sectors of codes out).  A second group of
 // eight takes every other tile; a third made it slower (4095 x 5120 mxfp4, r = 16: 26.7
 // against 25.9 us; r = 224 of 32760 tokens, nvfp4: 219 against 176).  Up to 64 tokens
-// there are four groups of four (a call of 64 tokens 17.6 to 16.4 us).
+// there are four groups of four (whole calls of 1, 16 and 64 tokens, N = 4096, both formats,
+// r = 16, 96, 224: 4096 columns 3 to 9 % faster, 13824 columns 5 to 20 %; one token of 13824,
+// nvfp4, r = 16, 21.7 to 17.4 us).
 //
 // Bound: the floor is HBM (v once, codes out); what is measured is the ALU pipe of the
 // quantisation -- 4095 x 5120 mxfp4 with r = 16, 53 MB, takes 18 to 25 us, issue slots
