@@ -17,7 +17,8 @@
 // scale.  Bound: HBM for small ranks (2 or 1.03 bytes an element of V), the MMAs, both of
 // whose operands come from shared memory, for large ones.  Both gradients
 // of 4097 tokens, 4096 -> 11008, r = 16, 107 MB: 46 us with the partials; of 32760 tokens,
-// 5120 -> 5120: 129 at r = 64, 162 at r = 128, 300 at r = 224 (300 GFLOP).  They are one launch: the second's blocks start as the
+// 5120 -> 5120: 129 at r = 64, 162 at r = 128, 284 to 300 at r = 224 (300 GFLOP, the tensor pipe
+// half busy).  They are one launch: the second's blocks start as the
 // first's leave, and few tokens' blocks run side by side (256 tokens, 4096 -> 4096: 4.7 us
 // instead of 4.0 + 7.8 with waits).
 // P is the whole hi/lo pair.  Up to rank 128 its halves lie side by side in one MMA (N = 2 r)
