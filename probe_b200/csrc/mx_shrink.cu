@@ -549,7 +549,11 @@ int launch_shrink(const MxShrinkOperands& o, cudaStream_t stream) {
     attr_err[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShSmemMax);
   });
   if (attr_err[dev] != cudaSuccess) return LORA_ERR_CUDA;
-  const size_t smem = static_cast<size_t>(a.stages) * a.stage_bytes + kFixed;
+  size_t smem = static_cast<size_t>(a.stages) * a.stage_bytes + kFixed;
+  // All of tensor memory: no CTA that takes some may share the SM.  A cluster's CTA that
+  // holds it while its peer waits for another cluster's, and the other way round on another
+  // SM, would wait for good (kernels of two streams).
+  if (2 * a.r16 > 256) smem = kShSmemMax;
   if (a.cluster && a.stages * a.stage_bytes < 128 * a.r16 * 4) return LORA_ERR_UNSUPPORTED;  // never: 167 KB and more
   const int64_t ctas = a.cluster ? (o.M + 127) / 128 * a.cluster : shrink_ctas(o.M, o.K, o.R);
   return mx_launch(kernel, dim3(static_cast<unsigned>(ctas)), kShThreads, smem, stream, a.cluster, maps, a);
