@@ -157,6 +157,31 @@ LORA_DEVINL bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, 
   return ok;
 }
 
+// The two halves of cluster_sync_all, and the arrival half of a named barrier.
+LORA_DEVINL void cluster_arrive_all() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+LORA_DEVINL void cluster_wait_all() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+LORA_DEVINL void named_bar_arrive(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// The cluster meets.  Warp 1 gives its CTA's tensor memory back in between, once the
+// reading warps (`readers`) are done with it: a CTA that held it and waited for a peer, which
+// may be waiting for another kernel's, could wait for good.  Barrier 2.
+LORA_DEVINL void cluster_sync_free_tmem(uint32_t tmem, uint32_t cols, int warp, bool reads, int readers) {
+  if (reads) {
+    tc_fence_before();
+    named_bar_arrive(2, 32 * (readers + 1));
+  }
+  cluster_arrive_all();
+  if (warp == 1) {
+    named_bar_sync(2, 32 * (readers + 1));
+    tc_fence_after();
+    tmem_dealloc(tmem, cols);
+  }
+  __syncwarp();
+  cluster_wait_all();
+}
+
 // 2^(byte - 127) of an E8M0 scale byte; 255 is NaN.
 LORA_DEVINL float mx_e8m0(uint32_t byte) {
   const uint32_t bits = byte == 0 ? 0x00400000u : (byte == 255 ? 0x7fffffffu : byte << 23);

@@ -320,17 +320,8 @@ __global__ void __launch_bounds__(dx_threads<NB>(), dx_ctas<NB>())
     }
   }
 
-  mx_tile_out<T, NB, dx_threads<NB>(), 2, kDxGroupWarps * dx_groups<NB>()>(
+  mx_tile_out<T, NB, dx_threads<NB>(), 2, kDxGroupWarps * dx_groups<NB>(), kTmemCols>(
       args.tile, reinterpret_cast<float*>(smem), tmem, 0, acc_full, abort_flag, args.err, splits, rank, k0, t0);
-  tc_fence_before();
-  if (splits > 1)
-    cluster_sync_all();  // no CTA leaves while another reads its partial tile
-  else
-    __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
-  }
 }
 
 template <typename T, int FMT, int NB>

@@ -433,9 +433,9 @@ __global__ void __launch_bounds__(kShThreads, 1)
       }
     }
   }
-  tc_fence_before();
   if (args.cluster) {
-    cluster_sync_all();  // every CTA's partial sums are in its shared memory
+    // every CTA's partial sums are in its shared memory
+    cluster_sync_free_tmem(tmem, tmem_cols, warp, warp >= 2, kShWorkers);
     // rows are dealt to the ranks, groups of four columns to the threads
     const int per = 128 / args.cluster, quads = args.r16 / 4;
     const int64_t row0 = static_cast<int64_t>(blockIdx.x / args.cluster) * 128 + crank * per;
@@ -466,11 +466,12 @@ __global__ void __launch_bounds__(kShThreads, 1)
     }
     cluster_sync_all();  // no CTA leaves while another reads its sums
   } else {
+    tc_fence_before();
     __syncthreads();
-  }
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem, tmem_cols);
+    if (warp == 1) {
+      tc_fence_after();
+      tmem_dealloc(tmem, tmem_cols);
+    }
   }
 }
 

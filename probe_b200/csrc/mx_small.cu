@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kSmThreads = 192;
 // Two CTAs an SM, each with at most half of TMEM, or (128 tokens) one with all of
-// it: a CTA must never wait for another's TMEM, whose cluster may wait for its own.
+// it: none of a launch waits for another's.
 template <int NB> __host__ __device__ constexpr int sm_smem_max() { return NB == 128 ? 220 * 1024 : 112 * 1024; }
 template <int NB> __host__ __device__ constexpr int sm_tmem_max() { return NB == 128 ? 512 : 256; }
 
@@ -236,17 +236,8 @@ __global__ void __launch_bounds__(kSmThreads)
     __syncwarp();
   }
 
-  mx_tile_out<T, NB, kSmThreads, 2, 4>(args.tile, reinterpret_cast<float*>(smem), tmem, tail_kb > 0 ? NB : 0, acc_full,
+  mx_tile_out<T, NB, kSmThreads, 2, 4, kTmemCols>(args.tile, reinterpret_cast<float*>(smem), tmem, tail_kb > 0 ? NB : 0, acc_full,
                                        abort_flag, args.err, splits, rank, n0, t0);
-  tc_fence_before();
-  if (splits > 1)
-    cluster_sync_all();  // no CTA leaves while another reads its partial tile
-  else
-    __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
-  }
 }
 
 template <typename T, int FMT, int NB>

@@ -16,9 +16,9 @@ struct MxTileOut {
 };
 
 // Threads of the block: THREADS; warps FIRST .. FIRST + WARPS - 1 read TMEM (WARPS a
-// multiple of 4).  part: NB x 128 fp32 over the drained stages.  second: TMEM column
-// of the second accumulator, 0 for none.
-template <typename T, int NB, int THREADS, int FIRST, int WARPS>
+// multiple of 4), whose COLS columns warp 1 gives back.  part: NB x 128 fp32 over the drained stages.  second: TMEM column of the second
+// accumulator, 0 for none.
+template <typename T, int NB, int THREADS, int FIRST, int WARPS, int COLS>
 LORA_DEVINL void mx_tile_out(const MxTileOut& args, float* part, uint32_t tmem, uint32_t second, uint64_t* acc_full,
                              volatile int* abort_flag, int* err, int splits, int rank, int n0, int t0) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -44,10 +44,12 @@ LORA_DEVINL void mx_tile_out(const MxTileOut& args, float* part, uint32_t tmem, 
       }
     }
   }
-  if (splits > 1)
-    cluster_sync_all();  // every rank's partial tile is in its shared memory
-  else
+  if (splits > 1) {  // every rank's partial tile is in its shared memory
+    cluster_sync_free_tmem(tmem, COLS, warp, warp >= FIRST && warp < FIRST + WARPS, WARPS);
+  } else {
+    tc_fence_before();
     __syncthreads();
+  }
   {
     const int b = count * rank / splits, e = count * (rank + 1) / splits;
     const int n = n0 + 4 * lane;
@@ -85,6 +87,12 @@ LORA_DEVINL void mx_tile_out(const MxTileOut& args, float* part, uint32_t tmem, 
         if (n + 3 < args.N) o[3] = from_f32<T>(v.w);
       }
     }
+  }
+  if (splits > 1) {
+    cluster_sync_all();  // no CTA leaves while another reads its partial tile
+  } else if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, COLS);
   }
 }
 
