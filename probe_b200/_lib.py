@@ -220,13 +220,16 @@ def stream_handle(device: torch.device | None = None):
 
 
 # ------------------------------------------------------------------ workspaces
+_GROWTH = 64 << 20  # the most that a growing workspace takes beyond what is asked for
+
+
 class _Workspace:
     """Zero-initialised byte buffers, one per (device, stream, slot).
 
     The split-K kernels leave their ticket counters at zero when they finish,
     so a buffer stays valid for every later call on the same stream.  Calls on
     one stream are ordered, so they never share a buffer concurrently.  A
-    buffer only grows (by allocating a new zeroed one).  A CUDA graph keeps the
+    buffer only grows (a new zeroed one, twice as large or 64 MB larger).  A CUDA graph keeps the
     addresses it was captured with: a buffer that a capture has taken stays
     allocated when a larger one replaces it.  Warm the shapes you will capture on
     the stream that captures them: a buffer allocated during a capture is zeroed
@@ -257,7 +260,7 @@ class _Workspace:
             if capturing:  # of the graph's own pool, which holds it
                 return torch.zeros(size, dtype=torch.uint8, device=device)
             if buf is not None:
-                size = max(size, buf.numel() * 2)
+                size = max(size, min(buf.numel() * 2, buf.numel() + _GROWTH))
                 if key in self._captured:
                     self._captured.discard(key)
                     self._retained.append(buf)

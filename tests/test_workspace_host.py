@@ -65,3 +65,12 @@ def test_a_buffer_of_a_capture_serves_that_call_alone(gpu):
     assert ws.get(9000, CPU, "linear") is not eager
     gpu.capturing = False
     assert ws.get(5000, CPU, "linear") is eager
+
+
+def test_growth_doubles_small_buffers_and_not_large_ones(gpu):
+    ws, mb = _lib._Workspace(), 1 << 20
+    assert ws.get(5 * mb, CPU, "a").numel() == 5 * mb
+    assert ws.get(6 * mb, CPU, "a").numel() == 10 * mb
+    ws.get(300 * mb, CPU, "b")
+    assert ws.get(301 * mb, CPU, "b").numel() == 364 * mb
+    assert ws.get(500 * mb, CPU, "b").numel() == 500 * mb
