@@ -140,6 +140,48 @@ LORA_DEVINL uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
   return v;
 }
 
+// MN-major operand in 64-wide chunks `lbo` bytes apart: rows of the contraction 128 bytes
+// apart, 8-row groups 1024 bytes apart, 128-byte swizzle.
+LORA_DEVINL uint64_t mx_desc_mn(uint32_t addr, uint32_t lbo) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((addr >> 4) & 0x3FFF);
+  d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFF) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+// A scale chunk in shared memory: 32 rows of 16 bytes, no swizzle, 8-row groups 128
+// bytes apart.
+LORA_DEVINL uint64_t mx_desc_scales(uint32_t addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((addr >> 4) & 0x3FFF);
+  d |= static_cast<uint64_t>(128 >> 4) << 16;
+  d |= static_cast<uint64_t>(128 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  return d;
+}
+
+// D (+)= A B^T of 4-bit codes with their block scales in TMEM, by one CTA (PAIR false) or a
+// pair of them.
+template <int FMT, bool PAIR>
+LORA_DEVINL void mx_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                        uint32_t accumulate) {
+#define LORA_MX_MMA(GROUP, VEC)                                                                                  \
+  asm volatile(                                                                                                  \
+      "{\n\t.reg .pred p;\n\t"                                                                                  \
+      "setp.ne.b32 p, %6, 0;\n\t"                                                                               \
+      "tcgen05.mma.cta_group::" GROUP ".kind::mxf4nvf4.block_scale.scale_vec::" VEC                              \
+      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),                                                        \
+      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                                            \
+      : "memory")
+  if constexpr (FMT == LORA_MXFP4 && PAIR) LORA_MX_MMA("2", "2X");
+  if constexpr (FMT == LORA_MXFP4 && !PAIR) LORA_MX_MMA("1", "2X");
+  if constexpr (FMT == LORA_NVFP4 && PAIR) LORA_MX_MMA("2", "4X");
+  if constexpr (FMT == LORA_NVFP4 && !PAIR) LORA_MX_MMA("1", "4X");
+#undef LORA_MX_MMA
+}
+
 // One lane of a converged warp.  Asked anew in front of each block that one lane
 // executes, never kept: the code generator may repeat the election where a kept
 // answer is used, and in diverged code that elects several lanes.

@@ -78,17 +78,6 @@ struct DxLayout {
   static_assert(kStages * kStage >= NB * 512, "the partial tile lies over the stages");
 };
 
-// MN-major operand in two 64-wide chunks.
-LORA_DEVINL uint64_t dx_desc_mn(uint32_t addr) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((addr >> 4) & 0x3FFF);
-  d |= static_cast<uint64_t>(kDxHalf >> 4) << 16;
-  d |= static_cast<uint64_t>(1024 >> 4) << 32;
-  d |= static_cast<uint64_t>(1) << 46;
-  d |= static_cast<uint64_t>(2) << 61;
-  return d;
-}
-
 // Factor of a block of codes as a pair of the type, where one packed multiplication
 // is exact: bf16 with 2^112 (see dx_decode8); fp16 in its normal range or zero.
 template <typename T> LORA_DEVINL bool dx_factor(float f, uint32_t& pair);
@@ -241,7 +230,7 @@ __global__ void __launch_bounds__(dx_threads<NB>(), dx_ctas<NB>())
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    const uint64_t wd0 = dx_desc_mn(smem_u32(smem));
+    const uint64_t wd0 = mx_desc_mn(smem_u32(smem), kDxHalf);
     const uint64_t xd0 = umma_desc_sw128(smem_u32(smem) + L::kXOffset);
     for (int i = 0; i < total; ++i) {
       if (!warp_wait(&full_w[stage], phase, abort_flag, args.err, kDevErrTimeoutFull) ||

@@ -78,41 +78,8 @@ struct MxSmem {
   static_assert(kOverlap % 16 == 0 && kBytes <= 227 * 1024, "layout");
 };
 
-// Descriptor of a scale chunk in shared memory: 32 rows of 16 bytes, no swizzle,
-// 8-row groups 128 bytes apart.
-LORA_DEVINL uint64_t mx_desc_scales(uint32_t addr) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((addr >> 4) & 0x3FFF);
-  d |= static_cast<uint64_t>(128 >> 4) << 16;
-  d |= static_cast<uint64_t>(128 >> 4) << 32;
-  d |= static_cast<uint64_t>(1) << 46;
-  return d;
-}
-
 LORA_DEVINL void mx_cp_scales_pair(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-
-template <int FMT>
-LORA_DEVINL void mx_mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
-                             uint32_t accumulate) {
-  if constexpr (FMT == LORA_MXFP4) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
-            d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
-  } else {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
-            d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
-  }
 }
 
 // D = A B^T + D 2^-S
@@ -422,7 +389,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMxGemmThreads, 1)
                 const int j = kMx ? k >> 1 : k;
                 const uint32_t id = kMx ? static_cast<uint32_t>(k & 1) * 2u : 0u;
                 if (k < nk)
-                  mx_mma_pair<FMT>(d, ad + static_cast<uint64_t>(2 * k), bd + static_cast<uint64_t>(2 * k),
+                  mx_mma<FMT, true>(d, ad + static_cast<uint64_t>(2 * k), bd + static_cast<uint64_t>(2 * k),
                                    kIdesc | (id << 4) | (id << 29), sf + 4 * j, sfb + 8 * j,
                                    (kb > -args.num_kb || k > 0) ? 1u : 0u);
               }

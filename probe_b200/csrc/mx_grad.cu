@@ -61,18 +61,6 @@ struct GrArgs {
   int stages, stage_bytes, steps_per_split, steps, splits, scale_gb;
 };
 
-// MN-major operand in 64-wide chunks: token rows 128 bytes apart, 8-row groups
-// 1024 bytes apart, chunks `lbo` bytes apart.
-LORA_DEVINL uint64_t gr_desc_mn(uint32_t addr, uint32_t lbo) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((addr >> 4) & 0x3FFF);
-  d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFF) << 16;
-  d |= static_cast<uint64_t>(1024 >> 4) << 32;
-  d |= static_cast<uint64_t>(1) << 46;
-  d |= static_cast<uint64_t>(2) << 61;
-  return d;
-}
-
 LORA_DEVINL uint32_t gr_mul_bf16x2(uint32_t a, uint32_t b) {
   const __nv_bfloat162 v =
       __hmul2_rn(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
@@ -185,8 +173,8 @@ LORA_DEVINL void gr_job(const GrMaps& maps, const GrArgs& args, int group, int s
     // operands MN-major (bits 15 and 16), M = 128.
     const uint32_t idesc = (umma_idesc_f16(128, 16, std::is_same<T, __nv_bfloat16>::value ? 1 : 0) & ~(0x3fu << 17)) |
                            (static_cast<uint32_t>(args.n >> 3) << 17) | (1u << 15) | (1u << 16);
-    const uint64_t desc0 = gr_desc_mn(smem_u32(smem), S::kChunk);
-    const uint64_t conv0 = gr_desc_mn(smem_u32(conv), S::kChunk);
+    const uint64_t desc0 = mx_desc_mn(smem_u32(smem), S::kChunk);
+    const uint64_t conv0 = mx_desc_mn(smem_u32(conv), S::kChunk);
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;

@@ -66,16 +66,6 @@ LORA_DEVINL int sh_start(const ShArgs& a, int cta) {
   return static_cast<int>(static_cast<uint32_t>(a.chunks_total) * static_cast<uint32_t>(cta) / gridDim.x);
 }
 
-LORA_DEVINL uint64_t sh_desc_mn(uint32_t addr, uint32_t lbo) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((addr >> 4) & 0x3FFF);
-  d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFF) << 16;
-  d |= static_cast<uint64_t>(1024 >> 4) << 32;
-  d |= static_cast<uint64_t>(1) << 46;
-  d |= static_cast<uint64_t>(2) << 61;
-  return d;
-}
-
 // hi/lo pair of 16 values to a row of z.
 template <typename T>
 LORA_DEVINL void sh_store_pair(T* z, int r16, const float* v) {
@@ -215,7 +205,7 @@ __global__ void __launch_bounds__(kShThreads, 1)
     const uint32_t idesc = (umma_idesc_f16(128, 16, std::is_same<T, __nv_bfloat16>::value ? 1 : 0) & ~(0x3fu << 17)) |
                            (static_cast<uint32_t>(args.r16 >> 3) << 17) | (AMN ? 1u << 16 : 0u);
     const uint64_t x0 = umma_desc_sw128(smem_u32(smem));
-    const uint64_t a0 = AMN ? sh_desc_mn(smem_u32(smem) + KB * kShBoxBytes, args.a_box_bytes)
+    const uint64_t a0 = AMN ? mx_desc_mn(smem_u32(smem) + KB * kShBoxBytes, args.a_box_bytes)
                             : umma_desc_sw128(smem_u32(smem) + KB * kShBoxBytes);
     int stage = 0, seg = 0;
     uint32_t phase = 0;

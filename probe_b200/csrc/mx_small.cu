@@ -37,39 +37,9 @@ struct SmArgs {
   int num_kb, last_step, rank_kb, last_k16, chunks, stages;
 };
 
-LORA_DEVINL uint64_t sm_desc_scales(uint32_t addr) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((addr >> 4) & 0x3FFF);
-  d |= static_cast<uint64_t>(128 >> 4) << 16;
-  d |= static_cast<uint64_t>(128 >> 4) << 32;
-  d |= static_cast<uint64_t>(1) << 46;
-  return d;
-}
 LORA_DEVINL void sm_cp_scales(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-template <int FMT>
-LORA_DEVINL void sm_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
-                        uint32_t accumulate) {
-  if constexpr (FMT == LORA_MXFP4) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
-            d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
-  } else {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
-            d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
-  }
-}
-
 template <int FMT, int NB>
 struct SmLayout {
   static constexpr int kChunks = 256 / MxFormat<FMT>::kBlock / 4;
@@ -184,7 +154,7 @@ __global__ void __launch_bounds__(kSmThreads)
     bool ok = true;
     const uint64_t wd0 = umma_desc_sw128(smem_u32(smem));
     const uint64_t xd0 = umma_desc_sw128(smem_u32(smem) + L::kXOffset);
-    const uint64_t sd0 = sm_desc_scales(smem_u32(smem) + L::kSfOffset);
+    const uint64_t sd0 = mx_desc_scales(smem_u32(smem) + L::kSfOffset);
     for (int i = 0; i < total; ++i) {
       if (!warp_wait(&full[stage], phase, abort_flag, args.err, kDevErrTimeoutFull)) {
         ok = false;
@@ -208,7 +178,7 @@ __global__ void __launch_bounds__(kSmThreads)
             const int j = kMx ? k >> 1 : k;
             const uint32_t id = kMx ? static_cast<uint32_t>(k & 1) * 2u : 0u;
             if (k < nk)
-              sm_mma<FMT>(tmem, wd + static_cast<uint32_t>(2 * k), xd + static_cast<uint32_t>(2 * k),
+              mx_mma<FMT, false>(tmem, wd + static_cast<uint32_t>(2 * k), xd + static_cast<uint32_t>(2 * k),
                           kIdesc | (id << 4) | (id << 29), sfa + 4 * j, sfb + 4 * j, (i > 0 || k > 0) ? 1u : 0u);
           }
           tc_commit(&empty[stage]);
