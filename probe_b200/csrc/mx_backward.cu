@@ -45,7 +45,8 @@ struct BackwardPlan {
 };
 
 // dy_rows, b_rows: TMA can read dy, b where they lie.
-BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need_dx, bool half, bool dy_rows, bool b_rows) {
+BackwardPlan backward_plan(int64_t M, int64_t N, int64_t K, int64_t R, bool need_dx, bool half, bool dy_rows,
+                           bool b_rows) {
   BackwardPlan p = {};
   const int64_t np = up(N, 8), rp = up(R, 16);
   const int dev = current_device();
@@ -123,9 +124,10 @@ __global__ void __launch_bounds__(256) mx_transpose_kernel(const TransposeJobs j
   }
 }
 
-TransposeJob transpose_job(const void* in, int64_t ldi, void* out, int64_t ldo, int64_t rows, int64_t cols, int64_t width,
-                           int copies, int lows) {
-  TransposeJob t{static_cast<const uint16_t*>(in), static_cast<uint16_t*>(out), ldi, ldo, rows, cols, width, copies, lows};
+TransposeJob transpose_job(const void* in, int64_t ldi, void* out, int64_t ldo, int64_t rows, int64_t cols,
+                           int64_t width, int copies, int lows) {
+  TransposeJob t{static_cast<const uint16_t*>(in), static_cast<uint16_t*>(out), ldi, ldo, rows, cols, width, copies,
+                 lows};
   t.blocks_c = static_cast<int>(up(cols, 32) / 32);
   t.blocks = t.blocks_c * static_cast<int>(up(width, 32) / 32);
   return t;
@@ -149,14 +151,15 @@ __global__ void __launch_bounds__(256) mx_split_rows_kernel(const uint16_t* __re
 #pragma unroll
   for (int i = 0; i < 8; ++i) split_half(c + i < cols ? in[row * ldi + c + i] : uint16_t{0}, h[i], l[i]);
   auto word = [](const uint16_t* v) { return v[0] | (static_cast<uint32_t>(v[1]) << 16); };
-  *reinterpret_cast<uint4*>(out + row * width + c) = make_uint4(word(h), word(h + 2), word(h + 4), word(h + 6));
-  *reinterpret_cast<uint4*>(out + (rows + row) * width + c) = make_uint4(word(l), word(l + 2), word(l + 4), word(l + 6));
+  uint16_t* dst = out + row * width + c;
+  *reinterpret_cast<uint4*>(dst) = make_uint4(word(h), word(h + 2), word(h + 4), word(h + 6));
+  *reinterpret_cast<uint4*>(dst + rows * width) = make_uint4(word(l), word(l + 2), word(l + 4), word(l + 6));
 }
 
 int split_rows(const void* in, int64_t ldi, void* out, int64_t rows, int64_t cols, int64_t width, cudaStream_t s) {
   const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>((width + 2047) / 2048));
-  mx_split_rows_kernel<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(in), ldi, static_cast<uint16_t*>(out), rows, cols,
-                                            width);
+  mx_split_rows_kernel<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(in), ldi, static_cast<uint16_t*>(out), rows,
+                                            cols, width);
   return cudaGetLastError() == cudaSuccess ? LORA_OK : LORA_ERR_CUDA;
 }
 

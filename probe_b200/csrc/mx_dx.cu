@@ -20,10 +20,10 @@
 // most four, so the product is exact wherever it is a normal number of the type.
 //
 // Bound: the chain load -> decode -> MMA of a stage over a ring of four (64 tokens: three),
-// whose 16-bit tiles fill the shared memory, then the decode's ALU work.  64 rows of 13824 x 5120 (nvfp4, r = 16) take 44 us, of which
-// 11 are the decode's and 6 the MMAs' (each left out in turn); 256 rows of 4096 x 4096
-// 18.  HBM's share is small, 0.53 or 0.56 bytes a weight.  So a tile takes up to 256
-// tokens, whose decode is then paid once (256 rows, whole backward pass: two tiles of 128
+// whose 16-bit tiles fill the shared memory, then the decode's ALU work.  64 rows of
+// 13824 x 5120 (nvfp4, r = 16) take 44 us, of which 11 are the decode's and 6 the MMAs'
+// (each left out in turn); 256 rows of 4096 x 4096 18.  HBM's share is small, 0.53 or
+// 0.56 bytes a weight.  So a tile takes up to 256 tokens, whose decode is then paid once (256 rows, whole backward pass: two tiles of 128
 // 33.8 us, one of 256 28.3; 512 rows 52.8 and 39.5); from 128 tokens on, where one CTA
 // fills an SM, two groups of eight warps decode stages in turn (128 rows, 4096 x 11008:
 // 53.3 to 49.3), below, two CTAs of one group each share it (64 rows, 13824 x 5120: 55.8

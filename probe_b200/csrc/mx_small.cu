@@ -206,8 +206,9 @@ __global__ void __launch_bounds__(kSmThreads)
     __syncwarp();
   }
 
-  mx_tile_out<T, NB, kSmThreads, 2, 4, kTmemCols>(args.tile, reinterpret_cast<float*>(smem), tmem, tail_kb > 0 ? NB : 0, acc_full,
-                                       abort_flag, args.err, splits, rank, n0, t0);
+  mx_tile_out<T, NB, kSmThreads, 2, 4, kTmemCols>(args.tile, reinterpret_cast<float*>(smem), tmem,
+                                                  tail_kb > 0 ? NB : 0, acc_full, abort_flag, args.err, splits, rank,
+                                                  n0, t0);
 }
 
 template <typename T, int FMT, int NB>
